@@ -28,6 +28,7 @@
 #include <tuple>
 #include <vector>
 
+#include "nanonemo_embedding.h"
 #include "nanonemo_fa.h"
 #include "nanonemo_linear.h"
 #include "nanonemo_loss.h"
@@ -57,6 +58,7 @@ void rope_done(int rc) { done(rc, nn_rope_last_error); }
 void rms_done(int rc) { done(rc, nn_rmsnorm_last_error); }
 void lin_done(int rc) { done(rc, nn_linear_last_error); }
 void loss_done(int rc) { done(rc, nn_loss_last_error); }
+void emb_done(int rc) { done(rc, nn_embedding_last_error); }
 
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
@@ -70,6 +72,11 @@ Tensor contig(const Tensor& t) { return t.is_contiguous() && !t.is_neg() ? t : r
 Tensor empty_of(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options()); }
 Tensor empty_f32(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
 Tensor bytes(const Tensor& like, size_t n) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
+// A contiguous tensor's values at a 16-byte boundary (a slice may start anywhere).
+Tensor dense(const Tensor& t) {
+    const Tensor c = contig(t);
+    return c.numel() == 0 || (uintptr_t)c.data_ptr() % 16 == 0 ? c : c.clone();
+}
 float scale_of(int64_t D) { return (float)(1.0 / std::sqrt((double)D)); }
 
 // The library reads raw addresses on x's device.
@@ -405,8 +412,8 @@ std::vector<Tensor> wgrad(const Tensor& dy_, const Tensor& x_, const std::vector
     const c10::DeviceGuard guard(x_.device());
     if (!wgrad_takes(T, N, K)) {
         // (dense rows are the library's to read whatever their width; an odd vocabulary's are not 16-byte aligned)
-        auto dense = [](const Tensor& t) { return t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0 ? t : rows_aligned(t); };
-        Tensor dw = at::mm(dense(dy_).t(), dense(x_), at::kFloat);
+        auto readable = [](const Tensor& t) { return t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0 ? t : rows_aligned(t); };
+        Tensor dw = at::mm(readable(dy_).t(), readable(x_), at::kFloat);
         if (rows.size() == 1) return {dw};
         std::vector<Tensor> out = dw.split_with_sizes(rows);
         for (Tensor& t : out) t = t.clone();
@@ -620,6 +627,53 @@ std::vector<OptTensor> head_bwd(const OptTensor& dlogits_, const OptTensor& dlos
     return out;
 }
 
+// ---- embedding ----------------------------------------------------------------------------------
+
+// The width of a token.
+int index_bits(const Tensor& idx) {
+    const auto t = idx.scalar_type();
+    need(t == at::kLong || t == at::kInt, "tokens must be int64 or int32");
+    return t == at::kLong ? 64 : 32;
+}
+
+Tensor embedding_fwd(const Tensor& idx_, const Tensor& weight_, double scale) {
+    check_on_device(weight_, {&idx_});
+    const int bits = index_bits(idx_);
+    need(weight_.dim() == 2 && code(weight_) >= 0, "weight must be a float16, bfloat16 or float32 matrix (V, N)");
+    const Tensor idx = contig(idx_), w = dense(weight_);
+    const int64_t M = idx.numel(), V = w.size(0), N = w.size(1);
+    std::vector<int64_t> shape = idx.sizes().vec();
+    shape.push_back(N);
+    Tensor out = empty_of(w, shape);
+    const c10::DeviceGuard guard(w.device());
+    emb_done(nn_embedding_fwd(w.data_ptr(), idx.data_ptr(), out.data_ptr(), M, V, N, (float)scale, code(w), bits, stream_of(w)));
+    return out;
+}
+
+Tensor embedding_bwd(const Tensor& dy_, const Tensor& idx_, int64_t rows, double scale, int64_t padding) {
+    check_on_device(dy_, {&idx_});
+    const int bits = index_bits(idx_);
+    need(code(dy_) >= 0 && dy_.dim() == idx_.dim() + 1 && dy_.sizes().slice(0, idx_.dim()) == idx_.sizes(),
+         "d_out must be a float16, bfloat16 or float32 tensor of the tokens' shape and one dimension more");
+    need(padding < rows, "padding_idx must be a row of the weight");
+    const Tensor idx = contig(idx_), dy = dense(dy_);
+    const int64_t M = idx.numel(), N = dy.size(-1);
+    Tensor dw = empty_of(dy, {rows, N});
+    const c10::DeviceGuard guard(dy.device());
+    const size_t n = nn_embedding_bwd_workspace_size(M, rows, N);
+    Tensor ws = bytes(dy, n ? n : 1);
+    emb_done(nn_embedding_bwd(dy.data_ptr(), idx.data_ptr(), dw.data_ptr(), ws.data_ptr(), n, M, rows, N, (float)scale, padding, code(dy), bits,
+                              stream_of(dy)));
+    return dw;
+}
+
+// The ops as the dispatcher calls them (padding is the backward's).
+Tensor embedding_op(const Tensor& idx, const Tensor& weight, double scale, int64_t) { return embedding_fwd(idx, weight, scale); }
+Tensor embedding_bwd_op(const Tensor& dy, const Tensor& idx, int64_t rows, double scale, int64_t padding) {
+    refuse_capture_from_engine("embedding backward op");
+    return embedding_bwd(dy, idx, rows, scale, padding);
+}
+
 // ---- routing ------------------------------------------------------------------------------------
 
 // Whether the tensor's values lie at its address, as dense values of its own type: not inside a transform's wrapper
@@ -677,6 +731,8 @@ TORCH_LIBRARY_IMPL(nanonemo, CUDA, m) {
     m.impl("rope_qk_bwd", rope_bwd_op);
     m.impl("cuda_add_rms_norm_fwd", norm_fwd);
     m.impl("cuda_add_rms_norm_bwd", norm_bwd);
+    m.impl("embedding", embedding_op);
+    m.impl("embedding_bwd", embedding_bwd_op);
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -693,6 +749,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("rope", rope, nogil);
     m.def("norm_fwd", norm_fwd, nogil);
     m.def("norm_bwd", norm_bwd, nogil);
+    m.def("embedding_fwd", embedding_fwd, nogil);
+    m.def("embedding_bwd", embedding_bwd, nogil);
     m.def("wgrad", wgrad, nogil);
     m.def("wgrad_takes", wgrad_takes);
     m.def("rows_aligned", rows_aligned);

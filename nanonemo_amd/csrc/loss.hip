@@ -13,57 +13,16 @@
 #include <stdio.h>
 
 #include <string>
-#include <type_traits>
 
 #include "nanonemo_loss.h"
-#include "tiles.h"
+#include "rows.h"
 
 #define NNLOSS_API extern "C" __attribute__((visibility("default")))
 
 namespace {
 
-constexpr int kF32 = 2;
 constexpr int kThreads = 256;
 constexpr long long kIgnore = -100;
-
-// Logits of type DT in groups of 16 bytes, as fp32.
-template <int DT>
-struct Row {
-    static constexpr int W = DT == kF32 ? 4 : 8;
-    using T = std::conditional_t<DT == kF32, float, u16>;
-    static __device__ float one(T x) {
-        if constexpr (DT == kF32)
-            return x;
-        else
-            return Elem<DT>::to_f32(x);
-    }
-    static __device__ T round(float x) {
-        if constexpr (DT == kF32)
-            return x;
-        else
-            return (T)(Elem<DT>::pack2(x, 0.f) & 0xffffu);
-    }
-    static __device__ void load(const T* p, float* v) {
-        if constexpr (DT == kF32) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(p);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = x[e];
-        } else {
-            const u16x8 x = ld8(p);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = Elem<DT>::to_f32(x[e]);
-        }
-    }
-    static __device__ void store(T* p, const float* v) {
-        if constexpr (DT == kF32)
-            *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-        else
-            *reinterpret_cast<u32x4*>(p) = u32x4{Elem<DT>::pack2(v[0], v[1]), Elem<DT>::pack2(v[2], v[3]),
-                                                 Elem<DT>::pack2(v[4], v[5]), Elem<DT>::pack2(v[6], v[7])};
-    }
-    // Values before the row's first 16-byte boundary (rows of an odd vocabulary start anywhere).
-    static __device__ int head(const T* row, int V) { return min(V, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T)); }
-};
 
 constexpr float kL2e = 1.4426950408889634f;
 // exp(x - m), the difference rounded once; 0 for x = -inf whatever a finite m.

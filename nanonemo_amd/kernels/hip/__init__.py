@@ -113,6 +113,11 @@ SIGNATURES: dict[str, tuple] = {
     "nn_cross_entropy_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp]),
     "nn_cross_entropy_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp]),
     "nn_loss_last_error": (ctypes.c_char_p, []),
+    # include/nanonemo_embedding.h
+    "nn_embedding_fwd": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _f32, _int, _int, _vp]),
+    "nn_embedding_bwd_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "nn_embedding_bwd": (_int, [_vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _f32, _i64, _int, _int, _vp]),
+    "nn_embedding_last_error": (ctypes.c_char_p, []),
 }
 
 ABI_VERSION = 11
@@ -183,6 +188,24 @@ def records(*ts) -> bool:
     return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
 
 
+def refuse_capture(where: str, *inputs) -> None:
+    """Raise when the current stream is capturing and autograd will record a call on these inputs (grad mode on and one of
+    them requires grad; without inputs: a backward, which autograd's engine runs): a HIP graph around a forward and its
+    autograd backward is not supported, a call without autograd is. Nothing has been launched when this raises; skipped
+    while torch.compile traces (no capture runs then)."""
+    import torch
+
+    if inputs and not records(*inputs):
+        return
+    if not torch.cuda.is_initialized() or torch.compiler.is_compiling() or not torch.cuda.is_current_stream_capturing():
+        return
+    raise RuntimeError(
+        f"{where}: capturing this op into a HIP graph while autograd records it (torch.cuda.graph around the forward and "
+        "its autograd backward, or torch.compile(mode='reduce-overhead')) is not supported. Capture it without autograd "
+        "(under torch.no_grad(), or the C ABI's calls), or run it eagerly."
+    )
+
+
 def strides3(b: int, h: int, t: int) -> ctypes.Array:
     """An int64[3] {batch, head, row} element-stride array for the *_strided entry points."""
     return (ctypes.c_int64 * 3)(b, h, t)
@@ -207,6 +230,13 @@ def check_loss(rc: int) -> None:
     if rc != 0:
         msg = lib().nn_loss_last_error().decode(errors="replace")
         raise RuntimeError(msg or f"nanonemo_loss call failed with code {rc}")
+
+
+def check_embedding(rc: int) -> None:
+    """Raise RuntimeError with the library's message when an nn_embedding_* entry point returns non-zero."""
+    if rc != 0:
+        msg = lib().nn_embedding_last_error().decode(errors="replace")
+        raise RuntimeError(msg or f"nanonemo_embedding call failed with code {rc}")
 
 
 def check_rmsnorm(rc: int) -> None:

@@ -16,7 +16,8 @@ tied input/output embedding, GPT-2 style init with the residual projections scal
 ``rope_kernel="hip"`` rotates q and k with this build's RoPE kernel (nanonemo::rope_qk), ``rope_kernel="fused"``
 rotates k with it and q inside the layout-fused attention op (nanonemo::flash_attn_bthd_rope), and
 ``norm_kernel="hip"`` runs the residual add + RMSNorm on either side of attention as this build's fused
-kernel (nanonemo::cuda_add_rms_norm_fwd / _bwd, the reference's norm_kernel="cuda").
+kernel (nanonemo::cuda_add_rms_norm_fwd / _bwd, the reference's norm_kernel="cuda"), and ``emb_kernel="hip"`` the token
+embedding and its gradient (nanonemo::embedding).
 
 A model with any of them set also runs its linear layers, SwiGLU and cross entropy on this build's kernels where it is
 called eagerly on a GPU under 16-bit autocast (kernels/hip/linear.py, layers.py and head.py say exactly when; there the
@@ -59,6 +60,8 @@ class ModelConfig:
     # op nanonemo::flash_attn_bthd_rope, k alone by nanonemo::rope_qk; needs attn_kernel="hip_bthd")
     rope_kernel: str = "torch"
     norm_kernel: str = "torch"  # "torch" | "hip" (fused residual add + RMSNorm, nanonemo::cuda_add_rms_norm_*)
+    emb_kernel: str = "torch"  # "torch" | "hip" (lookup, and the gradient by sorted tokens, nanonemo::embedding)
+    emb_scale: float = 1.0  # the embeddings times this (sqrt(d_model) in models that scale them)
 
     def __post_init__(self):
         if self.d_model % self.n_heads:
@@ -77,6 +80,8 @@ class ModelConfig:
             raise ValueError('rope_kernel="fused" needs attn_kernel="hip_bthd"')
         if self.norm_kernel not in ("torch", "hip"):
             raise ValueError(f"unknown norm_kernel {self.norm_kernel!r}")
+        if self.emb_kernel not in ("torch", "hip"):
+            raise ValueError(f"unknown emb_kernel {self.emb_kernel!r}")
 
     @property
     def head_dim(self) -> int:
@@ -85,7 +90,7 @@ class ModelConfig:
     @property
     def any_hip(self) -> bool:
         """Whether the model runs on this build's kernels; its linear layers then do too (kernels/hip/linear.py)."""
-        return self.attn_kernel != "torch" or self.rope_kernel != "torch" or self.norm_kernel != "torch"
+        return any(k != "torch" for k in (self.attn_kernel, self.rope_kernel, self.norm_kernel, self.emb_kernel))
 
 
 def _project(cfg: ModelConfig, x: torch.Tensor, *layers: nn.Module) -> tuple[torch.Tensor, ...]:
@@ -241,6 +246,28 @@ class MLP(nn.Module):
         return self.w_down(F.silu(self.w_gate(x)) * self.w_up(x))
 
 
+class Embedding(nn.Embedding):
+    """The tokens' embeddings times a scale. kernel="hip" looks them up, and sums their gradient, with this build's kernels
+    (nn.Embedding's other options keep its own)."""
+
+    def __init__(self, num: int, dim: int, scale: float = 1.0, kernel: str = "torch", **options):
+        super().__init__(num, dim, **options)
+        self.scale = scale
+        self.fused = None
+        if kernel == "hip":
+            from nanonemo_amd.kernels.hip.embedding import embedding  # raises without the library
+
+            self.fused = embedding
+
+    def forward(self, idx: torch.Tensor) -> torch.Tensor:
+        # (a module traced symbolically has no tensor here)
+        if self.fused is not None and isinstance(idx, torch.Tensor) and idx.is_cuda \
+                and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse:
+            return self.fused(idx, self.weight, self.scale, self.padding_idx)
+        x = super().forward(idx)
+        return x if self.scale == 1.0 else x * self.scale
+
+
 class Block(nn.Module):
     """Pre-norm block; returns (stream, pending MLP output) like layers.py:140-161."""
 
@@ -263,7 +290,8 @@ class NanoNemo(nn.Module):
     def __init__(self, cfg: ModelConfig):
         super().__init__()
         self.cfg = cfg
-        self.tok_emb = nn.Embedding(cfg.vocab_size, cfg.d_model)
+        plain = cfg.emb_kernel == "torch" and cfg.emb_scale == 1.0
+        self.tok_emb = nn.Embedding(cfg.vocab_size, cfg.d_model) if plain else Embedding(cfg.vocab_size, cfg.d_model, cfg.emb_scale, cfg.emb_kernel)
         self.blocks = nn.ModuleList(Block(cfg) for _ in range(cfg.n_layers))
         self.norm_out = AddRMSNorm(cfg.d_model, cfg.norm_eps, cfg.norm_kernel)
         self.lm_head = nn.Linear(cfg.d_model, cfg.vocab_size, bias=False)
