@@ -1,0 +1,662 @@
+// Distillation from a teacher's top logits for MI355X (gfx950): the selection of the top logits, and the loss of a
+// student's logits against them with its gradient.
+//
+// With z a row of the student's logits, t_i the teacher's values at the indices j_i, tau the temperature, w the weight:
+//   p_i = exp(t_i / tau - Lt)                     Lt = logsumexp(t / tau [, rest])
+//   q_j = exp(z_j / tau - L)                      L = logsumexp(z / tau),  q_rest = the sum of q outside the top set
+//   KL = sum p_i (log p_i - log q_{j_i}) [+ p_rest (log p_rest - log q_rest)]
+//   loss = mean of w tau^2 KL + (1 - w) (logsumexp(z) - z_target)
+//   dz_j = g / n (w tau (q_j f_j - p_j) + (1 - w) (s_j - [j = target])),  s = softmax(z),
+//   f_j = 1 - p_rest / q_rest outside the top set where rest is a class, else 1.
+//
+// A student near its teacher has a loss far below L, so the loss is a small difference of terms that share L. The sum over
+// the row, in fp32, therefore leaves out the top set and the target (a bitmap in LDS marks them); their terms, and all that
+// is joined from them, are computed in fp64, where the shared part cancels. An error of the row's sum then reaches KL only
+// times (q_rest - p_rest).
+//
+// All of it is bound by HBM: the forward reads the logits once, the backward reads them once and writes the gradient.
+// Built with NaN semantics: NaN and infinite logits reach the outputs.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "nanonemo_distill.h"
+#include "rows.h"
+
+#define NNDIS_API extern "C" __attribute__((visibility("default")))
+
+namespace {
+
+constexpr int kMaxTop = 512;
+constexpr int kMaxVocab = 393216;  // 48 KB of marks
+constexpr int kVocabBits = 19;
+constexpr long long kIgnore = -100;
+constexpr float kL2e = 1.4426950408889634f;
+
+struct Layout {  // row r at (r / T) * sb + (r % T) * st
+    long long sb, st;
+    int T;
+    __device__ long long at(int r) const {
+        const int b = r / T;
+        return b * sb + (r - b * T) * st;
+    }
+};
+
+// A 16-byte group at an address of the element's own alignment.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+template <int DT>
+__device__ inline u32x4 load_any(const typename Row<DT>::T* p) {
+    return *reinterpret_cast<const u32x4_any*>(p);
+}
+template <int DT>
+__device__ inline void store_any(typename Row<DT>::T* p, u32x4 v) {
+    *reinterpret_cast<u32x4_any*>(p) = v;
+}
+template <int DT>
+__device__ inline typename Row<DT>::T minus_inf() {
+    if constexpr (DT == kF32)
+        return -INFINITY;
+    else
+        return DT == kBF16 ? 0xff80 : 0xfc00;
+}
+// Group i of a row; values past the row's end are -inf.
+template <int DT>
+__device__ inline u32x4 group(const typename Row<DT>::T* row, int i, int V) {
+    using R = Row<DT>;
+    const int j = i * R::W;
+    if (j + R::W <= V) return load_any<DT>(row + j);
+    union {
+        u32x4 v;
+        typename R::T e[R::W];
+    } u;
+#pragma unroll
+    for (int e = 0; e < R::W; ++e) u.e[e] = j + e < V ? row[j + e] : minus_inf<DT>();
+    return u.v;
+}
+
+// Sums, maxima and the like over a block of TB threads: every thread gets the result. `tmp` is one value per wave, free for
+// the next call as soon as this one has returned everywhere.
+template <int TB, typename T, typename F>
+__device__ inline T block_all(T v, T* tmp, F f) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v = f(v, __shfl_xor(v, d));
+    if constexpr (TB > 64) {
+        if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = tmp[0];
+#pragma unroll
+        for (int w = 1; w < TB / 64; ++w) v = f(v, tmp[w]);
+        __syncthreads();
+    }
+    return v;
+}
+
+// ------------------------------------------------------------------------------------------
+// Softmax sums.
+// ------------------------------------------------------------------------------------------
+// exp((x - m) * c / log2(e)), the difference rounded first; 0 for x = -inf whatever a finite m.
+__device__ inline float exp_diff(float x, float m, float c) { return __builtin_amdgcn_exp2f((x - m) * c); }
+// What exponents are relative to: 0 where every value is -inf (their exp is 0 then) or one is +inf (infinite then).
+__device__ inline float base_of(float m) { return fabsf(m) == INFINITY ? 0.f : m; }
+
+// The factor that takes a sum relative to base_of(m) to another base; 0 for the empty sum, whose m is -inf.
+__device__ inline float rebase(float m, float base, float c) { return exp_diff(m == INFINITY ? 0.f : m, base, c); }
+
+struct MaxSum {  // s = sum of exp((x - base_of(m)) / tau); with a second sum at temperature 1
+    float m, s, s1;
+};
+template <bool BOTH>
+__device__ inline MaxSum merge(MaxSum a, MaxSum b, float c) {
+    const float m = fmaxf(a.m, b.m), base = base_of(m);
+    MaxSum r{m, a.s * rebase(a.m, base, c) + b.s * rebase(b.m, base, c), 0.f};
+    if constexpr (BOTH) r.s1 = a.s1 * rebase(a.m, base, kL2e) + b.s1 * rebase(b.m, base, kL2e);
+    return r;
+}
+// W further values.
+template <bool BOTH, int W>
+__device__ inline void take(MaxSum& a, const float* v, float c) {
+    float m = a.m;
+#pragma unroll
+    for (int e = 0; e < W; ++e) m = fmaxf(m, v[e]);
+    const float base = base_of(m);
+    float s = a.s * rebase(a.m, base, c), s1 = BOTH ? a.s1 * rebase(a.m, base, kL2e) : 0.f;
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+        s += exp_diff(v[e], base, c);
+        if constexpr (BOTH) s1 += exp_diff(v[e], base, kL2e);
+    }
+    a = {m, s, s1};
+}
+template <int TB, bool BOTH>
+__device__ inline MaxSum block_merge(MaxSum a, MaxSum* tmp, float c) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1)
+        a = merge<BOTH>(a, MaxSum{__shfl_xor(a.m, d), __shfl_xor(a.s, d), BOTH ? __shfl_xor(a.s1, d) : 0.f}, c);
+    if constexpr (TB > 64) {
+        if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = a;
+        __syncthreads();
+        a = tmp[0];
+#pragma unroll
+        for (int w = 1; w < TB / 64; ++w) a = merge<BOTH>(a, tmp[w], c);
+        __syncthreads();
+    }
+    return a;
+}
+
+// ------------------------------------------------------------------------------------------
+// The top logits: one block per row.
+// ------------------------------------------------------------------------------------------
+// A logit as a whole number of the same order: -0 as 0, NaN above everything; 0 is below every logit.
+template <int DT>
+struct Key {
+    static constexpr int kBits = DT == kF32 ? 32 : 16;
+    static constexpr uint32_t kSign = 1u << (kBits - 1), kAll = DT == kF32 ? 0xffffffffu : 0xffffu;
+    static constexpr uint32_t kInf = DT == kF32 ? 0x7f800000u : DT == kBF16 ? 0x7f80u : 0x7c00u;
+    using T = typename Row<DT>::T;
+    static __device__ uint32_t of(T x) {
+        uint32_t u;
+        if constexpr (DT == kF32)
+            u = __float_as_uint(x);
+        else
+            u = x;
+        const uint32_t mag = u & (kSign - 1);
+        if (mag > kInf) return kAll;
+        if (mag == 0) u = 0;
+        return u & kSign ? u ^ kAll : u | kSign;
+    }
+    static __device__ T value(uint32_t key) {
+        const uint32_t u = key & kSign ? key ^ kSign : key ^ kAll;
+        if constexpr (DT == kF32)
+            return __uint_as_float(u);
+        else
+            return (T)u;
+    }
+};
+__device__ inline uint64_t ranked(uint32_t key, int j) { return ((uint64_t)key << 32) | (0xffffffffu - (uint32_t)j); }
+
+template <int TB>
+constexpr int kCandidates = TB >= 1024 ? 2048 : TB >= 256 ? 1024 : 512;  // (at least kMaxTop)
+
+template <int DT, int TB>
+__global__ __launch_bounds__(TB) void top_kernel(const void* __restrict__ logits, Layout at, void* __restrict__ values,
+                                                 long long* __restrict__ indices, float* __restrict__ rest, int V, int k, float c,
+                                                 double inv_tau) {
+    using R = Row<DT>;
+    using T = typename R::T;
+    using K = Key<DT>;
+    const T* row = reinterpret_cast<const T*>(logits) + at.at(blockIdx.x);
+    const int tid = threadIdx.x, groups = (V + R::W - 1) / R::W;
+    __shared__ uint64_t cand[kCandidates<TB>];
+    __shared__ uint32_t maxima[TB];
+    __shared__ int tmp[TB / 64];
+    __shared__ int count;
+    __shared__ uint32_t bound;
+    __shared__ uint64_t last;
+    auto each = [&](auto f) {
+        for (int i = tid; i < groups; i += TB) {
+            union {
+                u32x4 v;
+                T e[R::W];
+            } u;
+            u.v = group<DT>(row, i, V);
+#pragma unroll
+            for (int e = 0; e < R::W; ++e)
+                if (i * R::W + e < V) f(u.e[e], i * R::W + e);
+        }
+    };
+    auto add = [](int a, int b) { return a + b; };
+    auto counted = [&](auto f) {
+        int n = 0;
+        each([&](T x, int j) { n += f(K::of(x), j) ? 1 : 0; });
+        return block_all<TB>(n, tmp, add);
+    };
+    auto collect = [&](auto f) {
+        if (tid == 0) count = 0;
+        __syncthreads();
+        each([&](T x, int j) {
+            const uint32_t key = K::of(x);
+            if (!f(key, j)) return;
+            const int p = atomicAdd(&count, 1);
+            if (p < kCandidates<TB>) cand[p] = ranked(key, j);
+        });
+        __syncthreads();
+        return count;
+    };
+
+    // The k-th largest of the threads' largest is a bound that at least k values reach, and few more do where k is a small
+    // share of the threads.
+    int n = kCandidates<TB> + 1;
+    if (2 * k <= min(TB, groups)) {
+        uint32_t most = 0;
+        each([&](T x, int) { most = max(most, K::of(x)); });
+        maxima[tid] = most;
+        __syncthreads();
+        if (tid < 64) {
+            uint32_t found = 0;
+            for (int b = K::kBits - 1; b >= 0; --b) {
+                const uint32_t t = found | (1u << b);
+                int reach = 0;
+#pragma unroll
+                for (int i = 0; i < TB / 64; ++i) reach += __popcll(__ballot(maxima[tid + 64 * i] >= t));
+                if (reach >= k) found = t;
+            }
+            if (tid == 0) bound = found;
+        }
+        __syncthreads();
+        const uint32_t least = bound;
+        n = collect([&](uint32_t key, int) { return key >= least; });
+    }
+    if (n > kCandidates<TB>) {
+        // Otherwise (many equal values, or k near the number of threads) the k-th largest key, bit by bit, and the place of
+        // the last of its equals that belongs to the k.
+        uint32_t key_k = 0;
+        for (int b = K::kBits - 1; b >= 0; --b) {
+            const uint32_t t = key_k | (1u << b);
+            if (counted([&](uint32_t key, int) { return key >= t; }) >= k) key_k = t;
+        }
+        const int need = k - counted([&](uint32_t key, int) { return key > key_k; });
+        int place = 0;
+        for (int b = kVocabBits - 1; b >= 0; --b) {
+            const int t = place | (1 << b);
+            if (counted([&](uint32_t key, int j) { return key == key_k && j < t; }) < need) place = t;
+        }
+        n = collect([&](uint32_t key, int j) { return key > key_k || (key == key_k && j <= place); });
+    }
+    // Every candidate's rank is the number of larger ones.
+    for (int i = tid; i < n; i += TB) {
+        const uint64_t mine = cand[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += cand[j] > mine ? 1 : 0;
+        if (rank < k) {
+            const size_t to = (size_t)blockIdx.x * k + rank;
+            reinterpret_cast<T*>(values)[to] = K::value((uint32_t)(mine >> 32));
+            indices[to] = (long long)(0xffffffffu - (uint32_t)mine);
+        }
+        if (rank == k - 1) last = mine;
+    }
+    __syncthreads();
+    const uint64_t end = last;
+    MaxSum a{-INFINITY, 0.f, 0.f};
+    each([&](T x, int j) {
+        if (ranked(K::of(x), j) >= end) return;
+        const float v = R::one(x);
+        take<false, 1>(a, &v, c);
+    });
+    __shared__ MaxSum sums[TB / 64];
+    a = block_merge<TB, false>(a, sums, c);
+    if (tid == 0) rest[blockIdx.x] = (float)(base_of(a.m) * inv_tau + log((double)a.s));
+}
+
+// ------------------------------------------------------------------------------------------
+// The loss: one block per row.
+// ------------------------------------------------------------------------------------------
+struct Loss {
+    const void* logits;
+    Layout at;
+    const void* values;
+    const long long* indices;
+    const float* rest;         // or nullptr
+    const long long* targets;  // or nullptr
+    double* stats;             // [R][kStats], then the rows' losses [R], then 1 / n
+    int V, k, vdt;
+    float c;  // log2(e) / tau
+    double tau, weight;
+    __device__ bool hard() const { return targets && weight < 1.0; }
+};
+// A row's statistics: L, logsumexp(z), Lt, f, what exponents are relative to, and whether an index is there twice.
+enum { kL, kL1, kLt, kF, kBase, kTwice, kStats };
+
+__device__ inline float value_at(const void* p, long long i, int dt) {
+    if (dt == kF32) return reinterpret_cast<const float*>(p)[i];
+    const u16 x = reinterpret_cast<const u16*>(p)[i];
+    return dt == kBF16 ? Elem<kBF16>::to_f32(x) : Elem<kF16>::to_f32(x);
+}
+
+// Whether entry e is the first with its index.
+__device__ inline bool first_of(const int* idx, int e) {
+    for (int i = 0; i < e; ++i)
+        if (idx[i] == idx[e]) return false;
+    return true;
+}
+
+struct Sums4 {
+    double a, p, z, z1;
+};
+__device__ inline Sums4 operator+(const Sums4& x, const Sums4& y) { return {x.a + y.a, x.p + y.p, x.z + y.z, x.z1 + y.z1}; }
+template <int TB>
+__device__ inline Sums4 block_sum(Sums4 v, Sums4* tmp) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v = v + Sums4{__shfl_xor(v.a, d), __shfl_xor(v.p, d), __shfl_xor(v.z, d), __shfl_xor(v.z1, d)};
+    if constexpr (TB > 64) {
+        if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = tmp[0];
+#pragma unroll
+        for (int w = 1; w < TB / 64; ++w) v = v + tmp[w];
+        __syncthreads();
+    }
+    return v;
+}
+
+// BOTH: sums at the temperature and at 1.
+template <int DT, int TB, bool BOTH>
+__global__ __launch_bounds__(TB) void loss_fwd_kernel(Loss x) {
+    using R = Row<DT>;
+    using T = typename R::T;
+    extern __shared__ uint32_t marks[];  // a bit per logit: the top set and the target
+    __shared__ int idx[kMaxTop];
+    __shared__ float zs[kMaxTop];
+    __shared__ int bad, twice, target_in_top;
+    __shared__ MaxSum sums[TB / 64];
+    __shared__ double tmp[TB / 64];
+    __shared__ Sums4 tmp4[TB / 64];
+    const int r = blockIdx.x, tid = threadIdx.x, V = x.V, k = x.k;
+    double* st = x.stats + (size_t)r * kStats;
+    double& loss = x.stats[(size_t)gridDim.x * kStats + r];
+    const long long target = x.targets ? x.targets[r] : 0;
+    if (x.targets && target == kIgnore) {
+        if (tid == 0) loss = 0.0;
+        return;
+    }
+    const bool hard = x.hard();
+    const T* row = reinterpret_cast<const T*>(x.logits) + x.at.at(r);
+    const int groups = (V + R::W - 1) / R::W;
+    for (int i = tid; i < (groups * R::W + 31) / 32; i += TB) marks[i] = 0;
+    if (tid == 0) bad = x.targets && (target < 0 || target >= V), twice = 0, target_in_top = 0;
+    __syncthreads();
+    for (int e = tid; e < k; e += TB) {
+        const long long j = x.indices[(size_t)r * k + e];
+        const bool ok = j >= 0 && j < V;
+        idx[e] = ok ? (int)j : 0;
+        zs[e] = R::one(row[idx[e]]);
+        if (!ok) {
+            bad = 1;
+            continue;
+        }
+        const uint32_t bit = 1u << (j & 31), old = atomicOr(&marks[j >> 5], bit);
+        if (hard && j == target) {  // (whose bit tells nothing: it is set below as well)
+            if (atomicAdd(&target_in_top, 1) > 0) twice = 1;
+        } else if (old & bit) {
+            twice = 1;
+        }
+    }
+    if (hard && tid == TB - 1 && target >= 0 && target < V) atomicOr(&marks[target >> 5], 1u << (target & 31));
+    __syncthreads();
+    if (bad) {
+        if (tid < kStats) st[tid] = tid == kTwice ? 0.0 : NAN;
+        if (tid == 0) loss = NAN;
+        return;
+    }
+    // The row without what is marked.
+    MaxSum s{-INFINITY, 0.f, 0.f};
+    const uint8_t* bytes = reinterpret_cast<const uint8_t*>(marks);
+    for (int i = tid; i < groups; i += TB) {
+        float v[R::W];
+        R::widen(group<DT>(row, i, V), v);
+        const uint32_t m = R::W == 8 ? bytes[i] : (bytes[i >> 1] >> (4 * (i & 1))) & 15;
+        if (m) {
+#pragma unroll
+            for (int e = 0; e < R::W; ++e) v[e] = (m >> e) & 1 ? -INFINITY : v[e];
+        }
+        take<BOTH, R::W>(s, v, x.c);
+    }
+    s = block_merge<TB, BOTH>(s, sums, x.c);
+    if constexpr (!BOTH) s.s1 = s.s;  // (read only where the temperature is 1)
+
+    // The rest in fp64. Exponents are relative to the row's largest logit, the teacher's to its largest term.
+    const double inv_tau = 1.0 / x.tau;
+    const double rest = x.rest ? (double)x.rest[r] : -INFINITY;
+    const float z_target = hard ? R::one(row[target]) : -INFINITY;
+    float zmax = fmaxf(s.m, z_target);
+    double tmax = rest;
+    for (int e = tid; e < k; e += TB) {
+        zmax = fmaxf(zmax, zs[e]);
+        tmax = fmax(tmax, value_at(x.values, (long long)r * k + e, x.vdt) * inv_tau);
+    }
+    auto larger = [](double a, double b) { return fmax(a, b); };
+    zmax = (float)block_all<TB>((double)zmax, tmp, larger);
+    tmax = block_all<TB>(tmax, tmp, larger);
+    const double base = base_of(zmax);  // (+inf: the row's results are NaN)
+    Sums4 top{0.0, 0.0, 0.0, 0.0};
+    for (int e = tid; e < k; e += TB) {
+        const double a = value_at(x.values, (long long)r * k + e, x.vdt) * inv_tau, z = zs[e], w = exp(a - tmax);
+        top.a += w;
+        if (!(w == 0.0)) top.p += w * (a - z * inv_tau);
+        if (!twice || first_of(idx, e)) {
+            top.z += exp((z - base) * inv_tau);
+            if (hard) top.z1 += exp(z - base);
+        }
+    }
+    top = block_sum<TB>(top, tmp4);
+    if (tid != 0) return;
+    const double from = s.m == -INFINITY ? -INFINITY : (double)base_of(s.m) - base;
+    double others = s.s * exp(from * inv_tau), others1 = s.s1 * exp(from);
+    if (hard && !target_in_top) {
+        others += exp((z_target - base) * inv_tau);
+        others1 += exp(z_target - base);
+    }
+    const double L = base * inv_tau + log(top.z + others), L1 = hard ? base + log(top.z1 + others1) : 0.0;
+    double A = top.a, P = top.p, f = 1.0;
+    if (x.rest) {
+        const double w = exp(rest - tmax);
+        A += w;
+        if (!(w == 0.0)) {
+            P += w * (rest - (base * inv_tau + log(others)));
+            f = 1.0 - (w / A) * ((top.z + others) / others);
+        }
+    }
+    const double Lt = tmax + log(A);
+    st[kL] = L, st[kL1] = L1, st[kLt] = Lt, st[kF] = f, st[kBase] = base, st[kTwice] = twice;
+    double v = 0.0;
+    if (zmax == INFINITY) v = st[kL] = NAN;  // as softmax has it: inf - inf
+    if (x.weight > 0.0) v += x.weight * x.tau * x.tau * (P / A - Lt + L);
+    if (hard) v += (1.0 - x.weight) * (L1 - z_target);
+    loss = v;
+}
+
+// loss = the rows' sum / n and 1 / n, n the rows that count: one block, in a fixed order.
+__global__ __launch_bounds__(1024) void loss_mean_kernel(const long long* __restrict__ targets, double* __restrict__ stats, float* __restrict__ loss, int R) {
+    const double* rows = stats + (size_t)R * kStats;
+    double s = 0.0;
+    int n = 0;
+    for (int i = threadIdx.x; i < R; i += 1024) {
+        s += rows[i];
+        n += !targets || targets[i] != kIgnore;
+    }
+    __shared__ double tmp[16];
+    __shared__ int tmpn[16];
+    s = block_all<1024>(s, tmp, [](double a, double b) { return a + b; });
+    n = block_all<1024>(n, tmpn, [](int a, int b) { return a + b; });
+    if (threadIdx.x == 0) {
+        *loss = (float)(s / n);
+        stats[(size_t)R * (kStats + 1)] = 1.0 / n;
+    }
+}
+
+template <int DT, int TB, bool BOTH>
+__global__ __launch_bounds__(TB) void loss_bwd_kernel(Loss x, const float* __restrict__ grad, void* __restrict__ dlogits) {
+    using R = Row<DT>;
+    using T = typename R::T;
+    __shared__ int idx[kMaxTop];
+    __shared__ int target_in_top;
+    const int r = blockIdx.x, tid = threadIdx.x, V = x.V, k = x.k;
+    T* dst = reinterpret_cast<T*>(dlogits) + (size_t)r * V;
+    const int whole = V / R::W, tail = whole * R::W;
+    const long long target = x.targets ? x.targets[r] : 0;
+    if (x.targets && target == kIgnore) {
+        for (int i = tid; i < whole; i += TB) store_any<DT>(dst + i * R::W, u32x4{});
+        if (tail + tid < V) dst[tail + tid] = (T)0;
+        return;
+    }
+    const bool hard = x.hard(), soft = x.weight > 0.0;
+    const T* row = reinterpret_cast<const T*>(x.logits) + x.at.at(r);
+    const double* st = x.stats + (size_t)r * kStats;
+    const double inv_tau = 1.0 / x.tau, L = st[kL], L1 = st[kL1], base = st[kBase], f = st[kF];
+    const double g = (double)grad[0] * x.stats[(size_t)gridDim.x * (kStats + 1)], gs = soft ? x.weight * x.tau * g : 0.0, gh = hard ? (1.0 - x.weight) * g : 0.0;
+    // Every logit as one outside the top set.
+    float A = soft ? (float)(gs * f * exp(base * inv_tau - L)) : 0.f;
+    const float B = hard ? (float)(gh * exp(base - L1)) : 0.f, b = (float)base;
+    if constexpr (!BOTH) A += B;  // (there is B only where the temperature is 1)
+    if (L != L) A = NAN;          // an index or target out of range, or a NaN or +inf in the row
+    auto of = [&](float z) {
+        const float d = z - b, v = A * __builtin_amdgcn_exp2f(d * x.c);
+        return BOTH ? v + B * __builtin_amdgcn_exp2f(d * kL2e) : v;
+    };
+    for (int i = tid; i < whole; i += TB) {
+        float v[R::W];
+        R::widen(load_any<DT>(row + i * R::W), v);
+#pragma unroll
+        for (int e = 0; e < R::W; ++e) v[e] = of(v[e]);
+        store_any<DT>(dst + i * R::W, R::narrow(v));
+    }
+    if (tail + tid < V) dst[tail + tid] = R::round(of(R::one(row[tail + tid])));
+    if (L != L) return;
+    // Then the top set and the target, over what was stored.
+    for (int e = tid; e < k; e += TB) {
+        const long long j = x.indices[(size_t)r * k + e];
+        idx[e] = j >= 0 && j < V ? (int)j : -1;  // (statistics of other indices lead to no access outside the row)
+    }
+    if (tid == 0) target_in_top = 0;
+    __syncthreads();
+    const bool twice = st[kTwice] != 0.0;
+    for (int e = tid; e < k; e += TB) {
+        const int j = idx[e];
+        if (j < 0) continue;
+        if (hard && j == target) target_in_top = 1;
+        if (twice && !first_of(idx, e)) continue;
+        const double z = R::one(row[j]);
+        double v = 0.0;
+        if (soft) {
+            double p = 0.0;
+            for (int i = e; i < (twice ? k : e + 1); ++i)
+                if (idx[i] == j) p += exp(value_at(x.values, (long long)r * k + i, x.vdt) * inv_tau - st[kLt]);
+            v = gs * (exp(z * inv_tau - L) - p);
+        }
+        if (hard) v += gh * (exp(z - L1) - (j == target ? 1.0 : 0.0));
+        dst[j] = R::round((float)v);
+    }
+    __syncthreads();
+    if (hard && tid == 0 && !target_in_top && target >= 0 && target < V) {
+        const double z = R::one(row[target]);
+        dst[target] = R::round((float)((soft ? gs * f * exp(z * inv_tau - L) : 0.0) + gh * (exp(z - L1) - 1.0)));
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// Host side.
+// ------------------------------------------------------------------------------------------
+thread_local std::string g_err;
+
+int fail(const char* what) {
+    g_err = what;
+    return -1;
+}
+
+int launched(const char* what) {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) {
+        g_err = std::string(what) + " launch failed: " + hipGetErrorString(e);
+        return (int)e;
+    }
+    return 0;
+}
+
+int check(int64_t T, int64_t sb, int64_t st, int64_t R, int64_t V, int64_t k, double temperature, int dtype, const void* logits) {
+    g_err.clear();
+    if (R < 1 || R >= (1 << 22) || V < 1 || V > kMaxVocab || T < 1 || T > R) return fail("invalid sizes");
+    if (k < 1 || k > V || k > kMaxTop) return fail("k must be in [1, min(V, 512)]");
+    if (sb < 0 || st < 0 || sb >= ((int64_t)1 << 40) || st >= ((int64_t)1 << 40)) return fail("invalid strides");
+    if (!(temperature >= 1e-4 && temperature <= 1e4)) return fail("temperature must be in [1e-4, 1e4]");
+    if (dtype != kF16 && dtype != kBF16 && dtype != kF32) return fail("dtype must be float16, bfloat16 or float32");
+    if ((uintptr_t)logits % (dtype == kF32 ? 4 : 2)) return fail("logits must be aligned to their type");
+    return 0;
+}
+
+template <typename F>
+int by_dtype(int dtype, F f) {
+    return dtype == kBF16 ? f(std::integral_constant<int, kBF16>()) : dtype == kF16 ? f(std::integral_constant<int, kF16>())
+                                                                                    : f(std::integral_constant<int, kF32>());
+}
+
+size_t mark_bytes(int64_t V) { return (size_t)((V + 7 + 31) / 32) * 4; }
+
+}  // namespace
+
+NNDIS_API const char* nn_distill_last_error(void) { return g_err.c_str(); }
+
+NNDIS_API int nn_top_logits(const void* logits, int64_t T, int64_t sb, int64_t st, void* values, int64_t* indices, float* rest, int64_t R,
+                            int64_t V, int64_t k, double temperature, int dtype, void* stream) {
+    if (int e = check(T, sb, st, R, V, k, temperature, dtype, logits)) return e;
+    if (!logits || !values || !indices || !rest) return fail("null pointer argument");
+    return by_dtype(dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        auto go = [&](auto kern, int threads) {
+            kern<<<dim3((unsigned)R), dim3(threads), 0, (hipStream_t)stream>>>(logits, Layout{sb, st, (int)T}, values, (long long*)indices, rest, (int)V,
+                                                                               (int)k, (float)(1.4426950408889634 / temperature), 1.0 / temperature);
+            return launched("top_kernel");
+        };
+        return V <= 2048 ? go(top_kernel<DT, 64>, 64) : V <= 8192 ? go(top_kernel<DT, 256>, 256) : go(top_kernel<DT, 1024>, 1024);
+    });
+}
+
+NNDIS_API size_t nn_distill_stats_size(int64_t R) { return R < 1 ? 0 : (size_t)R * (kStats + 1) + 1; }
+
+namespace {
+int check_loss(int64_t T, int64_t sb, int64_t st, int64_t R, int64_t V, int64_t k, double temperature, double weight, int dtype, int value_dtype,
+               const void* logits) {
+    if (int e = check(T, sb, st, R, V, k, temperature, dtype, logits)) return e;
+    if (!(weight >= 0.0 && weight <= 1.0)) return fail("weight must be in [0, 1]");
+    if (value_dtype != kF16 && value_dtype != kBF16 && value_dtype != kF32) return fail("dtype must be float16, bfloat16 or float32");
+    return 0;
+}
+// Launches a loss kernel: 64 threads for a short row, 256 for a long one.
+template <template <int, int, bool> class Kernel, typename F>
+int by_row(int dtype, int64_t V, bool both, F go) {
+    return by_dtype(dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (V <= 2048) return both ? go(Kernel<DT, 64, true>::fn, 64) : go(Kernel<DT, 64, false>::fn, 64);
+        return both ? go(Kernel<DT, 256, true>::fn, 256) : go(Kernel<DT, 256, false>::fn, 256);
+    });
+}
+template <int DT, int TB, bool BOTH>
+struct Fwd {
+    static constexpr auto fn = loss_fwd_kernel<DT, TB, BOTH>;
+};
+template <int DT, int TB, bool BOTH>
+struct Bwd {
+    static constexpr auto fn = loss_bwd_kernel<DT, TB, BOTH>;
+};
+}  // namespace
+
+NNDIS_API int nn_distill_fwd(const void* logits, int64_t T, int64_t sb, int64_t st, const void* values, const int64_t* indices, const float* rest,
+                             const int64_t* targets, float* loss, double* stats, int64_t R, int64_t V, int64_t k, double temperature,
+                             double weight, int dtype, int value_dtype, void* stream) {
+    if (int e = check_loss(T, sb, st, R, V, k, temperature, weight, dtype, value_dtype, logits)) return e;
+    if (!logits || !values || !indices || !loss || !stats) return fail("null pointer argument");
+    const Loss x{logits, Layout{sb, st, (int)T}, values, (const long long*)indices, rest, (const long long*)targets, stats, (int)V, (int)k, value_dtype,
+                 (float)(1.4426950408889634 / temperature), temperature, weight};
+    const bool both = targets && weight < 1.0 && temperature != 1.0;
+    if (int e = by_row<Fwd>(dtype, V, both, [&](auto kern, int threads) {
+            kern<<<dim3((unsigned)R), dim3(threads), mark_bytes(V), (hipStream_t)stream>>>(x);
+            return launched("loss_fwd_kernel");
+        }))
+        return e;
+    loss_mean_kernel<<<dim3(1), dim3(1024), 0, (hipStream_t)stream>>>((const long long*)targets, stats, loss, (int)R);
+    return launched("loss_mean_kernel");
+}
+
+NNDIS_API int nn_distill_bwd(const float* grad, const void* logits, int64_t T, int64_t sb, int64_t st, const void* values,
+                             const int64_t* indices, const int64_t* targets, const double* stats, void* dlogits, int64_t R, int64_t V, int64_t k,
+                             double temperature, double weight, int dtype, int value_dtype, void* stream) {
+    if (int e = check_loss(T, sb, st, R, V, k, temperature, weight, dtype, value_dtype, logits)) return e;
+    if ((uintptr_t)dlogits % (dtype == kF32 ? 4 : 2)) return fail("dlogits must be aligned to their type");
+    if (!grad || !logits || !values || !indices || !stats || !dlogits) return fail("null pointer argument");
+    const Loss x{logits, Layout{sb, st, (int)T}, values, (const long long*)indices, nullptr, (const long long*)targets, const_cast<double*>(stats), (int)V,
+                 (int)k, value_dtype, (float)(1.4426950408889634 / temperature), temperature, weight};
+    const bool both = targets && weight < 1.0 && temperature != 1.0;
+    return by_row<Bwd>(dtype, V, both, [&](auto kern, int threads) {
+        kern<<<dim3((unsigned)R), dim3(threads), 0, (hipStream_t)stream>>>(x, grad, dlogits);
+        return launched("loss_bwd_kernel");
+    });
+}

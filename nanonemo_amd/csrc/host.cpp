@@ -28,6 +28,7 @@
 #include <tuple>
 #include <vector>
 
+#include "nanonemo_distill.h"
 #include "nanonemo_embedding.h"
 #include "nanonemo_fa.h"
 #include "nanonemo_linear.h"
@@ -59,6 +60,7 @@ void rms_done(int rc) { done(rc, nn_rmsnorm_last_error); }
 void lin_done(int rc) { done(rc, nn_linear_last_error); }
 void loss_done(int rc) { done(rc, nn_loss_last_error); }
 void emb_done(int rc) { done(rc, nn_embedding_last_error); }
+void dis_done(int rc) { done(rc, nn_distill_last_error); }
 
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
@@ -674,6 +676,116 @@ Tensor embedding_bwd_op(const Tensor& dy, const Tensor& idx, int64_t rows, doubl
     return embedding_bwd(dy, idx, rows, scale, padding);
 }
 
+// ---- distillation -------------------------------------------------------------------------------
+
+// The rows of (..., V) logits as the library reads them: row r at (r / T) * sb + (r % T) * st. Tensors whose leading
+// dimensions are not two strided runs at most, or whose values are not side by side, are copied.
+struct RowsOf {
+    Tensor t;
+    int64_t R, V, T, sb, st;
+    explicit RowsOf(const Tensor& given) : t(real_values(given)) {
+        V = t.size(-1);
+        R = V ? t.numel() / V : 0;
+        if (!R || !(V == 1 || t.stride(-1) == 1) || !runs()) {
+            t = t.contiguous();
+            T = std::max<int64_t>(R, 1), sb = 0, st = V;
+        }
+    }
+
+   private:
+    bool runs() {
+        std::vector<std::array<int64_t, 2>> got;  // {size, stride}, innermost first
+        for (int64_t d = t.dim() - 2; d >= 0; --d) {
+            if (t.size(d) == 1) continue;
+            if (!got.empty() && t.stride(d) == got.back()[0] * got.back()[1])
+                got.back()[0] *= t.size(d);
+            else
+                got.push_back({t.size(d), t.stride(d)});
+        }
+        if (got.size() > 2) return false;
+        T = got.empty() ? 1 : got[0][0], st = got.empty() ? V : got[0][1], sb = got.size() > 1 ? got[1][1] : 0;
+        return true;
+    }
+};
+
+void check_logits(const Tensor& logits) {
+    need(logits.is_cuda(), "inputs must be CUDA tensors");
+    need(logits.dim() >= 1 && code(logits) >= 0, "logits must be a float16, bfloat16 or float32 tensor (..., V)");
+}
+
+T3 top_logits(const Tensor& logits, int64_t k, double temperature) {
+    check_logits(logits);
+    const c10::DeviceGuard guard(logits.device());
+    const RowsOf z(logits);
+    std::vector<int64_t> shape = logits.sizes().vec();
+    Tensor rest = empty_f32(logits, at::IntArrayRef(shape).slice(0, shape.size() - 1));
+    need(k >= 1 && k <= z.V, "k must be in [1, min(V, 512)]");
+    shape.back() = k;
+    Tensor values = empty_of(logits, shape), indices = at::empty(shape, logits.options().dtype(at::kLong));
+    if (z.R == 0) return {values, indices, rest};
+    dis_done(nn_top_logits(z.t.data_ptr(), z.T, z.sb, z.st, values.data_ptr(), indices.data_ptr<int64_t>(), rest.data_ptr<float>(), z.R, z.V, k,
+                           temperature, code(logits), stream_of(logits)));
+    return {values, indices, rest};
+}
+
+// What the loss and its backward read beside the logits, as the library reads it.
+struct Teacher {
+    Tensor values, indices, rest, targets;
+    int64_t k;
+    Teacher(const Tensor& logits, const Tensor& v, const Tensor& i, const OptTensor& r, const OptTensor& y) {
+        check_logits(logits);
+        check_on_device(logits, {&v, &i, r ? &*r : &v, y ? &*y : &v});
+        const auto rows = logits.sizes().slice(0, logits.dim() - 1);
+        need(code(v) >= 0 && v.dim() == logits.dim() && v.sizes().slice(0, v.dim() - 1) == rows,
+             "values must be a float16, bfloat16 or float32 tensor (..., k) of the logits' rows");
+        need(i.scalar_type() == at::kLong && i.sizes() == v.sizes(), "indices must be int64 and of the values' shape");
+        if (r) need(r->scalar_type() == at::kFloat && r->sizes() == rows, "rest must be float32, one for each row");
+        if (y) need(y->scalar_type() == at::kLong && y->sizes() == rows, "targets must be int64, one for each row");
+        k = v.size(-1);
+        values = contig(v), indices = contig(i);
+        if (r) rest = contig(*r);
+        if (y) targets = contig(*y);
+    }
+    const int64_t* target_at() const { return targets.defined() ? targets.data_ptr<int64_t>() : nullptr; }
+    const float* rest_at() const { return rest.defined() ? rest.data_ptr<float>() : nullptr; }
+};
+
+// (the loss, what the backward needs).
+T2 distill_fwd(const Tensor& logits, const Tensor& values, const Tensor& indices, const OptTensor& rest, const OptTensor& targets,
+               double temperature, double weight) {
+    const Teacher t(logits, values, indices, rest, targets);
+    const c10::DeviceGuard guard(logits.device());
+    const RowsOf z(logits);
+    Tensor loss = empty_f32(logits, {}), stats = at::empty({(int64_t)nn_distill_stats_size(z.R)}, logits.options().dtype(at::kDouble));
+    if (z.R == 0) return {loss.fill_(NAN), stats};  // the mean of no row
+    dis_done(nn_distill_fwd(z.t.data_ptr(), z.T, z.sb, z.st, t.values.data_ptr(), t.indices.data_ptr<int64_t>(), t.rest_at(), t.target_at(),
+                            loss.data_ptr<float>(), stats.data_ptr<double>(), z.R, z.V, t.k, temperature, weight, code(logits), code(t.values),
+                            stream_of(logits)));
+    return {loss, stats};
+}
+
+Tensor distill_bwd(const Tensor& d_loss, const Tensor& logits, const Tensor& values, const Tensor& indices, const OptTensor& targets,
+                   const Tensor& stats_, double temperature, double weight) {
+    const Teacher t(logits, values, indices, std::nullopt, targets);
+    check_on_device(logits, {&d_loss, &stats_});
+    const c10::DeviceGuard guard(logits.device());
+    const RowsOf z(logits);
+    need(d_loss.numel() == 1 && d_loss.scalar_type() == at::kFloat, "d_loss must be one float32");
+    need(stats_.scalar_type() == at::kDouble && stats_.numel() == (int64_t)nn_distill_stats_size(z.R), "stats must be what the forward returned");
+    const Tensor stats = contig(stats_), g = contig(d_loss);
+    Tensor out = empty_of(logits, logits.sizes());
+    if (z.R == 0) return out;
+    dis_done(nn_distill_bwd(g.data_ptr<float>(), z.t.data_ptr(), z.T, z.sb, z.st, t.values.data_ptr(), t.indices.data_ptr<int64_t>(), t.target_at(),
+                            stats.data_ptr<double>(), out.data_ptr(), z.R, z.V, t.k, temperature, weight, code(logits), code(t.values),
+                            stream_of(logits)));
+    return out;
+}
+Tensor distill_bwd_op(const Tensor& d_loss, const Tensor& logits, const Tensor& values, const Tensor& indices, const OptTensor& targets,
+                      const Tensor& stats, double temperature, double weight) {
+    refuse_capture_from_engine("distill_loss backward op");
+    return distill_bwd(d_loss, logits, values, indices, targets, stats, temperature, weight);
+}
+
 // ---- routing ------------------------------------------------------------------------------------
 
 // Whether the tensor's values lie at its address, as dense values of its own type: not inside a transform's wrapper
@@ -733,6 +845,9 @@ TORCH_LIBRARY_IMPL(nanonemo, CUDA, m) {
     m.impl("cuda_add_rms_norm_bwd", norm_bwd);
     m.impl("embedding", embedding_op);
     m.impl("embedding_bwd", embedding_bwd_op);
+    m.impl("top_logits", top_logits);
+    m.impl("distill_loss", distill_fwd);
+    m.impl("distill_loss_bwd", distill_bwd_op);
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -751,6 +866,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("norm_bwd", norm_bwd, nogil);
     m.def("embedding_fwd", embedding_fwd, nogil);
     m.def("embedding_bwd", embedding_bwd, nogil);
+    m.def("top_logits", top_logits, nogil);
+    m.def("distill_fwd", distill_fwd, nogil);
+    m.def("distill_bwd", distill_bwd, nogil);
     m.def("wgrad", wgrad, nogil);
     m.def("wgrad_takes", wgrad_takes);
     m.def("rows_aligned", rows_aligned);

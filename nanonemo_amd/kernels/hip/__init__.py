@@ -29,6 +29,7 @@ _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _sz = ctypes.c_size_t
 _i64p = ctypes.POINTER(ctypes.c_int64)
 
@@ -118,6 +119,16 @@ SIGNATURES: dict[str, tuple] = {
     "nn_embedding_bwd_workspace_size": (_sz, [_i64, _i64, _i64]),
     "nn_embedding_bwd": (_int, [_vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _f32, _i64, _int, _int, _vp]),
     "nn_embedding_last_error": (ctypes.c_char_p, []),
+    # include/nanonemo_distill.h
+    "nn_top_logits": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _f64, _int, _vp]),
+    "nn_distill_stats_size": (_sz, [_i64]),
+    "nn_distill_fwd": (
+        _int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f64, _f64, _int, _int, _vp]
+    ),
+    "nn_distill_bwd": (
+        _int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f64, _f64, _int, _int, _vp]
+    ),
+    "nn_distill_last_error": (ctypes.c_char_p, []),
 }
 
 ABI_VERSION = 11
@@ -237,6 +248,13 @@ def check_embedding(rc: int) -> None:
     if rc != 0:
         msg = lib().nn_embedding_last_error().decode(errors="replace")
         raise RuntimeError(msg or f"nanonemo_embedding call failed with code {rc}")
+
+
+def check_distill(rc: int) -> None:
+    """Raise RuntimeError with the library's message when an nn_top_logits or nn_distill_* entry point returns non-zero."""
+    if rc != 0:
+        msg = lib().nn_distill_last_error().decode(errors="replace")
+        raise RuntimeError(msg or f"nanonemo_distill call failed with code {rc}")
 
 
 def check_rmsnorm(rc: int) -> None:

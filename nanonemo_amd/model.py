@@ -22,13 +22,15 @@ embedding and its gradient (nanonemo::embedding).
 A model with any of them set also runs its linear layers, SwiGLU and cross entropy on this build's kernels where it is
 called eagerly on a GPU under 16-bit autocast (kernels/hip/linear.py, layers.py and head.py say exactly when; there the
 "hip_bthd" attention with either RoPE kernel is one autograd node, with q rotated by the RoPE kernel, whose result is
-bit-identical). Everything else, and every module whose layers carry hooks or are not plain nn.Linear, is PyTorch.
+bit-identical). So do its distillation from a teacher's top logits and that teacher's selection of them
+(kernels/hip/distill.py). Everything else, and every module whose layers carry hooks or are not plain nn.Linear, is PyTorch.
 """
 
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
@@ -284,6 +286,33 @@ class Block(nn.Module):
         return x, self.mlp(h)
 
 
+class Teacher(NamedTuple):
+    """What a student learns from (NanoNemo.teach): a teacher's top logits for the student's (B, T) tokens."""
+
+    values: torch.Tensor  # (B, T, k)
+    indices: torch.Tensor  # (B, T, k) int64
+    rest: torch.Tensor | None = None  # (B, T) fp32: logsumexp of the teacher's other logits / temperature
+    temperature: float = 1.0
+    weight: float = 0.5  # of the distillation; the rest of the loss is the targets' cross entropy
+
+
+def distill_loss(logits: torch.Tensor, teacher: Teacher, targets: torch.Tensor | None) -> torch.Tensor:
+    """The distillation loss as PyTorch operations (kernels/hip/distill.py states it), in fp32."""
+    values, indices, rest, tau, w = teacher
+    rows = torch.ones(indices.shape[:-1], dtype=torch.bool, device=logits.device) if targets is None else targets != -100
+    logits, indices = logits.float()[rows], indices[rows]
+    t = values.float()[rows] / tau
+    log_q = F.log_softmax(logits / tau, dim=-1)
+    on = log_q.gather(-1, indices)
+    if rest is not None:
+        t = torch.cat((t, rest[rows].unsqueeze(-1)), dim=-1)
+        others = torch.ones_like(log_q, dtype=torch.bool).scatter_(-1, indices, False)
+        on = torch.cat((on, log_q.masked_fill(~others, -math.inf).logsumexp(-1, keepdim=True)), dim=-1)
+    log_p = F.log_softmax(t, dim=-1)
+    loss = w * tau * tau * torch.where(log_p > -math.inf, log_p.exp() * (log_p - on), 0.0).sum(-1).mean()
+    return loss if targets is None or w == 1 else loss + (1 - w) * F.cross_entropy(logits, targets[rows])
+
+
 class NanoNemo(nn.Module):
     """Decoder-only LM (model.py:13-70): embedding, n_layers blocks, final norm, tied lm_head."""
 
@@ -307,14 +336,21 @@ class NanoNemo(nn.Module):
             nn.init.normal_(blk.attn.wo.weight, std=resid_std)
             nn.init.normal_(blk.mlp.w_down.weight, std=resid_std)
 
-    def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None):
+    def hidden(self, idx: torch.Tensor) -> torch.Tensor:
+        """The output layer's input for tokens (B, T)."""
         T = idx.shape[1]
         if T > self.cfg.max_seq_len:
             raise ValueError(f"sequence length {T} > max_seq_len {self.cfg.max_seq_len}")
         x, delta = self.tok_emb(idx), None
         for blk in self.blocks:
             x, delta = blk(x, self.rope_cos, self.rope_sin, delta)
-        h = self.norm_out(x, delta)[0]
+        return self.norm_out(x, delta)[0]
+
+    def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None, teacher: Teacher | None = None):
+        """(logits, loss): the targets' cross entropy, with a teacher the distillation loss, None without either."""
+        h = self.hidden(idx)
+        if teacher is not None:
+            return self._distill(h, teacher, targets)
         if targets is not None and self.cfg.any_hip and h.is_cuda:
             from nanonemo_amd.kernels.hip import head
 
@@ -325,6 +361,27 @@ class NanoNemo(nn.Module):
         if targets is not None:
             loss = F.cross_entropy(logits.float().view(-1, logits.size(-1)), targets.reshape(-1))
         return logits, loss
+
+    def _distill(self, h: torch.Tensor, teacher: Teacher, targets: torch.Tensor | None):
+        if not self.cfg.any_hip or not h.is_cuda:
+            logits = self.lm_head(h)
+            return logits, distill_loss(logits, teacher, targets)
+        from nanonemo_amd.kernels.hip import distill
+
+        logits = _project(self.cfg, h, self.lm_head)[0]
+        return logits, distill.distill_loss(logits, teacher.values, teacher.indices, teacher.rest, targets, teacher.temperature, teacher.weight)
+
+    @torch.no_grad()
+    def teach(self, idx: torch.Tensor, k: int, temperature: float = 1.0, weight: float = 0.5) -> Teacher:
+        """This model's k largest logits for tokens (B, T), for a student with the same vocabulary."""
+        logits = self.lm_head(self.hidden(idx))
+        if self.cfg.any_hip and logits.is_cuda:
+            from nanonemo_amd.kernels.hip import distill
+
+            return Teacher(*distill.top_logits(logits, k, temperature), temperature, weight)
+        values, indices = logits.topk(k, dim=-1)
+        rest = (logits.float() / temperature).scatter(-1, indices, -math.inf).logsumexp(-1)
+        return Teacher(values, indices, rest, temperature, weight)
 
     def num_params(self, non_embedding: bool = False) -> int:
         n = sum(p.numel() for p in self.parameters())  # the tied weight counts once

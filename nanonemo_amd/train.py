@@ -34,13 +34,13 @@ CURVE_BOUND = 0.12
 
 
 def train_step(model, opt, batches, grad_clip: float = 1.0, amp_dtype=torch.bfloat16):
-    """One optimizer step over the micro-batches ``batches`` [(x, y), ...]; returns (loss, grad_norm)
-    as device tensors (no host synchronisation)."""
+    """One optimizer step over the micro-batches ``batches`` [(x, y), ...] or, for a student, [(x, y, teacher), ...]
+    (``teacher_batches``); returns (loss, grad_norm) as device tensors (no host synchronisation)."""
     accum = len(batches)
     loss_sum = None
-    for x, y in batches:
+    for x, y, *teacher in batches:
         with torch.autocast(x.device.type, dtype=amp_dtype, enabled=amp_dtype is not None):
-            _, loss = model(x, y)
+            _, loss = model(x, y, *teacher)
         loss = loss / accum
         loss.backward()
         loss = loss.detach()
@@ -49,6 +49,16 @@ def train_step(model, opt, batches, grad_clip: float = 1.0, amp_dtype=torch.bflo
     opt.step()
     opt.zero_grad(set_to_none=True)
     return loss_sum, grad_norm
+
+
+def teacher_batches(teacher, batches, k: int, temperature: float = 2.0, weight: float = 0.5, amp_dtype=torch.bfloat16):
+    """The micro-batches [(x, y), ...] with what ``teacher`` (a NanoNemo with the student's vocabulary) says of them:
+    [(x, y, its top k logits), ...] for ``train_step``."""
+    out = []
+    for x, y in batches:
+        with torch.autocast(x.device.type, dtype=amp_dtype, enabled=amp_dtype is not None):
+            out.append((x, y, teacher.teach(x, k, temperature, weight)))
+    return out
 
 
 def synthetic_batches(steps: int, batch: int, seq: int, vocab: int, device, seed: int = 0):
