@@ -75,6 +75,32 @@ __device__ inline u32x4 group(const typename Row<DT>::T* row, int i, int V) {
     return u.v;
 }
 
+// Group i of a row of at least W values, from min(i W, V - W) on: the last one of a row that is not whole groups overlaps the
+// one before. Then own() makes what the group before holds (all of a group past the row's end) -inf: apart, so that many loads
+// can be under way.
+template <int DT>
+__device__ inline u32x4 group_at(const typename Row<DT>::T* row, int i, int V) {
+    constexpr int W = Row<DT>::W;
+    const uint32_t bytes = (uint32_t)min(i * W, V - W) * (uint32_t)sizeof(typename Row<DT>::T);  // (32 bits: the row's address stays scalar)
+    return load_any<DT>(reinterpret_cast<const typename Row<DT>::T*>(reinterpret_cast<const char*>(row) + bytes));
+}
+template <int DT>
+__device__ inline void own(u32x4& v, int i, int V) {
+    constexpr int W = Row<DT>::W;
+    const int twice = i * W - (V - W);
+    if (twice <= 0) return;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if constexpr (DT == kF32) {
+            if (w < twice) v[w] = 0xff800000u;
+        } else {
+            constexpr uint32_t ninf = DT == kBF16 ? 0xff80u : 0xfc00u;
+            if (2 * w < twice) v[w] = (v[w] & 0xffff0000u) | ninf;
+            if (2 * w + 1 < twice) v[w] = (v[w] & 0xffffu) | (ninf << 16);
+        }
+    }
+}
+
 // Sums, maxima and the like over a block of TB threads: every thread gets the result. `tmp` is one value per wave, free for
 // the next call as soon as this one has returned everywhere.
 template <int TB, typename T, typename F>
@@ -173,83 +199,306 @@ struct Key {
             return (T)u;
     }
 };
-__device__ inline uint64_t ranked(uint32_t key, int j) { return ((uint64_t)key << 32) | (0xffffffffu - (uint32_t)j); }
+// A key and the place of its value as one number: the larger key first, of equal ones the lower place. A double holds the 51
+// bits exactly, and two of them are compared in one instruction of full rate (two 64-bit integers take four times as long).
+__device__ inline double ranked(uint32_t key, int j) { return fma((double)key, (double)(1 << kVocabBits), (double)((1 << kVocabBits) - 1 - j)); }
+__device__ inline uint32_t key_in(double r) { return (uint32_t)(r * (1.0 / (1 << kVocabBits))); }
+__device__ inline int place_in(double r) { return (1 << kVocabBits) - 1 - (int)(r - (double)key_in(r) * (double)(1 << kVocabBits)); }
 
+// Largest values as whole numbers, for a group of 16 bytes at a time: like Key, but -0 below 0 and NaN by its sign. `mag` is the
+// largest value without its sign, which shows a NaN.
+template <int DT>
+struct Order {
+    using K = Key<DT>;
+    static __device__ uint32_t of(uint32_t u) { return u & K::kSign ? u ^ K::kAll : u | K::kSign; }
+    static __device__ typename K::T value(uint32_t order) { return K::value(order); }  // (the same for both orders)
+    static constexpr uint32_t kZero = K::kSign, kMinusZero = kZero - 1, kMinusInf = K::kAll ^ (K::kSign | K::kInf);
+    static __device__ uint32_t most(u32x4 raw, uint32_t& mag) {
+        if constexpr (DT == kF32) {
+            int m = INT32_MIN;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int x = (int)raw[w];
+                m = max(m, x ^ ((x >> 31) & 0x7fffffff));
+                mag = max(mag, raw[w] & 0x7fffffffu);
+            }
+            return (uint32_t)m ^ K::kSign;
+        } else {
+            typedef short s16x2 __attribute__((ext_vector_type(2)));
+            typedef u16 u16x2 __attribute__((ext_vector_type(2)));
+            s16x2 m = {INT16_MIN, INT16_MIN};
+            u16x2 g = __builtin_bit_cast(u16x2, mag);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const s16x2 x = __builtin_bit_cast(s16x2, (uint32_t)raw[w]);
+                m = __builtin_elementwise_max(m, x ^ ((x >> 15) & (short)0x7fff));
+                g = __builtin_elementwise_max(g, __builtin_bit_cast(u16x2, (uint32_t)raw[w] & 0x7fff7fffu));
+            }
+            mag = __builtin_bit_cast(uint32_t, g);
+            return (uint32_t)(max((int)m[0], (int)m[1]) + 0x8000);
+        }
+    }
+    static __device__ bool nan(uint32_t mag) {
+        if constexpr (DT == kF32)
+            return mag > K::kInf;
+        else
+            return (mag & 0xffffu) > K::kInf || (mag >> 16) > K::kInf;
+    }
+};
+
+// A bound that at least k of a wave's 64 P values reach, and at most k / 16 + 2 more where equal values allow it, found bit by
+// bit.
+template <int BITS, int P>
+__device__ inline uint32_t reached(const uint32_t (&v)[P], int k) {
+    uint32_t found = 0;
+    for (int b = BITS - 1; b >= 0; --b) {
+        const uint32_t t = found | (1u << b);
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < P; ++i) reach += __popcll(__ballot(v[i] >= t));
+        if (reach < k) continue;
+        found = t;
+        if (reach <= k + k / 16 + 2) break;
+    }
+    return found;
+}
+
+// What a row's selection keeps in LDS.
 template <int TB>
-constexpr int kCandidates = TB >= 1024 ? 2048 : TB >= 256 ? 1024 : 512;  // (at least kMaxTop)
+struct TopShared {
+    static constexpr int kWaves = TB / 64;
+    static constexpr int kCandidates = TB == 64 ? 640 : 1024;  // (at least kMaxTop)
+    static constexpr int kList = TB == 64 ? 1 : TB == 256 ? 64 : 1024 / kWaves;  // groups of a wave's list
+    double cand[kCandidates];  // (ranked)
+    u32x4 list[kWaves][kList];
+    int list_at[kWaves][kList];
+    float below[TB == 64 ? 1 : kCandidates];  // exponentials of the candidates that are not among the k
+    uint32_t bins[TB == 64 ? 1 : 1024];
+    int tmp[kWaves];
+    float tmpf[kWaves];
+    MaxSum sums[kWaves];
+    int count, special, full;
+    uint32_t bound;
+    double last;
+};
 
-template <int DT, int TB>
-__global__ __launch_bounds__(TB) void top_kernel(const void* __restrict__ logits, Layout at, void* __restrict__ values,
-                                                 long long* __restrict__ indices, float* __restrict__ rest, int V, int k, float c,
-                                                 double inv_tau) {
+// One block of TB threads per row. A thread holds NV groups of the row in registers from its one load to the end (the row is
+// read once); NV = 0 is for rows too long for that, which are read twice.
+//
+//   1  The k-th largest of some hundred parts' largest values is a bound that at least k values reach, and few more do.
+//   2  Values that reach it are the candidates (their groups go to a list of the wave's, so that the code for single values is
+//      there once); the exponentials of all others are summed.
+//   3  A candidate's rank is the number of larger ones; those behind the k join the sum.
+//
+// Measured at 8192 x 50304 bf16, k = 64: 200 us (4.1 TB/s), three rows to a CU at 80 registers, where a row's search and
+// ranking hide behind the others' loads; with the row read again for every step it took 700 us, with 1024 threads of 64
+// registers (7 groups each, 27 of them spilled) 390. A single row takes 11 us, most of it the steps' latency.
+// Rows for which the above does not do (many equal values, NaN, a k near the number of parts) take a search of the k-th value bit
+// by bit instead, and rows whose others lie far below the bound a sum relative to their own largest.
+template <int DT, int TB, int NV>
+__global__ __launch_bounds__(TB, TB == 512 ? 6 : 4) void top_kernel(const void* __restrict__ logits, Layout at, void* __restrict__ values,
+                                                    long long* __restrict__ indices, float* __restrict__ rest, int V, int k, float c,
+                                                    double inv_tau) {
     using R = Row<DT>;
     using T = typename R::T;
     using K = Key<DT>;
+    using O = Order<DT>;
+    using S = TopShared<TB>;
+    constexpr int N = NV ? NV : 1;
     const T* row = reinterpret_cast<const T*>(logits) + at.at(blockIdx.x);
-    const int tid = threadIdx.x, groups = (V + R::W - 1) / R::W;
-    __shared__ uint64_t cand[kCandidates<TB>];
-    __shared__ uint32_t maxima[TB];
-    __shared__ int tmp[TB / 64];
-    __shared__ int count;
-    __shared__ uint32_t bound;
-    __shared__ uint64_t last;
-    auto each = [&](auto f) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = (V + R::W - 1) / R::W;
+    __shared__ S sh;
+    union Group {
+        u32x4 v;
+        T e[R::W];
+    };
+    u32x4 raw[N];
+    uint32_t most[N];  // the order of each group's largest value
+    auto bits_of = [](T x) {
+        if constexpr (DT == kF32)
+            return __float_as_uint(x);
+        else
+            return (uint32_t)x;
+    };
+    auto begin_of = [&](int i) { return V < R::W ? 0 : min(i * R::W, V - R::W); };
+    auto one_group = [&](int i) {
+        u32x4 v = group_at<DT>(row, i, V);
+        own<DT>(v, i, V);
+        return v;
+    };
+    auto each = [&](auto f) {  // (the row again, for the steps that few rows take)
         for (int i = tid; i < groups; i += TB) {
-            union {
-                u32x4 v;
-                T e[R::W];
-            } u;
+            Group u;
             u.v = group<DT>(row, i, V);
 #pragma unroll
             for (int e = 0; e < R::W; ++e)
                 if (i * R::W + e < V) f(u.e[e], i * R::W + e);
         }
     };
-    auto add = [](int a, int b) { return a + b; };
-    auto counted = [&](auto f) {
-        int n = 0;
-        each([&](T x, int j) { n += f(K::of(x), j) ? 1 : 0; });
-        return block_all<TB>(n, tmp, add);
+    auto add = [](auto a, auto b) { return a + b; };
+    auto sync = [] {
+        if constexpr (TB > 64) __syncthreads();
     };
-    auto collect = [&](auto f) {
-        if (tid == 0) count = 0;
-        __syncthreads();
-        each([&](T x, int j) {
-            const uint32_t key = K::of(x);
-            if (!f(key, j)) return;
-            const int p = atomicAdd(&count, 1);
-            if (p < kCandidates<TB>) cand[p] = ranked(key, j);
-        });
-        __syncthreads();
-        return count;
-    };
+    if (tid == 0) sh.count = 0, sh.special = 0, sh.full = 0;
+    sync();
 
-    // The k-th largest of the threads' largest is a bound that at least k values reach, and few more do where k is a small
-    // share of the threads.
-    int n = kCandidates<TB> + 1;
-    if (2 * k <= min(TB, groups)) {
-        uint32_t most = 0;
-        each([&](T x, int) { most = max(most, K::of(x)); });
-        maxima[tid] = most;
-        __syncthreads();
-        if (tid < 64) {
-            uint32_t found = 0;
-            for (int b = K::kBits - 1; b >= 0; --b) {
-                const uint32_t t = found | (1u << b);
-                int reach = 0;
+    // 1. The parts: four threads' values, a thread's, a group's, or (one wave) every value. Of 256 parts, 64 leave 74
+    // candidates; of 1024, 512 leave 710.
+    uint32_t mag = 0, mine = 0, least = 0;
+    if constexpr (NV > 0) {
 #pragma unroll
-                for (int i = 0; i < TB / 64; ++i) reach += __popcll(__ballot(maxima[tid + 64 * i] >= t));
-                if (reach >= k) found = t;
-            }
-            if (tid == 0) bound = found;
+        for (int n = 0; n < NV; ++n) raw[n] = TB == 64 && V < R::W ? group<DT>(row, 0, tid + n ? 0 : V) : group_at<DT>(row, tid + n * TB, V);
+        if (TB > 64 || V >= R::W) {
+#pragma unroll
+            for (int n = 0; n < NV; ++n) own<DT>(raw[n], tid + n * TB, V);
         }
-        __syncthreads();
-        const uint32_t least = bound;
-        n = collect([&](uint32_t key, int) { return key >= least; });
+#pragma unroll
+        for (int n = 0; n < NV; ++n) mine = max(mine, most[n] = O::most(raw[n], mag));
+    } else {
+        for (int i = tid; i < groups; i += TB) mine = max(mine, O::most(one_group(i), mag));
     }
-    if (n > kCandidates<TB>) {
-        // Otherwise (many equal values, or k near the number of threads) the k-th largest key, bit by bit, and the place of
-        // the last of its equals that belongs to the k.
+    if constexpr (TB == 64) {
+        if (k <= groups) {
+            least = reached<K::kBits>(most, k);
+        } else {
+            uint32_t v[N * R::W];
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                Group u;
+                u.v = raw[n];
+#pragma unroll
+                for (int e = 0; e < R::W; ++e) v[n * R::W + e] = O::of(bits_of(u.e[e]));
+            }
+            least = reached<K::kBits>(v, k);
+        }
+        if (__ballot(O::nan(mag))) least = 0;
+        if (least == O::kZero) least = O::kMinusZero;  // (they are equal)
+    } else {
+        if (O::nan(mag)) sh.special = 1;
+        int parts = 0;
+        if (4 * k <= TB / 4) {
+            mine = max(mine, (uint32_t)__shfl_xor((int)mine, 1));
+            mine = max(mine, (uint32_t)__shfl_xor((int)mine, 2));
+            parts = TB / 4;
+            if (tid % 4 == 0) sh.bins[tid / 4] = mine;
+        } else if (NV > 0 ? 4 * k <= TB : 2 * k <= TB) {
+            parts = TB;
+            sh.bins[tid] = mine;
+        } else if (NV > 0 && k <= groups) {
+            parts = min(NV * TB, 1024);
+            // (of more groups than parts, several make one)
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                if (n * TB + tid < 1024) {
+                    uint32_t m = most[n];
+#pragma unroll
+                    for (int o = n + 1024 / TB; o < N; o += 1024 / TB) m = max(m, most[o]);
+                    sh.bins[n * TB + tid] = m;
+                }
+        }
+        sync();
+        if (tid < 64) {
+            auto search = [&](auto p) {
+                constexpr int P = decltype(p)::value;
+                uint32_t v[P];
+#pragma unroll
+                for (int i = 0; i < P; ++i) v[i] = sh.bins[64 * i + tid];
+                return reached<K::kBits>(v, k);
+            };
+            switch (parts / 64) {
+                case 0: break;
+                case 1: least = search(std::integral_constant<int, 1>()); break;
+                case 2: least = search(std::integral_constant<int, 2>()); break;
+                case 4: least = search(std::integral_constant<int, 4>()); break;
+                case 8: least = search(std::integral_constant<int, 8>()); break;
+                default: least = search(std::integral_constant<int, 16>());  // 1024
+            }
+            if (tid == 0) sh.bound = sh.special ? 0 : least == O::kZero ? O::kMinusZero : least;
+        }
+        sync();
+        least = sh.bound;
+    }
+
+    // 2. Exponents are in powers of two relative to 2^b, the whole number b next to the bound's own exponent (so that x c - b is
+    // rounded once).
+    const float v_b = R::one(O::value(least)), b = rintf(v_b * c);
+    float s = 0.f;
+    auto e_of = [&](T x) { return __builtin_amdgcn_exp2f(fmaf(R::one(x), c, -b)); };
+    bool quick = least > O::kMinusInf;  // (what lies past the row's end is -inf)
+    int n = 0;
+    if (quick) {
+        if constexpr (TB == 64) {
+#pragma unroll
+            for (int m = 0; m < N; ++m) {
+                Group u;
+                u.v = raw[m];
+#pragma unroll
+                for (int e = 0; e < R::W; ++e) {
+                    const bool hit = O::of(bits_of(u.e[e])) >= least;
+                    const uint64_t hits = __ballot(hit);
+                    s += hit ? 0.f : e_of(u.e[e]);
+                    if (hits) {
+                        const int to = n + __popcll(hits & ((1ull << lane) - 1));
+                        if (hit && to < S::kCandidates) sh.cand[to] = ranked(K::of(u.e[e]), begin_of(tid + m * TB) + e);
+                        n += __popcll(hits);
+                    }
+                }
+            }
+        } else {
+            int on_list = 0;
+            auto sweep = [&](u32x4 v, uint32_t m, int i) {
+                const uint64_t hits = __ballot(m >= least);
+                if (m >= least) {
+                    const int to = on_list + __popcll(hits & ((1ull << lane) - 1));
+                    if (to < S::kList) {
+                        sh.list[wave][to] = v;
+                        sh.list_at[wave][to] = i;
+                    }
+                } else {
+                    float f[R::W];
+                    R::widen(v, f);
+#pragma unroll
+                    for (int e = 0; e < R::W; ++e) s += __builtin_amdgcn_exp2f(fmaf(f[e], c, -b));
+                }
+                on_list += __popcll(hits);
+            };
+            if constexpr (NV > 0) {
+#pragma unroll
+                for (int m = 0; m < NV; ++m) sweep(raw[m], most[m], tid + m * TB);
+            } else {
+                for (int i = tid; i < groups; i += TB) {
+                    uint32_t none = 0;
+                    const u32x4 v = one_group(i);
+                    sweep(v, O::most(v, none), i);
+                }
+            }
+            on_list = __builtin_amdgcn_readfirstlane(on_list);  // (the first lane has seen every group of the wave)
+            if (on_list > S::kList) {
+                if (lane == 0) sh.full = 1;
+                on_list = S::kList;
+            }
+            for (int t = lane; t < on_list * R::W; t += 64) {  // the wave's own list: no other's is read
+                const int g = t / R::W;
+                const T x = reinterpret_cast<const T*>(sh.list[wave])[t];
+                if (O::of(bits_of(x)) >= least) {
+                    const int p = atomicAdd(&sh.count, 1);
+                    if (p < S::kCandidates) sh.cand[p] = ranked(K::of(x), begin_of(sh.list_at[wave][g]) + t % R::W);
+                } else {
+                    s += e_of(x);
+                }
+            }
+            sync();
+            n = sh.full ? S::kCandidates + 1 : sh.count;
+        }
+        quick = n <= S::kCandidates;
+    }
+    if (!quick) {
+        // The k-th largest key, and the place of the last of its equals that belongs to the k.
+        auto counted = [&](auto f) {
+            int n = 0;
+            each([&](T x, int j) { n += f(K::of(x), j) ? 1 : 0; });
+            return block_all<TB>(n, sh.tmp, add);
+        };
         uint32_t key_k = 0;
         for (int b = K::kBits - 1; b >= 0; --b) {
             const uint32_t t = key_k | (1u << b);
@@ -261,30 +510,79 @@ __global__ __launch_bounds__(TB) void top_kernel(const void* __restrict__ logits
             const int t = place | (1 << b);
             if (counted([&](uint32_t key, int j) { return key == key_k && j < t; }) < need) place = t;
         }
-        n = collect([&](uint32_t key, int j) { return key > key_k || (key == key_k && j <= place); });
+        sync();
+        if (tid == 0) sh.count = 0;
+        sync();
+        each([&](T x, int j) {
+            const uint32_t key = K::of(x);
+            if (key > key_k || (key == key_k && j <= place)) sh.cand[atomicAdd(&sh.count, 1)] = ranked(key, j);
+        });
+        sync();
+        n = k;
     }
-    // Every candidate's rank is the number of larger ones.
-    for (int i = tid; i < n; i += TB) {
-        const uint64_t mine = cand[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += cand[j] > mine ? 1 : 0;
-        if (rank < k) {
+    // 3. Every wave holds all candidates, and ranks every kWaves-th one: a comparison with all of them is one instruction a 64, and
+    // a count of its result bits.
+    auto rank_all = [&](auto parts) {
+        constexpr int P = decltype(parts)::value;
+        double x[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) x[i] = 64 * i + lane < n ? sh.cand[64 * i + lane] : -1.0;
+        for (int from = wave; from < n; from += 64 * S::kWaves) {  // 64 of the wave's, one for each lane in the end
+            const int own = min(64, (n - from + S::kWaves - 1) / S::kWaves);
+            const double my = lane < own ? sh.cand[from + lane * S::kWaves] : 0.0;
+            const int lo = (int)__builtin_bit_cast(uint64_t, my), hi = (int)(__builtin_bit_cast(uint64_t, my) >> 32);
+            int rank = 0;
+            for (int t = 0; t < own; ++t) {
+                const double y = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane(lo, t) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, t) << 32);
+                int larger = 0;
+#pragma unroll
+                for (int i = 0; i < P; ++i) larger += __popcll(__ballot(x[i] > y));
+                rank = lane == t ? larger : rank;
+            }
+            if (lane >= own) continue;
+            const T v = K::value(key_in(my));
+            if (rank >= k) {  // (one wave's candidates have one order; of several waves, they are summed by rank)
+                if constexpr (TB == 64)
+                    s += e_of(v);
+                else
+                    sh.below[rank - k] = e_of(v);
+                continue;
+            }
             const size_t to = (size_t)blockIdx.x * k + rank;
-            reinterpret_cast<T*>(values)[to] = K::value((uint32_t)(mine >> 32));
-            indices[to] = (long long)(0xffffffffu - (uint32_t)mine);
+            reinterpret_cast<T*>(values)[to] = v;
+            indices[to] = place_in(my);
+            if (rank == k - 1) sh.last = my;
         }
-        if (rank == k - 1) last = mine;
+    };
+    switch ((n + 63) / 64) {
+        case 1: rank_all(std::integral_constant<int, 1>()); break;
+        case 2: rank_all(std::integral_constant<int, 2>()); break;
+        case 3: rank_all(std::integral_constant<int, 3>()); break;
+        case 4: rank_all(std::integral_constant<int, 4>()); break;
+        case 5: case 6: rank_all(std::integral_constant<int, 6>()); break;
+        case 7: case 8: rank_all(std::integral_constant<int, 8>()); break;
+        default: rank_all(std::integral_constant<int, S::kCandidates / 64>());
     }
     __syncthreads();
-    const uint64_t end = last;
+    if (quick) {
+        if constexpr (TB > 64)
+            for (int i = tid; i < n - k; i += TB) s += sh.below[i];
+        s = block_all<TB>(s, sh.tmpf, add);
+        if (s > 1e-30f && s < 1e30f) {
+            // (c is log2(e) / tau rounded: what that puts on the exponents near the bound comes off again)
+            const double ln2 = 0.6931471805599453, off = v_b * (inv_tau / ln2 - (double)c);
+            if (tid == 0) rest[blockIdx.x] = (float)(ln2 * ((double)b + off + log2((double)s)));
+            return;
+        }
+    }
+    const double end = sh.last;
     MaxSum a{-INFINITY, 0.f, 0.f};
     each([&](T x, int j) {
         if (ranked(K::of(x), j) >= end) return;
         const float v = R::one(x);
         take<false, 1>(a, &v, c);
     });
-    __shared__ MaxSum sums[TB / 64];
-    a = block_merge<TB, false>(a, sums, c);
+    a = block_merge<TB, false>(a, sh.sums, c);
     if (tid == 0) rest[blockIdx.x] = (float)(base_of(a.m) * inv_tau + log((double)a.s));
 }
 
@@ -596,7 +894,13 @@ NNDIS_API int nn_top_logits(const void* logits, int64_t T, int64_t sb, int64_t s
                                                                                (int)k, (float)(1.4426950408889634 / temperature), 1.0 / temperature);
             return launched("top_kernel");
         };
-        return V <= 2048 ? go(top_kernel<DT, 64>, 64) : V <= 8192 ? go(top_kernel<DT, 256>, 256) : go(top_kernel<DT, 1024>, 1024);
+        const int64_t groups = (V + Row<DT>::W - 1) / Row<DT>::W;  // of 16 bytes, held by the block's threads
+        return groups <= 4 * 64      ? go(top_kernel<DT, 64, 4>, 64)
+               : groups <= 4 * 256   ? go(top_kernel<DT, 256, 4>, 256)
+               : groups <= 8 * 512   ? go(top_kernel<DT, 512, 8>, 512)
+               : groups <= 13 * 512  ? go(top_kernel<DT, 512, 13>, 512)
+               : groups <= 16 * 1024 ? go(top_kernel<DT, 1024, 16>, 1024)
+                                     : go(top_kernel<DT, 1024, 0>, 1024);
     });
 }
 
