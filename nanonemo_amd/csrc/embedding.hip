@@ -32,8 +32,8 @@ constexpr int kThreads = 256;
 // ------------------------------------------------------------------------------------------
 constexpr int kFwdUnits = 4;
 
-// UNIT: values of a unit, Row<DT>::W or 1.
-template <int DT, int UNIT, typename I>
+// UNIT: values of a unit, Row<DT>::W or 1. PAST: stored past the caches.
+template <int DT, int UNIT, bool PAST, typename I>
 __global__ __launch_bounds__(kThreads) void fwd_kernel(const void* __restrict__ weight, const I* __restrict__ idx,
                                                        void* __restrict__ out, long long units, int per_row, int V, float scale) {
     using R = Row<DT>;
@@ -73,7 +73,10 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(const void* __restrict__ 
             R::widen(raw[k], v);
 #pragma unroll
             for (int e = 0; e < R::W; ++e) v[e] = bad[k] ? NAN : v[e] * scale;
-            R::store(o + dst[k] * UNIT, v);
+            if constexpr (PAST)
+                __builtin_nontemporal_store(R::narrow(v), reinterpret_cast<u32x4*>(o + dst[k] * UNIT));
+            else
+                R::store(o + dst[k] * UNIT, v);
         }
     }
 }
@@ -125,7 +128,7 @@ struct Fill {
     int ntail;
 };
 __device__ inline void fill(const Fill& f, int block, int blocks) {
-    for (long long i = f.begin + (long long)block * blockDim.x + threadIdx.x; i < f.end; i += (long long)blocks * blockDim.x) f.at[i] = u32x4{};
+    for (long long i = f.begin + (long long)block * blockDim.x + threadIdx.x; i < f.end; i += (long long)blocks * blockDim.x) __builtin_nontemporal_store(u32x4{}, f.at + i);
     if (block == 0 && (int)threadIdx.x < f.ntail) f.tail[threadIdx.x] = 0;
 }
 __global__ __launch_bounds__(kSortThreads) void fill_kernel(Fill f) { fill(f, blockIdx.x, gridDim.x); }
@@ -157,16 +160,37 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(Pairs p, int M, int
                                                              uint32_t* __restrict__ key_out, int* __restrict__ pos_out, Fill f) {
     if ((int)blockIdx.x >= nb) return fill(f, blockIdx.x - nb, gridDim.x - nb);
     __shared__ int wave_count[kSortWaves][kBins];
+    __shared__ int wave_all[kSortWaves][kBins];
     __shared__ int wave_total[kSortWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    // Digit tid's first place for this block: all smaller digits' entries, and the blocks' before this one.
-    int before = 0, total = 0;
-#pragma unroll 8
-    for (int b = 0; b < nb; ++b) {
-        const int c = counts[b * kBins + tid];
-        before += b < (int)blockIdx.x ? c : 0;
-        total += c;
+    // Digit tid's first place for this block: all smaller digits' entries, and the blocks' before this one. Every wave adds up an
+    // eighth of the blocks' counts, eight digits a lane, with all loads under way (one after the other they took 10 us of 128
+    // blocks).
+    {
+        constexpr int PER = kBins / 64, EACH = kMostSortBlocks / kSortWaves;
+        int before[PER] = {}, total[PER] = {};
+#pragma unroll
+        for (int b = 0; b < EACH; ++b) {
+            const int block = b * kSortWaves + wave, on = block < nb, earlier = block < (int)blockIdx.x;
+            const int4* c = reinterpret_cast<const int4*>(counts + min(block, nb - 1) * kBins + lane * PER);
+#pragma unroll
+            for (int q = 0; q < PER / 4; ++q) {
+                const int4 v = c[q];
+                const int e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    total[4 * q + i] += on ? e[i] : 0;
+                    before[4 * q + i] += earlier ? e[i] : 0;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) wave_count[wave][lane * PER + i] = before[i], wave_all[wave][lane * PER + i] = total[i];
     }
+    __syncthreads();
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) before += wave_count[w][tid], total += wave_all[w][tid];
     int scan = total;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -224,17 +248,106 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(Pairs p, int M, int
     }
 }
 
+// Up to kSmall entries: one block sorts them in LDS, all passes in one launch, while the others zero dW. 8192 tokens: 11 us beside
+// 25 us of zeros for a 50304 x 768 fp32 weight; the launches above take 16 us beside them.
+constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64, kSmallItems = 16, kSmall = kSmallThreads * kSmallItems;
+template <typename I>
+__global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(Pairs p, int M, int passes, uint32_t* __restrict__ key_out, int* __restrict__ pos_out,
+                                                                   Fill f) {
+    if (blockIdx.x > 0) return fill(f, blockIdx.x - 1, gridDim.x - 1);
+    __shared__ uint32_t keys[kSmall];
+    __shared__ u16 positions[kSmall];
+    __shared__ int wave_count[kSmallWaves][kBins];
+    __shared__ int wave_total[kBins / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int items = (M + kSmallThreads - 1) / kSmallThreads, first = wave * 64 * items + lane;  // entries first + 64 i
+    uint32_t key[kSmallItems];
+    int pos[kSmallItems], rank[kSmallItems];
+#pragma unroll
+    for (int i = 0; i < kSmallItems; ++i) {
+        const int e = first + 64 * i;
+        const bool on = i < items && e < M;
+        key[i] = on ? key_at<I, true>(p, e) : 0;
+        pos[i] = e;
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * kDigit;
+        for (int i = tid; i < kSmallWaves * kBins; i += kSmallThreads) (&wave_count[0][0])[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kSmallItems; ++i) {
+            if (i >= items) continue;
+            const bool on = first + 64 * i < M;
+            const int d = (key[i] >> shift) & (kBins - 1);
+            const uint64_t m = same_digit(d, on);
+            const int leader = m ? __ffsll((unsigned long long)m) - 1 : 0;
+            int old = 0;
+            if (on && lane == leader) old = atomicAdd(&wave_count[wave][d], __popcll(m));
+            rank[i] = __shfl(old, leader) + __popcll(m & ((1ull << lane) - 1));
+        }
+        __syncthreads();
+        int total = 0, scan = 0;
+        if (tid < kBins) {  // (whole waves)
+#pragma unroll
+            for (int w = 0; w < kSmallWaves; ++w) total += wave_count[w][tid];
+            scan = total;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int t = __shfl_up(scan, d);
+                scan += lane >= d ? t : 0;
+            }
+            if (lane == 63) wave_total[wave] = scan;
+        }
+        __syncthreads();
+        if (tid < kBins) {
+            int run = scan - total;
+            for (int w = 0; w < wave; ++w) run += wave_total[w];
+#pragma unroll
+            for (int w = 0; w < kSmallWaves; ++w) {
+                const int c = wave_count[w][tid];
+                wave_count[w][tid] = run;
+                run += c;
+            }
+        }
+        __syncthreads();
+        const bool last = pass + 1 == passes;
+#pragma unroll
+        for (int i = 0; i < kSmallItems; ++i) {
+            if (i >= items || first + 64 * i >= M) continue;
+            const int at = wave_count[wave][(key[i] >> shift) & (kBins - 1)] + rank[i];
+            if (last) {
+                key_out[at] = key[i];
+                pos_out[at] = pos[i];
+            } else {
+                keys[at] = key[i];
+                positions[at] = (u16)pos[i];
+            }
+        }
+        if (last) break;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kSmallItems; ++i) {
+            const int e = first + 64 * i;
+            if (i < items && e < M) key[i] = keys[e], pos[i] = positions[e];
+        }
+        __syncthreads();
+    }
+}
+
 // ------------------------------------------------------------------------------------------
-// The sums. VEC values of a lane, 64 VEC columns of a wave: 4, or 1 where rows are not whole groups of 4.
+// The sums. VEC values of a lane, 64 VEC columns of a wave: 4, or 1 where rows are not whole groups of 4. dy is not needed again,
+// and its loads do not stay in the caches.
 // ------------------------------------------------------------------------------------------
 template <int DT, int VEC>
 __device__ inline void load_vec(const typename Row<DT>::T* p, float* v) {
     if constexpr (VEC == 1) {
         v[0] = Row<DT>::one(*p);
     } else if constexpr (DT == kF32) {
-        Row<DT>::load(p, v);
+        const f32x4 x = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = x[e];
     } else {
-        const u16x4 x = *reinterpret_cast<const u16x4*>(p);
+        const u16x4 x = __builtin_nontemporal_load(reinterpret_cast<const u16x4*>(p));
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = Elem<DT>::to_f32(x[e]);
     }
@@ -258,11 +371,11 @@ struct Sums {
     float scale;
 };
 
-// A wave per chunk and 64 VEC columns.
+// A wave per chunk and 64 VEC columns. 131072 x 768 bf16 (201 MB of dy): 41 us, with cached loads 62.
 template <int DT, int VEC>
 __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a, const void* __restrict__ dy_, void* __restrict__ dw_, long long waves) {
     using T = typename Row<DT>::T;
-    constexpr int U = 8;  // rows in flight
+    constexpr int U = 16;  // rows in flight
     const T* dy = reinterpret_cast<const T*>(dy_);
     T* dw = reinterpret_cast<T*>(dw_);
     const long long id = (long long)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -321,56 +434,97 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a, const void* __res
 }
 
 // Joins the sums of the token that begins in a chunk and goes on after it: the chunk's own, then the following ones', in
-// order (the waves take every kFixWaves-th of those and are added in order). A block per chunk and 64 VEC columns.
-constexpr int kFixWaves = 8;
+// order. A wave per chunk and 64 VEC columns joins up to kFew sums by itself; longer runs (a token that is there hundreds of
+// times) the block's waves join together, each every kFixWaves-th sum, and are added in order.
+constexpr int kFixWaves = 8, kFew = 16;
 template <int DT, int VEC>
 __global__ __launch_bounds__(64 * kFixWaves) void fixup_kernel(Sums a, void* __restrict__ dw_, int chunks) {
     using T = typename Row<DT>::T;
     constexpr int U = 8;
-    const int c = blockIdx.x / a.slabs, slab = blockIdx.x - c * a.slabs;
+    const int part_of = blockIdx.x / a.slabs, slab = blockIdx.x - part_of * a.slabs;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lo = c * a.chunk;
-    if (c + 1 >= chunks) return;
-    const uint32_t cur = a.key[lo + a.chunk - 1];
-    if (cur >= (uint32_t)a.V || a.key[lo + a.chunk] != cur) return;
-    if (a.key[lo] == cur && lo > 0 && a.key[lo - 1] == cur) return;
-    int last = c + 1, end = chunks;  // the last chunk that begins with this token: in [last, end)
-    while (end - last > 1) {
-        const int step = (end - last + 63) / 64;
-        const long long j = (long long)last + (long long)step * (lane + 1);
-        const int found = __popcll(__ballot(j < end && a.key[j * a.chunk] == cur));
-        last += found * step;
-        end = min(end, last + step);
-    }
     const int col = (slab * 64 + lane) * VEC;
     const bool mine = col < a.N;
     const float* part = a.part + (mine ? col : 0);
-    float acc[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = wave == 0 ? part[((size_t)c * 2 + 1) * a.ld + e] : 0.f;
-    for (long long j = c + 1 + wave; j <= last; j += kFixWaves * U) {
-        float v[U][VEC];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const long long k = j + u * kFixWaves;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[u][e] = k <= last ? part[(size_t)k * 2 * a.ld + e] : 0.f;
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] += v[u][e];
-    }
+    T* dw = reinterpret_cast<T*>(dw_);
+    __shared__ int ends[kFixWaves];  // the last chunk of a wave's run, for the block to join
+    __shared__ uint32_t tokens[kFixWaves];
     __shared__ float join[kFixWaves][64 * VEC];
+    // The sums of chunks j, j + step, ... up to last.
+    auto sum = [&](float* acc, int j, int last, int step) {
+        for (; j <= last; j += step * U) {
+            float v[U][VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) join[wave][lane * VEC + e] = acc[e];
+            for (int u = 0; u < U; ++u) {
+                const int k = j + u * step;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[u][e] = k <= last ? part[(size_t)k * 2 * a.ld + e] : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] += v[u][e];
+        }
+    };
+    auto own = [&](float* acc, int c) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] = part[((size_t)c * 2 + 1) * a.ld + e];
+    };
+    auto store = [&](const float* acc, uint32_t token) {
+        if (mine) store_vec<DT, VEC>(dw + (size_t)token * a.N + col, acc, a.scale);
+    };
+    // Whether chunk c is the first of a run, its token and the run's last chunk.
+    auto run = [&](int c, uint32_t& token, int& last) {
+        if (c + 1 >= chunks) return false;
+        const int lo = c * a.chunk;
+        token = a.key[lo + a.chunk - 1];
+        const uint32_t next = a.key[lo + a.chunk], first = a.key[lo], prev = lo > 0 ? a.key[lo - 1] : (uint32_t)a.V;
+        if (token >= (uint32_t)a.V || next != token || (first == token && prev == token)) return false;
+        last = c + 1;
+        for (int end = chunks, round = 0; end - last > 1; ++round) {  // (the last one that begins with the token: in [last, end))
+            const int step = round ? (end - last + 63) / 64 : 1;  // (most runs end within 64 chunks)
+            const long long j = (long long)last + (long long)step * (lane + 1);
+            const int found = __popcll(__ballot(j < end && a.key[j * a.chunk] == token));
+            last += found * step;
+            if (round || found < 64) end = min(end, last + step);
+        }
+        return true;
+    };
+    const int c = part_of * kFixWaves + wave;
+    uint32_t token;
+    int last;
+    int longer = 0;
+    float acc[VEC];
+    if (run(c, token, last)) {
+        if (last - c <= kFew) {
+            own(acc, c);
+            sum(acc, c + 1, last, 1);
+            store(acc, token);
+        } else {
+            longer = last;
+        }
+    }
+    if (lane == 0) ends[wave] = longer, tokens[wave] = token;
     __syncthreads();
-    if (wave != 0 || !mine) return;
+    for (int w = 0; w < kFixWaves; ++w) {
+        if (ends[w] == 0) continue;
+        const int c = part_of * kFixWaves + w;
 #pragma unroll
-    for (int w = 1; w < kFixWaves; ++w)
+        for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+        if (wave == 0) own(acc, c);
+        sum(acc, c + 1 + wave, ends[w], kFixWaves);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += join[w][lane * VEC + e];
-    store_vec<DT, VEC>(reinterpret_cast<T*>(dw_) + (size_t)cur * a.N + col, acc, a.scale);
+        for (int e = 0; e < VEC; ++e) join[wave][lane * VEC + e] = acc[e];
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int v = 1; v < kFixWaves; ++v)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] += join[v][lane * VEC + e];
+            store(acc, tokens[w]);
+        }
+        __syncthreads();
+    }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -404,7 +558,7 @@ struct Plan {
         nb = (int)((M + per - 1) / per);
         // Enough chunks for the chip, and chunks long enough that the borders' partial sums stay a small share.
         chunk = 8;
-        while (chunk < 64 && M / chunk > 4096) chunk *= 2;
+        while (chunk < 64 && M / chunk > 2048) chunk *= 2;
         chunks = (int)((M + chunk - 1) / chunk);
         ld = (int)((N + 3) & ~(int64_t)3);
         size_t n = 0;
@@ -463,7 +617,13 @@ NNEMB_API int nn_embedding_fwd(const void* weight, const void* idx, void* out, i
                 return launched("embedding fwd_kernel");
             };
             constexpr int W = Row<DT>::W;
-            return N % W == 0 ? go(fwd_kernel<DT, W, I>, N / W) : go(fwd_kernel<DT, 1, I>, N);
+            // What the next kernel can still find in the 256 MB cache is left there; half of it and more is stored past it.
+            // With the norm that follows: 8192 x 768 fp32 (25 MB) 20 us, 22 past the caches; 131072 x 768 bf16 (201 MB) 139 us
+            // either way, and the lookup itself 45 and 41 us (62 and 42 where other work has left the cache full).
+            const bool past = M * N * (dtype == kF32 ? 4 : 2) >= (int64_t)128 << 20;
+            return N % W     ? go(fwd_kernel<DT, 1, false, I>, N)
+                   : past    ? go(fwd_kernel<DT, W, true, I>, N / W)
+                             : go(fwd_kernel<DT, W, false, I>, N / W);
         });
     });
 }
@@ -481,7 +641,7 @@ NNEMB_API int nn_embedding_bwd(const void* dy, const void* idx, void* dw, void* 
     if (!dw || (M && (!dy || !idx || !workspace))) return fail("null pointer argument");
     const hipStream_t st = (hipStream_t)stream;
     const int64_t total = V * N * (dtype == kF32 ? 4 : 2), units = total / 16;
-    constexpr int kFillBlocks = 1024;
+    constexpr int kFillBlocks = 1024, kSmallFill = 255;  // (one block to a CU where their LDS is the sort's)
     // The i-th of n launches' share of dW.
     auto share = [&](int i, int n) {
         return Fill{(u32x4*)dw, units * i / n, units * (i + 1) / n, (u16*)((char*)dw + units * 16), i + 1 == n ? (int)(total - units * 16) / 2 : 0};
@@ -492,8 +652,19 @@ NNEMB_API int nn_embedding_bwd(const void* dy, const void* idx, void* dw, void* 
     }
     char* ws = (char*)workspace;
     int* counts = (int*)(ws + p.counts);
+    const bool small = M <= kSmall;
+    if (small) {
+        const int to = (p.passes - 1) & 1;
+        const Pairs in{idx, nullptr, nullptr, padding_idx, (int)V, 0};
+        const int e = by_index(idx_bits, [&](auto i) {
+            sort_small_kernel<decltype(i)><<<dim3(1 + kSmallFill), dim3(kSmallThreads), 0, st>>>(in, (int)M, p.passes, (uint32_t*)(ws + p.key[to]),
+                                                                                                 (int*)(ws + p.pos[to]), share(0, 1));
+            return launched("embedding sort_small_kernel");
+        });
+        if (e) return e;
+    }
     const int grid = p.nb + kFillBlocks, parts = 2 * p.passes;
-    for (int pass = 0; pass < p.passes; ++pass) {
+    for (int pass = 0; pass < p.passes && !small; ++pass) {
         const int from = (pass + 1) & 1, to = pass & 1;
         const Pairs in{idx, (const uint32_t*)(ws + p.key[from]), (const int*)(ws + p.pos[from]), padding_idx, (int)V, pass * kDigit};
         uint32_t* key = (uint32_t*)(ws + p.key[to]);
@@ -516,13 +687,13 @@ NNEMB_API int nn_embedding_bwd(const void* dy, const void* idx, void* dw, void* 
         auto go = [&](auto sum, auto fixup, int vec) {
             const int slabs = (int)((N + 64 * vec - 1) / (64 * vec));
             const int64_t waves = (int64_t)p.chunks * slabs, blocks = (waves + kThreads / 64 - 1) / (kThreads / 64);
-            if (waves >= ((int64_t)1 << 32) / (64 * kFixWaves)) return fail("invalid sizes");
+            if (waves >= ((int64_t)1 << 32) / 64 - 64 * kFixWaves * slabs) return fail("invalid sizes");
             const Sums a{(const uint32_t*)(ws + p.key[last]), (const int*)(ws + p.pos[last]), (float*)(ws + p.part), (int)M, (int)V, (int)N,
                          p.ld, p.chunk, slabs, scale};
             sum<<<dim3((unsigned)blocks), dim3(kThreads), 0, st>>>(a, dy, dw, (long long)waves);
             if (int err = launched("embedding sum_kernel")) return err;
             if (p.chunks == 1) return 0;
-            fixup<<<dim3((unsigned)waves), dim3(64 * kFixWaves), 0, st>>>(a, dw, p.chunks);
+            fixup<<<dim3((unsigned)((p.chunks + kFixWaves - 1) / kFixWaves * slabs)), dim3(64 * kFixWaves), 0, st>>>(a, dw, p.chunks);
             return launched("embedding fixup_kernel");
         };
         return N % 4 == 0 ? go(sum_kernel<DT, 4>, fixup_kernel<DT, 4>, 4) : go(sum_kernel<DT, 1>, fixup_kernel<DT, 1>, 1);
