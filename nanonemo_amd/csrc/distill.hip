@@ -7,7 +7,7 @@
 //   KL = sum p_i (log p_i - log q_{j_i}) [+ p_rest (log p_rest - log q_rest)]
 //   loss = mean of w tau^2 KL + (1 - w) (logsumexp(z) - z_target)
 //   dz_j = g / n (w tau (q_j f_j - p_j) + (1 - w) (s_j - [j = target])),  s = softmax(z),
-//   f_j = 1 - p_rest / q_rest outside the top set where rest is a class, else 1.
+//   f_j = 1 - p_rest / q_rest outside the top set where rest is a class, else 1 (p_j = 0 outside the top set).
 //
 // A student near its teacher has a loss far below L, so the loss is a small difference of terms that share L. The sum over
 // the row, in fp32, therefore leaves out the top set and the target (a bitmap in LDS marks them); their terms, and all that
@@ -298,7 +298,7 @@ struct TopShared {
 // Rows for which the above does not do (many equal values, NaN, a k near the number of parts) take a search of the k-th value bit
 // by bit instead, and rows whose others lie far below the bound a sum relative to their own largest.
 template <int DT, int TB, int NV>
-__global__ __launch_bounds__(TB, TB == 512 ? 6 : 4) void top_kernel(const void* __restrict__ logits, Layout at, void* __restrict__ values,
+__global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(const void* __restrict__ logits, Layout at, void* __restrict__ values,
                                                     long long* __restrict__ indices, float* __restrict__ rest, int V, int k, float c,
                                                     double inv_tau) {
     using R = Row<DT>;
@@ -604,8 +604,9 @@ struct Loss {
     double tau, weight;
     __device__ bool hard() const { return targets && weight < 1.0; }
 };
-// A row's statistics: L, logsumexp(z), Lt, f, what exponents are relative to, and whether an index is there twice.
-enum { kL, kL1, kLt, kF, kBase, kTwice, kStats };
+// A row's statistics: L, logsumexp(z), Lt, log of the rest's sum and p_rest, a logit that the gradient's exponents are relative to,
+// and whether an index is there twice.
+enum { kL, kL1, kLt, kLr, kPr, kBase, kTwice, kStats };
 
 __device__ inline float value_at(const void* p, long long i, int dt) {
     if (dt == kF32) return reinterpret_cast<const float*>(p)[i];
@@ -786,36 +787,39 @@ __global__ __launch_bounds__(TB, 8) void loss_fwd_kernel(Loss x) {
         from = base_of(a.m) * inv_tau, from1 = base_of(a.m);
     }
     if constexpr (!BOTH) s1 = s, from1 = from;  // (read only where the temperature is 1)
-    if (s == 0.f) from = from1 = -INFINITY;
     if (tid >= 64) return;
     const Sums4 top = top_sums;
     const float z_target = zt, zmax = fmaxf(near, z_target);
-    const double base = base_of(zmax), at = base * inv_tau;
+    const double base = base_of(zmax), at = base * inv_tau, z_soft = z_target * inv_tau;
     tmax = t_most;
 
-    // The exponentials and logarithms that join them, one a lane. Sums that lie above the base move it.
+    // All that is joined: logarithms and exponentials one a lane, since each takes as long as 64 of them.
     auto lane_of = [](double v, int lane) { return __shfl(v, lane); };
-    const double up = fmax(0.0, from - at), up1 = fmax(0.0, from1 - base), rest = x.rest ? (double)x.rest[r] : -INFINITY;
-    const double arg = tid == 0   ? from - at - up
-                       : tid == 1 ? from1 - base - up1
-                       : tid == 2 ? z_target * inv_tau - at - up
-                       : tid == 3 ? z_target - base - up1
+    const double rest = x.rest ? (double)x.rest[r] : -INFINITY, ls = log((double)(tid == 0 ? s : s1));
+    const double Ls = s == 0.f ? -INFINITY : from + lane_of(ls, 0), Ls1 = s == 0.f ? -INFINITY : from1 + lane_of(ls, 1);
+    const bool alone = hard && !target_in_top;  // (then the target is one of the others, but not in their sum)
+    const double to = fmax(at, Ls), to1 = fmax(base, Ls1), to_r = alone ? fmax(Ls, z_soft) : Ls;
+    const double arg = tid == 0   ? Ls - to
+                       : tid == 1 ? Ls1 - to1
+                       : tid == 2 ? z_soft - to
+                       : tid == 3 ? z_target - to1
                        : tid == 4 ? rest - tmax
-                       : tid == 5 ? -up
-                                  : -up1;
+                       : tid == 5 ? at - to
+                       : tid == 6 ? base - to1
+                       : tid == 7 ? Ls - to_r
+                                  : z_soft - to_r;
     const double ex = exp(arg);
-    const bool alone = hard && !target_in_top;
-    const double others = s * lane_of(ex, 0) + (alone ? lane_of(ex, 2) : 0.0), others1 = s1 * lane_of(ex, 1) + (alone ? lane_of(ex, 3) : 0.0);
-    const double w = x.rest ? lane_of(ex, 4) : 0.0, A = top.a + w, Z = top.z * lane_of(ex, 5) + others, Z1 = top.z1 * lane_of(ex, 6) + others1;
-    const double lg = log(tid == 0 ? Z : tid == 1 ? Z1 : tid == 2 ? A : others);
-    const double L = at + up + lane_of(lg, 0), L1 = hard ? base + up1 + lane_of(lg, 1) : 0.0, Lt = tmax + lane_of(lg, 2);
-    double P = top.p, f = 1.0;
-    if (x.rest && !(w == 0.0)) {
-        P += w * (rest - (at + up + lane_of(lg, 3)));
-        f = 1.0 - (w / A) * (Z / others);
-    }
+    const double w = x.rest ? lane_of(ex, 4) : 0.0, A = top.a + w;
+    const double Z = top.z * lane_of(ex, 5) + lane_of(ex, 0) + (alone ? lane_of(ex, 2) : 0.0);
+    const double Z1 = top.z1 * lane_of(ex, 6) + lane_of(ex, 1) + (alone ? lane_of(ex, 3) : 0.0);
+    const double lg = log(tid == 0 ? Z : tid == 1 ? Z1 : tid == 2 ? A : lane_of(ex, 7) + lane_of(ex, 8));
+    const double L = to + lane_of(lg, 0), L1 = hard ? to1 + lane_of(lg, 1) : 0.0, Lt = tmax + lane_of(lg, 2);
+    const double Lr = to_r == -INFINITY ? to_r : alone ? to_r + lane_of(lg, 3) : Ls;
     if (tid != 0) return;
-    st[kL] = L, st[kL1] = L1, st[kLt] = Lt, st[kF] = f, st[kBase] = base, st[kTwice] = twice;
+    double P = top.p;
+    if (!(w == 0.0)) P += w * (rest - Lr);
+    const float own = (float)(Ls * x.tau);
+    st[kL] = L, st[kL1] = L1, st[kLt] = Lt, st[kLr] = Lr, st[kPr] = w / A, st[kBase] = fabsf(own) < INFINITY ? own : 0.f, st[kTwice] = twice;
     double v = 0.0;
     if (zmax == INFINITY) v = st[kL] = NAN;  // (inf - inf again)
     if (x.weight > 0.0) v += x.weight * x.tau * x.tau * (P / A - Lt + L);
@@ -869,10 +873,15 @@ __global__ __launch_bounds__(TB, 8) void loss_bwd_kernel(Loss x, const float* __
     const bool hard = x.hard(), soft = x.weight > 0.0;
     const T* row = reinterpret_cast<const T*>(x.logits) + x.at.at(r);
     const double* st = x.stats + (size_t)r * kStats;
-    const double inv_tau = 1.0 / x.tau, L = st[kL], L1 = st[kL1], base = st[kBase], f = st[kF];
+    const double inv_tau = 1.0 / x.tau, L = st[kL], L1 = st[kL1], Lr = st[kLr], p_rest = st[kPr], base = st[kBase];
     const double g = (double)grad[0] * x.stats[(size_t)gridDim.x * (kStats + 1)], gs = soft ? x.weight * x.tau * g : 0.0, gh = hard ? (1.0 - x.weight) * g : 0.0;
-    // Every logit as one outside the top set.
-    float A = soft ? (float)(gs * f * exp(base * inv_tau - L)) : 0.f;
+    // q_j f_j of a logit outside the top set, which is q_j - p_rest times its share of the rest.
+    auto outside = [&](double z) {
+        const double share = p_rest == 0.0 ? 0.0 : p_rest * exp(z * inv_tau - Lr);
+        return gs * (exp(z * inv_tau - L) - share);
+    };
+    // Every logit as one of those, relative to one of their size: the rest may lie far below the top set.
+    float A = soft ? (float)outside(base) : 0.f;
     const float B = hard ? (float)(gh * exp(base - L1)) : 0.f, b = (float)base;
     if constexpr (S2 == kNoSecond) A += B;  // (there is B only where the temperature is 1)
     if (L != L) A = NAN;          // an index or target out of range, or a NaN or +inf in the row
@@ -919,7 +928,7 @@ __global__ __launch_bounds__(TB, 8) void loss_bwd_kernel(Loss x, const float* __
     __syncthreads();
     if (hard && tid == 0 && !target_in_top && target >= 0 && target < V) {
         const double z = R::one(row[target]);
-        dst[target] = R::round((float)((soft ? gs * f * exp(z * inv_tau - L) : 0.0) + gh * (exp(z - L1) - 1.0)));
+        dst[target] = R::round((float)((soft ? outside(z) : 0.0) + gh * (exp(z - L1) - 1.0)));
     }
 }
 
@@ -981,6 +990,7 @@ NNDIS_API int nn_top_logits(const void* logits, int64_t T, int64_t sb, int64_t s
                : groups <= 4 * 256   ? go(top_kernel<DT, 256, 4>, 256)
                : groups <= 8 * 512   ? go(top_kernel<DT, 512, 8>, 512)
                : groups <= 13 * 512  ? go(top_kernel<DT, 512, 13>, 512)
+               : groups <= 16 * 512  ? go(top_kernel<DT, 512, 16>, 512)
                : groups <= 16 * 1024 ? go(top_kernel<DT, 1024, 16>, 1024)
                                      : go(top_kernel<DT, 1024, 0>, 1024);
     });

@@ -50,7 +50,7 @@ def _distill_loss(
 @_distill_loss.register_fake
 def _(logits, values, indices, rest, targets, temperature, weight):
     rows = math.prod(logits.shape[:-1])
-    return logits.new_empty((), dtype=torch.float32), logits.new_empty(rows * 7 + 1, dtype=torch.float64)
+    return logits.new_empty((), dtype=torch.float32), logits.new_empty(rows * 8 + 1, dtype=torch.float64)
 
 
 @torch.library.custom_op("nanonemo::distill_loss_bwd", mutates_args=())

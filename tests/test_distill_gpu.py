@@ -145,8 +145,9 @@ def _reference(z, v, idx, rest, y, tau, w, grad=1.0):
     off = w * tau**2 * (q_rest - p_rest).abs().squeeze(-1) + (1 - w if hard else 0.0)
     loss_off = SUM * (off * keep).sum() / n + 2**-23 * loss.detach().abs() + 1e-12
     q = logq.detach().exp()
-    ratio = torch.where(p_rest > 0, p_rest / q_rest, 0.0)
-    size = w * tau * q * (1 + torch.where(others, ratio, 0.0)) + ((1 - w) * s.detach().exp() if hard else 0.0)
+    # (q p_rest / q_rest as a share of the rest: q and q_rest may both vanish, even in fp64)
+    share = torch.where(others & (p_rest > 0), p_rest * torch.softmax(logq.detach().masked_fill(~others, -INF), -1), 0.0).nan_to_num(0.0)
+    size = w * tau * (q + share) + ((1 - w) * s.detach().exp() if hard else 0.0)
     slack = SUM * size * (keep / n * abs(grad)).unsqueeze(-1)
     return loss.detach(), d.view(z.shape), loss_off, (half * (d.abs() + slack) + slack + tiny).view(z.shape)
 
@@ -211,6 +212,24 @@ def test_teacher_types_orders_and_scales():
     vm[..., 30:] = -INF  # a teacher that gives fewer than k
     _check_loss(z, vm, idx, rest, y, 2.0, 0.5, "fewer")
     _check_loss(z, v, idx, torch.full_like(rest, -INF), y, 2.0, 0.5, "nothing in the rest")
+
+
+@pytest.mark.parametrize("V", [300, 5000])
+def test_a_student_whose_top_set_stands_far_above_or_below_the_rest(V):
+    # 300 above: the rest's probabilities vanish in fp32 beside the top set's, its shares of the rest's gradient do not. 300
+    # below (and 900, past the exponents that fp32 sums reach): the top set's vanish.
+    g = _gen(13)
+    z, v, idx, rest, y = _case((6,), V, 9, torch.float32, 1.0, g)
+    for up in (300.0, -300.0, 900.0, -900.0):
+        x = z.scatter_add(-1, idx, torch.full_like(v, up))
+        y[0] = next(j for j in range(V) if j not in idx[0].tolist())
+        for r, t, w in ((rest, None, 1.0), (rest, y, 0.5), (None, y, 0.5)):
+            _check_loss(x, v, idx, r, t, 1.0, w, (up, r is not None, w))
+    # a masked vocabulary: all but the top set at the type's lowest value, or gone
+    low = torch.full_like(z, torch.finfo(z.dtype).min / 4).scatter(-1, idx, z.gather(-1, idx))
+    _check_loss(low, v, idx, None, None, 1.0, 1.0, "lowest")
+    _check_loss(low.masked_fill(low < -1e30, -INF), v, idx, None, None, 1.0, 1.0, "gone")
+    _check_loss(low, v, idx, torch.full_like(rest, -INF), None, 1.0, 1.0, "lowest, nothing in the rest")
 
 
 def test_strided_logits_and_teachers():

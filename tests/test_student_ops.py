@@ -156,7 +156,7 @@ def test_distill_c_abi_rejects_bad_arguments_before_any_launch(kw, msg):
 
 def test_distill_c_abi_checks_of_the_loss():
     L = lib()
-    assert L.nn_distill_stats_size(0) == 0 and L.nn_distill_stats_size(8192) == 8192 * 7 + 1
+    assert L.nn_distill_stats_size(0) == 0 and L.nn_distill_stats_size(8192) == 8192 * 8 + 1
     for weight, value_dtype, out, msg in ((-0.1, 1, 8192, "weight must be in"), (math.nan, 1, 8192, "weight must be in"), (0.5, 3, 8192, "dtype must be"), (0.5, 1, 8193, "dlogits must be aligned")):
         rc = L.nn_distill_bwd(2048, 256, 16, 0, 64, 512, 1024, None, 4096, out, 16, 64, 4, 1.0, weight, 1, value_dtype, None)
         assert rc != 0 and msg in L.nn_distill_last_error().decode()
