@@ -8,14 +8,17 @@
 // links: nothing here launches a kernel of its own.
 //
 // Every function allocates through PyTorch's caching allocator, launches on PyTorch's current stream of its inputs'
-// device, and neither synchronises nor keeps state between calls.
+// device, and neither synchronises nor keeps state between calls. (The embedding's and the distillation loss's autograd nodes
+// are here as well, see there.)
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 #include <torch/library.h>
@@ -786,6 +789,91 @@ Tensor distill_bwd_op(const Tensor& d_loss, const Tensor& logits, const Tensor& 
     return distill_bwd(d_loss, logits, values, indices, targets, stats, temperature, weight);
 }
 
+// ---- the two as autograd nodes ------------------------------------------------------------------
+// A student's small batch is paced by the host: with an autograd.Function in Python, a lookup and its gradient took 56 us of host
+// time around 20 us of kernels, of which the engine's own hand-off between threads is about 35.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void refuse_capture(const char* where) {
+    if (capturing())
+        raise(std::string(where) + ": capturing this op into a HIP graph while autograd records it (torch.cuda.graph around the forward and its "
+              "autograd backward, or torch.compile(mode='reduce-overhead')) is not supported. Capture it without autograd (under "
+              "torch.no_grad(), or the C ABI's calls), or run it eagerly.");
+}
+bool records(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+bool ordinary(const Tensor& t);
+void need_ordinary(const Tensor& grad) { need(ordinary(grad), "batched gradients (is_grads_batched) are not supported: the kernels read gradients by address"); }
+// A gradient that cannot be differentiated again: doing so is an error, as with once_differentiable.
+Tensor once(Tensor grad, const char* where) {
+    if (!at::GradMode::is_enabled()) return grad;
+    auto error = std::make_shared<torch::autograd::DelayedError>(std::string("trying to differentiate twice a function that was marked with once_differentiable: ") + where, 1);
+    return (*error)({grad.detach().requires_grad_()})[0];  // (of an input without a gradient it would make no node)
+}
+
+struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& idx, const Tensor& weight, double scale, int64_t padding) {
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({idx});
+        ctx->saved_data["rows"] = weight.size(0), ctx->saved_data["scale"] = scale, ctx->saved_data["padding"] = padding;
+        const at::AutoDispatchBelowADInplaceOrView below;
+        return embedding_fwd(idx, weight, scale);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_capture("embedding backward");
+        const auto saved = ctx->get_saved_variables();
+        if (!grads[0].defined()) return {{}, {}, {}, {}};
+        need_ordinary(grads[0]);
+        Tensor dw;
+        {
+            const at::AutoDispatchBelowADInplaceOrView below;
+            dw = embedding_bwd(grads[0], saved[0], ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt());
+        }
+        return {{}, once(dw, "embedding"), {}, {}};
+    }
+};
+Tensor embedding_call(const Tensor& idx, const Tensor& weight, double scale, int64_t padding) {
+    if (!records(weight)) return embedding_fwd(idx, weight, scale);
+    refuse_capture("embedding");
+    return EmbeddingNode::apply(idx, weight, scale, padding);
+}
+
+struct DistillNode : torch::autograd::Function<DistillNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& values, const Tensor& indices, const OptTensor& rest,
+                          const OptTensor& targets, double temperature, double weight) {
+        Tensor loss, stats;
+        {
+            const at::AutoDispatchBelowADInplaceOrView below;
+            std::tie(loss, stats) = distill_fwd(logits, values, indices, rest, targets, temperature, weight);
+        }
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({logits, values, indices, targets ? *targets : Tensor(), stats});
+        ctx->saved_data["temperature"] = temperature, ctx->saved_data["weight"] = weight;
+        return loss;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_capture("distill_loss backward");
+        const auto t = ctx->get_saved_variables();
+        if (!grads[0].defined()) return variable_list(7);
+        need_ordinary(grads[0]);
+        variable_list out(7);
+        Tensor d;
+        {
+            const at::AutoDispatchBelowADInplaceOrView below;
+            d = distill_bwd(grads[0], t[0], t[1], t[2], t[3].defined() ? OptTensor(t[3]) : std::nullopt, t[4], ctx->saved_data["temperature"].toDouble(),
+                            ctx->saved_data["weight"].toDouble());
+        }
+        out[0] = once(d, "distill_loss");
+        return out;
+    }
+};
+Tensor distill_call(const Tensor& logits, const Tensor& values, const Tensor& indices, const OptTensor& rest, const OptTensor& targets,
+                    double temperature, double weight) {
+    if (!records(logits)) return std::get<0>(distill_fwd(logits, values, indices, rest, targets, temperature, weight));
+    refuse_capture("distill_loss");
+    return DistillNode::apply(logits, values, indices, rest, targets, temperature, weight);
+}
+
 // ---- routing ------------------------------------------------------------------------------------
 
 // Whether the tensor's values lie at its address, as dense values of its own type: not inside a transform's wrapper
@@ -864,9 +952,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("rope", rope, nogil);
     m.def("norm_fwd", norm_fwd, nogil);
     m.def("norm_bwd", norm_bwd, nogil);
+    m.def("embedding", embedding_call, nogil);
     m.def("embedding_fwd", embedding_fwd, nogil);
     m.def("embedding_bwd", embedding_bwd, nogil);
     m.def("top_logits", top_logits, nogil);
+    m.def("distill", distill_call, nogil);
     m.def("distill_fwd", distill_fwd, nogil);
     m.def("distill_bwd", distill_bwd, nogil);
     m.def("wgrad", wgrad, nogil);

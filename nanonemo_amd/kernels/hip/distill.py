@@ -24,7 +24,6 @@ import math
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from nanonemo_amd.kernels.hip import eager, host, preload, records, refuse_capture
 
@@ -85,23 +84,6 @@ def _backward(ctx, d_loss, _d_stats):
 _distill_loss.register_autograd(_backward, setup_context=_setup_context)
 
 
-class _DistillLossFn(torch.autograd.Function):
-    """The eager path of distill_loss (plain CUDA tensors outside tracing; ``eager``): the op's launches without its
-    dispatch."""
-
-    @staticmethod
-    def forward(ctx, *inputs):
-        loss, stats = host().distill_fwd(*inputs)
-        _save(ctx, inputs, stats)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_loss):
-        refuse_capture("distill_loss backward")
-        return (None if d_loss is None else host().distill_bwd(d_loss, *ctx.saved_tensors, *ctx.call), *(None,) * 6)
-
-
 def _check_temperature(temperature: float) -> None:
     if not 1e-4 <= temperature <= 1e4:
         raise ValueError(f"temperature must be in [1e-4, 1e4], got {temperature}")
@@ -136,10 +118,10 @@ def distill_loss(
         raise ValueError("weight below 1 needs targets, whose cross entropy is the rest of the loss")
     if records(values) or rest is not None and records(rest):
         raise ValueError("the teacher's values take no gradient: detach them")
-    refuse_capture("distill_loss", logits)
     call = (logits, values, indices, rest, targets, float(temperature), float(weight))
-    if eager(*(t for t in call[:5] if t is not None)):
-        return _DistillLossFn.apply(*call) if records(logits) else host().distill_fwd(*call)[0]
+    if eager(*(t for t in call[:5] if t is not None)):  # the same launches as the op's, as one autograd node of the host module
+        return host().distill(*call)
+    refuse_capture("distill_loss", logits)
     return _distill_loss(*call)[0]
 
 

@@ -15,9 +15,8 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
-from nanonemo_amd.kernels.hip import eager, host, preload, records, refuse_capture
+from nanonemo_amd.kernels.hip import eager, host, preload, refuse_capture
 
 
 @torch.library.custom_op("nanonemo::embedding", mutates_args=())
@@ -58,21 +57,6 @@ def _backward(ctx, d_out):
 _embedding.register_autograd(_backward, setup_context=_setup_context)
 
 
-class _EmbeddingFn(torch.autograd.Function):
-    """The eager path of embedding (plain CUDA tensors outside tracing; ``eager``): the op's launches without its dispatch."""
-
-    @staticmethod
-    def forward(ctx, idx, weight, scale, padding_idx):
-        _save(ctx, idx, weight, scale, padding_idx)
-        return host().embedding_fwd(idx, weight, scale)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_out):
-        refuse_capture("embedding backward")
-        return None, host().embedding_bwd(d_out, *ctx.saved_tensors, *ctx.call), None, None
-
-
 def embedding(idx: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: int | None = None) -> Tensor:
     """scale * weight[idx]: idx (...) int64 or int32, weight (V, N) fp16, bf16 or fp32 -> (..., N) of the weight's type.
     Rows whose token is ``padding_idx`` (negative: from the end) give the weight no gradient."""
@@ -83,11 +67,9 @@ def embedding(idx: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: int 
         padding_idx %= rows
     else:
         raise ValueError(f"padding_idx {padding_idx} is not a row of the weight ({rows} rows)")
+    if eager(idx, weight):  # the same launches as the op's, as one autograd node of the host module
+        return host().embedding(idx, weight, scale, padding_idx)
     refuse_capture("embedding", weight)
-    if eager(idx, weight):
-        if records(weight):
-            return _EmbeddingFn.apply(idx, weight, scale, padding_idx)
-        return host().embedding_fwd(idx, weight, scale)
     return _embedding(idx, weight, scale, padding_idx)
 
 

@@ -342,7 +342,7 @@ def test_op_and_eager_path_give_the_same_bits_and_the_ops_pass_opcheck():
     z, v, idx, rest, y = _case((2, 5), 700, 6, torch.float32, 2.0, _gen(10))
     z.requires_grad_()
     loss, op = distill_loss(z, v, idx, rest, y, 2.0, 0.5), torch.ops.nanonemo.distill_loss(z, v, idx, rest, y, 2.0, 0.5)[0]
-    assert type(loss.grad_fn).__name__.startswith("_DistillLossFn") and torch.equal(loss, op)
+    assert 'DistillNode' in loss.grad_fn.name() and torch.equal(loss, op)
     (d,) = torch.autograd.grad(loss, z, retain_graph=True)
     assert torch.equal(d, torch.autograd.grad(loss, z)[0]) and torch.equal(d, torch.autograd.grad(op, z)[0])
     tests = ("test_schema", "test_autograd_registration", "test_faketensor")
@@ -354,6 +354,27 @@ def test_op_and_eager_path_give_the_same_bits_and_the_ops_pass_opcheck():
     eager = distill_loss(z * 1.0, *top_logits(z.flip(0), 6, 2.0), y, 2.0, 0.5)
     got = f(z)
     assert torch.equal(got, eager) and torch.equal(torch.autograd.grad(got, z)[0], torch.autograd.grad(eager, z)[0])
+
+
+def test_the_autograd_node_refuses_what_it_cannot_do():
+    from nanonemo_amd.kernels.hip.distill import distill_loss
+
+    z, v, idx, rest, y = _case((4,), 60, 5, torch.float32, 1.0, _gen(14))
+    z.requires_grad_()
+    (g,) = torch.autograd.grad(distill_loss(z, v, idx), z, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
+    with pytest.raises(RuntimeError, match="batched gradients"):
+        torch.autograd.grad(distill_loss(z, v, idx), z, torch.ones(2, device="cuda"), is_grads_batched=True)
+    loss = distill_loss(z, v, idx)
+    with torch.no_grad():
+        z.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    loss = distill_loss(z, v, idx, rest, y, 1.0, 0.5)
+    a, b = (torch.autograd.grad(loss * 2, z, retain_graph=True)[0] for _ in range(2))
+    assert torch.equal(a, b)
+    assert torch.autograd.grad(distill_loss(z * 1.0, v, idx, rest, y, 1.0, 0.5) * 2, z)[0].equal(a)
 
 
 def test_gradient_matches_differences():

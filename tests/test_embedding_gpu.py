@@ -135,7 +135,7 @@ def test_op_and_eager_path_give_the_same_bits_and_the_op_passes_opcheck():
     w = torch.randn(203, 96, device="cuda", requires_grad=True)
     dy = torch.randn(3, 50, 96, device="cuda")
     out, op = embedding(idx, w, 1.5, 7), torch.ops.nanonemo.embedding(idx, w, 1.5, 7)
-    assert type(out.grad_fn).__name__.startswith("_EmbeddingFn") and torch.equal(out, op)
+    assert 'EmbeddingNode' in out.grad_fn.name() and torch.equal(out, op)
     assert torch.equal(torch.autograd.grad(out, w, dy)[0], torch.autograd.grad(op, w, dy)[0])
     torch.library.opcheck(torch.ops.nanonemo.embedding, (idx, w, 1.5, 7))
     torch.library.opcheck(torch.ops.nanonemo.embedding_bwd, (dy, idx, 203, 1.5, 7))
@@ -145,6 +145,32 @@ def test_op_and_eager_path_give_the_same_bits_and_the_op_passes_opcheck():
     assert torch.equal(torch.autograd.grad(got, w, dy)[0], torch.autograd.grad(embedding(idx, w, 1.5, 7) * 2, w, dy)[0])
     with torch.no_grad():
         assert torch.equal(embedding(idx, w, 1.5, 7), out)
+
+
+def test_the_autograd_node_refuses_what_it_cannot_do():
+    from nanonemo_amd.kernels.hip.embedding import embedding
+
+    idx = torch.randint(0, 20, (3, 5), device="cuda")
+    w = torch.randn(20, 8, device="cuda", requires_grad=True)
+    out = embedding(idx, w)
+    (g,) = torch.autograd.grad(out.square().sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
+    with pytest.raises(RuntimeError, match="batched gradients"):
+        torch.autograd.grad(embedding(idx, w), w, torch.ones(2, 3, 5, 8, device="cuda"), is_grads_batched=True)
+    out = embedding(idx, w)
+    idx.add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    out = embedding(idx, w)  # twice over one graph, and a hook on the way
+    seen = []
+    out.register_hook(lambda d: seen.append(d.shape))
+    a, b = (torch.autograd.grad(out.sum(), w, retain_graph=True)[0] for _ in range(2))
+    assert torch.equal(a, b) and len(seen) == 2
+    loss = embedding(idx, w).sum()
+    del out
+    loss.backward()
+    assert torch.equal(w.grad, a)
 
 
 def test_on_another_stream_and_captured_into_a_graph():
