@@ -360,7 +360,7 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
         for (int i = tid; i < groups; i += TB) mine = max(mine, O::most(one_group(i), mag));
     }
     if constexpr (TB == 64) {
-        if (k <= groups) {
+        if (2 * k <= groups) {
             least = reached<K::kBits>(most, k);
         } else {
             uint32_t v[N * R::W];
@@ -986,7 +986,11 @@ NNDIS_API int nn_top_logits(const void* logits, int64_t T, int64_t sb, int64_t s
             return launched("top_kernel");
         };
         const int64_t groups = (V + Row<DT>::W - 1) / Row<DT>::W;  // of 16 bytes, held by the block's threads
-        return groups <= 4 * 64      ? go(top_kernel<DT, 64, 4>, 64)
+        // One wave a row up to 256 groups (groups past the row's end take as long as others: 468000 x 512 bf16, k = 6, 733 us with
+        // 4 a thread).
+        return groups <= 64          ? go(top_kernel<DT, 64, 1>, 64)
+               : groups <= 2 * 64    ? go(top_kernel<DT, 64, 2>, 64)
+               : groups <= 4 * 64    ? go(top_kernel<DT, 64, 4>, 64)
                : groups <= 4 * 256   ? go(top_kernel<DT, 256, 4>, 256)
                : groups <= 8 * 512   ? go(top_kernel<DT, 512, 8>, 512)
                : groups <= 13 * 512  ? go(top_kernel<DT, 512, 13>, 512)

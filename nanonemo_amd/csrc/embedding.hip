@@ -248,9 +248,10 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(Pairs p, int M, int
     }
 }
 
-// Up to kSmall entries: one block sorts them in LDS, all passes in one launch, while the others zero dW. 8192 tokens: 11 us beside
-// 25 us of zeros for a 50304 x 768 fp32 weight; the launches above take 16 us beside them.
-constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64, kSmallItems = 16, kSmall = kSmallThreads * kSmallItems;
+// Up to kSmall entries: one block sorts them in LDS, all passes in one launch, while the others zero dW. The whole gradient of
+// 8192 x 768 fp32 into 50304 rows: 46 us, with the four launches above 49 (and three more launches for the host); of 16384 tokens
+// 72 and 61: there the one block takes longer than the zeros.
+constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64, kSmallItems = 8, kSmall = kSmallThreads * kSmallItems;
 template <typename I>
 __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(Pairs p, int M, int passes, uint32_t* __restrict__ key_out, int* __restrict__ pos_out,
                                                                    Fill f) {
@@ -435,12 +436,13 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a, const void* __res
 
 // Joins the sums of the token that begins in a chunk and goes on after it: the chunk's own, then the following ones', in
 // order. A wave per chunk and 64 VEC columns joins up to kFew sums by itself; longer runs (a token that is there hundreds of
-// times) the block's waves join together, each every kFixWaves-th sum, and are added in order.
-constexpr int kFixWaves = 8, kFew = 16;
+// times) the block's waves join together, each every kFixWaves-th sum, and are added in order. A run of 1567 sums of 512 columns:
+// 21 us (85 with loads that wait for one another), beside 13 for the sums of its 50160 rows.
+constexpr int kFixWaves = 16, kFew = 16;
 template <int DT, int VEC>
 __global__ __launch_bounds__(64 * kFixWaves) void fixup_kernel(Sums a, void* __restrict__ dw_, int chunks) {
     using T = typename Row<DT>::T;
-    constexpr int U = 8;
+    constexpr int U = 16;
     const int part_of = blockIdx.x / a.slabs, slab = blockIdx.x - part_of * a.slabs;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = (slab * 64 + lane) * VEC;
@@ -450,26 +452,33 @@ __global__ __launch_bounds__(64 * kFixWaves) void fixup_kernel(Sums a, void* __r
     __shared__ int ends[kFixWaves];  // the last chunk of a wave's run, for the block to join
     __shared__ uint32_t tokens[kFixWaves];
     __shared__ float join[kFixWaves][64 * VEC];
+    auto sums_of = [&](float* v, int chunk, int which) {
+        const float* at = part + ((size_t)chunk * 2 + which) * a.ld;
+        if constexpr (VEC == 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = x[e];
+        } else {
+            v[0] = *at;
+        }
+    };
     // The sums of chunks j, j + step, ... up to last.
     auto sum = [&](float* acc, int j, int last, int step) {
         for (; j <= last; j += step * U) {
             float v[U][VEC];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int k = j + u * step;
+            for (int u = 0; u < U; ++u) sums_of(v[u], min(j + u * step, last), 0);  // (all under way, whether they count or not)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[u][e] = k <= last ? part[(size_t)k * 2 * a.ld + e] : 0.f;
-            }
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[u][e] = j + u * step <= last ? v[u][e] : 0.f;
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) acc[e] += v[u][e];
         }
     };
-    auto own = [&](float* acc, int c) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] = part[((size_t)c * 2 + 1) * a.ld + e];
-    };
+    auto own = [&](float* acc, int c) { sums_of(acc, c, 1); };
     auto store = [&](const float* acc, uint32_t token) {
         if (mine) store_vec<DT, VEC>(dw + (size_t)token * a.N + col, acc, a.scale);
     };
