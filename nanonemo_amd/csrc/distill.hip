@@ -338,11 +338,8 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
         }
     };
     auto add = [](auto a, auto b) { return a + b; };
-    auto sync = [] {
-        if constexpr (TB > 64) __syncthreads();
-    };
     if (tid == 0) sh.count = 0, sh.special = 0, sh.full = 0;
-    sync();
+    __syncthreads();
 
     // 1. The parts: four threads' values, a thread's, a group's, or (one wave) every value. Of 256 parts, 64 leave 74
     // candidates; of 1024, 512 leave 710.
@@ -398,7 +395,7 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
                     sh.bins[n * TB + tid] = m;
                 }
         }
-        sync();
+        __syncthreads();
         if (tid < 64) {
             auto search = [&](auto p) {
                 constexpr int P = decltype(p)::value;
@@ -417,7 +414,7 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
             }
             if (tid == 0) sh.bound = sh.special ? 0 : least == O::kZero ? O::kMinusZero : least;
         }
-        sync();
+        __syncthreads();
         least = sh.bound;
     }
 
@@ -446,6 +443,7 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
                     }
                 }
             }
+            __syncthreads();
         } else {
             int on_list = 0;
             auto sweep = [&](u32x4 v, uint32_t m, int i) {
@@ -479,7 +477,9 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
                 if (lane == 0) sh.full = 1;
                 on_list = S::kList;
             }
-            for (int t = lane; t < on_list * R::W; t += 64) {  // the wave's own list: no other's is read
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the wave's own list: no other's is read)
+            __builtin_amdgcn_wave_barrier();
+            for (int t = lane; t < on_list * R::W; t += 64) {
                 const int g = t / R::W;
                 const T x = reinterpret_cast<const T*>(sh.list[wave])[t];
                 if (O::of(bits_of(x)) >= least) {
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
                     s += e_of(x);
                 }
             }
-            sync();
+            __syncthreads();
             n = sh.full ? S::kCandidates + 1 : sh.count;
         }
         quick = n <= S::kCandidates;
@@ -512,14 +512,14 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
             const int t = place | (1 << b);
             if (counted([&](uint32_t key, int j) { return key == key_k && j < t; }) < need) place = t;
         }
-        sync();
+        __syncthreads();
         if (tid == 0) sh.count = 0;
-        sync();
+        __syncthreads();
         each([&](T x, int j) {
             const uint32_t key = K::of(x);
             if (key > key_k || (key == key_k && j <= place)) sh.cand[atomicAdd(&sh.count, 1)] = ranked(key, j);
         });
-        sync();
+        __syncthreads();
         n = k;
     }
     // 3. Every wave holds all candidates, and ranks every kWaves-th one: a comparison with all of them is one instruction a 64, and

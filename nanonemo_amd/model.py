@@ -363,6 +363,8 @@ class NanoNemo(nn.Module):
         return logits, loss
 
     def _distill(self, h: torch.Tensor, teacher: Teacher, targets: torch.Tensor | None):
+        if targets is None and teacher.weight < 1.0:
+            raise ValueError("a teacher's weight below 1 needs targets, whose cross entropy is the rest of the loss")
         if not self.cfg.any_hip or not h.is_cuda:
             logits = self.lm_head(h)
             return logits, distill_loss(logits, teacher, targets)

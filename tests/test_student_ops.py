@@ -232,5 +232,8 @@ def test_plain_distillation_of_a_model():
     torch.testing.assert_close(loss, 0.25 * 4 * kl + 0.75 * F.cross_entropy(logits.view(-1, 96), y.view(-1)))
     whole = Teacher(full, torch.arange(96).expand(2, 16, 96), None, 2.0, 1.0)
     torch.testing.assert_close(distill_loss(logits, whole, None), 4 * (p.exp() * (p - q)).sum(-1).mean())
+    with pytest.raises(ValueError, match="needs targets"):
+        student(idx, None, t)
+    assert student(idx, None, t._replace(weight=1.0))[1].isfinite()
     loss, norm = train_step(student, make_optimizer(student), [batch], amp_dtype=None)
     assert loss.isfinite() and norm > 0
