@@ -84,8 +84,8 @@ def run(attn: str, steps: int, batch: int, seq: int, cfg_kwargs: dict, device: s
         distinct: int = 0):
     """Train ``steps`` steps from the seed-0 init on the seed-0 synthetic stream; returns the per-step
     losses and the tokens/s over the steps after ``warmup``. ``attn`` is an attn_kernel, optionally
-    with "+rope" (rope_kernel="hip"), "+qrope" (rope_kernel="fused": q's RoPE inside the attention op)
-    and "+norm" (norm_kernel="hip") suffixes. ``distinct`` > 0 cycles through that many seed-0 batches instead of a
+    with "+rope" (rope_kernel="hip"), "+qrope" (rope_kernel="fused": q's RoPE inside the attention op),
+    "+norm" (norm_kernel="hip") and "+emb" (emb_kernel="hip") suffixes. ``distinct`` > 0 cycles through that many seed-0 batches instead of a
     fresh batch per step: a stream the model can memorise, so that the loss falls and the curves have something to
     track (on uniform fresh tokens the loss stays near ln(vocab))."""
     torch.manual_seed(0)
@@ -93,12 +93,13 @@ def run(attn: str, steps: int, batch: int, seq: int, cfg_kwargs: dict, device: s
     if backend:
         cfg_kwargs = {**cfg_kwargs, "attn_backend": backend}
     kernel, *extras = attn.split("+")
-    unknown = set(extras) - {"rope", "qrope", "norm"}
+    unknown = set(extras) - {"rope", "qrope", "norm", "emb"}
     if unknown:
         raise ValueError(f"unknown kernel suffixes {sorted(unknown)}")
     rope = "fused" if "qrope" in extras else "hip" if "rope" in extras else "torch"
     model = NanoNemo(ModelConfig(**cfg_kwargs, attn_kernel=kernel, rope_kernel=rope,
-                                 norm_kernel="hip" if "norm" in extras else "torch")).to(device)
+                                 norm_kernel="hip" if "norm" in extras else "torch",
+                                 emb_kernel="hip" if "emb" in extras else "torch")).to(device)
     opt = make_optimizer(model)
     data = synthetic_batches(distinct or steps, batch, seq, model.cfg.vocab_size, device)
     data = [data[i % len(data)] for i in range(steps)]
@@ -123,8 +124,8 @@ def main():
     p.add_argument("--seq", type=int, default=1024)
     p.add_argument("--attn", nargs="+",
                    default=["torch", "hip", "hip_bthd", "hip_bthd+rope", "hip_bthd+rope+norm", "hip_bthd+qrope+norm"],
-                   help="attention kernels; '+rope' / '+qrope' / '+norm' suffixes also select the HIP RoPE (separate / "
-                   "q folded into the attention) and add+RMSNorm kernels; 'torch@<backend>' runs the plain attention "
+                   help="attention kernels; '+rope' / '+qrope' / '+norm' / '+emb' suffixes also select the HIP RoPE (separate / "
+                   "q folded into the attention), add+RMSNorm and embedding kernels; 'torch@<backend>' runs the plain attention "
                    "on another SDPA backend (a control for the drift between two valid attentions)")
     p.add_argument("--small", action="store_true", help="a 2-layer model (quick check)")
     p.add_argument("--distinct", type=int, default=0,
