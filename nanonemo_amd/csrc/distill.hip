@@ -207,44 +207,31 @@ __device__ inline double ranked(uint32_t key, int j) { return fma((double)key, (
 __device__ inline uint32_t key_in(double r) { return (uint32_t)(r * (1.0 / (1 << kVocabBits))); }
 __device__ inline int place_in(double r) { return (1 << kVocabBits) - 1 - (int)(r - (double)key_in(r) * (double)(1 << kVocabBits)); }
 
-// Largest values as whole numbers, for a group of 16 bytes at a time: like Key, but -0 below 0 and NaN by its sign. `mag` is the
-// largest value without its sign, which shows a NaN.
+// Largest values as whole numbers, for a group of 16 bytes at a time: like Key, but -0 below 0 and a NaN by its sign (the largest
+// value shows one without it; one with it makes the sum of exponentials NaN).
 template <int DT>
 struct Order {
     using K = Key<DT>;
     static __device__ uint32_t of(uint32_t u) { return u & K::kSign ? u ^ K::kAll : u | K::kSign; }
     static __device__ typename K::T value(uint32_t order) { return K::value(order); }  // (the same for both orders)
-    static constexpr uint32_t kZero = K::kSign, kMinusZero = kZero - 1, kMinusInf = K::kAll ^ (K::kSign | K::kInf);
-    static __device__ uint32_t most(u32x4 raw, uint32_t& mag) {
+    static constexpr uint32_t kZero = K::kSign, kMinusZero = kZero - 1, kMinusInf = K::kAll ^ (K::kSign | K::kInf), kPlusInf = K::kSign | K::kInf;
+    // As signed whole numbers, values that are not negative have the order of floats and negative ones its reverse: the largest
+    // value is the largest of them, or the least where all are negative.
+    static __device__ uint32_t most(u32x4 raw) {
+        int hi, lo;
         if constexpr (DT == kF32) {
-            int m = INT32_MIN;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const int x = (int)raw[w];
-                m = max(m, x ^ ((x >> 31) & 0x7fffffff));
-                mag = max(mag, raw[w] & 0x7fffffffu);
-            }
-            return (uint32_t)m ^ K::kSign;
+            hi = max(max((int)raw[0], (int)raw[1]), max((int)raw[2], (int)raw[3]));
+            lo = min(min((int)raw[0], (int)raw[1]), min((int)raw[2], (int)raw[3]));
         } else {
             typedef short s16x2 __attribute__((ext_vector_type(2)));
-            typedef u16 u16x2 __attribute__((ext_vector_type(2)));
-            s16x2 m = {INT16_MIN, INT16_MIN};
-            u16x2 g = __builtin_bit_cast(u16x2, mag);
+            s16x2 x[4];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const s16x2 x = __builtin_bit_cast(s16x2, (uint32_t)raw[w]);
-                m = __builtin_elementwise_max(m, x ^ ((x >> 15) & (short)0x7fff));
-                g = __builtin_elementwise_max(g, __builtin_bit_cast(u16x2, (uint32_t)raw[w] & 0x7fff7fffu));
-            }
-            mag = __builtin_bit_cast(uint32_t, g);
-            return (uint32_t)(max((int)m[0], (int)m[1]) + 0x8000);
+            for (int w = 0; w < 4; ++w) x[w] = __builtin_bit_cast(s16x2, (uint32_t)raw[w]);
+            const s16x2 h = __builtin_elementwise_max(__builtin_elementwise_max(x[0], x[1]), __builtin_elementwise_max(x[2], x[3]));
+            const s16x2 l = __builtin_elementwise_min(__builtin_elementwise_min(x[0], x[1]), __builtin_elementwise_min(x[2], x[3]));
+            hi = max((int)h[0], (int)h[1]), lo = min((int)l[0], (int)l[1]);
         }
-    }
-    static __device__ bool nan(uint32_t mag) {
-        if constexpr (DT == kF32)
-            return mag > K::kInf;
-        else
-            return (mag & 0xffffu) > K::kInf || (mag >> 16) > K::kInf;
+        return of((uint32_t)(hi >= 0 ? hi : lo) & K::kAll);
     }
 };
 
@@ -292,9 +279,10 @@ struct TopShared {
 //      there once); the exponentials of all others are summed.
 //   3  A candidate's rank is the number of larger ones; those behind the k join the sum.
 //
-// Measured at 8192 x 50304 bf16, k = 64: 200 us (4.1 TB/s), three rows to a CU at 80 registers, where a row's search and
-// ranking hide behind the others' loads; with the row read again for every step it took 700 us, with 1024 threads of 64
-// registers (7 groups each, 27 of them spilled) 390. A single row takes 11 us, most of it the steps' latency.
+// Measured at 8192 x 50304 bf16, k = 64: 161 us (5.1 TB/s), three rows to a CU at 80 registers, where a row's search and
+// ranking hide behind the others' loads. With the row read again for every step it took 700 us, with 1024 threads of 64
+// registers (7 groups each, 27 of them spilled) 390, and 180 where a part's largest value took four instructions a pair of
+// values and NaN another two. A single row takes 10 us, most of it the steps' latency.
 // Rows for which the above does not do (many equal values, NaN, a k near the number of parts) take a search of the k-th value bit
 // by bit instead, and rows whose others lie far below the bound a sum relative to their own largest.
 template <int DT, int TB, int NV>
@@ -343,7 +331,7 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
 
     // 1. The parts: four threads' values, a thread's, a group's, or (one wave) every value. Of 256 parts, 64 leave 74
     // candidates; of 1024, 512 leave 710.
-    uint32_t mag = 0, mine = 0, least = 0;
+    uint32_t mine = 0, least = 0;
     if constexpr (NV > 0) {
 #pragma unroll
         for (int n = 0; n < NV; ++n) raw[n] = TB == 64 && V < R::W ? group<DT>(row, 0, tid + n ? 0 : V) : group_at<DT>(row, tid + n * TB, V);
@@ -352,9 +340,9 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
             for (int n = 0; n < NV; ++n) own<DT>(raw[n], tid + n * TB, V);
         }
 #pragma unroll
-        for (int n = 0; n < NV; ++n) mine = max(mine, most[n] = O::most(raw[n], mag));
+        for (int n = 0; n < NV; ++n) mine = max(mine, most[n] = O::most(raw[n]));
     } else {
-        for (int i = tid; i < groups; i += TB) mine = max(mine, O::most(one_group(i), mag));
+        for (int i = tid; i < groups; i += TB) mine = max(mine, O::most(one_group(i)));
     }
     if constexpr (TB == 64) {
         if (2 * k <= groups) {
@@ -370,10 +358,10 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
             }
             least = reached<K::kBits>(v, k);
         }
-        if (__ballot(O::nan(mag))) least = 0;
+        if (__ballot(mine > O::kPlusInf)) least = 0;
         if (least == O::kZero) least = O::kMinusZero;  // (they are equal)
     } else {
-        if (O::nan(mag)) sh.special = 1;
+        if (mine > O::kPlusInf) sh.special = 1;
         int parts = 0;
         if (4 * k <= TB / 4) {
             mine = max(mine, (uint32_t)__shfl_xor((int)mine, 1));
@@ -443,6 +431,7 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
                     }
                 }
             }
+            if (__ballot(s != s)) n = S::kCandidates + 1;  // (a NaN)
             __syncthreads();
         } else {
             int on_list = 0;
@@ -467,9 +456,8 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
                 for (int m = 0; m < NV; ++m) sweep(raw[m], most[m], tid + m * TB);
             } else {
                 for (int i = tid; i < groups; i += TB) {
-                    uint32_t none = 0;
                     const u32x4 v = one_group(i);
-                    sweep(v, O::most(v, none), i);
+                    sweep(v, O::most(v), i);
                 }
             }
             on_list = __builtin_amdgcn_readfirstlane(on_list);  // (the first lane has seen every group of the wave)
@@ -477,6 +465,7 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
                 if (lane == 0) sh.full = 1;
                 on_list = S::kList;
             }
+            if (s != s) sh.full = 1;  // (a NaN)
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the wave's own list: no other's is read)
             __builtin_amdgcn_wave_barrier();
             for (int t = lane; t < on_list * R::W; t += 64) {
@@ -487,6 +476,7 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
                     if (p < S::kCandidates) sh.cand[p] = ranked(K::of(x), begin_of(sh.list_at[wave][g]) + t % R::W);
                 } else {
                     s += e_of(x);
+                    if (s != s) sh.full = 1;
                 }
             }
             __syncthreads();
