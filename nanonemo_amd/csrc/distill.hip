@@ -720,6 +720,7 @@ __global__ __launch_bounds__(TB, 8) void loss_fwd_kernel(Loss x) {
         }
         top = block_sum<TB>(top, tmp.d4);
         if (tid == 0) top_sums = top, t_most = tmax;
+        if constexpr (TB == 64) __syncthreads();  // (else the row's sums have one)
     }
 
     // The row without what is marked. Exponents are in powers of two relative to 2^b, the whole number b next to the exponent of
@@ -808,8 +809,9 @@ __global__ __launch_bounds__(TB, 8) void loss_fwd_kernel(Loss x) {
     if (tid != 0) return;
     double P = top.p;
     if (!(w == 0.0)) P += w * (rest - Lr);
-    const float own = (float)(Ls * x.tau);
-    st[kL] = L, st[kL1] = L1, st[kLt] = Lt, st[kLr] = Lr, st[kPr] = w / A, st[kBase] = fabsf(own) < INFINITY ? own : 0.f, st[kTwice] = twice;
+    // (no others: the target's, or the top set's, so that the factors of exponentials that are 0 stay finite)
+    const float own = (float)(Ls * x.tau), no_own = alone && fabsf(z_target) < INFINITY ? z_target : (float)base;
+    st[kL] = L, st[kL1] = L1, st[kLt] = Lt, st[kLr] = Lr, st[kPr] = w / A, st[kBase] = fabsf(own) < INFINITY ? own : no_own, st[kTwice] = twice;
     double v = 0.0;
     if (zmax == INFINITY) v = st[kL] = NAN;  // (inf - inf again)
     if (x.weight > 0.0) v += x.weight * x.tau * x.tau * (P / A - Lt + L);

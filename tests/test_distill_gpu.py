@@ -232,6 +232,28 @@ def test_a_student_whose_top_set_stands_far_above_or_below_the_rest(V):
     _check_loss(low, v, idx, torch.full_like(rest, -INF), None, 1.0, 1.0, "lowest, nothing in the rest")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [300, 5000])
+def test_a_masked_vocabulary_at_any_level(V, dtype):
+    # All but the top set at -inf, and what is left far below (or above) 0: the gradient of the rest is 0, not 0 times e^100.
+    z, v, idx, rest, y = _case((6,), V, 9, torch.float32, 0.5, _gen(29))
+    y = idx[..., 3].clone()
+    other = next(j for j in range(V) if not (idx == j).any())
+    for level in (-300.0, 300.0):
+        gone = torch.full_like(z, -INF).scatter(-1, idx, z.gather(-1, idx) + level).to(dtype)
+        for tau in (0.5, 1.0, 2.0):
+            for t, w in ((None, 1.0), (y, 0.5), (y, 0.0)):
+                print(f"\n[case] masked V={V} {dtype} level={level} tau={tau} weight={w}", flush=True)
+                _check_loss(gone, v, idx, None, t, tau, w, ("gone", level, tau, w))
+        # the target as the only one of the rest, near the top set or far below it
+        for below in (2.0, 150.0):
+            alone = gone.clone()
+            alone[..., other] = level - below
+            for r in (None, rest):
+                print(f"\n[case] masked but the target V={V} {dtype} level={level} below={below} rest={r is not None}", flush=True)
+                _check_loss(alone, v, idx, r, torch.full_like(y, other), 0.5, 0.5, ("alone", level, below, r is not None))
+
+
 def test_strided_logits_and_teachers():
     g = _gen(6)
     z, v, idx, rest, y = _case((3, 6), 1003, 9, torch.bfloat16, 2.0, g)
