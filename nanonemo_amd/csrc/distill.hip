@@ -809,8 +809,11 @@ __global__ __launch_bounds__(TB, 8) void loss_fwd_kernel(Loss x) {
     if (tid != 0) return;
     double P = top.p;
     if (!(w == 0.0)) P += w * (rest - Lr);
-    // (no others: the target's, or the top set's, so that the factors of exponentials that are 0 stay finite)
-    const float own = (float)(Ls * x.tau), no_own = alone && fabsf(z_target) < INFINITY ? z_target : (float)base;
+    // The gradient's exponentials, at both temperatures, are relative to one logit, which has to lie near the others' largest: for
+    // temperatures above 1 their logsumexp at 1, below 1 the one at tau times tau (the lower one: the other lies up to tau ln V,
+    // or ln V, above, past fp32's exponents for a tau of 9). (No others: the target's, or the top set's, so that the factors of
+    // exponentials that are 0 stay finite.)
+    const float own = (float)(BOTH ? fmin(Ls * x.tau, Ls1) : Ls * x.tau), no_own = alone && fabsf(z_target) < INFINITY ? z_target : (float)base;
     st[kL] = L, st[kL1] = L1, st[kLt] = Lt, st[kLr] = Lr, st[kPr] = w / A, st[kBase] = fabsf(own) < INFINITY ? own : no_own, st[kTwice] = twice;
     double v = 0.0;
     if (zmax == INFINITY) v = st[kL] = NAN;  // (inf - inf again)

@@ -531,3 +531,53 @@ def test_refusals():
     ):
         with pytest.raises(error, match=msg):
             call()
+
+
+# ---- the whole range of temperatures ------------------------------------------------------------
+
+
+def _check_loss_at(z, v, idx, rest, y, tau, w, what):
+    """_check_loss with the rounding of fp64 added, which tau^2 makes count: the logsumexps, of terms up to `most` in size, are
+    sums of k values and of at most 256 + 16 partial ones, on either side."""
+    from nanonemo_amd.kernels.hip.distill import distill_loss
+
+    z = z.detach().requires_grad_()
+    loss = distill_loss(z, v, idx, rest, y, tau, w)
+    (d,) = torch.autograd.grad(loss, z)
+    rl, rd, loss_off, off = _reference(z, v, idx, rest, y, tau, w)
+    most = 13 + max(t.abs().max().item() for t in (z.detach().double() / tau, v.double() / tau))
+    loss_off = loss_off + w * tau**2 * 2 * (v.shape[-1] + 272) * 2.0**-53 * most
+    assert abs(loss.item() - rl.item()) <= loss_off.item(), what
+    assert d.isfinite().all(), what
+    worst = ((d.double() - rd).abs() / off).max().item()
+    assert worst <= 1.0, (what, worst)
+
+
+@pytest.mark.parametrize("tau", [1e-4, 0.01, 0.05, 2.0, 3.0, 4.0, 8.0, 9.0, 10.0, 20.0, 100.0, 1e4])
+@pytest.mark.parametrize("rows, V, k, dtype", [((1,), 512, 9, torch.float32), ((300,), 1003, 7, torch.float32), ((1,), 50304, 64, torch.float32), ((260,), 50304, 64, torch.bfloat16),
+                                               ((2,), 393216, 100, torch.float32)])
+def test_distill_loss_over_the_range_of_temperatures(rows, V, k, dtype, tau):
+    # The logsumexp of z / tau times tau lies up to tau ln V above the logits, their softmax at temperature 1 does not.
+    z, v, idx, rest, y = _case(rows, V, k, dtype, tau, _gen(V + k))
+    if y.numel() > 2:
+        y.view(-1)[1] = -100
+    for r, t, w in ((rest, y, 0.5), (rest, y, 0.0), (None, y, 0.9), (rest, None, 1.0), (None, None, 1.0)):
+        print(f"\n[case] distill rows={rows} V={V} k={k} {dtype} tau={tau} rest={r is not None} targets={t is not None} weight={w}", flush=True)
+        _check_loss_at(z, v, idx, r, t, tau, w, (r is not None, t is not None, w))
+
+
+@pytest.mark.parametrize("tau", [2.0, 4.0, 20.0])
+def test_the_cross_entropys_gradient_of_logits_far_below(tau):
+    # Probabilities down to 1e-30, of the cross entropy alone.
+    z, v, idx, _, y = _case((5,), 3001, 9, torch.float32, tau, _gen(31))
+    z[:, 100:200] -= 60.0
+    _check_loss_at(z, v, idx, None, y, tau, 0.0, tau)
+
+
+@pytest.mark.parametrize("tau", [1e-4, 0.01, 8.0, 100.0, 1e4])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [64, 1003, 5000, 50304, 140001])
+def test_top_logits_over_the_range_of_temperatures(V, dtype, tau):
+    print(f"\n[case] top logits V={V} {dtype} tau={tau}", flush=True)
+    for k in (1, 33):
+        _check_top(_logits("normal", (3,), V, dtype, _gen(V + k)), k, tau, k)
