@@ -781,7 +781,9 @@ __global__ __launch_bounds__(TB, 8) void loss_fwd_kernel(Loss x) {
     if (tid >= 64) return;
     const Sums4 top = top_sums;
     const float z_target = zt, zmax = fmaxf(near, z_target);
-    const double base = base_of(zmax), at = base * inv_tau, z_soft = z_target * inv_tau;
+    const double base = base_of(zmax), z_soft = z_target * inv_tau;
+    // (-inf where all of these are: the others' sum alone says then what the joined ones are relative to)
+    const double at1 = zmax == -INFINITY ? -INFINITY : base, at = at1 * inv_tau;
     tmax = t_most;
 
     // All that is joined: logarithms and exponentials one a lane, since each takes as long as 64 of them.
@@ -789,14 +791,14 @@ __global__ __launch_bounds__(TB, 8) void loss_fwd_kernel(Loss x) {
     const double rest = x.rest ? (double)x.rest[r] : -INFINITY, ls = log((double)(tid == 0 ? s : s1));
     const double Ls = s == 0.f ? -INFINITY : from + lane_of(ls, 0), Ls1 = s == 0.f ? -INFINITY : from1 + lane_of(ls, 1);
     const bool alone = hard && !target_in_top;  // (then the target is one of the others, but not in their sum)
-    const double to = fmax(at, Ls), to1 = fmax(base, Ls1), to_r = alone ? fmax(Ls, z_soft) : Ls;
+    const double to = fmax(at, Ls), to1 = fmax(at1, Ls1), to_r = alone ? fmax(Ls, z_soft) : Ls;
     const double arg = tid == 0   ? Ls - to
                        : tid == 1 ? Ls1 - to1
                        : tid == 2 ? z_soft - to
                        : tid == 3 ? z_target - to1
                        : tid == 4 ? rest - tmax
                        : tid == 5 ? at - to
-                       : tid == 6 ? base - to1
+                       : tid == 6 ? at1 - to1
                        : tid == 7 ? Ls - to_r
                                   : z_soft - to_r;
     const double ex = exp(arg);

@@ -581,3 +581,26 @@ def test_top_logits_over_the_range_of_temperatures(V, dtype, tau):
     print(f"\n[case] top logits V={V} {dtype} tau={tau}", flush=True)
     for k in (1, 33):
         _check_top(_logits("normal", (3,), V, dtype, _gen(V + k)), k, tau, k)
+
+
+@pytest.mark.parametrize("V", [300, 5000])
+def test_a_masked_top_set_at_any_level(V):
+    # The top set at -inf, the others far below (or above) 0. A teacher with mass in the top set makes the loss infinite, one
+    # with all its mass in the rest does not.
+    z, v, idx, rest, y = _case((6,), V, 9, torch.float32, 1.0, _gen(37))
+    y = torch.full_like(y, next(j for j in range(V) if not (idx == j).any()))
+    for level in (-3000.0, -800.0, -300.0, 300.0):
+        gone = (z + level).scatter(-1, idx, -INF)
+        for tau in (0.5, 1.0, 2.0, 3.0):
+            for values, r, t, w in ((v, rest, None, 1.0), (v, None, y, 0.5), (torch.full_like(v, -INF), rest, None, 1.0), (torch.full_like(v, -INF), rest, y, 0.5), (v, None, y, 0.0)):
+                what = (level, tau, bool(values[0, 0] == -INF), r is not None, w)
+                print(f"\n[case] masked top set V={V} {what}", flush=True)
+                from nanonemo_amd.kernels.hip.distill import distill_loss
+
+                x = gone.clone().requires_grad_()
+                loss = distill_loss(x, values, idx, r, t, tau, w)
+                (d,) = torch.autograd.grad(loss, x)
+                rl, rd, loss_off, off = _reference(x, values, idx, r, t, tau, w)
+                assert rl.isfinite() == bool(w == 0 or values[0, 0] == -INF), what
+                assert loss.item() == rl.item() or abs(loss.item() - rl.item()) <= loss_off.item(), what
+                assert ((d.double() - rd).abs() <= off).all(), what
