@@ -128,6 +128,10 @@ __device__ inline float exp_diff(float x, float m, float c) { return __builtin_a
 // What exponents are relative to: 0 where every value is -inf (their exp is 0 then) or one is +inf (infinite then).
 __device__ inline float base_of(float m) { return fabsf(m) == INFINITY ? 0.f : m; }
 
+// Whether a sum of exponentials relative to a value of the caller's choice can stand: those below 2^-126 count as 0, of up to
+// kMaxVocab of them 5e-33 in all, which has to be nothing beside the sum (5e-8 at 1e-25; of 1e-30 it was 0.5 %).
+__device__ inline bool stands(float s) { return s > 1e-25f && s < 1e30f; }
+
 // The factor that takes a sum relative to base_of(m) to another base; 0 for the empty sum, whose m is -inf.
 __device__ inline float rebase(float m, float base, float c) { return exp_diff(m == INFINITY ? 0.f : m, base, c); }
 
@@ -560,7 +564,7 @@ __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(
         if constexpr (TB > 64)
             for (int i = tid; i < n - k; i += TB) s += sh.below[i];
         s = block_all<TB>(s, sh.tmpf, add);
-        if (s > 1e-30f && s < 1e30f) {
+        if (stands(s)) {
             // (c is log2(e) / tau rounded: what that puts on the exponents near the bound comes off again)
             const double ln2 = 0.6931471805599453, off = v_b * (inv_tau / ln2 - (double)c);
             if (tid == 0) rest[blockIdx.x] = (float)(ln2 * ((double)b + off + log2((double)s)));
@@ -762,7 +766,7 @@ __global__ __launch_bounds__(TB, 8) void loss_fwd_kernel(Loss x) {
     // The sums times e^from (c is log2(e) / tau rounded: what that puts on the exponents near b comes off again).
     const double off = near * (inv_tau - (double)x.c * ln2);
     double from = ln2 * b + off, from1 = S2 == kOwn ? ln2 * b1 + near * (1.0 - (double)kL2e * ln2) : ln2 * b1 + off * x.tau;
-    if (!(s > 1e-30f && s < 1e30f && (!BOTH || (s1 > 1e-30f && s1 < 1e30f)))) {
+    if (!(stands(s) && (!BOTH || stands(s1)))) {
         // Far from the top set's: relative to their own largest.
         MaxSum a{-INFINITY, 0.f, 0.f};
         for (int i = tid; i < groups; i += TB) {

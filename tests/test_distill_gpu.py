@@ -604,3 +604,19 @@ def test_a_masked_top_set_at_any_level(V):
                 assert rl.isfinite() == bool(w == 0 or values[0, 0] == -INF), what
                 assert loss.item() == rl.item() or abs(loss.item() - rl.item()) <= loss_off.item(), what
                 assert ((d.double() - rd).abs() <= off).all(), what
+
+
+@pytest.mark.parametrize("V", [131072, 393216])
+def test_a_rest_of_one_logit_and_very_many_below_fp32s_exponents(V):
+    # e^-66.5 and some hundred thousand times e^-88, which fp32's normal numbers do not reach: 4e-5 to 2e-4 of the rest.
+    z = torch.full((2, V), -88.0, device="cuda")
+    z[:, 5:13] = torch.linspace(0.0, 1.0, 8, device="cuda")
+    z[:, 77] = -66.5
+    _check_top(z, 8, 1.0, V)
+    _check_top(4 * z, 8, 4.0, V)
+    idx = torch.arange(5, 13, device="cuda").expand(2, 8).contiguous()
+    v, y = z.gather(-1, idx), torch.full((2,), 5, device="cuda")
+    for tau in (1.0, 2.0, 4.0, 3.0):
+        for t, w in ((None, 1.0), (y, 0.5)):
+            print(f"\n[case] a rest of one logit V={V} tau={tau} weight={w}", flush=True)
+            _check_loss(tau * z, tau * v, idx, torch.ones(2, device="cuda"), t, tau, w, (tau, w))
