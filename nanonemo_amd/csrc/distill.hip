@@ -874,7 +874,9 @@ __global__ __launch_bounds__(TB, 8) void loss_bwd_kernel(Loss x, const float* __
     const bool hard = x.hard(), soft = x.weight > 0.0;
     const T* row = reinterpret_cast<const T*>(x.logits) + x.at.at(r);
     const double* st = x.stats + (size_t)r * kStats;
-    const double inv_tau = 1.0 / x.tau, L = st[kL], L1 = st[kL1], Lr = st[kLr], p_rest = st[kPr], base = st[kBase];
+    const double inv_tau = 1.0 / x.tau, L = st[kL], L1 = st[kL1], Lr = st[kLr], base = st[kBase];
+    // (where the student's rest is empty, its loss infinite, no logit has a share of the teacher's)
+    const double p_rest = Lr == -INFINITY && st[kPr] > 0.0 ? 0.0 : st[kPr];
     const double g = (double)grad[0] * x.stats[(size_t)gridDim.x * (kStats + 1)], gs = soft ? x.weight * x.tau * g : 0.0, gh = hard ? (1.0 - x.weight) * g : 0.0;
     // q_j f_j of a logit outside the top set, which is q_j - p_rest times its share of the rest.
     auto outside = [&](double z) {

@@ -620,3 +620,25 @@ def test_a_rest_of_one_logit_and_very_many_below_fp32s_exponents(V):
         for t, w in ((None, 1.0), (y, 0.5)):
             print(f"\n[case] a rest of one logit V={V} tau={tau} weight={w}", flush=True)
             _check_loss(tau * z, tau * v, idx, torch.ones(2, device="cuda"), t, tau, w, (tau, w))
+
+
+@pytest.mark.parametrize("V", [300, 5000])
+@pytest.mark.parametrize("tau", [1.0, 2.0, 5.0])
+def test_a_teachers_rest_where_the_student_has_none(V, tau):
+    # Infinite divergence; the gradient is that of the top set's terms, and 0 where nothing is left.
+    from nanonemo_amd.kernels.hip.distill import distill_loss
+
+    z, v, idx, rest, y = _case((6,), V, 9, torch.float32, tau, _gen(41))
+    x = torch.full_like(z, -INF).scatter(-1, idx, z.gather(-1, idx))
+    p = torch.softmax(torch.cat((v.double() / tau, rest.double().unsqueeze(-1)), -1), -1)[:, :-1]
+    on = x.double().gather(-1, idx)
+    for t, w in ((None, 1.0), (idx[:, 3].clone(), 0.5)):
+        x = x.detach().requires_grad_()
+        loss = distill_loss(x, v, idx, rest, t, tau, w)
+        (d,) = torch.autograd.grad(loss, x)
+        ref = w * tau * (torch.softmax(on / tau, -1) - p)
+        if t is not None:
+            ref = ref + (1 - w) * (torch.softmax(on, -1) - (idx == t.unsqueeze(-1)).double())
+        assert loss == INF and (d.scatter(-1, idx, 0.0) == 0).all()
+        # (fp64 throughout, rounded once)
+        assert ((d.gather(-1, idx).double() - ref / 6).abs() <= 2**-24 * (ref / 6).abs() + 1e-14).all()
