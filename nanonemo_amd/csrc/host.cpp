@@ -71,9 +71,10 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_de
 int code(at::ScalarType t) { return t == at::kHalf ? 0 : t == at::kBFloat16 ? 1 : t == at::kFloat ? 2 : -1; }
 int code(const Tensor& t) { return code(t.scalar_type()); }
 
-// The tensor's values at its address: a gradient may come as a lazy negation of what lies there.
-Tensor real_values(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
-Tensor contig(const Tensor& t) { return t.is_contiguous() && !t.is_neg() ? t : real_values(t).contiguous(); }
+// The tensor's values at its address: a gradient may come as a lazy negation of what lies there, or as zeros without memory.
+bool lazy(const Tensor& t) { return t.is_neg() || t._is_zerotensor(); }
+Tensor real_values(const Tensor& t) { return t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.is_neg() ? t.resolve_neg() : t; }
+Tensor contig(const Tensor& t) { return t.is_contiguous() && !lazy(t) ? t : real_values(t).contiguous(); }
 Tensor empty_of(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options()); }
 Tensor empty_f32(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
 Tensor bytes(const Tensor& like, size_t n) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
@@ -803,7 +804,12 @@ void refuse_capture(const char* where) {
 }
 bool records(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 bool ordinary(const Tensor& t);
-void need_ordinary(const Tensor& grad) { need(ordinary(grad), "batched gradients (is_grads_batched) are not supported: the kernels read gradients by address"); }
+// A gradient as the kernels can read it.
+Tensor readable_grad(const Tensor& grad) {
+    const Tensor g = lazy(grad) ? real_values(grad) : grad;
+    need(ordinary(g), "batched gradients (is_grads_batched) are not supported: the kernels read gradients by address");
+    return g;
+}
 // A gradient that cannot be differentiated again: doing so is an error, as with once_differentiable.
 Tensor once(Tensor grad, const char* where) {
     if (!at::GradMode::is_enabled()) return grad;
@@ -823,11 +829,11 @@ struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
         refuse_capture("embedding backward");
         const auto saved = ctx->get_saved_variables();
         if (!grads[0].defined()) return {{}, {}, {}, {}};
-        need_ordinary(grads[0]);
+        const Tensor dy = readable_grad(grads[0]);
         Tensor dw;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
-            dw = embedding_bwd(grads[0], saved[0], ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt());
+            dw = embedding_bwd(dy, saved[0], ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt());
         }
         return {{}, once(dw, "embedding"), {}, {}};
     }
@@ -855,12 +861,12 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
         refuse_capture("distill_loss backward");
         const auto t = ctx->get_saved_variables();
         if (!grads[0].defined()) return variable_list(7);
-        need_ordinary(grads[0]);
+        const Tensor d_loss = readable_grad(grads[0]);
         variable_list out(7);
         Tensor d;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
-            d = distill_bwd(grads[0], t[0], t[1], t[2], t[3].defined() ? OptTensor(t[3]) : std::nullopt, t[4], ctx->saved_data["temperature"].toDouble(),
+            d = distill_bwd(d_loss, t[0], t[1], t[2], t[3].defined() ? OptTensor(t[3]) : std::nullopt, t[4], ctx->saved_data["temperature"].toDouble(),
                             ctx->saved_data["weight"].toDouble());
         }
         out[0] = once(d, "distill_loss");

@@ -573,3 +573,11 @@ def test_lazy_negations_are_resolved_before_a_kernel_reads_them():
     assert t.is_neg()
     for out in (*host().readable(t), *host().readable(t, t)):
         assert not out.is_neg() and torch.equal(out, t)
+
+
+def test_zeros_without_memory_are_written_out_before_a_kernel_reads_them():
+    from nanonemo_amd.kernels.hip import host
+
+    t = torch._efficientzerotensor((1, 2, 16, 32))
+    for out in (*host().readable(t), *host().readable(t, t)):
+        assert not out._is_zerotensor() and out.data_ptr() and torch.equal(out, torch.zeros(1, 2, 16, 32))

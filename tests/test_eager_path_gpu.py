@@ -259,3 +259,36 @@ def test_lazily_negated_gradients():
             g = torch._neg_view(torch.randn_like(y))
         got = torch.autograd.grad(y, a, g, retain_graph=True)[0]
         assert torch.equal(got, torch.autograd.grad(y, a, g.resolve_neg())[0])
+
+
+def test_lazy_gradients_of_the_embedding_and_the_distillation_loss():
+    from nanonemo_amd.kernels.hip.distill import distill_loss
+    from nanonemo_amd.kernels.hip.embedding import embedding
+
+    idx = torch.randint(0, 50, (3, 7), device=DEV)
+    w = torch.randn(50, 16, device=DEV, requires_grad=True)
+    z = torch.randn(5, 50, device=DEV, requires_grad=True)
+    v, at = torch.randn(5, 50, device=DEV).topk(4)
+    for x, f in ((w, lambda: embedding(idx, w, 2.0, 3)), (z, lambda: distill_loss(z, v, at))):
+        y = f()
+        g = torch.randn(y.shape, dtype=torch.complex64, device=DEV).conj().imag
+        assert g.is_neg()
+        got = torch.autograd.grad(y, x, g, retain_graph=True)[0]
+        assert torch.equal(got, torch.autograd.grad(y, x, g.resolve_neg(), retain_graph=True)[0])
+        zeros = torch._efficientzerotensor(y.shape, device=DEV)  # (without memory)
+        assert zeros._is_zerotensor() and not torch.autograd.grad(y, x, zeros)[0].any()
+
+
+def test_gradients_that_are_zeros_without_memory():
+    import nanonemo_amd.kernels.hip.flash_attn as fa
+    from nanonemo_amd.kernels.hip import rmsnorm, rope
+    from nanonemo_amd.model import rope_tables
+
+    cos, sin = (t.to(DEV) for t in rope_tables(64, 16, 10000.0))
+    x, w = torch.randn(1, 16, 2, 64, device=DEV), torch.ones(64, device=DEV)
+    q = x.bfloat16()
+    for a, f in ((q, lambda a: fa.flash_attn(*[a.transpose(1, 2)] * 3)), (q, lambda a: fa.flash_attn_bthd(a, a, a)), (q, lambda a: fa.flash_attn_bthd_rope(a, a, a, cos, sin)),
+                 (x, lambda a: rope.rope_k(a, cos, sin)), (x, lambda a: rmsnorm.add_rms_norm(a, None, w, 1e-5)[0])):
+        a = a.clone().requires_grad_()
+        y = f(a)
+        assert not torch.autograd.grad(y, a, torch._efficientzerotensor(y.shape, dtype=y.dtype, device=DEV))[0].any()
