@@ -217,6 +217,19 @@ def refuse_capture(where: str, *inputs) -> None:
     )
 
 
+def refuse_forward_ad(where: str, *inputs) -> None:
+    """Raise where an input (None for one that is not given) carries a tangent (torch.autograd.forward_ad, torch.func.jvp):
+    the ops have no forward-mode formula, and a call that autograd does not record would return values without a tangent,
+    as if it were zero."""
+    import torch
+
+    ad = torch.autograd.forward_ad
+    if torch.compiler.is_compiling() or ad._current_level < 0:
+        return
+    if any(t is not None and ad.unpack_dual(t).tangent is not None for t in inputs):
+        raise NotImplementedError(f"{where}: forward-mode automatic differentiation is not supported")
+
+
 def strides3(b: int, h: int, t: int) -> ctypes.Array:
     """An int64[3] {batch, head, row} element-stride array for the *_strided entry points."""
     return (ctypes.c_int64 * 3)(b, h, t)

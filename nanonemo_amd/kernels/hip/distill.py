@@ -14,8 +14,8 @@ for neither term. Softmax statistics are joined in fp64, since a student near it
 
 Logits (..., V) may be strided rows (logits[:, :-1]); V up to 393216, k up to 512. An index or target that is out of range
 makes the loss and its row's gradient NaN; an index that is there twice adds up its probabilities. The loss is once
-differentiable in the logits; the teacher's side takes no gradient. Capturing a call that autograd records into a HIP graph
-is refused, as the attention's is; without autograd it captures.
+differentiable in the logits, in reverse mode (a tangent is refused); the teacher's side takes no gradient. Capturing a call
+that autograd records into a HIP graph is refused, as the attention's is; without autograd it captures.
 """
 
 from __future__ import annotations
@@ -25,7 +25,7 @@ import math
 import torch
 from torch import Tensor
 
-from nanonemo_amd.kernels.hip import eager, host, preload, records, refuse_capture
+from nanonemo_amd.kernels.hip import eager, host, preload, records, refuse_capture, refuse_forward_ad
 
 
 @torch.library.custom_op("nanonemo::top_logits", mutates_args=())
@@ -118,6 +118,7 @@ def distill_loss(
         raise ValueError("weight below 1 needs targets, whose cross entropy is the rest of the loss")
     if records(values) or rest is not None and records(rest):
         raise ValueError("the teacher's values take no gradient: detach them")
+    refuse_forward_ad("distill_loss", logits, values, rest)
     call = (logits, values, indices, rest, targets, float(temperature), float(weight))
     if eager(*(t for t in call[:5] if t is not None)):  # the same launches as the op's, as one autograd node of the host module
         return host().distill(*call)

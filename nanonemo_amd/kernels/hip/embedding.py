@@ -7,8 +7,8 @@ summed in fp32 in the order of the tokens and rounded once, whatever the weight'
 16-bit rows in 16 bits or with atomics. The model selects it with ``emb_kernel="hip"``.
 
 A token that is not in [0, V) makes its row of the output NaN and takes no part in the gradient (F.embedding ends the
-process with a device assertion). Tokens are int64 or int32. Once differentiable. Capturing a call that autograd records
-into a HIP graph is refused, as the attention's is; without autograd it captures.
+process with a device assertion). Tokens are int64 or int32. Once differentiable, in reverse mode: a tangent is refused.
+Capturing a call that autograd records into a HIP graph is refused, as the attention's is; without autograd it captures.
 """
 
 from __future__ import annotations
@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from nanonemo_amd.kernels.hip import eager, host, preload, refuse_capture
+from nanonemo_amd.kernels.hip import eager, host, preload, refuse_capture, refuse_forward_ad
 
 
 @torch.library.custom_op("nanonemo::embedding", mutates_args=())
@@ -67,6 +67,7 @@ def embedding(idx: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: int 
         padding_idx %= rows
     else:
         raise ValueError(f"padding_idx {padding_idx} is not a row of the weight ({rows} rows)")
+    refuse_forward_ad("embedding", weight)
     if eager(idx, weight):  # the same launches as the op's, as one autograd node of the host module
         return host().embedding(idx, weight, scale, padding_idx)
     refuse_capture("embedding", weight)

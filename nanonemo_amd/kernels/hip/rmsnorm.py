@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
-from nanonemo_amd.kernels.hip import eager, host, preload, records
+from nanonemo_amd.kernels.hip import eager, host, preload, records, refuse_forward_ad
 
 @torch.library.custom_op("nanonemo::cuda_add_rms_norm_fwd", mutates_args=())
 def _fwd(x: Tensor, delta: Tensor | None, weight: Tensor, eps: float, out_dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
@@ -101,6 +101,7 @@ def add_rms_norm(x: Tensor, delta: Tensor | None, weight: Tensor, eps: float) ->
     the normalized output takes the autocast dtype (the residual keeps its own)."""
     out_dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
     ins = (x, weight) if delta is None else (x, delta, weight)
+    refuse_forward_ad("add_rms_norm", *ins)
     if eager(*ins):
         if records(*ins):
             y, h = _AddRmsNormFn.apply(x, delta, weight, eps, out_dtype)

@@ -17,7 +17,7 @@ import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
-from nanonemo_amd.kernels.hip import eager, host, preload, records
+from nanonemo_amd.kernels.hip import eager, host, preload, records, refuse_forward_ad
 
 
 @torch.library.custom_op("nanonemo::rope_qk", mutates_args=())
@@ -72,6 +72,7 @@ class _RopeQkFn(torch.autograd.Function):
 
 
 def _rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> tuple[Tensor, Tensor]:
+    refuse_forward_ad("rope", q, k, cos, sin)
     if eager(q, k, cos, sin):
         if records(q, k, cos, sin):
             return _RopeQkFn.apply(q, k, cos, sin)

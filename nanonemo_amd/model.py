@@ -262,8 +262,8 @@ class Embedding(nn.Embedding):
             self.fused = embedding
 
     def forward(self, idx: torch.Tensor) -> torch.Tensor:
-        # (a module traced symbolically has no tensor here)
-        if self.fused is not None and isinstance(idx, torch.Tensor) and idx.is_cuda \
+        # (a module traced symbolically has no tensor here; PyTorch's lookup has a forward-mode formula)
+        if self.fused is not None and isinstance(idx, torch.Tensor) and idx.is_cuda and torch.autograd.forward_ad._current_level < 0 \
                 and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse:
             return self.fused(idx, self.weight, self.scale, self.padding_idx)
         x = super().forward(idx)

@@ -581,3 +581,26 @@ def test_zeros_without_memory_are_written_out_before_a_kernel_reads_them():
     t = torch._efficientzerotensor((1, 2, 16, 32))
     for out in (*host().readable(t), *host().readable(t, t)):
         assert not out._is_zerotensor() and out.data_ptr() and torch.equal(out, torch.zeros(1, 2, 16, 32))
+
+
+def test_forward_mode_differentiation_is_refused():
+    # Without it, a call that autograd does not record (nothing requires grad) would return values without a tangent.
+    from torch.autograd import forward_ad
+
+    from nanonemo_amd.kernels.hip import distill, embedding, flash_attn, rmsnorm, rope
+
+    q, cos, w = torch.randn(1, 16, 2, 32), torch.randn(16, 16), torch.ones(32)
+    idx, top = torch.zeros(3, dtype=torch.int64), torch.zeros(3, 2, dtype=torch.int64)
+    z, v, r = torch.randn(3, 8), torch.randn(3, 2), torch.randn(3)
+    calls = ((lambda t: flash_attn.flash_attn(q, q, t), q), (lambda t: flash_attn.flash_attn_bthd(t, q, q), q), (lambda t: flash_attn.flash_attn_bthd_rope(q, t, q, cos, cos), q),
+             (lambda t: rope.rope_qk(q, t, cos, cos), q), (lambda t: rope.rope_k(t, cos, cos), q), (lambda t: rmsnorm.add_rms_norm(q, t, w, 1e-5), q),
+             (lambda t: rmsnorm.add_rms_norm(q, None, t, 1e-5), w), (lambda t: embedding.embedding(idx, t), z), (lambda t: distill.distill_loss(t, v, top), z),
+             (lambda t: distill.distill_loss(z, t, top), v), (lambda t: distill.distill_loss(z, v, top, t), r))
+    for f, t in calls:
+        with forward_ad.dual_level():
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f(forward_ad.make_dual(t, torch.ones_like(t)))
+            with pytest.raises(RuntimeError, match="CUDA tensor|float16 or bfloat16"):  # no tangent: on to the op's own checks
+                f(t)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(f, (t,), (torch.ones_like(t),))

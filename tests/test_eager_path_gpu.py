@@ -292,3 +292,24 @@ def test_gradients_that_are_zeros_without_memory():
         a = a.clone().requires_grad_()
         y = f(a)
         assert not torch.autograd.grad(y, a, torch._efficientzerotensor(y.shape, dtype=y.dtype, device=DEV))[0].any()
+
+
+def test_forward_mode_is_refused_and_the_embedding_module_has_pytorchs():
+    from torch.autograd import forward_ad
+
+    from nanonemo_amd.kernels.hip import distill, embedding, rmsnorm
+    from nanonemo_amd.model import Embedding
+
+    idx = torch.randint(0, 50, (3, 7), device=DEV)
+    w, z = torch.randn(50, 16, device=DEV), torch.randn(5, 50, device=DEV)
+    v, at = z.topk(4)
+    for f, t in ((lambda t: embedding.embedding(idx, t), w), (lambda t: distill.distill_loss(t, v, at), z), (lambda t: rmsnorm.add_rms_norm(t, None, w[0], 1e-5), w)):
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            f(forward_ad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(f, (t,), (torch.ones_like(t),))
+    m = Embedding(50, 16, 3.0, "hip").to(DEV)
+    for grad in (False, True):
+        m.weight.requires_grad_(grad)
+        out, tangent = torch.func.jvp(lambda t: torch.func.functional_call(m, {"weight": t}, (idx,)), (m.weight,), (torch.full_like(m.weight, 2.0),))
+        assert torch.equal(out, m(idx)) and (tangent == 6.0).all()
