@@ -28,6 +28,9 @@ from torch import Tensor
 from nanonemo_amd.kernels.hip import eager, host, preload, records, refuse_capture, refuse_forward_ad
 
 
+_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+
+
 @torch.library.custom_op("nanonemo::top_logits", mutates_args=())
 def _top_logits(logits: Tensor, k: int, temperature: float) -> tuple[Tensor, Tensor, Tensor]:
     return host().top_logits(logits, k, temperature)
@@ -92,6 +95,14 @@ def _check_temperature(temperature: float) -> None:
 def _check_k(k: int, vocab: int) -> None:
     if not 1 <= k <= min(vocab, 512):
         raise ValueError(f"k must be in [1, min(V, 512)], got {k} of {vocab} logits")
+
+
+def takes(logits: Tensor, k: int, values: Tensor | None = None, rest: Tensor | None = None) -> bool:
+    """Whether logits (..., V) with k of a teacher's are within the kernels' sizes and types; other forms of them exist in
+    PyTorch's operations (model.py). What is no valid argument in any form is refused by the functions."""
+    V = logits.shape[-1]
+    return (logits.dtype in _DTYPES and k <= 512 and V <= 393216 and logits.numel() < V << 22
+            and (values is None or values.dtype in _DTYPES) and (rest is None or rest.dtype is torch.float32))
 
 
 def top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> tuple[Tensor, Tensor, Tensor]:

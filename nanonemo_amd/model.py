@@ -22,8 +22,9 @@ embedding and its gradient (nanonemo::embedding).
 A model with any of them set also runs its linear layers, SwiGLU and cross entropy on this build's kernels where it is
 called eagerly on a GPU under 16-bit autocast (kernels/hip/linear.py, layers.py and head.py say exactly when; there the
 "hip_bthd" attention with either RoPE kernel is one autograd node, with q rotated by the RoPE kernel, whose result is
-bit-identical). So do its distillation from a teacher's top logits and that teacher's selection of them
-(kernels/hip/distill.py). Everything else, and every module whose layers carry hooks or are not plain nn.Linear, is PyTorch.
+bit-identical). On a GPU its distillation from a teacher's top logits and that teacher's selection of them run there too,
+within the kernels' sizes and types (kernels/hip/distill.py). Everything else, and every module whose layers carry hooks or
+are not plain nn.Linear, is PyTorch.
 """
 
 from __future__ import annotations
@@ -371,6 +372,8 @@ class NanoNemo(nn.Module):
         from nanonemo_amd.kernels.hip import distill
 
         logits = _project(self.cfg, h, self.lm_head)[0]
+        if not distill.takes(logits, teacher.values.shape[-1], teacher.values, teacher.rest):
+            return logits, distill_loss(logits, teacher, targets)
         return logits, distill.distill_loss(logits, teacher.values, teacher.indices, teacher.rest, targets, teacher.temperature, teacher.weight)
 
     @torch.no_grad()
@@ -380,7 +383,8 @@ class NanoNemo(nn.Module):
         if self.cfg.any_hip and logits.is_cuda:
             from nanonemo_amd.kernels.hip import distill
 
-            return Teacher(*distill.top_logits(logits, k, temperature), temperature, weight)
+            if distill.takes(logits, k):
+                return Teacher(*distill.top_logits(logits, k, temperature), temperature, weight)
         values, indices = logits.topk(k, dim=-1)
         rest = (logits.float() / temperature).scatter(-1, indices, -math.inf).logsumexp(-1)
         return Teacher(values, indices, rest, temperature, weight)

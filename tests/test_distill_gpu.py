@@ -642,3 +642,28 @@ def test_a_teachers_rest_where_the_student_has_none(V, tau):
         assert loss == INF and (d.scatter(-1, idx, 0.0) == 0).all()
         # (fp64 throughout, rounded once)
         assert ((d.gather(-1, idx).double() - ref / 6).abs() <= 2**-24 * (ref / 6).abs() + 1e-14).all()
+
+
+def test_a_model_with_kernels_distils_what_they_do_not_take():
+    # k above 512, a vocabulary above 393216, a teacher in fp64: the PyTorch form, as a model without kernels has it.
+    from nanonemo_amd.model import ModelConfig, NanoNemo
+
+    for vocab, k, dtype in ((700, 600, None), (393300, 5, None), (512, 7, torch.float64)):
+        print(f"\n[case] model vocab={vocab} k={k} values {dtype}", flush=True)
+        out = []
+        for kernels in ({}, dict(norm_kernel="hip")):
+            torch.manual_seed(3)
+            m = NanoNemo(ModelConfig(**{**SMALL, "n_layers": 1, "d_model": 64, "d_ff": 64, "n_heads": 2, "n_kv_heads": 1, "vocab_size": vocab}, **kernels)).cuda()
+            idx = torch.randint(0, vocab, (1, 16), generator=torch.Generator().manual_seed(1)).cuda()
+            t = m.teach(idx, k, 2.0, 0.5)
+            if dtype is not None:
+                t = t._replace(values=t.values.to(dtype), rest=t.rest.to(dtype))
+            _, loss = m(idx, idx.roll(-1, 1), t)
+            out.append((t, loss, torch.autograd.grad(loss, m.tok_emb.weight)[0]))
+        assert out[1][0].values.shape == (1, 16, k)
+        for a, b in ((out[1][0].values, out[0][0].values), (out[1][0].rest, out[0][0].rest), (out[1][1], out[0][1]), (out[1][2], out[0][2])):
+            torch.testing.assert_close(a, b, rtol=1e-3, atol=1e-5)  # (the norms alone differ, by fp32 roundings)
+    with pytest.raises(ValueError, match="k must be"):
+        m.teach(idx, 0)
+    with pytest.raises(ValueError, match="temperature"):
+        m.teach(idx, 4, -1.0)
