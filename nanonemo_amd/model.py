@@ -251,23 +251,32 @@ class MLP(nn.Module):
 
 class Embedding(nn.Embedding):
     """The tokens' embeddings times a scale. kernel="hip" looks them up, and sums their gradient, with this build's kernels
-    (nn.Embedding's other options keep its own)."""
+    (nn.Embedding's other options and forward-mode differentiation keep its own)."""
 
     def __init__(self, num: int, dim: int, scale: float = 1.0, kernel: str = "torch", **options):
         super().__init__(num, dim, **options)
-        self.scale = scale
-        self.fused = None
-        if kernel == "hip":
-            from nanonemo_amd.kernels.hip.embedding import embedding  # raises without the library
+        self.scale = float(scale)
+        self.hip = kernel == "hip"
+        if self.hip:
+            import nanonemo_amd.kernels.hip.embedding  # noqa: F401  (registers the ops)
 
-            self.fused = embedding
+    @torch.jit.unused
+    def _fused(self, idx: torch.Tensor) -> torch.Tensor | None:
+        """The lookup on this build's kernels, for the calls that they take."""
+        from nanonemo_amd.kernels.hip.embedding import embedding
+
+        w = self.weight
+        if self.max_norm is not None or self.scale_grad_by_freq or self.sparse or torch.autograd.forward_ad._current_level >= 0:
+            return None
+        return embedding(idx, w, self.scale, self.padding_idx)
 
     def forward(self, idx: torch.Tensor) -> torch.Tensor:
-        # (a module traced symbolically has no tensor here; PyTorch's lookup has a forward-mode formula)
-        if self.fused is not None and isinstance(idx, torch.Tensor) and idx.is_cuda and torch.autograd.forward_ad._current_level < 0 \
-                and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse:
-            return self.fused(idx, self.weight, self.scale, self.padding_idx)
-        x = super().forward(idx)
+        # (a scripted module, and one traced symbolically, whose idx is no tensor, is PyTorch's)
+        if not torch.jit.is_scripting() and self.hip and isinstance(idx, torch.Tensor) and idx.is_cuda:
+            y = self._fused(idx)
+            if y is not None:
+                return y
+        x = F.embedding(idx, self.weight, self.padding_idx, self.max_norm, self.norm_type, self.scale_grad_by_freq, self.sparse)
         return x if self.scale == 1.0 else x * self.scale
 
 

@@ -237,3 +237,17 @@ def test_plain_distillation_of_a_model():
     assert student(idx, None, t._replace(weight=1.0))[1].isfinite()
     loss, norm = train_step(student, make_optimizer(student), [batch], amp_dtype=None)
     assert loss.isfinite() and norm > 0
+
+
+@pytest.mark.parametrize("kernel", ["torch", "hip"])
+@pytest.mark.parametrize("how", ["script", "trace"])
+def test_the_embedding_module_is_scripted_and_traced_as_pytorchs(kernel, how):
+    from nanonemo_amd.model import Embedding
+
+    m = Embedding(20, 8, 3.0, kernel, padding_idx=2)
+    idx = torch.randint(0, 20, (3, 5))
+    got = torch.jit.script(m) if how == "script" else torch.fx.symbolic_trace(m)
+    ref = F.embedding(idx, m.weight, 2) * 3.0
+    assert torch.equal(got(idx), ref) and torch.equal(m(idx), ref)
+    (g,), (r,) = (torch.autograd.grad(f(idx).square().sum(), m.weight) for f in (got, lambda i: F.embedding(i, m.weight, 2) * 3.0))
+    assert torch.equal(g, r) and not g[2].any()
