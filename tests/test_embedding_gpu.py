@@ -235,3 +235,17 @@ def test_refusals():
                       (lambda: host().embedding_bwd(w[:3], idx, 10, 1.0, 10), "padding_idx"), (lambda: host().embedding_bwd(w[:3], idx, 0, 1.0, -1), "invalid sizes")):
         with pytest.raises((RuntimeError, IndexError), match=msg):
             call()
+
+
+def test_the_module_keeps_pytorchs_lookup_for_what_the_kernels_do_not_take():
+    from nanonemo_amd.model import Embedding
+
+    idx = torch.randint(0, 50, (3, 7), device="cuda")
+    for options, dtype in ((dict(), torch.float64), (dict(max_norm=1.0), torch.float32), (dict(scale_grad_by_freq=True), torch.float32)):
+        m = Embedding(50, 16, 3.0, "hip", padding_idx=4, **options).cuda().to(dtype)
+        ref = F.embedding(idx, m.weight, 4, **options) * 3.0
+        out = m(idx)
+        assert out.dtype == dtype and torch.equal(out, ref)
+        assert torch.equal(torch.autograd.grad(out.sum(), m.weight)[0], torch.autograd.grad(ref.sum(), m.weight)[0])
+    m = Embedding(50, 16, 3.0, "hip").cuda()
+    assert "EmbeddingNode" in m(idx).grad_fn.name() and torch.equal(torch.jit.script(m)(idx), F.embedding(idx, m.weight) * 3.0)
