@@ -220,13 +220,11 @@ def refuse_capture(where: str, *inputs) -> None:
 def refuse_forward_ad(where: str, *inputs) -> None:
     """Raise where an input (None for one that is not given) carries a tangent (torch.autograd.forward_ad, torch.func.jvp):
     the ops have no forward-mode formula, and a call that autograd does not record would return values without a tangent,
-    as if it were zero."""
-    import torch
+    as if it were zero. For calls inside a dual level (forward_ad._current_level >= 0, which the callers ask themselves: the
+    small calls are paced by the host)."""
+    from torch.autograd import forward_ad
 
-    ad = torch.autograd.forward_ad
-    if torch.compiler.is_compiling() or ad._current_level < 0:
-        return
-    if any(t is not None and ad.unpack_dual(t).tangent is not None for t in inputs):
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in inputs):
         raise NotImplementedError(f"{where}: forward-mode automatic differentiation is not supported")
 
 

@@ -24,6 +24,7 @@ import math
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from nanonemo_amd.kernels.hip import eager, host, preload, records, refuse_capture, refuse_forward_ad
 
@@ -129,7 +130,8 @@ def distill_loss(
         raise ValueError("weight below 1 needs targets, whose cross entropy is the rest of the loss")
     if records(values) or rest is not None and records(rest):
         raise ValueError("the teacher's values take no gradient: detach them")
-    refuse_forward_ad("distill_loss", logits, values, rest)
+    if forward_ad._current_level >= 0:
+        refuse_forward_ad("distill_loss", logits, values, rest)
     call = (logits, values, indices, rest, targets, float(temperature), float(weight))
     if eager(*(t for t in call[:5] if t is not None)):  # the same launches as the op's, as one autograd node of the host module
         return host().distill(*call)

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from nanonemo_amd.kernels.hip import eager, host, preload, refuse_capture, refuse_forward_ad
 
@@ -67,7 +68,8 @@ def embedding(idx: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: int 
         padding_idx %= rows
     else:
         raise ValueError(f"padding_idx {padding_idx} is not a row of the weight ({rows} rows)")
-    refuse_forward_ad("embedding", weight)
+    if forward_ad._current_level >= 0:
+        refuse_forward_ad("embedding", weight)
     if eager(idx, weight):  # the same launches as the op's, as one autograd node of the host module
         return host().embedding(idx, weight, scale, padding_idx)
     refuse_capture("embedding", weight)

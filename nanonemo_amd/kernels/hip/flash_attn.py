@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from nanonemo_amd.kernels.hip import eager as _eager
@@ -135,7 +136,8 @@ class _FlashAttnFn(torch.autograd.Function):
 def flash_attn(q: Tensor, k: Tensor, v: Tensor) -> Tensor:
     """Causal GQA attention. q: (B, H, T, hd), k/v: (B, KVH, T, hd), fp16 or bf16, H % KVH == 0, hd in {32, 64}."""
     _refuse_capture_with_autograd("flash_attn", q, k, v)
-    refuse_forward_ad("flash_attn", q, k, v)
+    if forward_ad._current_level >= 0:
+        refuse_forward_ad("flash_attn", q, k, v)
     if _eager(q, k, v):
         return _FlashAttnFn.apply(q, k, v) if _records(q, k, v) else host().fa_fwd(q, k, v)[0]
     o, _ = _flash_attn(q, k, v)
@@ -210,7 +212,8 @@ class _FlashAttnBthdFn(torch.autograd.Function):
 def flash_attn_bthd(q: Tensor, k: Tensor, v: Tensor) -> Tensor:
     """Causal GQA attention in the projection layout: q (B, T, H, hd), k/v (B, T, KVH, hd) -> o (B, T, H, hd)."""
     _refuse_capture_with_autograd("flash_attn_bthd", q, k, v)
-    refuse_forward_ad("flash_attn_bthd", q, k, v)
+    if forward_ad._current_level >= 0:
+        refuse_forward_ad("flash_attn_bthd", q, k, v)
     if _eager(q, k, v):
         if _records(q, k, v):
             return _FlashAttnBthdFn.apply(q, k, v)
@@ -298,7 +301,8 @@ def flash_attn_bthd_rope(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tens
     """Causal GQA attention in the projection layout with q's RoPE folded in: q (B, T, H, hd) *before* RoPE,
     k (B, T, KVH, hd) already rotated, v (B, T, KVH, hd), cos/sin fp32 (T_max, hd/2) -> o (B, T, H, hd)."""
     _refuse_capture_with_autograd("flash_attn_bthd_rope", q, k, v)
-    refuse_forward_ad("flash_attn_bthd_rope", q, k, v, cos, sin)
+    if forward_ad._current_level >= 0:
+        refuse_forward_ad("flash_attn_bthd_rope", q, k, v, cos, sin)
     if _eager(q, k, v, cos, sin):
         if _records(q, k, v, cos, sin):
             return _FlashAttnBthdRopeFn.apply(q, k, v, cos, sin)

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from nanonemo_amd.kernels.hip import eager, host, preload, records, refuse_forward_ad
@@ -101,7 +102,8 @@ def add_rms_norm(x: Tensor, delta: Tensor | None, weight: Tensor, eps: float) ->
     the normalized output takes the autocast dtype (the residual keeps its own)."""
     out_dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
     ins = (x, weight) if delta is None else (x, delta, weight)
-    refuse_forward_ad("add_rms_norm", *ins)
+    if forward_ad._current_level >= 0:
+        refuse_forward_ad("add_rms_norm", *ins)
     if eager(*ins):
         if records(*ins):
             y, h = _AddRmsNormFn.apply(x, delta, weight, eps, out_dtype)

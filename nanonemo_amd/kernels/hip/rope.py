@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from nanonemo_amd.kernels.hip import eager, host, preload, records, refuse_forward_ad
@@ -72,7 +73,8 @@ class _RopeQkFn(torch.autograd.Function):
 
 
 def _rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> tuple[Tensor, Tensor]:
-    refuse_forward_ad("rope", q, k, cos, sin)
+    if forward_ad._current_level >= 0:
+        refuse_forward_ad("rope", q, k, cos, sin)
     if eager(q, k, cos, sin):
         if records(q, k, cos, sin):
             return _RopeQkFn.apply(q, k, cos, sin)
