@@ -667,3 +667,18 @@ def test_a_model_with_kernels_distils_what_they_do_not_take():
         m.teach(idx, 0)
     with pytest.raises(ValueError, match="temperature"):
         m.teach(idx, 4, -1.0)
+
+
+def test_logits_whose_values_are_not_side_by_side():
+    # Every other value of wider rows: copied, and the gradient is the view's.
+    z, v, idx, rest, y = _case((3, 6), 1003, 9, torch.bfloat16, 2.0, _gen(43))
+    wide = torch.randn(3, 6, 2006, device="cuda").bfloat16()
+    wide[..., ::2] = z
+    view = wide[..., ::2]
+    assert view.stride(-1) == 2 and not _twice(idx)
+    for r, t, w in ((rest, y, 0.5), (None, None, 1.0)):
+        _check_loss(view, v, idx, r, t, 2.0, w, w)
+    # and with indices that are there twice, as halved ones are
+    half = idx // 2
+    assert _twice(half)
+    _check_loss(view, v, half, rest, y, 2.0, 1.0, "twice")
