@@ -16,8 +16,9 @@
 extern "C" {
 #endif
 
-/* The k largest of each row, descending, equal ones by index (NaN above +inf): values [R][k] of the logits' dtype, indices
- * int64 [R][k], and rest[R] = logsumexp(the other logits / temperature) in fp32, -inf where there are none. Deterministic. */
+/* The k largest of each row, descending, equal ones by index (NaN above +inf; -0 equals 0 and is given as 0, a NaN of any
+ * bits as one of them): values [R][k] of the logits' dtype, indices int64 [R][k], and rest[R] = logsumexp(the other logits /
+ * temperature) in fp32, -inf where there are none. Deterministic. */
 int nn_top_logits(const void* logits, int64_t T, int64_t sb, int64_t st, void* values, int64_t* indices, float* rest, int64_t R,
                   int64_t V, int64_t k, double temperature, int dtype, void* stream);
 

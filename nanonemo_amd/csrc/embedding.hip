@@ -5,9 +5,10 @@
 //
 // Backward. The positions are sorted by token (a stable radix sort, so that equal tokens keep their order), the sorted
 // list is cut into chunks of equal length, and a wave sums a chunk's rows of dy token by token. A token whose rows lie in
-// one chunk is stored at once; the sums of one that is cut by chunk borders go to the workspace as fp32 and are joined in
-// chunk order by fixup_kernel. The work is even whatever the tokens are (a batch of one repeated token is as many waves
-// as any other), there are no atomics on values, and the order of every sum is fixed: the result is bit-reproducible.
+// one chunk is stored at once; the sums of one that is cut by chunk borders go to the workspace as fp32 and are joined by
+// fixup_kernel: in chunk order, or for a long run by 16 waves, each every 16th, and the waves' in order. The work is even
+// whatever the tokens are (a batch of one repeated token is as many waves as any other), there are no atomics on values, and the
+// order of every sum is fixed by the tokens and the sizes: the result is bit-reproducible.
 // Rows of dW without a token are zeroed by further blocks of the sort's launches, which leave the memory idle otherwise.
 // Bound by HBM: dy is read once and dW written once.
 //
@@ -434,10 +435,10 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a, const void* __res
         store();
 }
 
-// Joins the sums of the token that begins in a chunk and goes on after it: the chunk's own, then the following ones', in
-// order. A wave per chunk and 64 VEC columns joins up to kFew sums by itself; longer runs (a token that is there hundreds of
-// times) the block's waves join together, each every kFixWaves-th sum, and are added in order. A run of 1567 sums of 512 columns:
-// 21 us (85 with loads that wait for one another), beside 13 for the sums of its 50160 rows.
+// Joins the sums of the token that begins in a chunk and goes on after it, the chunk's own first. A wave per chunk and 64 VEC
+// columns joins up to kFew following sums by itself, in order; longer runs (a token that is there hundreds of times) the block's
+// waves join together, each every kFixWaves-th sum, and are added in order. A run of 1567 sums of 512 columns: 21 us (85 with
+// loads that wait for one another), beside 13 for the sums of its 50160 rows.
 constexpr int kFixWaves = 16, kFew = 16;
 template <int DT, int VEC>
 __global__ __launch_bounds__(64 * kFixWaves) void fixup_kernel(Sums a, void* __restrict__ dw_, int chunks) {
@@ -500,7 +501,7 @@ __global__ __launch_bounds__(64 * kFixWaves) void fixup_kernel(Sums a, void* __r
         return true;
     };
     const int c = part_of * kFixWaves + wave;
-    uint32_t token;
+    uint32_t token = 0;
     int last;
     int longer = 0;
     float acc[VEC];

@@ -108,8 +108,8 @@ def takes(logits: Tensor, k: int, values: Tensor | None = None, rest: Tensor | N
 
 def top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> tuple[Tensor, Tensor, Tensor]:
     """(values (..., k) of the logits' type, indices (..., k) int64, rest (...) fp32): the k largest of each row of logits
-    (..., V), descending, equal ones by index (NaN above +inf), and logsumexp(the others / temperature), -inf where there
-    are none. Not differentiable: what a frozen teacher gives its student."""
+    (..., V), descending, equal ones by index (NaN above +inf, -0 as 0), and logsumexp(the others / temperature), -inf
+    where there are none. Not differentiable: what a frozen teacher gives its student."""
     _check_temperature(temperature)
     _check_k(k, logits.shape[-1])
     logits = logits.detach()

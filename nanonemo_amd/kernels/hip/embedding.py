@@ -3,8 +3,8 @@ sorted tokens.
 
 ``embedding(idx, weight, scale, padding_idx)`` stands for ``F.embedding(idx, weight, padding_idx) * scale``
 (/root/reference/nanonemo/model/model.py:13-70 has it without a scale): the product in fp32, rounded once. Its gradient is
-summed in fp32 in the order of the tokens and rounded once, whatever the weight's type: bit-reproducible, where PyTorch adds
-16-bit rows in 16 bits or with atomics. The model selects it with ``emb_kernel="hip"``.
+summed in fp32 and rounded once, whatever the weight's type, in an order that the tokens and sizes alone decide:
+bit-reproducible, where PyTorch adds 16-bit rows in 16 bits or with atomics. The model selects it with ``emb_kernel="hip"``.
 
 A token that is not in [0, V) makes its row of the output NaN and takes no part in the gradient (F.embedding ends the
 process with a device assertion). Tokens are int64 or int32. Once differentiable, in reverse mode: a tangent is refused.
