@@ -251,7 +251,8 @@ class MLP(nn.Module):
 
 class Embedding(nn.Embedding):
     """The tokens' embeddings times a scale. kernel="hip" looks them up, and sums their gradient, with this build's kernels
-    (nn.Embedding's other options, other types than the kernels' and forward-mode differentiation keep its own)."""
+    (nn.Embedding's other options, other types than the kernels', torch.func's transforms and forward-mode differentiation keep
+    its own)."""
 
     def __init__(self, num: int, dim: int, scale: float = 1.0, kernel: str = "torch", **options):
         super().__init__(num, dim, **options)
@@ -266,8 +267,9 @@ class Embedding(nn.Embedding):
         from nanonemo_amd.kernels.hip.embedding import embedding
 
         w = self.weight
-        if self.max_norm is not None or self.scale_grad_by_freq or self.sparse or w.dtype not in (torch.float16, torch.bfloat16, torch.float32) \
-                or torch.autograd.forward_ad._current_level >= 0:
+        if self.max_norm is not None or self.scale_grad_by_freq or self.sparse or w.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+            return None
+        if not torch.compiler.is_compiling() and (torch.autograd.forward_ad._current_level >= 0 or any(map(torch._C._functorch.is_functorch_wrapped_tensor, (idx, w)))):
             return None
         return embedding(idx, w, self.scale, self.padding_idx)
 

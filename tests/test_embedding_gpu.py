@@ -249,3 +249,17 @@ def test_the_module_keeps_pytorchs_lookup_for_what_the_kernels_do_not_take():
         assert torch.equal(torch.autograd.grad(out.sum(), m.weight)[0], torch.autograd.grad(ref.sum(), m.weight)[0])
     m = Embedding(50, 16, 3.0, "hip").cuda()
     assert "EmbeddingNode" in m(idx).grad_fn.name() and torch.equal(torch.jit.script(m)(idx), F.embedding(idx, m.weight) * 3.0)
+
+
+def test_the_module_under_torch_funcs_transforms():
+    from nanonemo_amd.model import Embedding
+
+    m = Embedding(50, 16, 3.0, "hip", padding_idx=4).cuda()
+    idx = torch.randint(0, 50, (3, 7), device="cuda")
+    ref = torch.autograd.grad((F.embedding(idx, m.weight, 4) * 3.0).square().sum(), m.weight)[0]
+    got = torch.func.grad(lambda t: torch.func.functional_call(m, {"weight": t}, (idx,)).square().sum())(m.weight.detach())
+    assert torch.allclose(got, ref, rtol=21 * 2**-23, atol=0)  # (a sum of at most 21 equal terms, on either side)
+    ws = torch.stack([m.weight.detach(), 2 * m.weight.detach()])
+    both = torch.func.vmap(lambda t: torch.func.functional_call(m, {"weight": t}, (idx,)))(ws)
+    assert torch.equal(both, torch.stack([F.embedding(idx, t) * 3.0 for t in ws]))
+    assert torch.equal(torch.func.vmap(m)(idx), m(idx))
