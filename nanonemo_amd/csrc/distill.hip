@@ -288,7 +288,8 @@ struct TopShared {
 // registers (7 groups each, 27 of them spilled) 390, and 180 where a part's largest value took four instructions a pair of
 // values and NaN another two. A single row takes 10 us, most of it the steps' latency.
 // Rows for which the above does not do (many equal values, NaN, more candidates than the lists hold: with 256 threads from a k of
-// about 150 on, 8192 x 8192 bf16 takes 76 us at k = 128 and 1005 at 256) take a search of the k-th value bit by bit instead, and rows whose others lie far below the bound a sum relative to their own largest.
+// about 150 on, 8192 x 8192 bf16 takes 76 us at k = 128 and 1005 at 256) take a search of the k-th value bit by bit instead, and
+// rows whose others lie far below the bound a sum relative to their own largest.
 template <int DT, int TB, int NV>
 __global__ __launch_bounds__(TB, TB == 512 && NV <= 13 ? 6 : 4) void top_kernel(const void* __restrict__ logits, Layout at, void* __restrict__ values,
                                                     long long* __restrict__ indices, float* __restrict__ rest, int V, int k, float c,

@@ -102,7 +102,7 @@ def takes(logits: Tensor, k: int, values: Tensor | None = None, rest: Tensor | N
     """Whether logits (..., V) with k of a teacher's are within the kernels' sizes and types; other forms of them exist in
     PyTorch's operations (model.py). What is no valid argument in any form is refused by the functions."""
     V = logits.shape[-1]
-    return (logits.dtype in _DTYPES and k <= 512 and V <= 393216 and logits.numel() < V << 22
+    return (logits.dtype in _DTYPES and k <= 512 and V <= 393216 and logits.numel() < V * (1 << 22)
             and (values is None or values.dtype in _DTYPES) and (rest is None or rest.dtype is torch.float32))
 
 
