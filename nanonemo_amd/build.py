@@ -21,7 +21,7 @@ from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
-SRCS = [PKG / "csrc" / f"{n}.hip" for n in ("flash_attn", "rope", "rmsnorm", "linear", "loss", "embedding", "distill")]
+SRCS = [PKG / "csrc" / f"{n}.hip" for n in ("flash_attn", "rope", "rmsnorm", "linear", "loss", "embedding", "distill", "qk_norm")]
 LIB_DIR = PKG / "lib"
 LIB = LIB_DIR / "libnanonemo_fa.so"
 # Block timelines for `bench.py --timeline`: the attention kernels built with NN_TIMELINE=1, so that every block
@@ -57,7 +57,7 @@ HIPCC_FLAGS = [
 # which must show NaN and infinite values and tokens out of range; without this every fmaxf of an MFMA result is preceded by a canonicalising
 # v_max_f32 x, x.
 NO_NANS = ["-Xarch_device", "-fno-honor-nans"]
-HONOR_NANS = {"loss", "embedding", "distill"}
+HONOR_NANS = {"loss", "embedding", "distill", "qk_norm"}
 
 
 # The host side of the operations, a torch extension over the library (g++: it has no device code).

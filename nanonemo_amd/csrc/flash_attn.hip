@@ -37,6 +37,7 @@
 #include <type_traits>
 
 #include "nanonemo_fa.h"
+#include "nanonemo_packed.h"
 #include "tiles.h"
 
 #define NNFA_API extern "C" __attribute__((visibility("default")))
@@ -191,15 +192,66 @@ __device__ inline float sub_rn(float a, float b) {
     return a - b;
 }
 
+// Sequences of different lengths behind one another in one [tokens][heads][D] tensor (include/nanonemo_packed.h). Each is a
+// problem of its own to the kernels below: what a block works on, and where its sequence lies, is one entry of a list that the
+// host laid out and sorted (nn_fa_packed_plan), the tensors' pointers move to the sequence's first row, T is its length, and
+// the loops, masks and sums are those of the dense kernels. So a sequence's outputs are the same bits as a dense call's on it
+// alone (its dk and dv too where the same blocks share the work).
+struct PackedTile {  // forward and dQ: 128 query rows of one sequence, for the query heads of one KV head
+    int start, len, qb, kvh;  // len 0: nothing to do (the list is padded to a multiple of 8)
+};
+struct PackedUnit {  // dK/dV: a unit of 64 keys, or the pair pj and nkb - 1 - pj of them, of one sequence and KV head
+    int start, len, pj, kvh;
+    int nsplit, sidx, slot;  // this block's share of the pair's iterations, and its place among the partial sums
+    int paired;
+};
+template <bool PACKED>
+struct PackedArg {};
+template <>
+struct PackedArg<true> {
+    const void* list;  // PackedTile or PackedUnit
+    int count;         // entries
+    int tokens;        // of all sequences: the stride of the per-head vectors lse, -lse/scale and -D
+};
+using Packed = PackedArg<true>;
+constexpr int kPairRows = 128;  // rows of a partial sum of packed dK/dV: the pair's two units
+// A forward or dQ block's batch, head and query block; packed: its sequence's start and length, and bh * T as the place of the
+// sequence's row 0 in the per-head fp32 vectors. Entry i of the packed list is for XCD i % 8 (block i goes to XCD i % 8), where
+// the heads of its group follow one another and share its K and V tiles in that XCD's L2.
+struct Place {
+    int bh, qb, b, h, kvh, start, T;
+};
+// Row 0 of the block's head (and sequence) in the per-head fp32 vectors.
+template <bool PACKED>
+__device__ inline size_t vec_row(const PackedArg<PACKED>& pk, int bh, int h, int start, int T) {
+    if constexpr (PACKED)
+        return (size_t)h * pk.tokens + start;
+    else
+        return (size_t)bh * T;
+}
+template <bool PACKED>
+__device__ inline Place place(const PackedArg<PACKED>& pk, int BH, int H, int KVH, int T, int nqb) {
+    if constexpr (PACKED) {
+        const int group = H / KVH, slot = (int)blockIdx.x >> 3, at = slot / group;
+        const PackedTile e = static_cast<const PackedTile*>(pk.list)[at * 8 + ((int)blockIdx.x & 7)];
+        return {0, e.qb, 0, e.kvh * group + (slot - at * group), e.kvh, e.start, e.len};
+    } else {
+        const QBlk blk = qblock_of(blockIdx.x, BH, H / KVH, nqb);
+        const int b = blk.bh / H, h = blk.bh - b * H;
+        return {blk.bh, blk.qb, b, h, h / (H / KVH), 0, T};
+    }
+}
+
 // ------------------------------------------------------------------------------------------
 // Forward. Block = 4 waves = 128 query rows of one (batch, head); 128-key tiles of K and V,
 // double-buffered in LDS by DMA. Q stays in registers for the whole block.
 // ------------------------------------------------------------------------------------------
-template <int HD, int DT, bool ROPE>
+template <int HD, int DT, bool ROPE, bool PACKED = false>
 __global__ __launch_bounds__(256, 2) void fa_fwd_kernel(const u16* __restrict__ Q, const u16* __restrict__ K,
                                                         const u16* __restrict__ V, u16* __restrict__ O,
                                                         float* __restrict__ LSE, int BH, int H, int KVH, int T,
-                                                        int nqb, float sl2, Lay lq, Lay lk, Lay lo, RopeArgs ra) {
+                                                        int nqb, float sl2, Lay lq, Lay lk, Lay lo, RopeArgs ra,
+                                                        PackedArg<PACKED> pk) {
     using E = Elem<DT>;
     NN_TL_START(kTlFwd);
     constexpr int BM = 128, BN = 128, NW = 4;
@@ -212,13 +264,13 @@ __global__ __launch_bounds__(256, 2) void fa_fwd_kernel(const u16* __restrict__ 
     __shared__ __attribute__((aligned(16))) u16 kB[TILE];
     __shared__ __attribute__((aligned(16))) u16 vB[TILE];
 
-    const QBlk blk = qblock_of(blockIdx.x, BH, H / KVH, nqb);
-    const int bh = blk.bh, qb = blk.qb;
-    const int b = bh / H, h = bh - b * H;
-    const int kvh = h / (H / KVH);
-    const size_t qoff = lq.at(b, h);
-    const u16* Kp = K + lk.at(b, kvh);
-    const u16* Vp = V + lk.at(b, kvh);
+    const Place at = place<PACKED>(pk, BH, H, KVH, T, nqb);
+    if (PACKED && at.T == 0) return;
+    if constexpr (PACKED) T = at.T;
+    const int bh = at.bh, qb = at.qb, b = at.b, h = at.h, kvh = at.kvh, start = at.start;
+    const size_t qoff = lq.at(b, h) + (PACKED ? (size_t)start * lq.st : 0);
+    const u16* Kp = K + lk.at(b, kvh) + (PACKED ? (size_t)start * lk.st : 0);
+    const u16* Vp = V + lk.at(b, kvh) + (PACKED ? (size_t)start * lk.st : 0);
 
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -440,7 +492,7 @@ __global__ __launch_bounds__(256, 2) void fa_fwd_kernel(const u16* __restrict__ 
             for (int s = 0; s < NS; ++s) *reinterpret_cast<u16x8*>(qo + 16 * s + 8 * hh) = qf[s];
         }
         const float inv = 1.f / ltot;
-        u16* op = O + lo.at(b, h) + (size_t)qrow * lo.st;
+        u16* op = O + lo.at(b, h) + (size_t)(start + qrow) * lo.st;
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
@@ -449,7 +501,7 @@ __global__ __launch_bounds__(256, 2) void fa_fwd_kernel(const u16* __restrict__ 
                 u32x2 w = {E::pack2(a[4 * g] * inv, a[4 * g + 1] * inv), E::pack2(a[4 * g + 2] * inv, a[4 * g + 3] * inv)};
                 *reinterpret_cast<u32x2*>(op + 32 * dt + 8 * g + 4 * hh) = w;
             }
-        if (hh == 0) LSE[(size_t)bh * T + qrow] = (mb + fast_log2(ltot)) * kLn2;
+        if (hh == 0) LSE[vec_row<PACKED>(pk, bh, h, start, T) + qrow] = (mb + fast_log2(ltot)) * kLn2;
     }
     NN_TL_END(kTlFwd);
 }
@@ -511,12 +563,12 @@ __global__ __launch_bounds__(256) void fa_bwd_pre_kernel(const u16* __restrict__
 // (each wave a quarter, by DMA), and every wave reads its K / V operands from there, instead of each wave
 // loading all 64 rows from memory; the second unit's rows are copied a whole unit ahead, while the first
 // unit's loop runs, so its unit change carries only the first tiles' copies.
-template <int HD, int DT, int WPP, bool KVL>
+template <int HD, int DT, int WPP, bool KVL, bool PACKED = false>
 __global__ __launch_bounds__(256, 1) void fa_bwd_dkdv_kernel(
     const u16* __restrict__ Q, const u16* __restrict__ K, const u16* __restrict__ V, const u16* __restrict__ dO,
     const float* __restrict__ nLvec, const float* __restrict__ nDvec, u16* __restrict__ dK, u16* __restrict__ dV,
     int BKV, int H, int KVH, int T, int nkb, int nqt, float sl2, float scale, Lay lq, Lay lk, Lay ldk,
-    int nsplit, float* __restrict__ part, int paired) {
+    int nsplit, float* __restrict__ part, int paired, PackedArg<PACKED> pk) {
     using E = Elem<DT>;
     NN_TL_START(kTlDkdv);
     constexpr int BNK = 64, BM = 64, NW = 4, NSL = BNK / 32;
@@ -535,12 +587,12 @@ __global__ __launch_bounds__(256, 1) void fa_bwd_dkdv_kernel(
     static_assert(!KVL || WPP == NW, "K / V through LDS needs the block's four waves on one pair");
     __shared__ __attribute__((aligned(16))) u16 kvS[KVL ? 2 * BNK * HD : 8];  // a unit's K rows, then its V rows
 
-    const int nbk = (BKV + PPB - 1) / PPB;   // blocks per unit-pair index (and split)
-    const int nbase = nbk * (paired ? (nkb + 1) / 2 : nkb);  // blocks of one split
-    const int sidx = blockIdx.x / nbase;      // this block's split
+    const int nbk = PACKED ? 1 : (BKV + PPB - 1) / PPB;   // blocks per unit-pair index (and split)
+    const int nbase = PACKED ? 1 : nbk * (paired ? (nkb + 1) / 2 : nkb);  // blocks of one split
+    int sidx = PACKED ? 0 : blockIdx.x / nbase;      // this block's split
     const int bid = blockIdx.x - sidx * nbase;
     const int bgrp = bid % nbk;               // the block's pairs are (batch, KV head) bgrp PPB .. + PPB - 1
-    const int pj = bid / nbk;  // the pair's first unit (the block's only unit when unpaired)
+    int pj = bid / nbk;  // the pair's first unit (the block's only unit when unpaired)
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
     const int wave = tid >> 6;  // a uniform copy in an SGPR costs this kernel more than it saves
     const int wp = wave % WPP;  // this wave's place among its pair's waves
@@ -549,8 +601,20 @@ __global__ __launch_bounds__(256, 1) void fa_bwd_dkdv_kernel(
     // tile copies' addressing stays in SALU. (With one wave per pair the scalar form breaks the compiler's
     // AGPR-copy rewrite pass.)
     const int bk = WPP == NW ? bgrp : WPP == 2 ? __builtin_amdgcn_readfirstlane(bgrp * PPB + wave / WPP) : bgrp * PPB + wave / WPP;
-    const bool active = bk < BKV;
-    const int b = bk / KVH, kvh = bk - b * KVH, group = H / KVH;
+    bool active = bk < BKV;
+    const int b = PACKED ? 0 : bk / KVH, group = H / KVH;
+    int kvh = bk - b * KVH, slot0 = 0, vecT = T;
+    if constexpr (PACKED) {  // this wave's entry of the list (with every wave on one pair the block's)
+        const int at = (int)blockIdx.x * PPB + (WPP == NW ? 0 : wave / WPP);
+        active = at < pk.count;
+        const PackedUnit u = static_cast<const PackedUnit*>(pk.list)[min(at, pk.count - 1)];
+        T = u.len, pj = u.pj, kvh = u.kvh, nsplit = u.nsplit, sidx = u.sidx, slot0 = u.slot, paired = u.paired;
+        nkb = nqt = (T + 63) / 64, vecT = pk.tokens;
+        Q += (size_t)u.start * lq.st, dO += (size_t)u.start * lq.st;
+        K += (size_t)u.start * lk.st, V += (size_t)u.start * lk.st;
+        dK += (size_t)u.start * ldk.st, dV += (size_t)u.start * ldk.st;
+        nLvec += u.start, nDvec += u.start;
+    }
     const DmaOffs<HD, BM, 1> dfo = dma_offsets<HD, BM, 1>(lane, 0, lq.st);
     // This split's iterations [first, end) of a unit with n of them.
     // 32-bit: the host splits only units whose (sidx + 1) n stays below 2^31 (dkdv_split).
@@ -612,7 +676,7 @@ __global__ __launch_bounds__(256, 1) void fa_bwd_dkdv_kernel(
         const int bu = __builtin_amdgcn_readfirstlane(b), ku = __builtin_amdgcn_readfirstlane(kvh);
         const uint32_t iq = (uint32_t)itu / (uint32_t)group, ih = (uint32_t)itu - iq * (uint32_t)group;
         const uint32_t hq = (uint32_t)(ku * group) + ih;
-        const size_t ro = (uint64_t)((uint32_t)(bu * H) + hq) * (uint32_t)T;  // first row of the head's [T] vectors
+        const size_t ro = (uint64_t)((uint32_t)(bu * H) + hq) * (uint32_t)vecT;  // the head's row 0 in the vectors
         const size_t qo = lq.at(bu, hq);
         const uint32_t q0 = (uint32_t)(qtf == pj ? nqt - 1 - (int)iq : qtf + (int)iq) * BM;
         const uint64_t at = qo + (uint64_t)q0 * (uint32_t)lq.st;
@@ -957,12 +1021,13 @@ __global__ __launch_bounds__(256, 1) void fa_bwd_dkdv_kernel(
                     for (int k = 0; k < NO; ++k)
                         reinterpret_cast<u32x2*>(row16(wave, owned(k), which, l32))[hh] =
                             u32x2{E::pack2(sum[k][0], sum[k][1]), E::pack2(sum[k][2], sum[k][3])};
-                } else {  // this split's partial: part[split][dK | dV][bk][key][HD]
+                } else {  // this split's partial: part[split][dK | dV][bk][key][HD], or packed part[slot][dK | dV][pair's row][HD]
 #pragma unroll
                     for (int sl = 0; sl < NSL; ++sl) {
                         const int key = kb0 + 32 * sl + l32;
                         if (active && key < T) {
                             float* row = part + (((size_t)sidx * 2 + which) * BKV + bk) * T * HD + (size_t)key * HD;
+                            if constexpr (PACKED) row = part + (((size_t)slot0 * 2 + which) * kPairRows + ui * BNK + 32 * sl + l32) * HD;
 #pragma unroll
                             for (int k = 0; k < NO; ++k)
                                 if (owned(k) / (4 * ND) == sl) *reinterpret_cast<f32x4*>(row + col_of(owned(k))) = sum[k];
@@ -1007,7 +1072,6 @@ __global__ __launch_bounds__(256, 1) void fa_bwd_dkdv_kernel(
     }
     NN_TL_END(kTlDkdv);
 }
-
 // ------------------------------------------------------------------------------------------
 // Backward, dK / dV with nsplit > 1: dK, dV = the sum over splits s = 0, 1, ... (in that order) of
 // part[s][dK | dV][bk][key][HD] (fp32, dK already scaled), rounded once to the output dtype. One
@@ -1035,6 +1099,27 @@ __global__ __launch_bounds__(256) void fa_bwd_dkdv_sum_kernel(const float* __res
     }
 }
 
+// The same for packed sequences: the pairs of units that several blocks shared, one block per pair and KV head (its PackedUnit:
+// nsplit partial sums from `slot` on).
+template <int HD, int DT>
+__global__ __launch_bounds__(256) void fa_packed_sum_kernel(const float* __restrict__ part, u16* __restrict__ dK, u16* __restrict__ dV,
+                                                            const PackedUnit* __restrict__ list, Lay ldk) {
+    using E = Elem<DT>;
+    const PackedUnit u = list[blockIdx.x];
+    const int nkb = (u.len + 63) / 64;
+    constexpr int kOne = kPairRows * HD;  // values of one gradient's partial sum
+    const float* from = part + (size_t)u.slot * 2 * kOne;
+    for (int i = threadIdx.x * 4; i < 2 * kOne; i += 1024) {
+        const int which = i / kOne, row = i % kOne / HD, col = i % HD;
+        const int unit = row < 64 ? u.pj : nkb - 1 - u.pj, key = unit * 64 + row % 64;
+        if (key >= u.len || (row >= 64 && unit <= u.pj)) continue;  // (a middle unit has no partner)
+        f32x4 acc = *reinterpret_cast<const f32x4*>(from + i);
+        for (int s = 1; s < u.nsplit; ++s) acc += *reinterpret_cast<const f32x4*>(from + (size_t)s * 2 * kOne + i);
+        u16* dst = (which == 0 ? dK : dV) + ldk.at(0, u.kvh) + (size_t)(u.start + key) * ldk.st + col;
+        *reinterpret_cast<u32x2*>(dst) = u32x2{E::pack2(acc[0], acc[1]), E::pack2(acc[2], acc[3])};
+    }
+}
+
 // ------------------------------------------------------------------------------------------
 // Backward, dQ. Shaped like the forward: block = 4 waves = 128 query rows of one (batch, head),
 // 128-key tiles of K and V double-buffered in LDS by DMA and processed in 64-key halves, Q and dO rows
@@ -1044,14 +1129,14 @@ __global__ __launch_bounds__(256) void fa_bwd_dkdv_sum_kernel(const float* __res
 //   dQ^T += K^T dS^T                    (A = columns of the K tile, B = dS^T registers)
 // dQ stays in registers for the whole key loop and is stored once, scaled, in the output dtype.
 // ------------------------------------------------------------------------------------------
-template <int HD, int DT, bool ROPE>
+template <int HD, int DT, bool ROPE, bool PACKED = false>
 __global__ __launch_bounds__(256, 2) void fa_bwd_dq_kernel(const u16* __restrict__ Q, const u16* __restrict__ K,
                                                            const u16* __restrict__ V, const u16* __restrict__ O,
                                                            const u16* __restrict__ dO, const float* __restrict__ LSE,
                                                            float* __restrict__ nLvec, float* __restrict__ nDvec,
                                                            u16* __restrict__ dQ, int BH, int H, int KVH, int T, int nqb,
                                                            float sl2, float scale, Lay lq, Lay lk, Lay lo, Lay ldq,
-                                                           RopeArgs ra) {
+                                                           RopeArgs ra, PackedArg<PACKED> pk) {
     using E = Elem<DT>;
     NN_TL_START(kTlDq);
     // LDS tiles of BT = 128 keys (one barrier and one tile wait per 128 keys), each processed as two BN = 64-key
@@ -1067,12 +1152,12 @@ __global__ __launch_bounds__(256, 2) void fa_bwd_dq_kernel(const u16* __restrict
     __shared__ __attribute__((aligned(16))) u16 vB[TILE];
     __shared__ __attribute__((aligned(16))) u16 oS[BM * HD];  // the block's O rows (for D)
 
-    const QBlk blk = qblock_of(blockIdx.x, BH, H / KVH, nqb);
-    const int bh = blk.bh, qb = blk.qb;
-    const int b = bh / H, h = bh - b * H;
-    const int kvh = h / (H / KVH);
-    const u16* Kp = K + lk.at(b, kvh);
-    const u16* Vp = V + lk.at(b, kvh);
+    const Place at = place<PACKED>(pk, BH, H, KVH, T, nqb);
+    if (PACKED && at.T == 0) return;
+    if constexpr (PACKED) T = at.T;
+    const int bh = at.bh, qb = at.qb, b = at.b, h = at.h, kvh = at.kvh, start = at.start;
+    const u16* Kp = K + lk.at(b, kvh) + (PACKED ? (size_t)start * lk.st : 0);
+    const u16* Vp = V + lk.at(b, kvh) + (PACKED ? (size_t)start * lk.st : 0);
 
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1097,13 +1182,14 @@ __global__ __launch_bounds__(256, 2) void fa_bwd_dq_kernel(const u16* __restrict
     // Q and dO into its slices of the second tile buffers, which the loop's first copy overwrites only after
     // the block barrier, O into oS. Rows past T read as zeros.
     issue(0, kA, vA);
-    const float lse = LSE[(size_t)bh * T + qc_];
+    const float lse = LSE[vec_row<PACKED>(pk, bh, h, start, T) + qc_];
     if (qw < T) {
         const DmaOffs<HD, 32, 1> rfo = dma_offsets<HD, 32, 1>(lane, 0, lq.st);
         const DmaOffs<HD, 32, 1> ofo = dma_offsets<HD, 32, 1>(lane, 0, lo.st);
-        dma_rows<HD, 32, 1>(Q + lq.at(b, h), lq.st, qw, T, kB + 32 * wave * HD, 0, rfo);
-        dma_rows<HD, 32, 1>(dO + lq.at(b, h), lq.st, qw, T, vB + 32 * wave * HD, 0, rfo);
-        dma_rows<HD, 32, 1>(O + lo.at(b, h), lo.st, qw, T, oS + 32 * wave * HD, 0, ofo);
+        const size_t qoff = lq.at(b, h) + (PACKED ? (size_t)start * lq.st : 0);
+        dma_rows<HD, 32, 1>(Q + qoff, lq.st, qw, T, kB + 32 * wave * HD, 0, rfo);
+        dma_rows<HD, 32, 1>(dO + qoff, lq.st, qw, T, vB + 32 * wave * HD, 0, rfo);
+        dma_rows<HD, 32, 1>(O + lo.at(b, h) + (PACKED ? (size_t)start * lo.st : 0), lo.st, qw, T, oS + 32 * wave * HD, 0, ofo);
     }
     wait_vmem();
     // The preprocessing pass, for this block's rows: D = rowsum(dO * O) from the 16-bit O (each half-wave
@@ -1122,8 +1208,8 @@ __global__ __launch_bounds__(256, 2) void fa_bwd_dq_kernel(const u16* __restrict
     const float nd = -pair_sum(dacc);
     const float nl2 = -lse * kLog2e;  // (-lse/scale) * sl2
     if (hh == 0 && qrow < T) {
-        nDvec[(size_t)bh * T + qrow] = nd;
-        nLvec[(size_t)bh * T + qrow] = -lse / scale;
+        nDvec[vec_row<PACKED>(pk, bh, h, start, T) + qrow] = nd;
+        nLvec[vec_row<PACKED>(pk, bh, h, start, T) + qrow] = -lse / scale;
     }
     NN_TL_BLOCK(kTlDq, kTlExtra, __builtin_amdgcn_s_memtime());
 
@@ -1222,7 +1308,7 @@ __global__ __launch_bounds__(256, 2) void fa_bwd_dq_kernel(const u16* __restrict
     }
 
     if (qrow < T) {
-        u16* dst = dQ + ldq.at(b, h) + (size_t)qrow * ldq.st;
+        u16* dst = dQ + ldq.at(b, h) + (size_t)(start + qrow) * ldq.st;
         if constexpr (ROPE) {
             // The gradient reaching the rotated Q, rounded to the 16-bit type as a stored dQ would be, then the
             // rotation by -theta. Element i of dq[dt] is column c = 32 dt + (i / 4) * 8 + 4 hh + i % 4; its pair
@@ -1391,7 +1477,7 @@ int fwd_impl(const void* q, const void* k, const void* v, void* o, float* lse, i
     const int BH = (int)(B * H);
     auto launch = [&](auto kern) {
         kern<<<dim3(nqb * BH), dim3(256), 0, st>>>((const u16*)q, (const u16*)k, (const u16*)v, (u16*)o, lse, BH, (int)H,
-                                                   (int)KVH, (int)T, nqb, scale * kLog2e, l.q, l.k, l.o, ra);
+                                                   (int)KVH, (int)T, nqb, scale * kLog2e, l.q, l.k, l.o, ra, PackedArg<false>{});
     };
     if (ra.cosT)
         launch(fa_fwd_kernel<HD, DT, true>);
@@ -1427,7 +1513,8 @@ int dkdv_impl(const void* q, const void* k, const void* v, const void* dO, const
     auto launch = [&](auto kern, int ppb) {
         kern<<<dim3((unsigned)dkdv_blocks(B, KVH, T, mode, w.nsplit)), dim3(256), 0, st>>>(
             (const u16*)q, (const u16*)k, (const u16*)v, (const u16*)dO, w.nL, w.nD, (u16*)dk, (u16*)dv, BKV, (int)H,
-            (int)KVH, (int)T, nkb, nqt, scale * kLog2e, scale, l.q, l.k, l.dk, w.nsplit, w.part, paired ? 1 : 0);
+            (int)KVH, (int)T, nkb, nqt, scale * kLog2e, scale, l.q, l.k, l.dk, w.nsplit, w.part, paired ? 1 : 0,
+            PackedArg<false>{});
     };
     // K / V through LDS (KVL) for pairs at head_dim 64 up to T = 2048: measured 1-3.4 % faster there (config 2:
     // -3 %), within noise or slower at T >= 4096 and at head_dim 32, where the direct loads stay.
@@ -1458,7 +1545,8 @@ int dq_impl(const void* q, const void* k, const void* v, const void* o, const vo
     auto launch = [&](auto kern) {
         kern<<<dim3(nqb * BH), dim3(256), 0, st>>>((const u16*)q, (const u16*)k, (const u16*)v, (const u16*)o,
                                                    (const u16*)dO, lse, w.nL, w.nD, (u16*)dq, BH, (int)H, (int)KVH,
-                                                   (int)T, nqb, scale * kLog2e, scale, l.q, l.k, l.o, l.dq, ra);
+                                                   (int)T, nqb, scale * kLog2e, scale, l.q, l.k, l.o, l.dq, ra,
+                                                   PackedArg<false>{});
     };
     if (ra.cosT)
         launch(fa_bwd_dq_kernel<HD, DT, true>);
@@ -1808,6 +1896,263 @@ NNFA_API int nn_fa_bwd_noalloc(const void* dO, const void* q, const void* k, con
     void* ws = nullptr;
     if (int e = scratch_ptr(stream, &ws)) return e;
     return bwd_entry(dO, q, k, v, o, lse, dq, dk, dv, ws, kNoAllocScratchBytes, B, H, KVH, T, D, dtype, scale, {}, stream);
+}
+
+// ------------------------------------------------------------------------------------------
+// Packed sequences (include/nanonemo_packed.h): the plan, and the launches over its lists.
+// ------------------------------------------------------------------------------------------
+namespace {
+
+constexpr int32_t kPlanMagic = 0x6e6e7031;
+struct PlanHead {
+    int32_t magic, words, n, H, KVH, tokens, longest;
+    int32_t ntiles, nunits, nsums;  // entries of the lists
+    int32_t nslots;                 // partial sums
+    int32_t wpp;                    // waves per entry of the dK/dV list: 1 or 4
+    int32_t tiles, units, sums, positions;  // words where they begin
+};
+static_assert(sizeof(PlanHead) == 64 && offsetof(PlanHead, positions) == 4 * NN_FA_PACKED_POSITIONS, "16 words");
+
+// What the lists are made by: one pass over the lengths counts, a second writes.
+struct PlanRule {
+    int64_t g;        // query heads per KV head
+    int64_t target;   // iterations (query head, query tile) that each of kDkdvFill blocks would do if all did the same
+    bool paired;
+    int wpp;
+    int64_t iters(int64_t nkb, int64_t pj) const { return paired && nkb - 1 - pj > pj ? g * (nkb + 1) : g * (nkb - pj); }
+    // Blocks that share a pair: as many as bring its iterations down to a block's even share, each with kDkdvMinIters at least.
+    // A quarter over the share is left alone: the blocks end unevenly by about as much anyway, and partial sums cost a pass.
+    int64_t splits(int64_t it) const {
+        if (!paired || wpp != 4 || target <= 0) return 1;
+        return std::max<int64_t>(1, std::min({kDkdvMaxSplit, (4 * it - target + 4 * target - 1) / (4 * target), it / kDkdvMinIters}));
+    }
+};
+
+struct PlanSize {
+    PlanRule rule;
+    int64_t tokens = 0, longest = 0, ntiles = 0, nunits = 0, nsums = 0, nslots = 0;
+    int64_t padded() const { return (ntiles + 7) / 8 * 8; }
+    int64_t words() const { return 16 + 4 * padded() + 8 * (nunits + nsums) + tokens; }
+};
+
+int plan_size(const int64_t* lengths, int64_t n, int64_t H, int64_t KVH, PlanSize* out) {
+    g_last_error.clear();
+    if (n < 0 || (n > 0 && !lengths)) return fail(-1, "invalid list of lengths");
+    if (int e = check_dims(1, H, KVH, 1, 64, kBF16)) return e;
+    PlanSize z;
+    int64_t pairs = 0, units = 0, work = 0;
+    const int64_t g = H / KVH;
+    for (int64_t i = 0; i < n; ++i) {
+        const int64_t len = lengths[i];
+        if (len < 0) return fail(-1, "sequence %lld has the length %lld", (long long)i, (long long)len);
+        if (len >= (int64_t)1 << 30 || (z.tokens += len) >= (int64_t)1 << 30) return fail(-1, "sizes too large");
+        z.longest = std::max(z.longest, len);
+        const int64_t nkb = (len + 63) / 64;
+        z.ntiles += (len + 127) / 128 * KVH;
+        pairs += (nkb + 1) / 2 * KVH, units += nkb * KVH;
+        work += g * nkb * (nkb + 1) / 2 * KVH;
+    }
+    // (blocks of 256 threads, fewer than 2^32 threads to a launch; 32-bit words and split bounds)
+    const int64_t most = g * ((z.longest + 63) / 64 + 1);
+    if (z.padded() * g >= (int64_t)1 << 24 || units * kDkdvMaxSplit >= (int64_t)1 << 28 || most * kDkdvMaxSplit >= (int64_t)1 << 31)
+        return fail(-1, "sizes too large");
+    // The dense kernels' choices (dkdv_waves_per_pair, dkdv_mode), for work that differs from pair to pair: a wave of its own
+    // for each pair where there are enough of them and the longest does not outlast an even share of all.
+    PlanRule r{g, work / kDkdvFill, true, 4};
+    if (pairs >= 3 * kDkdvFill && most <= kDkdvFewWavesMaxIters && most <= work / (4 * kDkdvFill) * 5 / 4) r.wpp = 1;
+    if (units <= kDkdvFill && r.splits(most) == 1) r.paired = false;
+    z.rule = r;
+    for (int64_t i = 0; i < n; ++i) {
+        const int64_t nkb = (lengths[i] + 63) / 64, np = r.paired ? (nkb + 1) / 2 : nkb;
+        for (int64_t pj = 0; pj < np; ++pj) {
+            const int64_t ns = r.splits(r.iters(nkb, pj));
+            z.nunits += ns * KVH;
+            if (ns > 1) z.nsums += KVH, z.nslots += ns * KVH;
+        }
+    }
+    if (z.words() >= (int64_t)1 << 31) return fail(-1, "sizes too large");
+    *out = z;
+    return 0;
+}
+
+// The header of a plan that nn_fa_packed_plan filled.
+int take_plan(const int32_t* plan, const int32_t* device_plan, int64_t D, int dtype, PlanHead* out) {
+    if (!plan || !device_plan) return fail(-1, "null plan");
+    if (!aligned16(device_plan)) return fail(-1, "the device's plan must be 16-byte aligned");
+    memcpy(out, plan, sizeof *out);
+    if (out->magic != kPlanMagic) return fail(-1, "not a plan of nn_fa_packed_plan");
+    return check_dims(1, out->H, out->KVH, out->tokens, D, dtype);
+}
+
+// The layouts of packed tensors: {head, row} strides, `count` pairs of them, or dense.
+int take_packed_lays(const int64_t* strides, const PlanHead& p, int64_t D, bool bwd, Lays* out) {
+    const Lay q{0, (long long)D, (int)(p.H * D)}, k{0, (long long)D, (int)(p.KVH * D)};
+    *out = shared_lays(q, k);
+    if (!strides) {
+        if ((int64_t)p.longest * p.H * D >= (int64_t)1 << 30) return fail(-1, "sizes too large");
+        return 0;
+    }
+    Lays l{};
+    const struct {
+        Lay* to;
+        int64_t heads;
+        const char* what;
+    } all[5] = {{&l.q, p.H, "q/dO"}, {&l.k, p.KVH, "k/v"}, {&l.o, p.H, "o"}, {&l.dq, p.H, "dq"}, {&l.dk, p.KVH, "dk/dv"}};
+    for (int i = 0; i < (bwd ? 5 : 3); ++i) {
+        const int64_t three[3] = {8, strides[2 * i], strides[2 * i + 1]};
+        if (int e = take_layout(three, all[i].heads, p.longest, D, all[i].what, all[i].to)) return e;
+        all[i].to->sb = 0;
+    }
+    *out = l;
+    return 0;
+}
+
+Workspace carve_packed(void* base, const PlanHead& p, int64_t D) {
+    const size_t vec = round256(4 * (size_t)p.H * p.tokens);
+    Workspace w;
+    w.nsplit = p.nslots > 0 ? 2 : 1;
+    w.nD = (float*)base;
+    w.nL = (float*)((char*)base + vec);
+    w.part = (float*)((char*)base + 2 * vec);
+    w.bytes = 2 * vec + (size_t)p.nslots * 2 * kPairRows * D * 4;
+    return w;
+}
+
+template <int HD, int DT>
+int packed_fwd_impl(const void* q, const void* k, const void* v, void* o, float* lse, const PlanHead& p, const int32_t* dp, float scale,
+                    const Lays& l, hipStream_t st) {
+    const int g = p.H / p.KVH;
+    fa_fwd_kernel<HD, DT, false, true><<<dim3((unsigned)(p.ntiles * g)), dim3(256), 0, st>>>(
+        (const u16*)q, (const u16*)k, (const u16*)v, (u16*)o, lse, p.H, p.H, p.KVH, 0, 0, scale * kLog2e, l.q, l.k, l.o, RopeArgs{},
+        Packed{dp + p.tiles, p.ntiles, p.tokens});
+    return launch_status("fa_fwd_kernel (packed)");
+}
+
+template <int HD, int DT>
+int packed_bwd_impl(const void* dO, const void* q, const void* k, const void* v, const void* o, const float* lse, void* dq, void* dk, void* dv,
+                    const Workspace& w, const PlanHead& p, const int32_t* dp, float scale, const Lays& l, hipStream_t st) {
+    const int g = p.H / p.KVH;
+    fa_bwd_dq_kernel<HD, DT, false, true><<<dim3((unsigned)(p.ntiles * g)), dim3(256), 0, st>>>(
+        (const u16*)q, (const u16*)k, (const u16*)v, (const u16*)o, (const u16*)dO, lse, w.nL, w.nD, (u16*)dq, p.H, p.H, p.KVH, 0, 0, scale * kLog2e,
+        scale, l.q, l.k, l.o, l.dq, RopeArgs{}, Packed{dp + p.tiles, p.ntiles, p.tokens});
+    if (int e = launch_status("fa_bwd_dq_kernel (packed)")) return e;
+    auto launch = [&](auto kern, int per) {
+        kern<<<dim3((unsigned)((p.nunits + per - 1) / per)), dim3(256), 0, st>>>(
+            (const u16*)q, (const u16*)k, (const u16*)v, (const u16*)dO, w.nL, w.nD, (u16*)dk, (u16*)dv, p.KVH, p.H, p.KVH, 0, 0, 0, scale * kLog2e,
+            scale, l.q, l.k, l.dk, 1, w.part, 1, Packed{dp + p.units, p.nunits, p.tokens});
+    };
+    if (p.wpp == 1)
+        launch(fa_bwd_dkdv_kernel<HD, DT, 1, false, true>, 4);
+    else if (HD == 64 && p.longest <= 2048)  // (as the dense pairs', see dkdv_impl)
+        launch(fa_bwd_dkdv_kernel<HD, DT, 4, true, true>, 1);
+    else
+        launch(fa_bwd_dkdv_kernel<HD, DT, 4, false, true>, 1);
+    if (int e = launch_status("fa_bwd_dkdv_kernel (packed)")) return e;
+    if (p.nsums == 0) return 0;
+    fa_packed_sum_kernel<HD, DT><<<dim3((unsigned)p.nsums), dim3(256), 0, st>>>(w.part, (u16*)dk, (u16*)dv, (const PackedUnit*)(dp + p.sums), l.dk);
+    return launch_status("fa_packed_sum_kernel");
+}
+
+}  // namespace
+
+NNFA_API size_t nn_fa_packed_plan_words(const int64_t* lengths, int64_t n, int64_t H, int64_t KVH) {
+    PlanSize z;
+    return plan_size(lengths, n, H, KVH, &z) ? 0 : (size_t)z.words();
+}
+
+NNFA_API int nn_fa_packed_plan(const int64_t* lengths, int64_t n, int64_t H, int64_t KVH, int32_t* plan, size_t words) {
+    PlanSize z;
+    if (int e = plan_size(lengths, n, H, KVH, &z)) return e;
+    if (!plan || ((uintptr_t)plan & 3u)) return fail(-1, "plan must be a 4-byte aligned buffer");
+    if (words != (size_t)z.words()) return fail(-1, "the plan has %lld words, %zu given", (long long)z.words(), words);
+    const PlanRule& r = z.rule;
+    PlanHead p{};
+    p.magic = kPlanMagic, p.words = (int32_t)words, p.n = (int32_t)std::min<int64_t>(n, INT32_MAX), p.H = (int32_t)H, p.KVH = (int32_t)KVH;
+    p.tokens = (int32_t)z.tokens, p.longest = (int32_t)z.longest;
+    p.ntiles = (int32_t)z.padded(), p.nunits = (int32_t)z.nunits, p.nsums = (int32_t)z.nsums, p.nslots = (int32_t)z.nslots, p.wpp = r.wpp;
+    p.tiles = 16, p.units = p.tiles + 4 * p.ntiles, p.sums = p.units + 8 * p.nunits, p.positions = p.sums + 8 * p.nsums;
+    memcpy(plan, &p, sizeof p);
+    PackedTile* tile = (PackedTile*)(plan + p.tiles);
+    PackedUnit* unit = (PackedUnit*)(plan + p.units);
+    PackedUnit* sum = (PackedUnit*)(plan + p.sums);
+    int32_t* pos = plan + p.positions;
+    PackedTile* const tile0 = tile;
+    PackedUnit* const unit0 = unit;
+    int start = 0, slot = 0;
+    for (int64_t i = 0; i < n; ++i) {
+        const int len = (int)lengths[i], nkb = (len + 63) / 64, np = r.paired ? (nkb + 1) / 2 : nkb;
+        for (int t = 0; t < len; ++t) *pos++ = t;
+        for (int kvh = 0; kvh < KVH; ++kvh) {
+            for (int qb = 0; qb < (len + 127) / 128; ++qb) *tile++ = PackedTile{start, len, qb, kvh};
+            for (int pj = 0; pj < np; ++pj) {
+                const int ns = (int)r.splits(r.iters(nkb, pj));
+                if (ns > 1) *sum++ = PackedUnit{start, len, pj, kvh, ns, 0, slot, 1};
+                for (int s = 0; s < ns; ++s) *unit++ = PackedUnit{start, len, pj, kvh, ns, s, ns > 1 ? slot++ : 0, r.paired ? 1 : 0};
+            }
+        }
+        start += len;
+    }
+    // Longest work first, so that what is left at the end is short; the rest of the order is any that is always the same.
+    std::sort(tile0, tile, [](const PackedTile& a, const PackedTile& b) {
+        return a.qb != b.qb ? a.qb > b.qb : a.start != b.start ? a.start < b.start : a.kvh < b.kvh;
+    });
+    std::sort(unit0, unit, [&](const PackedUnit& a, const PackedUnit& b) {
+        const int64_t wa = r.iters((a.len + 63) / 64, a.pj) * b.nsplit, wb = r.iters((b.len + 63) / 64, b.pj) * a.nsplit;
+        if (wa != wb) return wa > wb;
+        return a.start != b.start ? a.start < b.start : a.pj != b.pj ? a.pj < b.pj : a.sidx != b.sidx ? a.sidx < b.sidx : a.kvh < b.kvh;
+    });
+    while (tile < tile0 + p.ntiles) *tile++ = PackedTile{0, 0, 0, 0};
+    return 0;
+}
+
+NNFA_API int nn_fa_packed_plan_info(const int32_t* plan, nn_fa_packed_info* info) {
+    g_last_error.clear();
+    if (!plan || !info) return fail(-1, "null pointer argument");
+    PlanHead p;
+    memcpy(&p, plan, sizeof p);
+    if (p.magic != kPlanMagic) return fail(-1, "not a plan of nn_fa_packed_plan");
+    *info = nn_fa_packed_info{p.words, p.n, p.H, p.KVH, p.tokens, p.longest};
+    return 0;
+}
+
+NNFA_API int nn_fa_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* plan, const int32_t* device_plan,
+                              int64_t D, const int64_t* strides, int dtype, float scale, void* stream) {
+    g_last_error.clear();
+    PlanHead p;
+    if (int e = take_plan(plan, device_plan, D, dtype, &p)) return e;
+    if (p.tokens == 0) return 0;
+    if (!q || !k || !v || !o || !lse) return fail(-1, "null pointer argument");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)) return fail(-1, "inputs must be 16-byte aligned");
+    Lays l;
+    if (int e = take_packed_lays(strides, p, D, false, &l)) return e;
+    return NNFA_DISPATCH(packed_fwd_impl, D, dtype, q, k, v, o, lse, p, device_plan, scale, l, (hipStream_t)stream);
+}
+
+NNFA_API size_t nn_fa_packed_bwd_workspace_size(const int32_t* plan, int64_t D) {
+    if (!plan || plan[0] != kPlanMagic || D < 0) return 0;
+    PlanHead p;
+    memcpy(&p, plan, sizeof p);
+    return carve_packed(nullptr, p, D).bytes;
+}
+
+NNFA_API int nn_fa_packed_bwd(const void* dO, const void* q, const void* k, const void* v, const void* o, const float* lse, void* dq, void* dk,
+                              void* dv, void* workspace, size_t workspace_bytes, const int32_t* plan, const int32_t* device_plan, int64_t D,
+                              const int64_t* strides, int dtype, float scale, void* stream) {
+    g_last_error.clear();
+    PlanHead p;
+    if (int e = take_plan(plan, device_plan, D, dtype, &p)) return e;
+    if (p.tokens == 0) return 0;
+    if (!dO || !q || !k || !v || !o || !lse || !dq || !dk || !dv) return fail(-1, "null pointer argument");
+    if (!aligned16(dO) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
+        return fail(-1, "inputs must be 16-byte aligned");
+    if (!(scale > 0.f)) return fail(-1, "scale must be positive");
+    if (!workspace) return fail(-1, "null workspace");
+    if (((uintptr_t)workspace & 255u) != 0) return fail(-1, "workspace must be 256-byte aligned");
+    const Workspace w = carve_packed(workspace, p, D);
+    if (workspace_bytes < w.bytes) return fail(-1, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, w.bytes);
+    Lays l;
+    if (int e = take_packed_lays(strides, p, D, true, &l)) return e;
+    return NNFA_DISPATCH(packed_bwd_impl, D, dtype, dO, q, k, v, o, lse, dq, dk, dv, w, p, device_plan, scale, l, (hipStream_t)stream);
 }
 
 #if NN_TIMELINE

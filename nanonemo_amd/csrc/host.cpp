@@ -9,7 +9,7 @@
 //
 // Every function allocates through PyTorch's caching allocator, launches on PyTorch's current stream of its inputs'
 // device, and neither synchronises nor keeps state between calls. (The embedding's and the distillation loss's autograd nodes
-// are here as well, see there.)
+// are here as well, see there, and so are the packed attention's and the query and key norm's.)
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
@@ -36,6 +36,8 @@
 #include "nanonemo_fa.h"
 #include "nanonemo_linear.h"
 #include "nanonemo_loss.h"
+#include "nanonemo_packed.h"
+#include "nanonemo_qk_norm.h"
 #include "nanonemo_rmsnorm.h"
 #include "nanonemo_rope.h"
 
@@ -64,6 +66,7 @@ void lin_done(int rc) { done(rc, nn_linear_last_error); }
 void loss_done(int rc) { done(rc, nn_loss_last_error); }
 void emb_done(int rc) { done(rc, nn_embedding_last_error); }
 void dis_done(int rc) { done(rc, nn_distill_last_error); }
+void qkn_done(int rc) { done(rc, nn_qk_norm_last_error); }
 
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
@@ -790,7 +793,202 @@ Tensor distill_bwd_op(const Tensor& d_loss, const Tensor& logits, const Tensor& 
     return distill_bwd(d_loss, logits, values, indices, targets, stats, temperature, weight);
 }
 
-// ---- the two as autograd nodes ------------------------------------------------------------------
+// ---- attention over packed sequences ------------------------------------------------------------
+
+// The plan of a batch of sequences (nn_fa_packed_plan), an int32 vector in host memory.
+Tensor packed_plan(const std::vector<int64_t>& lengths, int64_t H, int64_t KVH) {
+    const size_t n = nn_fa_packed_plan_words(lengths.data(), (int64_t)lengths.size(), H, KVH);
+    if (!n) fa_done(-1);
+    Tensor plan = at::empty({(int64_t)n}, at::kInt);
+    fa_done(nn_fa_packed_plan(lengths.data(), (int64_t)lengths.size(), H, KVH, plan.data_ptr<int32_t>(), n));
+    return plan;
+}
+
+// A call's plan: in host memory and, the same, on the tensors' device.
+struct Plan {
+    Tensor host, device;
+    nn_fa_packed_info info;
+    Plan(const Tensor& device_, const Tensor& host_) : host(host_), device(device_) {
+        need(host.device().is_cpu() && host.scalar_type() == at::kInt && host.dim() == 1 && host.is_contiguous() && host.numel() >= 16 &&
+                 device.scalar_type() == at::kInt && device.sizes() == host.sizes() && device.is_contiguous(),
+             "plan and plan_host must be a Packing's");
+        fa_done(nn_fa_packed_plan_info(at_host(), &info));
+        need(info.words == host.numel(), "plan and plan_host must be a Packing's");
+    }
+    const int32_t* at_host() const { return host.data_ptr<int32_t>(); }
+    const int32_t* at_device() const { return device.data_ptr<int32_t>(); }
+};
+
+using S2 = std::array<int64_t, 2>;
+// The {head, row} strides through which the kernels can read the (tokens, heads, hd) tensor in place, if they can (strides_of).
+std::optional<S2> packed_strides(const Tensor& t) {
+    if (t.dim() != 3 || t.numel() == 0) return std::nullopt;
+    const auto s = strides_of(t.transpose(0, 1).unsqueeze(0));
+    if (!s) return std::nullopt;
+    return S2{(*s)[1], (*s)[2]};
+}
+// The two as the kernels read them, through strides that they share.
+void packed_readable(Tensor& a, Tensor& b) {
+    a = real_values(a), b = real_values(b);
+    const auto sa = packed_strides(a), sb = packed_strides(b);
+    if (a.size(-2) == b.size(-2) && sa && sb && *sa == *sb) return;
+    a = dense(a), b = dense(b);
+}
+S2 packed_known(const Tensor& t) { return t.is_contiguous() ? S2{t.size(2), t.size(1) * t.size(2)} : *packed_strides(t); }
+
+void check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Plan& p) {
+    need(q.is_cuda(), "inputs must be CUDA tensors");
+    check_on_device(q, {&k, &v, &p.device});
+    const int c = code(q);
+    need((c == 0 || c == 1) && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+         "inputs must be float16 or bfloat16 (all the same dtype)");
+    need(q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() && q.size(0) == k.size(0) && q.size(2) == k.size(2),
+         "expected q (tokens, H, hd) and k, v (tokens, KVH, hd)");
+    need(q.size(2) == 32 || q.size(2) == 64, "head_dim must be 32 or 64");
+    if (q.size(0) != p.info.tokens || q.size(1) != p.info.H || k.size(1) != p.info.KVH)
+        raise("the packing is of " + std::to_string(p.info.tokens) + " tokens, " + std::to_string(p.info.H) + " query and " + std::to_string(p.info.KVH) +
+              " KV heads, the tensors of " + std::to_string(q.size(0)) + ", " + std::to_string(q.size(1)) + " and " + std::to_string(k.size(1)));
+}
+
+T2 packed_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& plan, const Tensor& plan_host) {
+    const Plan p(plan, plan_host);
+    check_packed(q_, k_, v_, p);
+    const c10::DeviceGuard guard(q_.device());
+    Tensor q = q_, k = k_, v = v_, same = q_;
+    packed_readable(q, same);
+    packed_readable(k, v);
+    const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
+    Tensor o = empty_of(q, q.sizes()), lse = empty_f32(q, {H, T});
+    if (T == 0) return {o, lse};
+    const S2 s[3] = {packed_known(q), packed_known(k), packed_known(o)};
+    fa_done(nn_fa_packed_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(), p.at_host(), p.at_device(), D, s[0].data(),
+                             code(q), scale_of(D), stream_of(q)));
+    return {o, lse};
+}
+
+T3 packed_bwd(const Tensor& d_o_, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& o_, const Tensor& lse_, const Tensor& plan,
+              const Tensor& plan_host) {
+    const Plan p(plan, plan_host);
+    check_packed(q_, k_, v_, p);
+    check_on_device(q_, {&d_o_, &o_, &lse_});
+    const int64_t T = q_.size(0), H = q_.size(1), D = q_.size(2);
+    need(d_o_.sizes() == q_.sizes() && d_o_.scalar_type() == q_.scalar_type() && o_.sizes() == q_.sizes() && o_.scalar_type() == q_.scalar_type(),
+         "d_o and o must be of q's shape and type");
+    need(lse_.sizes() == at::IntArrayRef({H, T}) && lse_.scalar_type() == at::kFloat, "lse must be a float32 tensor of shape (H, tokens)");
+    const c10::DeviceGuard guard(q_.device());
+    Tensor q = q_, d_o = d_o_, k = k_, v = v_;
+    packed_readable(q, d_o);
+    packed_readable(k, v);
+    const Tensor o = dense(o_), lse = contig(lse_);
+    Tensor dq = empty_of(q, q.sizes()), dk = empty_of(k, k.sizes()), dv = empty_of(v, v.sizes());
+    if (T == 0) return {dq, dk, dv};
+    const size_t n = nn_fa_packed_bwd_workspace_size(p.at_host(), D);
+    Tensor ws = bytes(q, n);
+    const S2 s[5] = {packed_known(q), packed_known(k), packed_known(o), packed_known(dq), packed_known(dk)};
+    fa_done(nn_fa_packed_bwd(d_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
+                             dv.data_ptr(), ws.data_ptr(), n, p.at_host(), p.at_device(), D, s[0].data(), code(q), scale_of(D), stream_of(q)));
+    return {dq, dk, dv};
+}
+T3 packed_bwd_op(const Tensor& d_o, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& plan,
+                 const Tensor& plan_host) {
+    refuse_capture_from_engine("flash_attn_packed backward op");
+    return packed_bwd(d_o, q, k, v, o, lse, plan, plan_host);
+}
+
+// ---- norm and rotation of queries and keys ------------------------------------------------------
+
+// (..., heads, hd) with one or two leading dimensions, as the library reads it: tokens of one stride, 16-byte groups.
+struct Tokens {
+    Tensor t;
+    int64_t M, heads, D;
+    S2 s;  // {token, head}
+    explicit Tokens(const Tensor& given) : t(real_values(given)) {
+        const int64_t n = t.dim();
+        D = t.size(n - 1), heads = t.size(n - 2), M = n == 4 ? t.size(0) * t.size(1) : t.size(0);
+        const int64_t T = t.size(n - 3), st = T > 1 ? t.stride(n - 3) : n == 4 && t.size(0) > 1 ? t.stride(0) : heads * D;
+        s = {st, heads > 1 ? t.stride(n - 2) : 8};
+        const bool flat = n == 3 || t.size(0) <= 1 || t.stride(0) == T * st;
+        if (t.numel() && flat && t.stride(n - 1) == 1 && s[0] > 0 && s[0] % 8 == 0 && s[1] > 0 && s[1] % 8 == 0 && (uintptr_t)t.data_ptr() % 16 == 0) return;
+        t = dense(t);
+        s = {heads * D, D};
+    }
+};
+
+// What the two directions check and read alike.
+struct NormCall {
+    Tensor wq, wk, cos, sin, positions;
+    int64_t T, period;
+    int bits = 0;
+    NormCall(const Tensor& q, const Tensor& k, const Tensor& wq_, const Tensor& wk_, const Tensor& cos_, const Tensor& sin_, const OptTensor& pos) {
+        check_on_device(q, {&k, &wq_, &wk_, &cos_, &sin_, pos ? &*pos : &q});
+        const int64_t n = q.dim();
+        need((n == 3 || n == 4) && k.dim() == n && q.sizes().slice(0, n - 2) == k.sizes().slice(0, n - 2) && q.size(n - 1) == k.size(n - 1),
+             "expected q (tokens, H, hd) and k (tokens, KVH, hd), or (B, T, heads, hd)");
+        need(code(q) >= 0 && k.scalar_type() == q.scalar_type(), "q and k must share a dtype in {float16, bfloat16, float32}");
+        const int64_t D = q.size(n - 1);
+        need(D > 0 && D % 16 == 0 && D <= 256, "head_dim must be a multiple of 16, up to 256");
+        need(q.size(n - 2) > 0 && k.size(n - 2) > 0, "q and k must have heads");
+        for (const Tensor* w : {&wq_, &wk_}) need(w->scalar_type() == at::kFloat && w->dim() == 1 && w->size(0) == D, "weights must be float32 of head_dim values");
+        need(cos_.scalar_type() == at::kFloat && sin_.scalar_type() == at::kFloat && cos_.sizes() == sin_.sizes() && cos_.dim() == 2 && cos_.size(1) == D / 2,
+             "cos/sin must be float32 (T_max, hd/2) tables");
+        T = period = q.size(n - 3);
+        if (pos) {
+            need(pos->scalar_type() == at::kLong || pos->scalar_type() == at::kInt, "positions must be int64 or int32");
+            need(pos->sizes() == q.sizes().slice(0, n - 2) || (pos->dim() == 1 && pos->size(0) == T), "positions must have one value for each token");
+            positions = contig(*pos);
+            bits = positions.scalar_type() == at::kLong ? 64 : 32;
+            period = positions.numel();
+        } else {
+            need(cos_.size(0) >= T, "cos/sin must be float32 tables of at least T rows");
+        }
+        wq = dense(wq_), wk = dense(wk_), cos = dense(cos_), sin = dense(sin_);
+    }
+    const void* at() const { return bits ? positions.data_ptr() : nullptr; }
+};
+
+T2 qk_norm_fwd(const Tensor& q_, const Tensor& k_, const Tensor& wq, const Tensor& wk, const Tensor& cos, const Tensor& sin, const OptTensor& positions,
+               double eps) {
+    need(q_.is_cuda(), "inputs must be CUDA tensors");
+    const NormCall c(q_, k_, wq, wk, cos, sin, positions);
+    const c10::DeviceGuard guard(q_.device());
+    Tensor qo = empty_of(q_, q_.sizes()), ko = empty_of(k_, k_.sizes());
+    if (qo.numel() == 0) return {qo, ko};
+    const Tokens q(q_), k(k_);
+    const S2 s[4] = {q.s, k.s, {q.heads * q.D, q.D}, {k.heads * k.D, k.D}};
+    qkn_done(nn_qk_norm_rope_fwd(q.t.data_ptr(), k.t.data_ptr(), c.wq.data_ptr<float>(), c.wk.data_ptr<float>(), c.cos.data_ptr<float>(),
+                                 c.sin.data_ptr<float>(), c.cos.size(0), c.at(), c.bits, c.period, qo.data_ptr(), ko.data_ptr(), q.M, q.heads, k.heads,
+                                 q.D, s[0].data(), (float)eps, code(q_), stream_of(q_)));
+    return {qo, ko};
+}
+
+using T4 = std::tuple<Tensor, Tensor, Tensor, Tensor>;
+T4 qk_norm_bwd(const Tensor& dq_, const Tensor& dk_, const Tensor& q_, const Tensor& k_, const Tensor& wq, const Tensor& wk, const Tensor& cos,
+               const Tensor& sin, const OptTensor& positions, double eps) {
+    need(q_.is_cuda(), "inputs must be CUDA tensors");
+    const NormCall c(q_, k_, wq, wk, cos, sin, positions);
+    check_on_device(q_, {&dq_, &dk_});
+    need(dq_.sizes() == q_.sizes() && dk_.sizes() == k_.sizes() && dq_.scalar_type() == q_.scalar_type() && dk_.scalar_type() == q_.scalar_type(),
+         "the gradients must be of the outputs' shapes and type");
+    const c10::DeviceGuard guard(q_.device());
+    Tensor dq = empty_of(q_, q_.sizes()), dk = empty_of(k_, k_.sizes()), dwq = empty_of(c.wq, c.wq.sizes()), dwk = empty_of(c.wk, c.wk.sizes());
+    if (dq.numel() == 0) return {dq, dk, dwq.zero_(), dwk.zero_()};
+    const Tokens q(q_), k(k_), gq(dq_), gk(dk_);
+    const S2 s[6] = {gq.s, gk.s, q.s, k.s, {q.heads * q.D, q.D}, {k.heads * k.D, k.D}};
+    const size_t n = nn_qk_norm_rope_bwd_workspace_size(q.M, q.heads, k.heads, q.D);
+    Tensor ws = bytes(q_, n);
+    qkn_done(nn_qk_norm_rope_bwd(gq.t.data_ptr(), gk.t.data_ptr(), q.t.data_ptr(), k.t.data_ptr(), c.wq.data_ptr<float>(), c.wk.data_ptr<float>(),
+                                 c.cos.data_ptr<float>(), c.sin.data_ptr<float>(), c.cos.size(0), c.at(), c.bits, c.period, dq.data_ptr(), dk.data_ptr(),
+                                 dwq.data_ptr<float>(), dwk.data_ptr<float>(), ws.data_ptr(), n, q.M, q.heads, k.heads, q.D, s[0].data(), (float)eps,
+                                 code(q_), stream_of(q_)));
+    return {dq, dk, dwq, dwk};
+}
+T4 qk_norm_bwd_op(const Tensor& dq, const Tensor& dk, const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& cos,
+                  const Tensor& sin, const OptTensor& positions, double eps) {
+    refuse_capture_from_engine("qk_norm_rope backward op");
+    return qk_norm_bwd(dq, dk, q, k, wq, wk, cos, sin, positions, eps);
+}
+
+// ---- these four as autograd nodes ---------------------------------------------------------------
 // A student's small batch is paced by the host: with an autograd.Function in Python, a lookup and its gradient took 56 us of host
 // time around 20 us of kernels, of which the engine's own hand-off between threads is about 35.
 using torch::autograd::AutogradContext;
@@ -880,6 +1078,75 @@ Tensor distill_call(const Tensor& logits, const Tensor& values, const Tensor& in
     return DistillNode::apply(logits, values, indices, rest, targets, temperature, weight);
 }
 
+struct PackedNode : torch::autograd::Function<PackedNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& plan, const Tensor& plan_host) {
+        Tensor q = q_, k = k_, v = v_, o, lse;
+        {
+            const at::AutoDispatchBelowADInplaceOrView below;
+            if (k.dim() == 3 && v.dim() == 3) packed_readable(k, v);  // copies that the backward would make again
+            std::tie(o, lse) = packed_fwd(q, k, v, plan, plan_host);
+        }
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({q, k, v, o, lse, plan, plan_host});
+        return o;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_capture("flash_attn_packed backward");
+        const auto t = ctx->get_saved_variables();
+        variable_list out(5);
+        if (!grads[0].defined()) return out;
+        const Tensor d_o = readable_grad(grads[0]);
+        {
+            const at::AutoDispatchBelowADInplaceOrView below;
+            std::tie(out[0], out[1], out[2]) = packed_bwd(d_o, t[0], t[1], t[2], t[3], t[4], t[5], t[6]);
+        }
+        for (int i = 0; i < 3; ++i) out[i] = once(out[i], "flash_attn_packed");
+        return out;
+    }
+};
+Tensor packed_call(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& plan, const Tensor& plan_host) {
+    if (!records(q) && !records(k) && !records(v)) return std::get<0>(packed_fwd(q, k, v, plan, plan_host));
+    refuse_capture("flash_attn_packed");
+    return PackedNode::apply(q, k, v, plan, plan_host);
+}
+
+struct QkNormNode : torch::autograd::Function<QkNormNode> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& cos,
+                                 const Tensor& sin, const OptTensor& positions, double eps) {
+        Tensor qo, ko;
+        {
+            const at::AutoDispatchBelowADInplaceOrView below;
+            std::tie(qo, ko) = qk_norm_fwd(q, k, wq, wk, cos, sin, positions, eps);
+        }
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({q, k, wq, wk, cos, sin, positions ? *positions : Tensor()});
+        ctx->saved_data["eps"] = eps;
+        return {qo, ko};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_capture("qk_norm_rope backward");
+        const auto t = ctx->get_saved_variables();
+        variable_list out(8);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        {
+            const Tensor dq = grads[0].defined() ? readable_grad(grads[0]) : at::zeros(t[0].sizes(), t[0].options());
+            const Tensor dk = grads[1].defined() ? readable_grad(grads[1]) : at::zeros(t[1].sizes(), t[1].options());
+            const at::AutoDispatchBelowADInplaceOrView below;
+            std::tie(out[0], out[1], out[2], out[3]) =
+                qk_norm_bwd(dq, dk, t[0], t[1], t[2], t[3], t[4], t[5], t[6].defined() ? OptTensor(t[6]) : std::nullopt, ctx->saved_data["eps"].toDouble());
+        }
+        for (int i = 0; i < 4; ++i) out[i] = once(out[i], "qk_norm_rope");
+        return out;
+    }
+};
+T2 qk_norm_call(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& cos, const Tensor& sin, const OptTensor& positions,
+                double eps) {
+    if (!records(q) && !records(k) && !records(wq) && !records(wk)) return qk_norm_fwd(q, k, wq, wk, cos, sin, positions, eps);
+    refuse_capture("qk_norm_rope");
+    const variable_list out = QkNormNode::apply(q, k, wq, wk, cos, sin, positions, eps);
+    return {out[0], out[1]};
+}
+
 // ---- routing ------------------------------------------------------------------------------------
 
 // Whether the tensor's values lie at its address, as dense values of its own type: not inside a transform's wrapper
@@ -942,6 +1209,10 @@ TORCH_LIBRARY_IMPL(nanonemo, CUDA, m) {
     m.impl("top_logits", top_logits);
     m.impl("distill_loss", distill_fwd);
     m.impl("distill_loss_bwd", distill_bwd_op);
+    m.impl("flash_attn_packed", packed_fwd);
+    m.impl("flash_attn_packed_bwd", packed_bwd_op);
+    m.impl("qk_norm_rope", qk_norm_fwd);
+    m.impl("qk_norm_rope_bwd", qk_norm_bwd_op);
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -965,6 +1236,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("distill", distill_call, nogil);
     m.def("distill_fwd", distill_fwd, nogil);
     m.def("distill_bwd", distill_bwd, nogil);
+    m.def("packed_plan", packed_plan, nogil);
+    m.def("packed", packed_call, nogil);
+    m.def("packed_fwd", packed_fwd, nogil);
+    m.def("packed_bwd", packed_bwd, nogil);
+    m.def("qk_norm_rope", qk_norm_call, nogil);
+    m.def("qk_norm_fwd", qk_norm_fwd, nogil);
+    m.def("qk_norm_bwd", qk_norm_bwd, nogil);
     m.def("wgrad", wgrad, nogil);
     m.def("wgrad_takes", wgrad_takes);
     m.def("rows_aligned", rows_aligned);

@@ -77,6 +77,15 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "nn_fa_last_error": (ctypes.c_char_p, []),
     "nn_fa_abi_version": (_int, []),
+    # include/nanonemo_packed.h
+    "nn_fa_packed_plan_words": (_sz, [_i64p, _i64, _i64, _i64]),
+    "nn_fa_packed_plan": (_int, [_i64p, _i64, _i64, _i64, _vp, _sz]),
+    "nn_fa_packed_plan_info": (_int, [_vp, _i64p]),
+    "nn_fa_packed_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64p, _int, _f32, _vp]),
+    "nn_fa_packed_bwd_workspace_size": (_sz, [_vp, _i64]),
+    "nn_fa_packed_bwd": (
+        _int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _i64, _i64p, _int, _f32, _vp]
+    ),
     # include/nanonemo_rope.h
     "nn_rope_qk": (
         _int,
@@ -129,6 +138,18 @@ SIGNATURES: dict[str, tuple] = {
         _int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f64, _f64, _int, _int, _vp]
     ),
     "nn_distill_last_error": (ctypes.c_char_p, []),
+    # include/nanonemo_qk_norm.h
+    "nn_qk_norm_rope_fwd": (
+        _int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _int, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64p, _f32, _int, _vp],
+    ),
+    "nn_qk_norm_rope_bwd_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
+    "nn_qk_norm_rope_bwd": (
+        _int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _int, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i64, _i64p, _f32,
+         _int, _vp],
+    ),
+    "nn_qk_norm_last_error": (ctypes.c_char_p, []),
 }
 
 ABI_VERSION = 11
@@ -266,6 +287,13 @@ def check_distill(rc: int) -> None:
     if rc != 0:
         msg = lib().nn_distill_last_error().decode(errors="replace")
         raise RuntimeError(msg or f"nanonemo_distill call failed with code {rc}")
+
+
+def check_qk_norm(rc: int) -> None:
+    """Raise RuntimeError with the library's message when an nn_qk_norm_* entry point returns non-zero."""
+    if rc != 0:
+        msg = lib().nn_qk_norm_last_error().decode(errors="replace")
+        raise RuntimeError(msg or f"nanonemo_qk_norm call failed with code {rc}")
 
 
 def check_rmsnorm(rc: int) -> None:

@@ -1,0 +1,281 @@
+"""GPU tests of attention over packed sequences (kernels/hip/packed.py): against float64, against the dense attention on each
+sequence alone, bit for bit, and where it is called from."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tests.common import TOL, TOL_GRAD, assert_close_tol
+
+pytestmark = pytest.mark.gpu
+
+# lengths, H, KVH, hd: tile and unit edges with empty sequences; an odd group; one long sequence among short ones, whose pairs
+# are split; few tokens, a block for each unit; many sequences, a wave for each pair; lengths of 1 and 2; long and split, MQA.
+CASES = [
+    ([63, 0, 64, 65, 1, 127, 128, 129, 0, 191, 192, 193, 0], 12, 4, 64),
+    ([63, 64, 65, 1, 127, 128, 129, 300], 6, 2, 32),
+    ([2500, 17, 130, 3], 12, 4, 64),
+    ([200, 56], 12, 4, 64),
+    ([100, 37, 64, 70] * 60, 12, 4, 64),
+    ([1, 2, 1, 1, 3] * 80, 8, 8, 32),
+    ([3000], 12, 1, 64),
+    ([1111, 999, 1], 4, 4, 32),
+]
+IDS = [f"{len(c[0])}x{max(c[0])}-{c[1]}-{c[2]}-{c[3]}" for c in CASES]
+
+
+def _packing(lengths, H, KVH):
+    from nanonemo_amd.kernels.hip.packed import Packing
+
+    return Packing(lengths, H, KVH)
+
+
+def _call(*args):
+    from nanonemo_amd.kernels.hip.packed import flash_attn_packed
+
+    return flash_attn_packed(*args)
+
+
+def _inputs(lengths, H, KVH, D, dtype, seed=0, mult=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    T = sum(lengths)
+    q, k, v = ((mult * torch.randn(T, n, D, device="cuda", generator=g)).to(dtype) for n in (H, KVH, KVH))
+    return q, k, v, torch.randn(T, H, D, device="cuda", generator=g).to(dtype)
+
+
+def _float64(q, k, v, do, lengths):
+    """(o, dq, dk, dv) of the definition, a sequence and a head at a time."""
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    o, dq, dk, dv = (torch.zeros_like(t) for t in (q, q, k, v))
+    group, scale, a = q.shape[1] // k.shape[1], 1 / math.sqrt(q.shape[2]), 0
+    for n in lengths:
+        r = slice(a, a + n)
+        a += n
+        future = torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1)
+        for h in range(q.shape[1] if n else 0):
+            j = h // group
+            p = torch.softmax((q[r, h] @ k[r, j].t() * scale).masked_fill(future, -math.inf), -1)
+            o[r, h] = p @ v[r, j]
+            dp = do[r, h] @ v[r, j].t()
+            ds = p * (dp - (do[r, h] * o[r, h]).sum(-1, keepdim=True)) * scale
+            dq[r, h] = ds @ k[r, j]
+            dk[r, j] += ds.t() @ q[r, h]
+            dv[r, j] += p.t() @ do[r, h]
+    return o, dq, dk, dv
+
+
+def _run(q, k, v, do, packing):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = _call(*leaves, packing)
+    return (o.detach(), *torch.autograd.grad(o, leaves, do))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths, H, KVH, D", CASES, ids=IDS)
+def test_matches_float64(lengths, H, KVH, D, dtype):
+    print(f"\n[case] packed {len(lengths)} sequences of up to {max(lengths)}, H={H} KVH={KVH} D={D} {dtype}", flush=True)
+    q, k, v, do = _inputs(lengths, H, KVH, D, dtype)
+    got = _run(q, k, v, do, _packing(lengths, H, KVH))
+    for name, x, ref, tol in zip(("o", "dq", "dk", "dv"), got, _float64(q, k, v, do, lengths), (TOL, TOL_GRAD, TOL_GRAD, TOL_GRAD)):
+        assert_close_tol(x, ref, tol[dtype], name)
+
+
+@pytest.mark.parametrize("lengths, H, KVH, D", CASES, ids=IDS)
+def test_a_sequence_is_the_dense_attention_on_it_alone(lengths, H, KVH, D):
+    from nanonemo_amd.kernels.hip.flash_attn import flash_attn_bthd
+
+    print(f"\n[case] packed against dense, {len(lengths)} sequences of up to {max(lengths)}, H={H} KVH={KVH} D={D}", flush=True)
+    q, k, v, do = _inputs(lengths, H, KVH, D, torch.bfloat16, seed=1)
+    o, dq, dk, dv = _run(q, k, v, do, _packing(lengths, H, KVH))
+    a = 0
+    for n in lengths[:20]:
+        if n:
+            alone = [t[None, a : a + n].clone().requires_grad_() for t in (q, k, v)]
+            y = flash_attn_bthd(*alone)
+            gq, gk, gv = torch.autograd.grad(y, alone, do[None, a : a + n].contiguous())
+            assert torch.equal(y[0], o[a : a + n]) and torch.equal(gq[0], dq[a : a + n]), (a, n)
+            # (dk and dv: other blocks may share the sums, each rounded to bf16 at the end: two roundings apart, and the fp32 sums' order)
+            for x, y in ((gk[0], dk[a : a + n]), (gv[0], dv[a : a + n])):
+                torch.testing.assert_close(x.float(), y.float(), rtol=2**-7, atol=1e-5 * x.abs().max().item())
+        a += n
+
+
+def test_two_runs_give_the_same_bits():
+    for lengths, H, KVH, D in (CASES[2], CASES[4]):
+        q, k, v, do = _inputs(lengths, H, KVH, D, torch.bfloat16, seed=2)
+        packing = _packing(lengths, H, KVH)
+        first = _run(q, k, v, do, packing)
+        for again in (packing, _packing(torch.tensor(lengths), H, KVH)):
+            assert all(torch.equal(a, b) for a, b in zip(first, _run(q, k, v, do, again)))
+
+
+@pytest.mark.parametrize("lengths, H, KVH, D", [CASES[0], CASES[2], CASES[4]], ids=[IDS[0], IDS[2], IDS[4]])
+def test_sequences_do_not_see_each_other(lengths, H, KVH, D):
+    print(f"\n[case] packed among NaN, {len(lengths)} sequences", flush=True)
+    q, k, v, do = _inputs(lengths, H, KVH, D, torch.bfloat16, seed=3)
+    packing = _packing(lengths, H, KVH)
+    ref = _run(q, k, v, do, packing)
+    for parity in (0, 1):  # every other sequence of NaN and infinity
+        bad = torch.cat([torch.full((n,), i % 2 == parity, device="cuda") for i, n in enumerate(lengths)])
+        q2, k2, v2, do2 = (t.clone() for t in (q, k, v, do))
+        for t, x in ((q2, math.nan), (k2, math.inf), (v2, math.nan), (do2, -math.inf)):
+            t[bad] = x
+        for a, b in zip(_run(q2, k2, v2, do2, packing), ref):
+            assert torch.equal(a[~bad], b[~bad])
+
+
+def test_rows_of_equal_and_of_large_scores():
+    lengths, H, KVH, D = [300, 77, 1], 4, 2, 64
+    q, k, v, do = _inputs(lengths, H, KVH, D, torch.bfloat16, seed=4)
+    packing = _packing(lengths, H, KVH)
+    o = _call(torch.zeros_like(q), k, v, packing)  # the mean of the values so far
+    a = 0
+    for n in lengths:
+        mean = v[a : a + n].double().cumsum(0) / torch.arange(1, n + 1, device="cuda").view(-1, 1, 1)
+        assert_close_tol(o[a : a + n], mean.repeat_interleave(2, 1), TOL[torch.bfloat16], "mean")
+        a += n
+    q, k, v, do = _inputs(lengths, H, KVH, D, torch.bfloat16, seed=5, mult=3.0)
+    for name, x, ref, tol in zip(("o", "dq", "dk", "dv"), _run(q, k, v, do, packing), _float64(q, k, v, do, lengths), (TOL, TOL_GRAD, TOL_GRAD, TOL_GRAD)):
+        assert_close_tol(x, ref, tol[torch.bfloat16], name)
+
+
+def test_gradients_match_differences():
+    lengths, H, KVH, D = [5, 1, 9], 4, 2, 32
+    q, k, v, do = _inputs(lengths, H, KVH, D, torch.float16, seed=6)
+    packing = _packing(lengths, H, KVH)
+    _, *grads = _run(q, k, v, do, packing)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    for i, grad in enumerate(grads):
+        # Along a direction of 0.25 steps, which fp16 holds beside values of up to 4 but for their own rounding (taken from what
+        # the call is given). The loss is a sum of 15 * 4 * 32 products of outputs rounded to 11 bits: an error of 2^-11 of
+        # about 1 each, of random sign: 2^-11 sqrt(1920) = 0.02 a side, over 2 * 0.25; third derivatives 0.25^2 / 6 of the
+        # same order as the derivative.
+        step = 0.25 * torch.sign(torch.randn(grad.shape, device="cuda", generator=g))
+        ends = []
+        for sign in (1, -1):
+            ins = [q, k, v]
+            ins[i] = (ins[i] + sign * step).half()
+            ends.append((ins[i], (_call(*ins, packing).double() * do.double()).sum()))
+        moved = ends[0][0].double() - ends[1][0].double()
+        want, got = (ends[0][1] - ends[1][1]).item(), (grad.double() * moved).sum().item()
+        size = (grad.double() * moved).norm().item()  # random signs: the size of the sum that is compared
+        assert abs(got - want) <= 0.1 + 0.5 * size, (i, got, want, size)
+
+
+def test_projections_are_read_in_place_and_other_layouts_copied():
+    lengths, H, KVH, D = [70, 1, 200, 33], 12, 4, 64
+    T = sum(lengths)
+    packing = _packing(lengths, H, KVH)
+    q, k, v, do = _inputs(lengths, H, KVH, D, torch.bfloat16, seed=8)
+    ref = _run(q, k, v, do, packing)
+    qkv = torch.cat([t.view(T, -1) for t in (q, k, v)], 1)
+    cols = [t.view(T, -1, D) for t in qkv.split([H * D, KVH * D, KVH * D], 1)]  # a projection's column ranges
+    turned = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]  # heads outermost
+    odd = [torch.cat([t.new_zeros(4), t.flatten()])[4:].view(t.shape) for t in (q, k, v)]  # 8 bytes off
+    wide = [torch.stack([t, t], -1)[..., 0] for t in (q, k, v)]  # values not side by side
+    mixed = [cols[0], k, cols[2]]
+    for views in (cols, turned, odd, wide, mixed):
+        assert all(torch.equal(a, b) for a, b in zip(_run(*views, do, packing), ref))
+    for d in (do.transpose(0, 1).contiguous().transpose(0, 1), torch.cat([do.new_zeros(1), do.flatten()])[1:].view(do.shape)):
+        assert all(torch.equal(a, b) for a, b in zip(_run(q, k, v, d, packing), ref))
+    one = do[:, :1, :1].expand(T, H, D)  # a gradient without memory of its own
+    assert all(torch.equal(a, b) for a, b in zip(_run(q, k, v, one, packing), _run(q, k, v, one.contiguous(), packing)))
+    leaf = qkv.clone().requires_grad_()
+    qs, ks, vs = (t.view(T, -1, D) for t in leaf.split([H * D, KVH * D, KVH * D], 1))
+    (g,) = torch.autograd.grad(_call(qs, ks, vs, packing), leaf, do)
+    assert torch.equal(g, torch.cat([t.view(T, -1) for t in ref[1:]], 1))
+
+
+def test_nothing_to_do():
+    for lengths in ([], [0], [0, 0]):
+        packing = _packing(lengths, 4, 2)
+        q, k, v, do = _inputs(lengths, 4, 2, 64, torch.bfloat16)
+        assert [t.shape[0] for t in _run(q, k, v, do, packing)] == [0] * 4 and packing.positions.numel() == 0
+
+
+def test_op_and_eager_path_give_the_same_bits_and_the_op_passes_opcheck():
+    lengths, H, KVH, D = [70, 1, 0, 200, 33], 4, 2, 32
+    packing = _packing(lengths, H, KVH)
+    q, k, v, do = _inputs(lengths, H, KVH, D, torch.float16, seed=9)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = _call(*leaves, packing)
+    op, lse = torch.ops.nanonemo.flash_attn_packed(*leaves, packing.plan, packing.plan_host)
+    assert "PackedNode" in o.grad_fn.name() and torch.equal(o, op) and lse.shape == (H, sum(lengths))
+    ref = torch.autograd.grad(o, leaves, do, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(ref, torch.autograd.grad(op, leaves, do)))
+    torch.library.opcheck(torch.ops.nanonemo.flash_attn_packed, (*leaves, packing.plan, packing.plan_host))
+    torch.library.opcheck(torch.ops.nanonemo.flash_attn_packed_bwd, (do, *(t.detach() for t in leaves), op.detach(), lse.detach(), packing.plan, packing.plan_host))
+    f = torch.compile(lambda a, b, c: _call(a, b, c, packing) * 2, fullgraph=True, backend="aot_eager")
+    got = f(*leaves)
+    assert torch.equal(got, o * 2)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, leaves, do), torch.autograd.grad(o * 2, leaves, do)))
+    with torch.no_grad():
+        assert torch.equal(_call(*leaves, packing), o)
+
+
+def test_the_autograd_node_refuses_what_it_cannot_do():
+    lengths, H, KVH, D = [20, 5], 4, 2, 32
+    packing = _packing(lengths, H, KVH)
+    q, k, v, do = _inputs(lengths, H, KVH, D, torch.float16, seed=10)
+    q.requires_grad_()
+    (g,) = torch.autograd.grad(_call(q, k, v, packing).float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
+    with pytest.raises(RuntimeError, match="batched gradients"):
+        torch.autograd.grad(_call(q, k, v, packing), q, torch.ones(2, *q.shape, device="cuda", dtype=q.dtype), is_grads_batched=True)
+    o = _call(q, k, v, packing)
+    v.add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    o = _call(q, k, v, packing)
+    a, b = (torch.autograd.grad(o, q, do, retain_graph=True)[0] for _ in range(2))
+    assert torch.equal(a, b)
+
+
+def test_refusals():
+    packing = _packing([20, 5], 4, 2)
+    q, k, v, _ = _inputs([20, 5], 4, 2, 32, torch.float16)
+    for call, msg in ((lambda: _call(q[:24], k[:24], v[:24], packing), "the packing is of 25 tokens"), (lambda: _call(q[:, :2], k, v, packing), "the packing is of"), (lambda: _call(q, q, q, packing), "the packing is of"),
+                      (lambda: _call(q.float(), k.float(), v.float(), packing), "float16 or bfloat16"), (lambda: _call(q, k, v[:, :1], packing), "expected"), (lambda: _call(q[None], k[None], v[None], packing), "expected"),
+                      (lambda: _call(q[..., :16], k[..., :16], v[..., :16], packing), "head_dim"), (lambda: _call(q, k.cpu(), v, packing), "same device|CUDA"), (lambda: _call(q, k.bfloat16(), v, packing), "same dtype"),
+                      (lambda: torch.ops.nanonemo.flash_attn_packed(q, k, v, packing.plan[:-1], packing.plan_host), "Packing's"),
+                      (lambda: torch.ops.nanonemo.flash_attn_packed(q, k, v, packing.plan, packing.plan), "Packing's"),
+                      (lambda: torch.ops.nanonemo.flash_attn_packed(q, k, v, torch.zeros_like(packing.plan), torch.zeros_like(packing.plan_host)), "not a plan")):
+        with pytest.raises(RuntimeError, match=msg):
+            call()
+
+
+def test_on_another_stream_and_captured_into_a_graph():
+    from nanonemo_amd.kernels.hip import host
+
+    print("\n[case] packed attention on a side stream and in a graph", flush=True)
+    lengths, H, KVH, D = [1500, 70, 33], 12, 4, 64  # split: the partial sums' launch too
+    packing = _packing(lengths, H, KVH)
+    q, k, v, do = _inputs(lengths, H, KVH, D, torch.bfloat16, seed=11)
+
+    def both():
+        o, lse = host().packed_fwd(q, k, v, packing.plan, packing.plan_host)
+        return (o, *host().packed_bwd(do, q, k, v, o, lse, packing.plan, packing.plan_host))
+
+    ref = both()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = both()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = both()
+    for i in range(4):
+        for t in (q, k, v, do):
+            t.copy_(torch.randn_like(t))
+        for t in outs:
+            t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, both())), i
