@@ -1099,8 +1099,10 @@ __global__ __launch_bounds__(256) void fa_bwd_dkdv_sum_kernel(const float* __res
     }
 }
 
-// The same for packed sequences: the pairs of units that several blocks shared, one block per pair and KV head (its PackedUnit:
-// nsplit partial sums from `slot` on).
+// The same for packed sequences: the pairs of units that several blocks shared, kSumBlocks blocks for each pair and KV head (its
+// PackedUnit: nsplit partial sums from `slot` on). A thread has two groups of 4 columns at head_dim 64, whose loads are under way
+// together. (One block for each: 8 us for 32 pairs of 4 parts, latency.)
+constexpr int kSumBlocks = 8;
 template <int HD, int DT>
 __global__ __launch_bounds__(256) void fa_packed_sum_kernel(const float* __restrict__ part, u16* __restrict__ dK, u16* __restrict__ dV,
                                                             const PackedUnit* __restrict__ list, Lay ldk) {
@@ -1109,11 +1111,14 @@ __global__ __launch_bounds__(256) void fa_packed_sum_kernel(const float* __restr
     const int nkb = (u.len + 63) / 64;
     constexpr int kOne = kPairRows * HD;  // values of one gradient's partial sum
     const float* from = part + (size_t)u.slot * 2 * kOne;
-    for (int i = threadIdx.x * 4; i < 2 * kOne; i += 1024) {
+#pragma unroll
+    for (int n = 0; n < 2 * kOne / (kSumBlocks * 1024); ++n) {
+        const int i = ((int)blockIdx.y * (2 * kOne / (kSumBlocks * 1024)) + n) * 1024 + (int)threadIdx.x * 4;
         const int which = i / kOne, row = i % kOne / HD, col = i % HD;
         const int unit = row < 64 ? u.pj : nkb - 1 - u.pj, key = unit * 64 + row % 64;
         if (key >= u.len || (row >= 64 && unit <= u.pj)) continue;  // (a middle unit has no partner)
         f32x4 acc = *reinterpret_cast<const f32x4*>(from + i);
+#pragma unroll 4
         for (int s = 1; s < u.nsplit; ++s) acc += *reinterpret_cast<const f32x4*>(from + (size_t)s * 2 * kOne + i);
         u16* dst = (which == 0 ? dK : dV) + ldk.at(0, u.kvh) + (size_t)(u.start + key) * ldk.st + col;
         *reinterpret_cast<u32x2*>(dst) = u32x2{E::pack2(acc[0], acc[1]), E::pack2(acc[2], acc[3])};
@@ -1354,6 +1359,294 @@ __global__ __launch_bounds__(256, 2) void fa_bwd_dq_kernel(const u16* __restrict
         }
     }
     NN_TL_END(kTlDq);
+}
+
+// ------------------------------------------------------------------------------------------
+// Packed sequences of up to kShort tokens: one wave for each 32 query rows of a head (forward, dQ), one for each 32 keys of a KV
+// head (dK/dV). A block of the kernels above carries 128 rows and its barriers for them: 7872 blocks of 24 tokens on average
+// took 44 us, mostly latency, where these waves, independent of each other and more of them to a CU, take 17 (and the backward 50 instead of 89). The
+// arithmetic of a row is that of the kernels above in the same order, so its bits are too (dk and dv: sums over the group's
+// heads in one wave instead of four).
+// Operands that need rows come straight from memory in their lanes' layout, those that need columns through the wave's own LDS
+// tile by DMA, whose rows past the sequence read as zeros. List entries: PackedTile with qb = the 32-row tile.
+// ------------------------------------------------------------------------------------------
+constexpr int kShort = 64;
+
+// A wave's 32 x HD result, held transposed (lane: row l32; element i of acc[dt]: column 32 dt + (i / 4) * 8 + 4 hh + i % 4),
+// times mul and rounded, to rows [0, left) of p: through the wave's own LDS tile, so that a store instruction writes whole rows.
+// (Stored from the lanes, each of 2 ND x 4 instructions touches 32 rows 16 bytes at a time.)
+template <int HD, int DT>
+__device__ inline void store_rows(const f32x16* acc, float mul, u16* lds, u16* p, int st, int left, int lane) {
+    using E = Elem<DT>;
+    constexpr int ND = HD / 32, CH = HD / 8;
+    const int l32 = lane & 31, hh = lane >> 5;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x16& a = acc[dt];
+            *reinterpret_cast<u32x2*>(lds + swz<HD>(l32, 32 * dt + 8 * g) + 4 * hh) =
+                u32x2{E::pack2(a[4 * g] * mul, a[4 * g + 1] * mul), E::pack2(a[4 * g + 2] * mul, a[4 * g + 3] * mul)};
+        }
+#pragma unroll
+    for (int n = 0; n < CH / 2; ++n) {
+        const int i = n * 64 + lane, r = i / CH, c = i % CH;
+        const u16x8 v = ld8(lds + swz<HD>(r, 8 * c));
+        if (r < left) *reinterpret_cast<u16x8*>(p + (size_t)r * st + 8 * c) = v;
+    }
+}
+
+template <int HD, int DT>
+__global__ __launch_bounds__(256, 4) void fa_short_fwd_kernel(const u16* __restrict__ Q, const u16* __restrict__ K, const u16* __restrict__ V,
+                                                              u16* __restrict__ O, float* __restrict__ LSE, Packed pk, int H, int KVH, float sl2,
+                                                              Lay lq, Lay lk, Lay lo) {
+    using E = Elem<DT>;
+    constexpr int NS = HD / 16, ND = HD / 32, TILE = 32 * HD;
+    __shared__ __attribute__((aligned(16))) u16 vS[4 * 2 * TILE];
+    const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5, g16 = (lane >> 4) & 1;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int item = (int)blockIdx.x * 4 + wave, at = item / H;
+    if (at >= pk.count) return;
+    const int h = item - at * H, kvh = h / (H / KVH);
+    const PackedTile e = static_cast<const PackedTile*>(pk.list)[at];
+    const int T = e.len, nt = e.qb + 1, qrow = 32 * e.qb + l32;  // nt: 32-key sub-tiles with a visible key
+    u16* vb = vS + wave * 2 * TILE;
+    const u16* Vp = V + lk.at(0, kvh) + (size_t)e.start * lk.st;
+    const u16* Kp = K + lk.at(0, kvh) + (size_t)e.start * lk.st;
+    const DmaOffs<HD, 32, 1> vfo = dma_offsets<HD, 32, 1>(lane, 0, lk.st);
+    u16x8 qf[NS], kq[2][NS];
+    {
+        const u16* qp = Q + lq.at(0, h) + (size_t)(e.start + min(qrow, T - 1)) * lq.st + 8 * hh;  // (rows past T: the last, not stored)
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qf[s] = ld8(qp + 16 * s);
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        if (t >= nt) break;
+        const u16* kp = Kp + (size_t)min(32 * t + l32, T - 1) * lk.st + 8 * hh;  // (keys past T are masked)
+#pragma unroll
+        for (int s = 0; s < NS; ++s) kq[t][s] = ld8(kp + 16 * s);
+        dma_rows<HD, 32, 1>(Vp, lk.st, 32 * t, T, vb + t * TILE, 0, vfo);
+    }
+    int voff[ND][2];
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) voff[dt][x] = col_off<HD>(8 * x + 4 * hh, 32 * dt + 16 * g16, lane);
+    f32x16 oacc[ND];
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) oacc[dt] = f32x16{};
+    float mb = -INFINITY, lsum = 0.f;
+    const int lim = min(qrow, T - 1) - 4 * hh;  // key offsets beyond this are masked
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        if (t >= nt) break;
+        f32x16 cur = f32x16{};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) cur = E::mfma(kq[t][s], qf[s], cur);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) cur[i] = 32 * t + (i >> 2) * 8 + (i & 3) > lim ? -INFINITY : cur[i];
+        u16x8 pf[2];
+        float psum = 0.f;
+        auto exps = [&]() {
+            f32x16 pv;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pv[i] = fast_exp2(fmaf(cur[i], sl2, -mb));
+            psum = 0.f;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                pf[half] = pack8<DT>(pv, 8 * half);
+                const u32x4 pw = __builtin_bit_cast(u32x4, pf[half]);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) psum = E::add_pair(pw[x], psum);
+            }
+        };
+        auto rescale = [&]() {
+            float mx = cur[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, cur[i]);
+            mx = pair_max(mx);
+            const float mnew = fmaxf(mb, mx * sl2);
+            const float corr = fast_exp2(mb - mnew);
+            mb = mnew;
+            lsum *= corr;
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) oacc[dt] *= corr;
+            exps();
+        };
+        if (t == 0) {  // (sub-tile 0 holds key 0: every row's max is finite)
+            rescale();
+        } else {
+            exps();
+            if (__builtin_amdgcn_ballot_w64(psum > kPsumMax)) rescale();
+        }
+        lsum += psum;
+        if (t == 0) wait_vmem();  // the V rows
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) {
+                const u16* vc = vb + (2 * t + half) * 16 * HD;
+                oacc[dt] = E::mfma(cat4(ld_tr(vc + voff[dt][0]), ld_tr(vc + voff[dt][1])), pf[half], oacc[dt]);
+            }
+    }
+    const float ltot = pair_sum(lsum);
+    store_rows<HD, DT>(oacc, 1.f / ltot, vb, O + lo.at(0, h) + (size_t)(e.start + 32 * e.qb) * lo.st, lo.st, T - 32 * e.qb, lane);
+    if (hh == 0 && qrow < T) LSE[(size_t)h * pk.tokens + e.start + qrow] = (mb + fast_log2(ltot)) * kLn2;
+}
+
+// Waves 0 .. count KVH - 1: dk and dv of 32 keys; the next count H: dq of 32 rows. Either computes D for its rows itself.
+template <int HD, int DT>
+__global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restrict__ Q, const u16* __restrict__ K, const u16* __restrict__ V,
+                                                              const u16* __restrict__ O, const u16* __restrict__ dO, const float* __restrict__ LSE,
+                                                              u16* __restrict__ dQ, u16* __restrict__ dK, u16* __restrict__ dV, Packed pk, int H, int KVH,
+                                                              float sl2, float scale, Lay lq, Lay lk, Lay lo, Lay ldq, Lay ldk) {
+    using E = Elem<DT>;
+    constexpr int NS = HD / 16, ND = HD / 32, TILE = 32 * HD;
+    __shared__ __attribute__((aligned(16))) u16 tS[4 * 4 * TILE];  // per wave: two Q and two dO tiles, or the K rows
+    __shared__ __attribute__((aligned(16))) float vecS[4 * 64];    // per wave: -lse/scale | -D
+    const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5, g16 = (lane >> 4) & 1;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = H / KVH;
+    int item = (int)blockIdx.x * 4 + wave;
+    const bool keys = item < pk.count * KVH;
+    if (!keys) item -= pk.count * KVH;
+    const int per = keys ? KVH : H, at = item / per;
+    if (at >= pk.count) return;
+    const PackedTile e = static_cast<const PackedTile*>(pk.list)[at];
+    const int T = e.len, tile = e.qb;
+    u16* lds = tS + wave * 4 * TILE;
+    int roff[NS], coff[ND][2];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) roff[s] = row_off<HD>(l32, 16 * s + 8 * hh);
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) coff[dt][x] = col_off<HD>(8 * x + 4 * hh, 32 * dt + 16 * g16, lane);
+    // Row r (the last for rows past T) of a head's matrix, in an operand's layout.
+    auto rows_of = [&](const u16* p, const Lay& l, int head, int r, u16x8* to) {
+        const u16* at_ = p + l.at(0, head) + (size_t)(e.start + min(r, T - 1)) * l.st + 8 * hh;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) to[s] = ld8(at_ + 16 * s);
+    };
+    auto rowsum = [&](const u16x8* g, const u16x8* o) {  // D of the lane's row
+        float acc = 0.f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc = fmaf(E::to_f32(g[s][j]), E::to_f32(o[s][j]), acc);
+        return pair_sum(acc);
+    };
+    if (keys) {
+        const int kvh = item - at * per, key = 32 * tile + l32;
+        const int nq = (T + 31) / 32 - tile, n = group * nq;  // (query head, 32-row tile) iterations
+        u16x8 kf[NS], vf[NS], of[NS];
+        rows_of(K, lk, kvh, key, kf);
+        rows_of(V, lk, kvh, key, vf);
+        const DmaOffs<HD, 32, 1> fo = dma_offsets<HD, 32, 1>(lane, 0, lq.st);
+        float lse = 0.f;
+        auto fetch = [&](int it) {  // iteration it's Q and dO tiles, O rows and lse
+            const int iq = it / group, h = kvh * group + (it - iq * group), q0 = 32 * (tile + iq);
+            u16* to = lds + (it & 1) * 2 * TILE;
+            const size_t off = lq.at(0, h) + (size_t)e.start * lq.st;
+            dma_rows<HD, 32, 1>(Q + off, lq.st, q0, T, to, 0, fo);
+            dma_rows<HD, 32, 1>(dO + off, lq.st, q0, T, to + TILE, 0, fo);
+            rows_of(O, lo, h, q0 + l32, of);
+            lse = LSE[(size_t)h * pk.tokens + e.start + min(q0 + l32, T - 1)];
+        };
+        f32x16 dk[ND], dv[ND];
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) dk[dt] = dv[dt] = f32x16{};
+        float* vec = vecS + wave * 64;
+        fetch(0);
+        for (int it = 0; it < n; ++it) {
+            wait_vmem();
+            const u16* qt = lds + (it & 1) * 2 * TILE;
+            const u16* ot = qt + TILE;
+            u16x8 qa[NS], oa[NS];
+#pragma unroll
+            for (int s = 0; s < NS; ++s) qa[s] = ld8(qt + roff[s]), oa[s] = ld8(ot + roff[s]);
+            const int iq = it / group, row = 32 * (tile + iq) + l32;
+            const float nd = -rowsum(oa, of);
+            if (hh == 0) vec[l32] = row < T ? -lse / scale : -INFINITY, vec[32 + l32] = row < T ? nd : 0.f;  // rows past T: p is 0
+            if (it + 1 < n) fetch(it + 1);
+            const f32x4* v4 = reinterpret_cast<const f32x4*>(vec + 4 * hh);
+            f32x16 s = cat16(v4[0], v4[2], v4[4], v4[6]), dp = cat16(v4[8], v4[10], v4[12], v4[14]);
+#pragma unroll
+            for (int ks = 0; ks < NS; ++ks) {
+                s = E::mfma(qa[ks], kf[ks], s);
+                dp = E::mfma(oa[ks], vf[ks], dp);
+            }
+            if (iq == 0) {  // the diagonal: keys past the row
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = (i >> 2) * 8 + (i & 3) >= l32 - 4 * hh ? s[i] : -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = fast_exp2(s[i] * sl2);
+                dp[i] *= p;
+                s[i] = p;
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const u16x8 pf = pack8<DT>(s, 8 * half), sf = pack8<DT>(dp, 8 * half);
+#pragma unroll
+                for (int dt = 0; dt < ND; ++dt) {
+                    const u16 *oc = ot + half * 16 * HD, *qc = qt + half * 16 * HD;
+                    dv[dt] = E::mfma(cat4(ld_tr(oc + coff[dt][0]), ld_tr(oc + coff[dt][1])), pf, dv[dt]);
+                    dk[dt] = E::mfma(cat4(ld_tr(qc + coff[dt][0]), ld_tr(qc + coff[dt][1])), sf, dk[dt]);
+                }
+            }
+        }
+        const size_t off = ldk.at(0, kvh) + (size_t)(e.start + 32 * tile) * ldk.st;
+        store_rows<HD, DT>(dk, scale, lds, dK + off, ldk.st, T - 32 * tile, lane);
+        store_rows<HD, DT>(dv, 1.f, lds + TILE, dV + off, ldk.st, T - 32 * tile, lane);
+    } else {
+        const int h = item - at * per, kvh = h / group, qrow = 32 * tile + l32, nt = tile + 1;
+        const u16* Kp = K + lk.at(0, kvh) + (size_t)e.start * lk.st;
+        const DmaOffs<HD, 32, 1> fo = dma_offsets<HD, 32, 1>(lane, 0, lk.st);
+        u16x8 qf[NS], gf[NS], of[NS], ka[2][NS], va[2][NS];
+        rows_of(dO, lq, h, qrow, gf);
+        rows_of(O, lo, h, qrow, of);
+        rows_of(Q, lq, h, qrow, qf);
+        const float lse = LSE[(size_t)h * pk.tokens + e.start + min(qrow, T - 1)];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            if (t >= nt) break;
+            rows_of(K, lk, kvh, 32 * t + l32, ka[t]);
+            rows_of(V, lk, kvh, 32 * t + l32, va[t]);
+            dma_rows<HD, 32, 1>(Kp, lk.st, 32 * t, T, lds + t * TILE, 0, fo);
+        }
+        const float nd = -rowsum(gf, of), nl2 = -lse * kLog2e;
+        f32x16 dq[ND];
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) dq[dt] = f32x16{};
+        const int lim = min(qrow, T - 1) - 4 * hh;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            if (t >= nt) break;
+            f32x16 s = f32x16{}, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] = nd;
+#pragma unroll
+            for (int ks = 0; ks < NS; ++ks) {
+                s = E::mfma(ka[t][ks], qf[ks], s);
+                dp = E::mfma(va[t][ks], gf[ks], dp);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = 32 * t + (i >> 2) * 8 + (i & 3) > lim ? -INFINITY : s[i];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] = fast_exp2(fmaf(s[i], sl2, nl2)) * dp[i];
+            if (t == 0) wait_vmem();  // the K rows
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const u16x8 sf = pack8<DT>(dp, 8 * half);
+                const u16* kc = lds + (2 * t + half) * 16 * HD;
+#pragma unroll
+                for (int dt = 0; dt < ND; ++dt) dq[dt] = E::mfma(cat4(ld_tr(kc + coff[dt][0]), ld_tr(kc + coff[dt][1])), sf, dq[dt]);
+            }
+        }
+        store_rows<HD, DT>(dq, scale, lds + 2 * TILE, dQ + ldq.at(0, h) + (size_t)(e.start + 32 * tile) * ldq.st, ldq.st, T - 32 * tile, lane);
+    }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1910,29 +2203,41 @@ struct PlanHead {
     int32_t nslots;                 // partial sums
     int32_t wpp;                    // waves per entry of the dK/dV list: 1 or 4
     int32_t tiles, units, sums, positions;  // words where they begin
+    int32_t nshort, shorts;                 // 32-row tiles of the short sequences, and the word where they begin
+    int32_t unused[14];
 };
-static_assert(sizeof(PlanHead) == 64 && offsetof(PlanHead, positions) == 4 * NN_FA_PACKED_POSITIONS, "16 words");
+static_assert(sizeof(PlanHead) == 128 && offsetof(PlanHead, positions) == 4 * NN_FA_PACKED_POSITIONS, "32 words");
 
 // What the lists are made by: one pass over the lengths counts, a second writes.
+constexpr int64_t kSplitGain = 64;
 struct PlanRule {
+    int64_t upto;     // sequences of up to this many tokens take the kernels for short ones
     int64_t g;        // query heads per KV head
     int64_t target;   // iterations (query head, query tile) that each of kDkdvFill blocks would do if all did the same
     bool paired;
     int wpp;
     int64_t iters(int64_t nkb, int64_t pj) const { return paired && nkb - 1 - pj > pj ? g * (nkb + 1) : g * (nkb - pj); }
-    // Blocks that share a pair: as many as bring its iterations down to a block's even share, each with kDkdvMinIters at least.
-    // A quarter over the share is left alone: the blocks end unevenly by about as much anyway, and partial sums cost a pass.
+    // Blocks that share a pair: as many as bring its iterations down to a block's even share, each with kDkdvMinIters at least,
+    // where that takes kSplitGain iterations off its block. Partial sums cost their traffic, another launch and 8 us or so:
+    // backwards of one sequence of 2048 (74 off) 65 us instead of 77, of 4096 (97) 130 instead of 147, of 4096 among 30 short ones
+    // (89) 145 instead of 150; but of 8192 tokens in 12 sequences of up to 2048 (43) 88 instead of 85, of 4096 in 6 (41) 66
+    // instead of 56.
     int64_t splits(int64_t it) const {
-        if (!paired || wpp != 4 || target <= 0) return 1;
+        if (!paired || wpp != 4 || target <= 0 || it - target < kSplitGain) return 1;
         return std::max<int64_t>(1, std::min({kDkdvMaxSplit, (4 * it - target + 4 * target - 1) / (4 * target), it / kDkdvMinIters}));
     }
 };
 
+constexpr int64_t kSinglesMost = 9 * kDkdvFill / 4, kSinglesIters = 128;
+// From this many waves of short sequences on, their kernels pay beside the others' launches (below, a few blocks more in those
+// cost less than a launch, about 3 us; 512 of them run at once and take 2.9 us).
+constexpr int64_t kShortWaves = 1024;
+
 struct PlanSize {
     PlanRule rule;
-    int64_t tokens = 0, longest = 0, ntiles = 0, nunits = 0, nsums = 0, nslots = 0;
+    int64_t tokens = 0, longest = 0, ntiles = 0, nunits = 0, nsums = 0, nslots = 0, nshort = 0;
     int64_t padded() const { return (ntiles + 7) / 8 * 8; }
-    int64_t words() const { return 16 + 4 * padded() + 8 * (nunits + nsums) + tokens; }
+    int64_t words() const { return 32 + 4 * (padded() + nshort) + 8 * (nunits + nsums) + tokens; }
 };
 
 int plan_size(const int64_t* lengths, int64_t n, int64_t H, int64_t KVH, PlanSize* out) {
@@ -1940,13 +2245,20 @@ int plan_size(const int64_t* lengths, int64_t n, int64_t H, int64_t KVH, PlanSiz
     if (n < 0 || (n > 0 && !lengths)) return fail(-1, "invalid list of lengths");
     if (int e = check_dims(1, H, KVH, 1, 64, kBF16)) return e;
     PlanSize z;
-    int64_t pairs = 0, units = 0, work = 0;
+    int64_t pairs = 0, units = 0, work = 0, few = 0;
     const int64_t g = H / KVH;
     for (int64_t i = 0; i < n; ++i) {
         const int64_t len = lengths[i];
         if (len < 0) return fail(-1, "sequence %lld has the length %lld", (long long)i, (long long)len);
         if (len >= (int64_t)1 << 30 || (z.tokens += len) >= (int64_t)1 << 30) return fail(-1, "sizes too large");
         z.longest = std::max(z.longest, len);
+        if (len <= kShort) few += (len + 31) / 32;
+    }
+    const int64_t upto = z.longest <= kShort || few * H >= kShortWaves ? kShort : 0;
+    if (upto) z.nshort = few;
+    for (int64_t i = 0; i < n; ++i) {
+        const int64_t len = lengths[i];
+        if (len <= upto) continue;
         const int64_t nkb = (len + 63) / 64;
         z.ntiles += (len + 127) / 128 * KVH;
         pairs += (nkb + 1) / 2 * KVH, units += nkb * KVH;
@@ -1954,15 +2266,19 @@ int plan_size(const int64_t* lengths, int64_t n, int64_t H, int64_t KVH, PlanSiz
     }
     // (blocks of 256 threads, fewer than 2^32 threads to a launch; 32-bit words and split bounds)
     const int64_t most = g * ((z.longest + 63) / 64 + 1);
-    if (z.padded() * g >= (int64_t)1 << 24 || units * kDkdvMaxSplit >= (int64_t)1 << 28 || most * kDkdvMaxSplit >= (int64_t)1 << 31)
+    if (z.padded() * g >= (int64_t)1 << 24 || z.nshort * (H + KVH) >= (int64_t)1 << 24 || units * kDkdvMaxSplit >= (int64_t)1 << 28 || most * kDkdvMaxSplit >= (int64_t)1 << 31)
         return fail(-1, "sizes too large");
-    // The dense kernels' choices (dkdv_waves_per_pair, dkdv_mode), for work that differs from pair to pair: a wave of its own
-    // for each pair where there are enough of them and the longest does not outlast an even share of all.
-    PlanRule r{g, work / kDkdvFill, true, 4};
-    if (pairs >= 3 * kDkdvFill && most <= kDkdvFewWavesMaxIters && most <= work / (4 * kDkdvFill) * 5 / 4) r.wpp = 1;
-    if (units <= kDkdvFill && r.splits(most) == 1) r.paired = false;
+    // The dense kernels' choices (dkdv_waves_per_pair, dkdv_mode), for work that differs from pair to pair. A wave of its own for
+    // each pair where there are enough of them and the longest does not outlast a wave's even share of all (65536 tokens in
+    // sequences of up to 512: 250 us instead of 295; of up to 4096, where it would, 703 instead of 692). Single units where they
+    // fill the chip little more than twice and none is long: their blocks even out better than pairs' (4096 tokens in 6
+    // sequences 56 us instead of 60, 8192 in 12 84.5 instead of 86.5, in 8 of 1024 the same; one of 8192 363 instead of 352).
+    PlanRule r{upto, g, work / kDkdvFill, true, 4};
+    if (pairs >= 3 * kDkdvFill && most <= kDkdvFewWavesMaxIters && most <= work / (4 * kDkdvFill)) r.wpp = 1;
+    if (r.wpp == 4 && units <= kSinglesMost && most <= kSinglesIters && r.splits(most) == 1) r.paired = false;
     z.rule = r;
     for (int64_t i = 0; i < n; ++i) {
+        if (lengths[i] <= upto) continue;
         const int64_t nkb = (lengths[i] + 63) / 64, np = r.paired ? (nkb + 1) / 2 : nkb;
         for (int64_t pj = 0; pj < np; ++pj) {
             const int64_t ns = r.splits(r.iters(nkb, pj));
@@ -2022,6 +2338,12 @@ template <int HD, int DT>
 int packed_fwd_impl(const void* q, const void* k, const void* v, void* o, float* lse, const PlanHead& p, const int32_t* dp, float scale,
                     const Lays& l, hipStream_t st) {
     const int g = p.H / p.KVH;
+    if (p.nshort) {
+        fa_short_fwd_kernel<HD, DT><<<dim3((unsigned)(((int64_t)p.nshort * p.H + 3) / 4)), dim3(256), 0, st>>>(
+            (const u16*)q, (const u16*)k, (const u16*)v, (u16*)o, lse, Packed{dp + p.shorts, p.nshort, p.tokens}, p.H, p.KVH, scale * kLog2e, l.q, l.k, l.o);
+        if (int e = launch_status("fa_short_fwd_kernel")) return e;
+    }
+    if (p.ntiles == 0) return 0;
     fa_fwd_kernel<HD, DT, false, true><<<dim3((unsigned)(p.ntiles * g)), dim3(256), 0, st>>>(
         (const u16*)q, (const u16*)k, (const u16*)v, (u16*)o, lse, p.H, p.H, p.KVH, 0, 0, scale * kLog2e, l.q, l.k, l.o, RopeArgs{},
         Packed{dp + p.tiles, p.ntiles, p.tokens});
@@ -2032,6 +2354,13 @@ template <int HD, int DT>
 int packed_bwd_impl(const void* dO, const void* q, const void* k, const void* v, const void* o, const float* lse, void* dq, void* dk, void* dv,
                     const Workspace& w, const PlanHead& p, const int32_t* dp, float scale, const Lays& l, hipStream_t st) {
     const int g = p.H / p.KVH;
+    if (p.nshort) {
+        fa_short_bwd_kernel<HD, DT><<<dim3((unsigned)(((int64_t)p.nshort * (p.H + p.KVH) + 3) / 4)), dim3(256), 0, st>>>(
+            (const u16*)q, (const u16*)k, (const u16*)v, (const u16*)o, (const u16*)dO, lse, (u16*)dq, (u16*)dk, (u16*)dv,
+            Packed{dp + p.shorts, p.nshort, p.tokens}, p.H, p.KVH, scale * kLog2e, scale, l.q, l.k, l.o, l.dq, l.dk);
+        if (int e = launch_status("fa_short_bwd_kernel")) return e;
+    }
+    if (p.ntiles == 0) return 0;
     fa_bwd_dq_kernel<HD, DT, false, true><<<dim3((unsigned)(p.ntiles * g)), dim3(256), 0, st>>>(
         (const u16*)q, (const u16*)k, (const u16*)v, (const u16*)o, (const u16*)dO, lse, w.nL, w.nD, (u16*)dq, p.H, p.H, p.KVH, 0, 0, scale * kLog2e,
         scale, l.q, l.k, l.o, l.dq, RopeArgs{}, Packed{dp + p.tiles, p.ntiles, p.tokens});
@@ -2049,7 +2378,7 @@ int packed_bwd_impl(const void* dO, const void* q, const void* k, const void* v,
         launch(fa_bwd_dkdv_kernel<HD, DT, 4, false, true>, 1);
     if (int e = launch_status("fa_bwd_dkdv_kernel (packed)")) return e;
     if (p.nsums == 0) return 0;
-    fa_packed_sum_kernel<HD, DT><<<dim3((unsigned)p.nsums), dim3(256), 0, st>>>(w.part, (u16*)dk, (u16*)dv, (const PackedUnit*)(dp + p.sums), l.dk);
+    fa_packed_sum_kernel<HD, DT><<<dim3((unsigned)p.nsums, kSumBlocks), dim3(256), 0, st>>>(w.part, (u16*)dk, (u16*)dv, (const PackedUnit*)(dp + p.sums), l.dk);
     return launch_status("fa_packed_sum_kernel");
 }
 
@@ -2070,19 +2399,24 @@ NNFA_API int nn_fa_packed_plan(const int64_t* lengths, int64_t n, int64_t H, int
     p.magic = kPlanMagic, p.words = (int32_t)words, p.n = (int32_t)std::min<int64_t>(n, INT32_MAX), p.H = (int32_t)H, p.KVH = (int32_t)KVH;
     p.tokens = (int32_t)z.tokens, p.longest = (int32_t)z.longest;
     p.ntiles = (int32_t)z.padded(), p.nunits = (int32_t)z.nunits, p.nsums = (int32_t)z.nsums, p.nslots = (int32_t)z.nslots, p.wpp = r.wpp;
-    p.tiles = 16, p.units = p.tiles + 4 * p.ntiles, p.sums = p.units + 8 * p.nunits, p.positions = p.sums + 8 * p.nsums;
+    p.nshort = (int32_t)z.nshort;
+    p.tiles = 32, p.units = p.tiles + 4 * p.ntiles, p.sums = p.units + 8 * p.nunits, p.shorts = p.sums + 8 * p.nsums;
+    p.positions = p.shorts + 4 * p.nshort;
     memcpy(plan, &p, sizeof p);
     PackedTile* tile = (PackedTile*)(plan + p.tiles);
     PackedUnit* unit = (PackedUnit*)(plan + p.units);
     PackedUnit* sum = (PackedUnit*)(plan + p.sums);
+    PackedTile* few = (PackedTile*)(plan + p.shorts);
     int32_t* pos = plan + p.positions;
+    PackedTile* const few0 = few;
     PackedTile* const tile0 = tile;
     PackedUnit* const unit0 = unit;
     int start = 0, slot = 0;
     for (int64_t i = 0; i < n; ++i) {
         const int len = (int)lengths[i], nkb = (len + 63) / 64, np = r.paired ? (nkb + 1) / 2 : nkb;
         for (int t = 0; t < len; ++t) *pos++ = t;
-        for (int kvh = 0; kvh < KVH; ++kvh) {
+        for (int t = 0; len <= r.upto && 32 * t < len; ++t) *few++ = PackedTile{start, len, t, 0};
+        for (int kvh = 0; kvh < KVH && len > r.upto; ++kvh) {
             for (int qb = 0; qb < (len + 127) / 128; ++qb) *tile++ = PackedTile{start, len, qb, kvh};
             for (int pj = 0; pj < np; ++pj) {
                 const int ns = (int)r.splits(r.iters(nkb, pj));
@@ -2096,6 +2430,7 @@ NNFA_API int nn_fa_packed_plan(const int64_t* lengths, int64_t n, int64_t H, int
     std::sort(tile0, tile, [](const PackedTile& a, const PackedTile& b) {
         return a.qb != b.qb ? a.qb > b.qb : a.start != b.start ? a.start < b.start : a.kvh < b.kvh;
     });
+    std::sort(few0, few, [](const PackedTile& a, const PackedTile& b) { return a.qb != b.qb ? a.qb > b.qb : a.start < b.start; });
     std::sort(unit0, unit, [&](const PackedUnit& a, const PackedUnit& b) {
         const int64_t wa = r.iters((a.len + 63) / 64, a.pj) * b.nsplit, wb = r.iters((b.len + 63) / 64, b.pj) * a.nsplit;
         if (wa != wb) return wa > wb;

@@ -806,7 +806,7 @@ Tensor packed_plan(const std::vector<int64_t>& lengths, int64_t H, int64_t KVH) 
 
 // A call's plan: in host memory and, the same, on the tensors' device.
 struct Plan {
-    Tensor host, device;
+    const Tensor &host, &device;
     nn_fa_packed_info info;
     Plan(const Tensor& device_, const Tensor& host_) : host(host_), device(device_) {
         need(host.device().is_cpu() && host.scalar_type() == at::kInt && host.dim() == 1 && host.is_contiguous() && host.numel() >= 16 &&
@@ -820,21 +820,32 @@ struct Plan {
 };
 
 using S2 = std::array<int64_t, 2>;
-// The {head, row} strides through which the kernels can read the (tokens, heads, hd) tensor in place, if they can (strides_of).
+// The {head, row} strides through which the kernels can read the (tokens, heads, hd) tensor's values in place, if they can (the
+// library's limits; a dimension of size 1 has no stride of its own).
 std::optional<S2> packed_strides(const Tensor& t) {
-    if (t.dim() != 3 || t.numel() == 0) return std::nullopt;
-    const auto s = strides_of(t.transpose(0, 1).unsqueeze(0));
-    if (!s) return std::nullopt;
-    return S2{(*s)[1], (*s)[2]};
+    const int64_t T = t.size(0), H = t.size(1), D = t.size(2);
+    const S2 s{H > 1 ? t.stride(1) : D, T > 1 ? t.stride(0) : H * D};
+    if (T == 0 || t.stride(2) != 1 || s[0] <= 0 || s[0] % 8 || s[1] < D || s[1] % 8 || (uintptr_t)t.data_ptr() % 16) return std::nullopt;
+    if (s[0] == D && s[1] == H * D) return s;  // dense: the library knows how long a sequence may be
+    if (T * s[1] >= (int64_t)1 << 30 || s[0] * H >= (int64_t)1 << 40) return std::nullopt;
+    return s;
 }
-// The two as the kernels read them, through strides that they share.
-void packed_readable(Tensor& a, Tensor& b) {
-    a = real_values(a), b = real_values(b);
-    const auto sa = packed_strides(a), sb = packed_strides(b);
-    if (a.size(-2) == b.size(-2) && sa && sb && *sa == *sb) return;
-    a = dense(a), b = dense(b);
+// The tensors as the kernels read them, through strides that they share.
+S2 packed_readable(std::initializer_list<Tensor*> ts) {
+    std::optional<S2> first;
+    bool ok = true;
+    for (Tensor* t : ts) {
+        if (lazy(*t)) *t = real_values(*t);
+        const auto s = packed_strides(*t);
+        ok = ok && s && (!first || *first == *s);
+        first = s;
+    }
+    if (ok) return *first;
+    for (Tensor* t : ts) *t = dense(*t);
+    const Tensor& t = **ts.begin();
+    return {t.size(2), t.size(1) * t.size(2)};
 }
-S2 packed_known(const Tensor& t) { return t.is_contiguous() ? S2{t.size(2), t.size(1) * t.size(2)} : *packed_strides(t); }
+S2 dense_packed(const Tensor& t) { return {t.size(2), t.size(1) * t.size(2)}; }
 
 void check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Plan& p) {
     need(q.is_cuda(), "inputs must be CUDA tensors");
@@ -854,13 +865,12 @@ T2 packed_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor
     const Plan p(plan, plan_host);
     check_packed(q_, k_, v_, p);
     const c10::DeviceGuard guard(q_.device());
-    Tensor q = q_, k = k_, v = v_, same = q_;
-    packed_readable(q, same);
-    packed_readable(k, v);
+    Tensor q = q_, k = k_, v = v_;
+    const S2 sq = packed_readable({&q}), sk = packed_readable({&k, &v});
     const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
     Tensor o = empty_of(q, q.sizes()), lse = empty_f32(q, {H, T});
     if (T == 0) return {o, lse};
-    const S2 s[3] = {packed_known(q), packed_known(k), packed_known(o)};
+    const S2 s[3] = {sq, sk, dense_packed(o)};
     fa_done(nn_fa_packed_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(), p.at_host(), p.at_device(), D, s[0].data(),
                              code(q), scale_of(D), stream_of(q)));
     return {o, lse};
@@ -877,14 +887,13 @@ T3 packed_bwd(const Tensor& d_o_, const Tensor& q_, const Tensor& k_, const Tens
     need(lse_.sizes() == at::IntArrayRef({H, T}) && lse_.scalar_type() == at::kFloat, "lse must be a float32 tensor of shape (H, tokens)");
     const c10::DeviceGuard guard(q_.device());
     Tensor q = q_, d_o = d_o_, k = k_, v = v_;
-    packed_readable(q, d_o);
-    packed_readable(k, v);
+    const S2 sq = packed_readable({&q, &d_o}), sk = packed_readable({&k, &v});
     const Tensor o = dense(o_), lse = contig(lse_);
     Tensor dq = empty_of(q, q.sizes()), dk = empty_of(k, k.sizes()), dv = empty_of(v, v.sizes());
     if (T == 0) return {dq, dk, dv};
     const size_t n = nn_fa_packed_bwd_workspace_size(p.at_host(), D);
     Tensor ws = bytes(q, n);
-    const S2 s[5] = {packed_known(q), packed_known(k), packed_known(o), packed_known(dq), packed_known(dk)};
+    const S2 s[5] = {sq, sk, dense_packed(o), dense_packed(dq), dense_packed(dk)};
     fa_done(nn_fa_packed_bwd(d_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
                              dv.data_ptr(), ws.data_ptr(), n, p.at_host(), p.at_device(), D, s[0].data(), code(q), scale_of(D), stream_of(q)));
     return {dq, dk, dv};
@@ -1083,7 +1092,7 @@ struct PackedNode : torch::autograd::Function<PackedNode> {
         Tensor q = q_, k = k_, v = v_, o, lse;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
-            if (k.dim() == 3 && v.dim() == 3) packed_readable(k, v);  // copies that the backward would make again
+            if (k.dim() == 3 && k.sizes() == v.sizes()) packed_readable({&k, &v});  // copies that the backward would make again
             std::tie(o, lse) = packed_fwd(q, k, v, plan, plan_host);
         }
         ctx->set_materialize_grads(false);

@@ -13,7 +13,8 @@ from tests.common import TOL, TOL_GRAD, assert_close_tol
 pytestmark = pytest.mark.gpu
 
 # lengths, H, KVH, hd: tile and unit edges with empty sequences; an odd group; one long sequence among short ones, whose pairs
-# are split; few tokens, a block for each unit; many sequences, a wave for each pair; lengths of 1 and 2; long and split, MQA.
+# are split; few tokens, a block for each unit; many sequences, a wave for each pair; lengths of 1 and 2; long and split, MQA; short
+# sequences alone, and many of them beside a longer one.
 CASES = [
     ([63, 0, 64, 65, 1, 127, 128, 129, 0, 191, 192, 193, 0], 12, 4, 64),
     ([63, 64, 65, 1, 127, 128, 129, 300], 6, 2, 32),
@@ -23,6 +24,9 @@ CASES = [
     ([1, 2, 1, 1, 3] * 80, 8, 8, 32),
     ([3000], 12, 1, 64),
     ([1111, 999, 1], 4, 4, 32),
+    ([1, 31, 32, 33, 63, 64, 0, 2, 50] * 3, 12, 4, 64),
+    ([40, 7, 64, 32, 5], 5, 1, 32),
+    ([20, 64, 33] * 40 + [500], 8, 2, 64),
 ]
 IDS = [f"{len(c[0])}x{max(c[0])}-{c[1]}-{c[2]}-{c[3]}" for c in CASES]
 
@@ -104,7 +108,7 @@ def test_a_sequence_is_the_dense_attention_on_it_alone(lengths, H, KVH, D):
 
 
 def test_two_runs_give_the_same_bits():
-    for lengths, H, KVH, D in (CASES[2], CASES[4]):
+    for lengths, H, KVH, D in (CASES[2], CASES[4], CASES[10]):
         q, k, v, do = _inputs(lengths, H, KVH, D, torch.bfloat16, seed=2)
         packing = _packing(lengths, H, KVH)
         first = _run(q, k, v, do, packing)
@@ -112,7 +116,7 @@ def test_two_runs_give_the_same_bits():
             assert all(torch.equal(a, b) for a, b in zip(first, _run(q, k, v, do, again)))
 
 
-@pytest.mark.parametrize("lengths, H, KVH, D", [CASES[0], CASES[2], CASES[4]], ids=[IDS[0], IDS[2], IDS[4]])
+@pytest.mark.parametrize("lengths, H, KVH, D", [CASES[0], CASES[2], CASES[4], CASES[8], CASES[10]], ids=[IDS[0], IDS[2], IDS[4], IDS[8], IDS[10]])
 def test_sequences_do_not_see_each_other(lengths, H, KVH, D):
     print(f"\n[case] packed among NaN, {len(lengths)} sequences", flush=True)
     q, k, v, do = _inputs(lengths, H, KVH, D, torch.bfloat16, seed=3)

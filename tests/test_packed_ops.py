@@ -32,12 +32,17 @@ def _plan(lengths, H, KVH):
 def _check_plan(lengths, H, KVH):
     """Every tile, unit, iteration and partial sum once, whole, and within its sequence and the workspace."""
     w, g, tokens = _plan(lengths, H, KVH), H // KVH, sum(lengths)
-    magic, words, n, h, kvh, total, longest, ntiles, nunits, nsums, nslots, wpp, tiles, units, sums, positions = w[:16]
+    magic, words, n, h, kvh, total, longest, ntiles, nunits, nsums, nslots, wpp, tiles, units, sums, positions, nshort, shorts = w[:18]
     assert (words, n, h, kvh, total, longest) == (len(w), len(lengths), H, KVH, tokens, max(lengths, default=0))
-    assert tiles == 16 and units == tiles + 4 * ntiles and sums == units + 8 * nunits and positions == sums + 8 * nsums and len(w) == positions + tokens
-    assert tiles % 4 == 0 and units % 4 == 0 and sums % 4 == 0 and ntiles % 8 == 0 and wpp in (1, 4)
+    assert tiles == 32 and units == tiles + 4 * ntiles and sums == units + 8 * nunits and shorts == sums + 8 * nsums
+    assert positions == shorts + 4 * nshort and len(w) == positions + tokens and ntiles % 8 == 0 and wpp in (1, 4)
     assert w[positions:] == [t for n in lengths for t in range(n)]
     starts = [sum(lengths[:i]) for i in range(len(lengths))]
+
+    few = [tuple(w[shorts + 4 * i : shorts + 4 * i + 4]) for i in range(nshort)]  # sequences of up to 64 tokens, or none of them
+    upto = 64 if few or longest <= 64 else 0
+    assert sorted(few) == sorted((s, n, t, 0) for s, n in zip(starts, lengths) if n <= upto for t in range(-(-n // 32)))
+    starts, lengths = [s for s, n in zip(starts, lengths) if n > upto], [n for n in lengths if n > upto]
 
     got = [tuple(w[tiles + 4 * i : tiles + 4 * i + 4]) for i in range(ntiles)]
     real = [t for t in got if t[1]]
@@ -68,7 +73,7 @@ def _check_plan(lengths, H, KVH):
     plan = (ctypes.c_int32 * len(w))(*w)
     for D in (32, 64):
         assert lib().nn_fa_packed_bwd_workspace_size(plan, D) == 2 * rnd(4 * H * tokens) + nslots * 2 * 128 * D * 4
-    return w[:16]
+    return w[:18]
 
 
 @pytest.mark.parametrize("lengths, H, KVH", CASES, ids=[f"{len(c[0])}x{max(c[0], default=0)}-{c[1]}-{c[2]}" for c in CASES])
@@ -86,12 +91,14 @@ def test_plan_of_random_sequences(seed):
 
 
 def test_plan_shares_out_the_work():
-    # equal long sequences that fill the chip are not split; one long sequence is, down to an even share of the whole
+    # equal long sequences that fill the chip are not split; one long sequence is, also beside short ones, and short ones never
     assert _check_plan([1024] * 8, 12, 4)[10] == 0
     assert _check_plan([2048], 12, 4)[10] > 0
-    assert _check_plan([2048] + [64] * 30, 12, 4)[10] > 0
-    assert _check_plan([256], 12, 4)[8] == 16  # a block for each unit
+    assert _check_plan([4096] + [100] * 30, 12, 4)[10] > 0 and _check_plan([1000, 500], 12, 4)[10] == 0
+    assert _check_plan([256], 12, 4)[8] == 16 and _check_plan([900, 1024], 12, 4)[8] == 124  # a block for each unit
     assert _check_plan([1024] * 32, 12, 4)[11] == 1  # a wave for each pair
+    assert _check_plan([20, 64], 12, 4)[16] == 3 and _check_plan([20, 64, 65], 12, 4)[16] == 0  # short sequences alone,
+    assert _check_plan([20] * 100 + [300], 12, 4)[16] == 100  # or many of them
 
 
 @pytest.mark.parametrize(
