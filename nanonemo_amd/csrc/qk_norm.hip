@@ -7,13 +7,17 @@
 // r is computed again from x, which the backward reads anyway. Everything is fp32; an output is rounded once.
 //
 // Work decomposition. A vector belongs to a team of R lanes (R the power of two at or above D/16); a lane holds 8 pairs: two
-// groups of 8 values. A team takes NH heads of one token, queries or keys, one after the other in registers: they share the
-// token's angles and the weight, whose fp32 values are twice as many bytes as a head's 16-bit ones and come from the caches.
-// Sums over a vector are xor-butterflies over the team. The kernels are bound by memory.
+// groups of 8 values. Sums over a vector are xor-butterflies over the team. The kernels are bound by memory.
 //
-// Backward: a fixed grid whose blocks work on queries or on keys, in proportion; every team walks its kind's units and keeps
+// Forward: a team takes two heads of one token, queries or keys, which share the token's angles and the weight, whose fp32 values
+// are twice as many bytes as a head's 16-bit ones and come from the caches (131072 tokens of 12 + 4 heads of 64 in bf16: 109 us,
+// 4.9 TB/s; one head 113, four 115).
+//
+// Backward: a fixed grid whose blocks work on queries or on keys, in proportion; every team walks its kind's vectors and keeps
 // its lanes' part of dw in registers. A block's teams are joined by butterflies within the waves and in LDS in wave order, into
-// one partial row per block; sum_kernel adds a kind's rows in a fixed order: no atomics, bit-reproducible.
+// one partial row per block; sum_kernel adds a kind's rows in a fixed order: no atomics, bit-reproducible. 1024 blocks are what
+// the chip holds at once (the same tokens: 165 us, 4.9 TB/s with the sums' 5; 768 blocks 172, 1280 222, 2048 173; two heads of
+// a token at a time 174 to 203, four 178).
 #include <hip/hip_runtime.h>
 #include <stdarg.h>
 #include <stdint.h>
@@ -31,6 +35,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kBwdBlocks = 1024;  // most blocks of the backward, each of which leaves one partial row of dw
+constexpr int kFwdHeads = 2;      // heads of a token to a team of the forward
 constexpr int kSumWaves = 16;
 
 // 8 values of a row as fp32, and back.
@@ -136,7 +141,8 @@ __global__ __launch_bounds__(kThreads) void qk_norm_fwd_kernel(Side q, Side k, A
     }
 }
 
-template <int DT, int R, int NH>
+// Blocks [0, qblocks) take the queries' vectors, the others the keys'.
+template <int DT, int R>
 __global__ __launch_bounds__(kThreads) void qk_norm_bwd_kernel(Side q, Side k, Angles a, unsigned tokens, unsigned qblocks, float* __restrict__ part,
                                                                int D, float inv_d, float eps) {
     __shared__ float red[kWaves][16 * 16];
@@ -149,56 +155,50 @@ __global__ __launch_bounds__(kThreads) void qk_norm_bwd_kernel(Side q, Side k, A
     const float* w = isq ? q.w : k.w;
     const long long xt = isq ? q.xt : k.xt, xh = isq ? q.xh : k.xh, dt = isq ? q.dt : k.dt, dh = isq ? q.dh : k.dh, yt = isq ? q.yt : k.yt,
                     yh = isq ? q.yh : k.yh;
-    const int heads = isq ? q.heads : k.heads;
-    const unsigned per = (heads + NH - 1) / NH, units = tokens * per, teams = blocks * (kThreads / R);
+    const unsigned heads = isq ? q.heads : k.heads, vectors = tokens * heads, teams = blocks * (kThreads / R);
     float w1[8] = {}, w2[8] = {}, a1[8] = {}, a2[8] = {};
     if (on) {
         load8f(w + i0, w1);
         load8f(w + half + i0, w2);
     }
-    for (unsigned u = block * (kThreads / R) + threadIdx.x / R; u < units; u += teams) {
-        const unsigned token = u / per;
-        const int h0 = (int)(u - token * per) * NH;
-        const long long xo = token * xt + h0 * xh + i0, go = token * dt + h0 * dh + i0, yo = token * yt + h0 * yh + i0;
-        float x1[NH][8], x2[NH][8], d1[NH][8], d2[NH][8], c[8], s[8];
-#pragma unroll
-        for (int n = 0; n < NH; ++n) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x1[n][j] = x2[n][j] = d1[n][j] = d2[n][j] = 0.f;
-            if (on && h0 + n < heads) {
-                load8<DT>(x, xo + n * xh, x1[n]);
-                load8<DT>(x, xo + n * xh + half, x2[n]);
-                load8<DT>(dy, go + n * dh, d1[n]);
-                load8<DT>(dy, go + n * dh + half, d2[n]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) c[j] = s[j] = 0.f;
-        const bool ok = on ? angles(a, token, half, i0, c, s) : true;
-#pragma unroll
-        for (int n = 0; n < NH; ++n) {
-            float ss = 0.f, gx = 0.f;
+    for (unsigned u = block * (kThreads / R) + threadIdx.x / R; u < vectors; u += teams) {
+        const unsigned token = u / heads, h = u - token * heads;
+        float x1[8] = {}, x2[8] = {}, g1[8] = {}, g2[8] = {};
+        bool ok = true;
+        if (on) {
+            const long long xo = token * xt + h * xh + i0, go = token * dt + h * dh + i0;
+            float d1[8], d2[8], c[8], s[8];
+            load8<DT>(x, xo, x1);
+            load8<DT>(x, xo + half, x2);
+            load8<DT>(dy, go, d1);
+            load8<DT>(dy, go + half, d2);
+            ok = angles(a, token, half, i0, c, s);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                ss = fmaf(x1[n][j], x1[n][j], fmaf(x2[n][j], x2[n][j], ss));
-                const float g1 = d1[n][j] * c[j] + d2[n][j] * s[j], g2 = d2[n][j] * c[j] - d1[n][j] * s[j];
-                d1[n][j] = g1, d2[n][j] = g2;
-                gx = fmaf(g1 * w1[j], x1[n][j], fmaf(g2 * w2[j], x2[n][j], gx));
+                g1[j] = d1[j] * c[j] + d2[j] * s[j];
+                g2[j] = d2[j] * c[j] - d1[j] * s[j];
             }
-            const float r = ok ? rsqrtf(team_sum<R>(ss) * inv_d + eps) : NAN, m = r * team_sum<R>(gx) * inv_d;
-            if (!on || h0 + n >= heads) continue;
-            float y1[8], y2[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float n1 = x1[n][j] * r, n2 = x2[n][j] * r;
-                a1[j] = fmaf(d1[n][j], n1, a1[j]);
-                a2[j] = fmaf(d2[n][j], n2, a2[j]);
-                y1[j] = r * (d1[n][j] * w1[j] - n1 * m);
-                y2[j] = r * (d2[n][j] * w2[j] - n2 * m);
-            }
-            store8<DT>(dx, yo + n * yh, y1);
-            store8<DT>(dx, yo + n * yh + half, y2);
         }
+        float ss = 0.f, gx = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            ss = fmaf(x1[j], x1[j], fmaf(x2[j], x2[j], ss));
+            gx = fmaf(g1[j] * w1[j], x1[j], fmaf(g2[j] * w2[j], x2[j], gx));
+        }
+        const float r = ok ? rsqrtf(team_sum<R>(ss) * inv_d + eps) : NAN, m = r * team_sum<R>(gx) * inv_d;
+        if (!on) continue;
+        float y1[8], y2[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float n1 = x1[j] * r, n2 = x2[j] * r;
+            a1[j] = fmaf(g1[j], n1, a1[j]);
+            a2[j] = fmaf(g2[j], n2, a2[j]);
+            y1[j] = r * (g1[j] * w1[j] - n1 * m);
+            y2[j] = r * (g2[j] * w2[j] - n2 * m);
+        }
+        const long long yo = token * yt + h * yh + i0;
+        store8<DT>(dx, yo, y1);
+        store8<DT>(dx, yo + half, y2);
     }
     // The wave's teams, then the block's waves.
 #pragma unroll
@@ -258,8 +258,6 @@ int launched(const char* what) {
 }
 bool aligned(const void* p, int n) { return ((uintptr_t)p % n) == 0; }
 
-constexpr int kFwdHeads = 4, kBwdHeads = 2;  // NH
-
 // Lanes per vector.
 int team_of(int64_t D) {
     int r = 1;
@@ -276,13 +274,13 @@ Grid grid_of(int64_t M, int64_t H, int64_t KVH, int64_t D, int NH) {
     const int64_t qu = M * ((H + NH - 1) / NH), ku = M * ((KVH + NH - 1) / NH);
     return {(unsigned)((qu + teams - 1) / teams), (unsigned)((ku + teams - 1) / teams)};
 }
-// The backward's: kBwdBlocks at most, in proportion to the units.
+// The backward's: kBwdBlocks at most, in proportion to the heads.
 Grid bwd_grid(int64_t M, int64_t H, int64_t KVH, int64_t D) {
     if (M <= 0) return {0, 0};
-    const Grid all = grid_of(M, H, KVH, D, kBwdHeads);
-    const int64_t qb = all.q, kb = all.k, qu = (H + kBwdHeads - 1) / kBwdHeads, ku = (KVH + kBwdHeads - 1) / kBwdHeads;
+    const Grid all = grid_of(M, H, KVH, D, 1);
+    const int64_t qb = all.q, kb = all.k;
     if (qb + kb <= kBwdBlocks) return all;
-    const int64_t q = std::min<int64_t>(kBwdBlocks - 1, std::max<int64_t>(1, (kBwdBlocks * qu + (qu + ku) / 2) / (qu + ku)));
+    const int64_t q = std::min<int64_t>(kBwdBlocks - 1, std::max<int64_t>(1, (kBwdBlocks * H + (H + KVH) / 2) / (H + KVH)));
     return {(unsigned)std::min(q, qb), (unsigned)std::min(kBwdBlocks - q, kb)};
 }
 
@@ -378,7 +376,7 @@ NNQK_API int nn_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, const v
         const Angles a{cos_table, sin_table, positions, table_rows, (unsigned)period, position_bits};
         const int e = with_type(dtype, [&](auto dt) {
             return with_team(team_of(D), [&](auto r) {
-                qk_norm_bwd_kernel<dt(), r(), kBwdHeads><<<dim3(g.q + g.k), dim3(kThreads), 0, st>>>(qs, ks, a, (unsigned)M, g.q, (float*)workspace, (int)D,
+                qk_norm_bwd_kernel<dt(), r()><<<dim3(g.q + g.k), dim3(kThreads), 0, st>>>(qs, ks, a, (unsigned)M, g.q, (float*)workspace, (int)D,
                                                                                                           1.f / (float)D, eps);
                 return launched("qk_norm_bwd_kernel");
             });
