@@ -19,6 +19,11 @@ rotates k with it and q inside the layout-fused attention op (nanonemo::flash_at
 kernel (nanonemo::cuda_add_rms_norm_fwd / _bwd, the reference's norm_kernel="cuda"), and ``emb_kernel="hip"`` the token
 embedding and its gradient (nanonemo::embedding).
 
+``qk_norm`` normalises each head's queries and keys before their rotation (RMSNorm over head_dim, one weight for queries and one
+for keys); a HIP RoPE kernel then gives way to nanonemo::qk_norm_rope, which does both in one pass. A ``packing``
+(kernels/hip/packed.py; ``NanoNemo.pack``) makes a batch's tokens, in order, sequences of different lengths: attention stays within
+each (nanonemo::flash_attn_packed with a HIP attention) and positions begin anew.
+
 A model with any of them set also runs its linear layers, SwiGLU and cross entropy on this build's kernels where it is
 called eagerly on a GPU under 16-bit autocast (kernels/hip/linear.py, layers.py and head.py say exactly when; there the
 "hip_bthd" attention with either RoPE kernel is one autograd node, with q rotated by the RoPE kernel, whose result is
@@ -64,6 +69,7 @@ class ModelConfig:
     rope_kernel: str = "torch"
     norm_kernel: str = "torch"  # "torch" | "hip" (fused residual add + RMSNorm, nanonemo::cuda_add_rms_norm_*)
     emb_kernel: str = "torch"  # "torch" | "hip" (lookup, and the gradient by sorted tokens, nanonemo::embedding)
+    qk_norm: bool = False  # RMSNorm of each query and key head's vector before RoPE
     emb_scale: float = 1.0  # the embeddings times this (sqrt(d_model) in models that scale them)
 
     def __post_init__(self):
@@ -162,7 +168,8 @@ def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, seq_dim: int) ->
 
 
 class Attention(nn.Module):
-    """Causal GQA self-attention (layers.py:77-116)."""
+    """Causal GQA self-attention (layers.py:77-116). With a packing, x is one row of all its tokens and cos and sin hold a row
+    for each of them."""
 
     def __init__(self, cfg: ModelConfig):
         super().__init__()
@@ -172,18 +179,40 @@ class Attention(nn.Module):
         self.wk = nn.Linear(cfg.d_model, self.KVH * self.hd, bias=False)
         self.wv = nn.Linear(cfg.d_model, self.KVH * self.hd, bias=False)
         self.wo = nn.Linear(self.H * self.hd, cfg.d_model, bias=False)
+        if cfg.qk_norm:
+            self.q_norm, self.k_norm = RMSNorm(self.hd, cfg.norm_eps), RMSNorm(self.hd, cfg.norm_eps)
         if cfg.attn_kernel != "torch":
             from nanonemo_amd.kernels.hip import flash_attn as fa  # registers the ops; raises without the library
+            from nanonemo_amd.kernels.hip.packed import flash_attn_packed
 
-            self._fa = fa
+            self._fa, self._packed = fa, flash_attn_packed
         if cfg.rope_kernel in ("hip", "fused"):
+            from nanonemo_amd.kernels.hip.qk_norm import qk_norm_rope
             from nanonemo_amd.kernels.hip.rope import rope_k, rope_qk
 
-            self._rope_qk, self._rope_k = rope_qk, rope_k
+            self._rope_qk, self._rope_k, self._qk_norm_rope = rope_qk, rope_k, qk_norm_rope
 
-    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+    def _rotated(self, q, k, cos, sin):
+        """q and k (B, T, heads, hd), normalised if the model does, and rotated."""
+        if self.cfg.rope_kernel == "torch":
+            if self.cfg.qk_norm:
+                q, k = self.q_norm(q), self.k_norm(k)
+            return rope(q, cos, sin, seq_dim=1), rope(k, cos, sin, seq_dim=1)
+        if self.cfg.qk_norm:
+            return self._qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, eps=self.cfg.norm_eps)
+        return self._rope_qk(q, k, cos, sin)  # in the projection layout, q and k in one launch
+
+    def _attend_packed(self, q, k, v, packing):
+        """Attention within each of the packing's sequences: q, k, v (tokens, heads, hd) -> (tokens, H, hd)."""
+        if self.cfg.attn_kernel != "torch":
+            return self._packed(q, k, v, packing)
+        ys = [self._attend_torch(*(t[None].transpose(1, 2) for t in ts)) for ts in zip(*(t.split(packing.lengths) for t in (q, k, v))) if len(ts[0])]
+        return torch.cat(ys, dim=2)[0].transpose(0, 1)
+
+    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, packing=None) -> torch.Tensor:
         B, T, _ = x.shape
-        if self.cfg.attn_kernel == "hip_bthd" and self.cfg.rope_kernel != "torch" and x.is_cuda:
+        fusible = self.cfg.attn_kernel == "hip_bthd" and self.cfg.rope_kernel != "torch" and not self.cfg.qk_norm and packing is None
+        if fusible and x.is_cuda:
             from nanonemo_amd.kernels.hip import layers
 
             call = (x, cos, sin, self.H, self.KVH)
@@ -194,6 +223,16 @@ class Attention(nn.Module):
         q = q.view(B, T, self.H, self.hd)
         k = k.view(B, T, self.KVH, self.hd)
         v = v.view(B, T, self.KVH, self.hd)
+        if packing is not None:
+            q, k = self._rotated(q, k, cos, sin)
+            return _project(self.cfg, self._attend_packed(q[0], k[0], v[0], packing).reshape(B, T, -1), self.wo)[0]
+        if self.cfg.qk_norm:
+            q, k = self._rotated(q, k, cos, sin)
+            if self.cfg.attn_kernel == "hip_bthd":
+                return _project(self.cfg, self._fa.flash_attn_bthd(q, k, v).view(B, T, -1), self.wo)[0]
+            q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+            y = self._fa.flash_attn(q, k, v) if self.cfg.attn_kernel == "hip" else self._attend_torch(q, k, v)
+            return _project(self.cfg, y.transpose(1, 2).reshape(B, T, -1), self.wo)[0]
         if self.cfg.rope_kernel == "fused":  # k rotated here, q inside the attention op
             k = self._rope_k(k, cos, sin)
             return _project(self.cfg, self._fa.flash_attn_bthd_rope(q, k, v, cos, sin).view(B, T, -1), self.wo)[0]
@@ -207,19 +246,19 @@ class Attention(nn.Module):
         q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)  # (B, heads, T, hd) views
         if not hip_rope:
             q, k = rope(q, cos, sin, seq_dim=2), rope(k, cos, sin, seq_dim=2)
-        if self.cfg.attn_kernel == "hip":
-            y = self._fa.flash_attn(q, k, v)
-        else:
-            g = self.H // self.KVH
-            kr, vr = k.repeat_interleave(g, dim=1), v.repeat_interleave(g, dim=1)
-            if self.cfg.attn_backend == "math_fp32":
-                with torch.autocast(q.device.type, enabled=False), sdpa_kernel(SDPBackend.MATH):
-                    y = F.scaled_dot_product_attention(q.float(), kr.float(), vr.float(), is_causal=True).to(q.dtype)
-            else:
-                backend = {"math": SDPBackend.MATH, "mem_efficient": SDPBackend.EFFICIENT_ATTENTION}[self.cfg.attn_backend]
-                with sdpa_kernel(backend):
-                    y = F.scaled_dot_product_attention(q, kr, vr, is_causal=True)
+        y = self._fa.flash_attn(q, k, v) if self.cfg.attn_kernel == "hip" else self._attend_torch(q, k, v)
         return _project(self.cfg, y.transpose(1, 2).reshape(B, T, -1), self.wo)[0]
+
+    def _attend_torch(self, q, k, v):
+        """The "torch" attention of (B, heads, T, hd)."""
+        g = self.H // self.KVH
+        kr, vr = k.repeat_interleave(g, dim=1), v.repeat_interleave(g, dim=1)
+        if self.cfg.attn_backend == "math_fp32":
+            with torch.autocast(q.device.type, enabled=False), sdpa_kernel(SDPBackend.MATH):
+                return F.scaled_dot_product_attention(q.float(), kr.float(), vr.float(), is_causal=True).to(q.dtype)
+        backend = {"math": SDPBackend.MATH, "mem_efficient": SDPBackend.EFFICIENT_ATTENTION}[self.cfg.attn_backend]
+        with sdpa_kernel(backend):
+            return F.scaled_dot_product_attention(q, kr, vr, is_causal=True)
 
 
 class MLP(nn.Module):
@@ -293,9 +332,9 @@ class Block(nn.Module):
         self.norm_mlp = AddRMSNorm(cfg.d_model, cfg.norm_eps, cfg.norm_kernel)
         self.mlp = MLP(cfg)
 
-    def forward(self, x, cos, sin, delta=None):
+    def forward(self, x, cos, sin, delta=None, packing=None):
         h, x = self.norm_attn(x, delta)
-        h, x = self.norm_mlp(x, self.attn(h, cos, sin))
+        h, x = self.norm_mlp(x, self.attn(h, cos, sin) if packing is None else self.attn(h, cos, sin, packing))
         return x, self.mlp(h)
 
 
@@ -349,19 +388,37 @@ class NanoNemo(nn.Module):
             nn.init.normal_(blk.attn.wo.weight, std=resid_std)
             nn.init.normal_(blk.mlp.w_down.weight, std=resid_std)
 
-    def hidden(self, idx: torch.Tensor) -> torch.Tensor:
-        """The output layer's input for tokens (B, T)."""
-        T = idx.shape[1]
+    def pack(self, lengths):
+        """The packing of sequences of these lengths, one behind the other, in a batch for this model (kernels/hip/packed.py)."""
+        from nanonemo_amd.kernels.hip.packed import Packing
+
+        return Packing(lengths, self.cfg.n_heads, self.cfg.n_kv_heads, self.rope_cos.device)
+
+    def hidden(self, idx: torch.Tensor, packing=None) -> torch.Tensor:
+        """The output layer's input for tokens (B, T), with a packing its sequences row by row."""
+        T = idx.shape[1] if packing is None else packing.longest
         if T > self.cfg.max_seq_len:
             raise ValueError(f"sequence length {T} > max_seq_len {self.cfg.max_seq_len}")
+        if packing is not None:
+            return self._hidden_packed(idx, packing)
         x, delta = self.tok_emb(idx), None
         for blk in self.blocks:
             x, delta = blk(x, self.rope_cos, self.rope_sin, delta)
         return self.norm_out(x, delta)[0]
 
-    def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None, teacher: Teacher | None = None):
-        """(logits, loss): the targets' cross entropy, with a teacher the distillation loss, None without either."""
-        h = self.hidden(idx)
+    def _hidden_packed(self, idx: torch.Tensor, packing) -> torch.Tensor:
+        if idx.numel() != packing.tokens:
+            raise ValueError(f"{idx.numel()} tokens, but a packing of {packing.tokens}")
+        x, delta = self.tok_emb(idx.reshape(1, -1)), None
+        cos, sin = self.rope_cos[packing.positions], self.rope_sin[packing.positions]  # once for all blocks
+        for blk in self.blocks:
+            x, delta = blk(x, cos, sin, delta, packing)
+        return self.norm_out(x, delta)[0].view(*idx.shape, -1)
+
+    def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None, teacher: Teacher | None = None, packing=None):
+        """(logits, loss): the targets' cross entropy, with a teacher the distillation loss, None without either. With a packing
+        (``pack``) the tokens, row by row, are its sequences."""
+        h = self.hidden(idx) if packing is None else self.hidden(idx, packing)
         if teacher is not None:
             return self._distill(h, teacher, targets)
         if targets is not None and self.cfg.any_hip and h.is_cuda:
@@ -389,9 +446,9 @@ class NanoNemo(nn.Module):
         return logits, distill.distill_loss(logits, teacher.values, teacher.indices, teacher.rest, targets, teacher.temperature, teacher.weight)
 
     @torch.no_grad()
-    def teach(self, idx: torch.Tensor, k: int, temperature: float = 1.0, weight: float = 0.5) -> Teacher:
+    def teach(self, idx: torch.Tensor, k: int, temperature: float = 1.0, weight: float = 0.5, packing=None) -> Teacher:
         """This model's k largest logits for tokens (B, T), for a student with the same vocabulary."""
-        logits = self.lm_head(self.hidden(idx))
+        logits = self.lm_head(self.hidden(idx) if packing is None else self.hidden(idx, packing))
         if self.cfg.any_hip and logits.is_cuda:
             from nanonemo_amd.kernels.hip import distill
 

@@ -35,12 +35,12 @@ CURVE_BOUND = 0.12
 
 def train_step(model, opt, batches, grad_clip: float = 1.0, amp_dtype=torch.bfloat16):
     """One optimizer step over the micro-batches ``batches`` [(x, y), ...] or, for a student, [(x, y, teacher), ...]
-    (``teacher_batches``); returns (loss, grad_norm) as device tensors (no host synchronisation)."""
+    (``teacher_batches``), or of packed documents, [(x, y, None, packing), ...] (``packed_batches``); returns (loss, grad_norm) as device tensors (no host synchronisation)."""
     accum = len(batches)
     loss_sum = None
-    for x, y, *teacher in batches:
+    for x, y, *more in batches:
         with torch.autocast(x.device.type, dtype=amp_dtype, enabled=amp_dtype is not None):
-            _, loss = model(x, y, *teacher)
+            _, loss = model(x, y, *more)
         loss = loss / accum
         loss.backward()
         loss = loss.detach()
@@ -53,11 +53,31 @@ def train_step(model, opt, batches, grad_clip: float = 1.0, amp_dtype=torch.bflo
 
 def teacher_batches(teacher, batches, k: int, temperature: float = 2.0, weight: float = 0.5, amp_dtype=torch.bfloat16):
     """The micro-batches [(x, y), ...] with what ``teacher`` (a NanoNemo with the student's vocabulary) says of them:
-    [(x, y, its top k logits), ...] for ``train_step``."""
+    [(x, y, its top k logits), ...] for ``train_step``. Packed ones, [(x, y, None, packing), ...], keep their packing, which must
+    suit the teacher's heads too."""
     out = []
-    for x, y in batches:
+    for x, y, *more in batches:
         with torch.autocast(x.device.type, dtype=amp_dtype, enabled=amp_dtype is not None):
-            out.append((x, y, teacher.teach(x, k, temperature, weight)))
+            out.append((x, y, teacher.teach(x, k, temperature, weight, *more[1:]), *more[1:]))
+    return out
+
+
+def packed_batches(model, documents, tokens: int):
+    """Documents (1-D tensors of token ids) as micro-batches of at most ``tokens`` tokens for ``train_step``, without padding:
+    [(x, y, None, packing), ...], x and y (1, n). Every document is a sequence that predicts its next tokens; longer ones than
+    the model's context or a batch go on in another sequence, which begins with the last token of the one before."""
+    device = model.rope_cos.device
+    most = min(model.cfg.max_seq_len, tokens)
+    pieces = [d[a : a + most + 1] for d in documents for a in range(0, len(d) - 1, most)]
+    out, here, room = [], [], tokens
+    for piece in [*pieces, None]:
+        if here and (piece is None or len(piece) - 1 > room):
+            x, y = (torch.cat(ts).unsqueeze(0).to(device) for ts in ([p[:-1] for p in here], [p[1:] for p in here]))
+            out.append((x, y, None, model.pack([len(p) - 1 for p in here])))
+            here, room = [], tokens
+        if piece is not None:
+            here.append(piece)
+            room -= len(piece) - 1
     return out
 
 
@@ -71,6 +91,17 @@ def synthetic_batches(steps: int, batch: int, seq: int, vocab: int, device, seed
     return out
 
 
+def synthetic_documents(steps: int, tokens: int, mean: int, vocab: int, seed: int = 0):
+    """Documents of uniform token ids with lengths spread log-normally about ``mean``, enough for ``steps`` batches of ``tokens``."""
+    g = torch.Generator(device="cpu").manual_seed(seed)
+    out, left = [], steps * tokens
+    while left > 0:
+        n = 2 + int(mean * torch.exp(0.8 * torch.randn((), generator=g) - 0.32))
+        out.append(torch.randint(0, vocab, (n,), generator=g))
+        left -= n - 1
+    return out
+
+
 def make_optimizer(model, lr: float = 6e-4):
     decay = [p for p in model.parameters() if p.dim() >= 2]
     no_decay = [p for p in model.parameters() if p.dim() < 2]
@@ -81,13 +112,14 @@ def make_optimizer(model, lr: float = 6e-4):
 
 
 def run(attn: str, steps: int, batch: int, seq: int, cfg_kwargs: dict, device: str = "cuda", warmup: int = 3,
-        distinct: int = 0):
+        distinct: int = 0, docs: int = 0):
     """Train ``steps`` steps from the seed-0 init on the seed-0 synthetic stream; returns the per-step
     losses and the tokens/s over the steps after ``warmup``. ``attn`` is an attn_kernel, optionally
     with "+rope" (rope_kernel="hip"), "+qrope" (rope_kernel="fused": q's RoPE inside the attention op),
     "+norm" (norm_kernel="hip") and "+emb" (emb_kernel="hip") suffixes. ``distinct`` > 0 cycles through that many seed-0 batches instead of a
     fresh batch per step: a stream the model can memorise, so that the loss falls and the curves have something to
-    track (on uniform fresh tokens the loss stays near ln(vocab))."""
+    track (on uniform fresh tokens the loss stays near ln(vocab)). ``docs`` > 0 trains on batches of packed documents of that mean
+    length instead of full sequences."""
     torch.manual_seed(0)
     attn, _, backend = attn.partition("@")  # "torch@mem_efficient": the plain attention on another SDPA backend
     if backend:
@@ -101,19 +133,22 @@ def run(attn: str, steps: int, batch: int, seq: int, cfg_kwargs: dict, device: s
                                  norm_kernel="hip" if "norm" in extras else "torch",
                                  emb_kernel="hip" if "emb" in extras else "torch")).to(device)
     opt = make_optimizer(model)
-    data = synthetic_batches(distinct or steps, batch, seq, model.cfg.vocab_size, device)
+    if docs:
+        data = packed_batches(model, synthetic_documents(distinct or steps, batch * seq, docs, model.cfg.vocab_size), batch * seq)
+    else:
+        data = synthetic_batches(distinct or steps, batch, seq, model.cfg.vocab_size, device)
     data = [data[i % len(data)] for i in range(steps)]
     losses = []
     t0 = None
-    for i, (x, y) in enumerate(data):
+    for i, micro in enumerate(data):
         if i == warmup:
             torch.cuda.synchronize()
             t0 = time.perf_counter()
-        loss, _ = train_step(model, opt, [(x, y)])
+        loss, _ = train_step(model, opt, [micro])
         losses.append(loss)
     torch.cuda.synchronize()
     dt = time.perf_counter() - t0 if t0 is not None else float("nan")
-    tokens = (steps - warmup) * batch * seq
+    tokens = sum(micro[0].numel() for micro in data[warmup:])
     return [float(v) for v in torch.stack(losses).cpu()], tokens / dt, model.flops_per_token(seq)
 
 
@@ -131,15 +166,18 @@ def main():
     p.add_argument("--distinct", type=int, default=0,
                    help="cycle through this many fixed batches (a stream the model can memorise) instead of fresh "
                    "uniform batches; 0: a fresh batch per step (BASELINE config 5)")
+    p.add_argument("--docs", type=int, default=0,
+                   help="train on packed documents of this mean length (packed attention) instead of full sequences")
+    p.add_argument("--qk-norm", action="store_true", help="a model that normalises queries and keys before RoPE")
     p.add_argument("--torch-backend", default="math_fp32", choices=["math", "mem_efficient", "math_fp32"],
                    help="SDPA backend of the torch attention (math_fp32: fp32 math on upcast q, k, v)")
     a = p.parse_args()
     cfg_kwargs = dict(n_layers=2, d_model=256, n_heads=4, n_kv_heads=2, d_ff=512, vocab_size=512, max_seq_len=a.seq) \
         if a.small else dict(max_seq_len=a.seq)
-    cfg_kwargs["attn_backend"] = a.torch_backend
+    cfg_kwargs.update(attn_backend=a.torch_backend, qk_norm=a.qk_norm)
     res = {}
     for attn in a.attn:
-        losses, tps, fpt = run(attn, a.steps, a.batch, a.seq, cfg_kwargs, distinct=a.distinct)
+        losses, tps, fpt = run(attn, a.steps, a.batch, a.seq, cfg_kwargs, distinct=a.distinct, docs=a.docs)
         res[attn] = {"tokens_per_s": round(tps, 1), "model_tflops": round(tps * fpt / 1e12, 2), "loss_first": losses[0],
                      "loss_last": losses[-1], "losses": [round(v, 5) for v in losses]}
         print(f"[train] attn={attn}: {tps:,.0f} tokens/s, loss {losses[0]:.4f} -> {losses[-1]:.4f}", flush=True)
@@ -154,6 +192,8 @@ def main():
                 res[attn]["first_step_past_0.01"] = next((i for i, x in enumerate(d) if x > 0.01), None)
                 res[attn]["curve_within_bounds"] = bool(d[0] <= STEP0_BOUND and max(d) <= CURVE_BOUND)
     stream = f"{a.distinct} fixed batches of uniform tokens, cycled" if a.distinct else "uniform synthetic tokens"
+    if a.docs:
+        stream += f", packed documents of about {a.docs} tokens"
     print(json.dumps({"workload": f"114M NanoNemo bf16 autocast, B={a.batch} T={a.seq}, {a.steps} AdamW steps, "
                       f"seed 0, {stream}; torch attention: SDPA {a.torch_backend}",
                       "bounds": {"step0_abs_loss_diff": STEP0_BOUND, "max_abs_loss_diff": CURVE_BOUND},

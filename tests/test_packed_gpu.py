@@ -283,3 +283,108 @@ def test_on_another_stream_and_captured_into_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, both())), i
+
+
+SMALL = dict(n_layers=2, d_model=256, n_heads=4, n_kv_heads=2, d_ff=512, vocab_size=512, max_seq_len=256, attn_backend="math_fp32")
+
+
+def _step(cfg, state, idx, y, lengths):
+    from nanonemo_amd.model import ModelConfig, NanoNemo
+
+    model = NanoNemo(ModelConfig(**SMALL, **cfg)).cuda()
+    model.load_state_dict(state)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        logits, loss = model(idx, y, None, model.pack(lengths) if lengths else None)
+    loss.backward()
+    return loss.item(), logits.float(), {n: p.grad for n, p in model.named_parameters()}
+
+
+@pytest.mark.parametrize("qk_norm", [False, True])
+@pytest.mark.parametrize("attn, rope", [("hip_bthd", "hip"), ("hip", "hip"), ("hip_bthd", "torch"), ("hip_bthd", "fused")])
+@pytest.mark.parametrize("lengths", [None, [200, 1, 55, 0, 130, 126]])
+def test_model_with_the_kernels_matches_the_plain_one(lengths, attn, rope, qk_norm):
+    from nanonemo_amd.model import ModelConfig, NanoNemo
+
+    if lengths is None and not qk_norm:
+        pytest.skip("the dense model without the norm is tested elsewhere")
+    print(f"\n[case] model attn={attn} rope={rope} qk_norm={qk_norm} lengths={lengths}", flush=True)
+    torch.manual_seed(0)
+    state = NanoNemo(ModelConfig(**SMALL, qk_norm=qk_norm)).state_dict()
+    for n, t in state.items():
+        if n.endswith(("q_norm.weight", "k_norm.weight")):
+            t.normal_(1.0, 0.2)
+    idx, y = (torch.randint(0, 512, (2, 256), device="cuda") for _ in range(2))
+    y[0, 199] = -100
+    plain = _step(dict(qk_norm=qk_norm), state, idx, y, lengths)
+    got = _step(dict(qk_norm=qk_norm, attn_kernel=attn, rope_kernel=rope, norm_kernel="hip"), state, idx, y, lengths)
+    # bf16 activations: 2^-8 for each of some ten roundings a block on values that the norms keep at 1, at random: 2^-8 sqrt(20),
+    # times the output weights' 0.02 sqrt(256) = 0.32 for a logit; the loss averages 511 of them. Gradients: as the model's other
+    # kernels are held to, a twentieth of the tensor's norm.
+    assert abs(got[0] - plain[0]) < 5e-3
+    assert (got[1] - plain[1]).abs().max() < 5 * 2**-8 * math.sqrt(20) * 0.32
+    for n, g in plain[2].items():
+        assert (got[2][n] - g).norm() <= 0.05 * g.norm() + 1e-6, n
+
+
+def test_packed_training_step():
+    from nanonemo_amd.model import ModelConfig, NanoNemo
+    from nanonemo_amd.train import make_optimizer, packed_batches, synthetic_documents, teacher_batches, train_step
+
+    torch.manual_seed(0)
+    cfg = ModelConfig(**SMALL, attn_kernel="hip_bthd", rope_kernel="hip", norm_kernel="hip", emb_kernel="hip", qk_norm=True)
+    model, teacher = NanoNemo(cfg).cuda(), NanoNemo(cfg).cuda()
+    batches = packed_batches(model, synthetic_documents(2, 600, 70, 512), 600)
+    assert len(batches) >= 2 and all(x.is_cuda and p.device.type == "cuda" for x, _, _, p in batches)
+    before = {n: p.clone() for n, p in model.named_parameters()}
+    opt = make_optimizer(model)
+    for some in (batches[:2], teacher_batches(teacher, batches[:2], 8)):
+        loss, norm = train_step(model, opt, some)
+        assert loss.isfinite() and norm.isfinite()
+    assert all(not torch.equal(before[n], p) for n, p in model.named_parameters())
+
+
+def test_the_two_operators_together():
+    """A model's attention between its projections: norm and rotation of q and k where they lie, attention within sequences, and
+    the gradient of the projection and the norms' weights, against float64 with the roundings between the two counted."""
+    from nanonemo_amd.kernels.hip.qk_norm import qk_norm_rope
+
+    lengths, H, KVH, D = [130, 1, 0, 64, 45, 260], 12, 4, 64
+    T = sum(lengths)
+    packing = _packing(lengths, H, KVH)
+    g = torch.Generator(device="cuda").manual_seed(12)
+    qkv = (2 * torch.randn(T, (H + 2 * KVH) * D, device="cuda", generator=g)).bfloat16().requires_grad_()
+    wq, wk = ((1 + 0.2 * torch.randn(D, device="cuda", generator=g)).requires_grad_() for _ in range(2))
+    do = torch.randn(T, H, D, device="cuda", generator=g).bfloat16()
+    angle = torch.outer(torch.arange(300, dtype=torch.float64), 10000.0 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D))
+    cos, sin = angle.cos().float().cuda(), angle.sin().float().cuda()
+
+    def chain(qkv, wq, wk, cos, sin, rotate, attend):
+        q, k, v = (t.view(T, -1, D) for t in qkv.split([H * D, KVH * D, KVH * D], 1))
+        return attend(*rotate(q, k, wq, wk, cos, sin), v)
+
+    o = chain(qkv, wq, wk, cos, sin, lambda *a: qk_norm_rope(*a, packing.positions), lambda *a: _call(*a, packing))
+    got = (o.detach(), *torch.autograd.grad(o, (qkv, wq, wk), do))
+
+    def rotate64(q, k, wq, wk, cos, sin):
+        c, s = (t[packing.positions].unsqueeze(1) for t in (cos, sin))
+        outs = []
+        for x, w in ((q, wq), (k, wk)):
+            a, b = (w * x / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-5)).chunk(2, -1)
+            outs.append(torch.cat((a * c - b * s, a * s + b * c), -1))
+        return outs
+
+    def attend64(q, k, v):
+        outs = []
+        for a, b, c in zip(q.split(lengths), k.split(lengths), v.split(lengths)):
+            b, c = b.repeat_interleave(H // KVH, 1), c.repeat_interleave(H // KVH, 1)
+            x = torch.matmul(a.transpose(0, 1), b.permute(1, 2, 0)) / math.sqrt(D)
+            x = x.masked_fill(torch.ones(x.shape[1:], dtype=torch.bool, device="cuda").triu(1), -math.inf)
+            outs.append(torch.matmul(x.softmax(-1), c.transpose(0, 1)).transpose(0, 1))
+        return torch.cat(outs)
+
+    ins = [t.detach().double().requires_grad_() for t in (qkv, wq, wk)]
+    ref = chain(*ins, cos.double(), sin.double(), rotate64, attend64)
+    want = (ref.detach(), *torch.autograd.grad(ref, ins, do.double()))
+    # (q and k between the two are rounded to bf16: the errors of o and the gradients double at most in the norm, 2 * TOL's fro)
+    for name, x, y, tol in zip(("o", "dqkv", "dwq", "dwk"), got, want, (TOL, TOL_GRAD, TOL_GRAD, TOL_GRAD)):
+        assert_close_tol(x, y, {**tol[torch.bfloat16], "fro": 2 * tol[torch.bfloat16]["fro"]}, name)

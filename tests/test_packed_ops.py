@@ -258,3 +258,59 @@ def test_capture_through_autograd_is_refused(monkeypatch):
         packed.flash_attn_packed(q, k, k, packing)
     with pytest.raises(RuntimeError, match="while a HIP graph is captured"):
         packed.Packing([3], 4, 2, device="cuda")
+
+
+SMALL = dict(n_layers=2, d_model=128, n_heads=4, n_kv_heads=2, d_ff=256, vocab_size=97, max_seq_len=64)
+
+
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_a_packed_model_is_the_model_on_each_sequence(qk_norm):
+    from nanonemo_amd.model import ModelConfig, NanoNemo
+
+    torch.manual_seed(0)
+    model = NanoNemo(ModelConfig(**SMALL, qk_norm=qk_norm))
+    assert ("blocks.0.attn.q_norm.weight" in model.state_dict()) == qk_norm
+    if qk_norm:
+        for p in (model.blocks[0].attn.q_norm.weight, model.blocks[1].attn.k_norm.weight):
+            torch.nn.init.normal_(p, 1.0, 0.2)
+    lengths = [5, 0, 1, 64, 20]
+    idx, y = (torch.randint(0, 97, (2, 45)) for _ in range(2))
+    y[0, 4] = -100
+    packing = model.pack(lengths)
+    logits, loss = model(idx, y, None, packing)
+    alone = torch.cat([model(t[None])[0][0] for t in idx.flatten().split(lengths) if len(t)])
+    # the same fp32 sums in another order: 2^-24 of about 1 each, some hundred of them
+    torch.testing.assert_close(logits.view(90, -1), alone, rtol=1e-4, atol=1e-4)
+    torch.testing.assert_close(loss, torch.nn.functional.cross_entropy(alone, y.flatten()), rtol=1e-5, atol=1e-5)
+    assert model(idx, None, None, packing)[1] is None
+    t = model.teach(idx, 3, packing=packing)
+    assert torch.equal(t.indices, logits.topk(3).indices)
+    loss = model(idx, y, t, packing)[1]
+    loss.backward()
+    assert all(p.grad is not None for p in model.parameters())
+    with pytest.raises(ValueError, match="90 tokens, but a packing of 89"):
+        model(idx, None, None, model.pack([64, 25]))
+    with pytest.raises(ValueError, match="max_seq_len"):
+        model(idx, None, None, model.pack([65, 25]))
+
+
+def test_packed_batches():
+    from nanonemo_amd.model import ModelConfig, NanoNemo
+    from nanonemo_amd.train import packed_batches, synthetic_documents, teacher_batches, train_step
+
+    model = NanoNemo(ModelConfig(**SMALL))
+    docs = [torch.arange(n) % 97 for n in (10, 1, 0, 2, 150, 33)]
+    batches = packed_batches(model, docs, 80)
+    assert [p.lengths for *_, p in batches] == [(9, 1, 64), (64,), (21, 32)]
+    for x, y, none, p in batches:
+        assert none is None and x.shape == y.shape == (1, p.tokens) and torch.equal(y, (x + 1) % 97)
+    assert torch.equal(batches[1][0][0], torch.arange(64, 128) % 97)  # a long document goes on where it was cut
+    assert packed_batches(model, [], 80) == []
+    assert [p.lengths for *_, p in packed_batches(model, docs[:1], 4)] == [(4,), (4,), (1,)]
+    docs = synthetic_documents(3, 80, 20, 97)
+    assert sum(len(d) - 1 for d in docs) >= 240 and max(int(d.max()) for d in docs) < 97
+    student = NanoNemo(ModelConfig(**SMALL))
+    opt = torch.optim.SGD(student.parameters(), 0.1)
+    for some in (batches[:2], teacher_batches(model, batches[:2], 3, amp_dtype=None)):
+        loss, norm = train_step(student, opt, some, amp_dtype=None)
+        assert loss.isfinite() and norm > 0
