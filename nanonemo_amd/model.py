@@ -225,7 +225,8 @@ class Attention(nn.Module):
         v = v.view(B, T, self.KVH, self.hd)
         if packing is not None:
             q, k = self._rotated(q, k, cos, sin)
-            return _project(self.cfg, self._attend_packed(q[0], k[0], v[0], packing).reshape(B, T, -1), self.wo)[0]
+            q, k, v = (t.flatten(0, 1) for t in (q, k, v))  # (views; an index would fill and copy in the backward)
+            return _project(self.cfg, self._attend_packed(q, k, v, packing).reshape(B, T, -1), self.wo)[0]
         if self.cfg.qk_norm:
             q, k = self._rotated(q, k, cos, sin)
             if self.cfg.attn_kernel == "hip_bthd":
