@@ -6,8 +6,12 @@
  *   q, o, dO, dq   [tokens, H,   D]    k, v, dk, dv   [tokens, KVH, D]    lse   [H, tokens] fp32
  * with tokens their sum: row t of sequence i is row lengths[0] + .. + lengths[i - 1] + t. A query sees the keys of its own
  * sequence up to itself; otherwise everything is as in nanonemo_fa.h (types, head_dim 32 or 64, scale, lse, errors through
- * nn_fa_last_error, work only enqueued on `stream`, no atomics), and a sequence's o, lse and dq are the same bits as
- * nn_fa_fwd's and nn_fa_bwd's on it alone.
+ * nn_fa_last_error, work only enqueued on `stream`, no atomics), and a sequence's o and lse are the same bits as nn_fa_fwd's on
+ * it alone.
+ *
+ * rest: tokens * H * D bytes, or null. The forward writes into it what rounding o to 16 bits took off each value, in 8 bits, and
+ * a backward that is given it computes D = rowsum(dO * o) from both: dq and dk then carry the rounding of dS and their own, and
+ * none of o's. Without it dq is the same bits as nn_fa_bwd's.
  *
  * The work is laid out once for a batch, on the host: nn_fa_packed_plan fills `plan` (int32 words, in host memory), which the
  * caller copies to the device as it is (16-byte aligned) and keeps while it uses it, in both places. Its layout is the
@@ -40,7 +44,7 @@ int nn_fa_packed_plan_info(const int32_t* plan, nn_fa_packed_info* info);
 
 /* Forward. strides: element strides {head, row} of q, of k and v, and of o (6 values; positive multiples of 8, rows at
  * least D apart), or null for dense tensors. */
-int nn_fa_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* plan,
+int nn_fa_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* rest, const int32_t* plan,
                      const int32_t* device_plan, int64_t D, const int64_t* strides, int dtype, float scale, void* stream);
 
 /* Bytes of device workspace of the backward, 256-byte aligned: -rowsum(dO * o) and -lse / scale, and where pairs of 64-key
@@ -48,8 +52,8 @@ int nn_fa_packed_fwd(const void* q, const void* k, const void* v, void* o, float
 size_t nn_fa_packed_bwd_workspace_size(const int32_t* plan, int64_t D);
 
 /* Backward. strides: {head, row} of q and dO, of k and v, of o, of dq, and of dk and dv (10 values), or null. */
-int nn_fa_packed_bwd(const void* dO, const void* q, const void* k, const void* v, const void* o, const float* lse, void* dq,
-                     void* dk, void* dv, void* workspace, size_t workspace_bytes, const int32_t* plan,
+int nn_fa_packed_bwd(const void* dO, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                     const void* rest, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, const int32_t* plan,
                      const int32_t* device_plan, int64_t D, const int64_t* strides, int dtype, float scale, void* stream);
 
 #ifdef __cplusplus

@@ -212,8 +212,92 @@ struct PackedArg<true> {
     const void* list;  // PackedTile or PackedUnit
     int count;         // entries
     int tokens;        // of all sequences: the stride of the per-head vectors lse, -lse/scale and -D
+    uint32_t* rest;    // [tokens][H][HD] bytes: what rounding o to 16 bits took off (below), or null
 };
 using Packed = PackedArg<true>;
+// D = rowsum(dO * O) enters every dS, and an O of 16 bits puts an error of its own into it: with dS rounded to 16 bits before its
+// products, which the matrix unit asks for, and the gradients rounded once more, dq and dk come out 1.5 to 1.6 times as far from
+// the formula's as a single rounding; without O's share 1.4 (by arithmetic sqrt(2)). So a forward whose backward will be run
+// also writes the rest of each value in 8 bits, the difference of the two as fp32 words (one sign, so of their magnitudes) less
+// its last bits, and D is summed from the two: 1.44 to 1.49 times, for 2 us of 79 (8192 tokens of documents, forward and backward)
+// and 0.5 % where sequences are long. A row's bytes lie in the order in which the backward's lanes hold a
+// row, 16-byte pieces of theirs side by side: byte hh HD/2 + 8 s + j is column 16 s + 8 hh + j's. (In the columns' order, a lane's
+// 4 at a time, the stores took 4 us instead.)
+template <int DT>
+constexpr int kRestShift = DT == kBF16 ? 8 : 5;  // half a step is 2^15 or 2^12 of an fp32 word's
+// The 16-bit value in half j of w as an fp32 word.
+template <int DT>
+__device__ inline uint32_t word_of(uint32_t w, int j) {
+    if constexpr (DT == kBF16)
+        return j ? w & 0xffff0000u : w << 16;
+    else
+        return __float_as_uint(Elem<DT>::to_f32((u16)(w >> (16 * j))));
+}
+// The rests of four values v * mul whose roundings are w. (At the type's smallest values, where steps are larger than that, the
+// nearest there is.)
+template <int DT>
+__device__ inline uint32_t rest4(const f32x16& v, int at, float mul, u32x2 w) {
+    constexpr int most = (128 << kRestShift<DT>) - 1;
+    uint32_t d[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int diff = (int)(__float_as_uint(v[at + j] * mul) - word_of<DT>(w[j >> 1], j & 1));
+        d[j] = (uint32_t)min(max(diff, -most - 1), most) << (8 - kRestShift<DT>);  // the rest in bits 8 to 15
+    }
+    // (v_perm_b32: byte 1 of the second operand, byte 1 of the first, zeros)
+    return __builtin_amdgcn_perm(d[1], d[0], 0x0c0c0501u) | __builtin_amdgcn_perm(d[3], d[2], 0x0c0c0501u) << 16;
+}
+// x and y of lanes l < 32 and of lanes l + 32 as (x of the lower, x of the upper) in the lower and (y of the lower, y of the upper)
+// in the upper: from 4 columns of each of two groups of 8 (an accumulator's) to one whole group (an operand's).
+__device__ inline u32x2 pair_groups(uint32_t x, uint32_t y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    return u32x2{r[0], r[1]};
+}
+// A row's results acc * mul, held transposed (element i of acc[dt]: column 32 dt + (i / 4) * 8 + 4 hh + i % 4), rounded and stored
+// to `row`, 16 bytes at a time, and their rests to `rest` (null: none).
+template <int HD, int DT>
+__device__ inline void store_row(const f32x16* acc, float mul, int hh, u16* row, uint32_t* rest) {
+    using E = Elem<DT>;
+    constexpr int NS = HD / 16;
+    uint32_t r[2 * NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        const f32x16& a = acc[s / 2];
+        const int x = 8 * (s & 1), y = x + 4;  // where groups 2 s and 2 s + 1 of 8 columns begin
+        const u32x2 wx = {E::pack2(a[x] * mul, a[x + 1] * mul), E::pack2(a[x + 2] * mul, a[x + 3] * mul)};
+        const u32x2 wy = {E::pack2(a[y] * mul, a[y + 1] * mul), E::pack2(a[y + 2] * mul, a[y + 3] * mul)};
+        const u32x2 lo = pair_groups(wx[0], wy[0]), hi = pair_groups(wx[1], wy[1]);
+        if (row) *reinterpret_cast<u32x4*>(row + 16 * s + 8 * hh) = u32x4{lo[0], hi[0], lo[1], hi[1]};
+        if (rest) {
+            const u32x2 both = pair_groups(rest4<DT>(a, x, mul, wx), rest4<DT>(a, y, mul, wy));
+            r[2 * s] = both[0], r[2 * s + 1] = both[1];
+        }
+    }
+    if (rest) {
+#pragma unroll
+        for (int i = 0; i < 2 * NS; i += 4) *reinterpret_cast<u32x4*>(rest + hh * (HD / 8) + i) = u32x4{r[i], r[i + 1], r[i + 2], r[i + 3]};
+    }
+}
+// A row's rests as the lane's operands have its columns.
+template <int HD>
+__device__ inline void load_rests(const uint32_t* rest, int hh, u32x2* to) {
+#pragma unroll
+    for (int s = 0; s < HD / 16; s += 2) {
+        const u32x4 r = *reinterpret_cast<const u32x4*>(rest + hh * (HD / 8) + 2 * s);
+        to[s] = u32x2{r[0], r[1]}, to[s + 1] = u32x2{r[2], r[3]};
+    }
+}
+// acc + rowsum(g * o) over 8 values with their rests r.
+template <int DT>
+__device__ inline float dot_rest(u16x8 g, u16x8 o, u32x2 r, float acc) {
+    const u32x4 ow = __builtin_bit_cast(u32x4, o);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t q = (uint32_t)((int)(r[j >> 2] << (24 - 8 * (j & 3))) >> 24);
+        acc = fmaf(Elem<DT>::to_f32(g[j]), __uint_as_float(word_of<DT>(ow[j >> 1], j & 1) + (q << kRestShift<DT>)), acc);
+    }
+    return acc;
+}
 constexpr int kPairRows = 128;  // rows of a partial sum of packed dK/dV: the pair's two units
 // A forward or dQ block's batch, head and query block; packed: its sequence's start and length, and bh * T as the place of the
 // sequence's row 0 in the per-head fp32 vectors. Entry i of the packed list is for XCD i % 8 (block i goes to XCD i % 8), where
@@ -493,14 +577,18 @@ __global__ __launch_bounds__(256, 2) void fa_fwd_kernel(const u16* __restrict__ 
         }
         const float inv = 1.f / ltot;
         u16* op = O + lo.at(b, h) + (size_t)(start + qrow) * lo.st;
+        if constexpr (PACKED) {
+            store_row<HD, DT>(oacc, inv, hh, op, pk.rest ? pk.rest + ((size_t)(start + qrow) * H + h) * (HD / 4) : nullptr);
+        } else {
 #pragma unroll
-        for (int dt = 0; dt < ND; ++dt)
+            for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x16& a = oacc[dt];
-                u32x2 w = {E::pack2(a[4 * g] * inv, a[4 * g + 1] * inv), E::pack2(a[4 * g + 2] * inv, a[4 * g + 3] * inv)};
-                *reinterpret_cast<u32x2*>(op + 32 * dt + 8 * g + 4 * hh) = w;
-            }
+                for (int g = 0; g < 4; ++g) {
+                    const f32x16& a = oacc[dt];
+                    u32x2 w = {E::pack2(a[4 * g] * inv, a[4 * g + 1] * inv), E::pack2(a[4 * g + 2] * inv, a[4 * g + 3] * inv)};
+                    *reinterpret_cast<u32x2*>(op + 32 * dt + 8 * g + 4 * hh) = w;
+                }
+        }
         if (hh == 0) LSE[vec_row<PACKED>(pk, bh, h, start, T) + qrow] = (mb + fast_log2(ltot)) * kLn2;
     }
     NN_TL_END(kTlFwd);
@@ -1202,13 +1290,20 @@ __global__ __launch_bounds__(256, 2) void fa_bwd_dq_kernel(const u16* __restrict
     // one dQ block, which also writes both into the workspace for the dK/dV kernel that runs next.
     u16x8 qf[NS], gf[NS];
     float dacc = 0.f;
+    u32x2 rests[NS] = {};
+    if constexpr (PACKED)
+        if (pk.rest) load_rests<HD>(pk.rest + ((size_t)(start + qc_) * H + h) * (HD / 4), hh, rests);
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
         qf[s] = ld8(kB + 32 * wave * HD + koff[s]);
         gf[s] = ld8(vB + 32 * wave * HD + koff[s]);
         const u16x8 of = ld8(oS + 32 * wave * HD + koff[s]);
+        if constexpr (PACKED) {
+            dacc = dot_rest<DT>(gf[s], of, rests[s], dacc);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dacc = fmaf(E::to_f32(gf[s][j]), E::to_f32(of[j]), dacc);
+            for (int j = 0; j < 8; ++j) dacc = fmaf(E::to_f32(gf[s][j]), E::to_f32(of[j]), dacc);
+        }
     }
     const float nd = -pair_sum(dacc);
     const float nl2 = -lse * kLog2e;  // (-lse/scale) * sl2
@@ -1347,6 +1442,8 @@ __global__ __launch_bounds__(256, 2) void fa_bwd_dq_kernel(const u16* __restrict
                 *reinterpret_cast<u32x2*>(dst + clo) = u32x2{E::pack2(r1[0], r1[1]), E::pack2(r1[2], r1[3])};
                 *reinterpret_cast<u32x2*>(dst + chi) = u32x2{E::pack2(r2[0], r2[1]), E::pack2(r2[2], r2[3])};
             }
+        } else if constexpr (PACKED) {
+            store_row<HD, DT>(dq, scale, hh, dst, nullptr);
         } else {
 #pragma unroll
             for (int dt = 0; dt < ND; ++dt)
@@ -1491,6 +1588,7 @@ __global__ __launch_bounds__(256, 4) void fa_short_fwd_kernel(const u16* __restr
             }
     }
     const float ltot = pair_sum(lsum);
+    if (pk.rest && qrow < T) store_row<HD, DT>(oacc, 1.f / ltot, hh, nullptr, pk.rest + ((size_t)(e.start + qrow) * H + h) * (HD / 4));
     store_rows<HD, DT>(oacc, 1.f / ltot, vb, O + lo.at(0, h) + (size_t)(e.start + 32 * e.qb) * lo.st, lo.st, T - 32 * e.qb, lane);
     if (hh == 0 && qrow < T) LSE[(size_t)h * pk.tokens + e.start + qrow] = (mb + fast_log2(ltot)) * kLn2;
 }
@@ -1528,12 +1626,13 @@ __global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restr
 #pragma unroll
         for (int s = 0; s < NS; ++s) to[s] = ld8(at_ + 16 * s);
     };
-    auto rowsum = [&](const u16x8* g, const u16x8* o) {  // D of the lane's row
+    auto rests_of = [&](int head, int r, u32x2* to) {
+        if (pk.rest) load_rests<HD>(pk.rest + ((size_t)(e.start + min(r, T - 1)) * H + head) * (HD / 4), hh, to);
+    };
+    auto rowsum = [&](const u16x8* g, const u16x8* o, const u32x2* r) {  // D of the lane's row
         float acc = 0.f;
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc = fmaf(E::to_f32(g[s][j]), E::to_f32(o[s][j]), acc);
+        for (int s = 0; s < NS; ++s) acc = dot_rest<DT>(g[s], o[s], r[s], acc);
         return pair_sum(acc);
     };
     if (keys) {
@@ -1543,6 +1642,7 @@ __global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restr
         rows_of(K, lk, kvh, key, kf);
         rows_of(V, lk, kvh, key, vf);
         const DmaOffs<HD, 32, 1> fo = dma_offsets<HD, 32, 1>(lane, 0, lq.st);
+        u32x2 rs[NS] = {};
         float lse = 0.f;
         auto fetch = [&](int it) {  // iteration it's Q and dO tiles, O rows and lse
             const int iq = it / group, h = kvh * group + (it - iq * group), q0 = 32 * (tile + iq);
@@ -1551,6 +1651,7 @@ __global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restr
             dma_rows<HD, 32, 1>(Q + off, lq.st, q0, T, to, 0, fo);
             dma_rows<HD, 32, 1>(dO + off, lq.st, q0, T, to + TILE, 0, fo);
             rows_of(O, lo, h, q0 + l32, of);
+            rests_of(h, q0 + l32, rs);
             lse = LSE[(size_t)h * pk.tokens + e.start + min(q0 + l32, T - 1)];
         };
         f32x16 dk[ND], dv[ND];
@@ -1566,7 +1667,7 @@ __global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restr
 #pragma unroll
             for (int s = 0; s < NS; ++s) qa[s] = ld8(qt + roff[s]), oa[s] = ld8(ot + roff[s]);
             const int iq = it / group, row = 32 * (tile + iq) + l32;
-            const float nd = -rowsum(oa, of);
+            const float nd = -rowsum(oa, of, rs);
             if (hh == 0) vec[l32] = row < T ? -lse / scale : -INFINITY, vec[32 + l32] = row < T ? nd : 0.f;  // rows past T: p is 0
             if (it + 1 < n) fetch(it + 1);
             const f32x4* v4 = reinterpret_cast<const f32x4*>(vec + 4 * hh);
@@ -1606,7 +1707,9 @@ __global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restr
         const DmaOffs<HD, 32, 1> fo = dma_offsets<HD, 32, 1>(lane, 0, lk.st);
         u16x8 qf[NS], gf[NS], of[NS], ka[2][NS], va[2][NS];
         rows_of(dO, lq, h, qrow, gf);
+        u32x2 rs[NS] = {};
         rows_of(O, lo, h, qrow, of);
+        rests_of(h, qrow, rs);
         rows_of(Q, lq, h, qrow, qf);
         const float lse = LSE[(size_t)h * pk.tokens + e.start + min(qrow, T - 1)];
 #pragma unroll
@@ -1616,7 +1719,7 @@ __global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restr
             rows_of(V, lk, kvh, 32 * t + l32, va[t]);
             dma_rows<HD, 32, 1>(Kp, lk.st, 32 * t, T, lds + t * TILE, 0, fo);
         }
-        const float nd = -rowsum(gf, of), nl2 = -lse * kLog2e;
+        const float nd = -rowsum(gf, of, rs), nl2 = -lse * kLog2e;
         f32x16 dq[ND];
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) dq[dt] = f32x16{};
@@ -2335,40 +2438,40 @@ Workspace carve_packed(void* base, const PlanHead& p, int64_t D) {
 }
 
 template <int HD, int DT>
-int packed_fwd_impl(const void* q, const void* k, const void* v, void* o, float* lse, const PlanHead& p, const int32_t* dp, float scale,
-                    const Lays& l, hipStream_t st) {
+int packed_fwd_impl(const void* q, const void* k, const void* v, void* o, float* lse, uint32_t* rest, const PlanHead& p, const int32_t* dp,
+                    float scale, const Lays& l, hipStream_t st) {
     const int g = p.H / p.KVH;
     if (p.nshort) {
         fa_short_fwd_kernel<HD, DT><<<dim3((unsigned)(((int64_t)p.nshort * p.H + 3) / 4)), dim3(256), 0, st>>>(
-            (const u16*)q, (const u16*)k, (const u16*)v, (u16*)o, lse, Packed{dp + p.shorts, p.nshort, p.tokens}, p.H, p.KVH, scale * kLog2e, l.q, l.k, l.o);
+            (const u16*)q, (const u16*)k, (const u16*)v, (u16*)o, lse, Packed{dp + p.shorts, p.nshort, p.tokens, rest}, p.H, p.KVH, scale * kLog2e, l.q, l.k, l.o);
         if (int e = launch_status("fa_short_fwd_kernel")) return e;
     }
     if (p.ntiles == 0) return 0;
     fa_fwd_kernel<HD, DT, false, true><<<dim3((unsigned)(p.ntiles * g)), dim3(256), 0, st>>>(
         (const u16*)q, (const u16*)k, (const u16*)v, (u16*)o, lse, p.H, p.H, p.KVH, 0, 0, scale * kLog2e, l.q, l.k, l.o, RopeArgs{},
-        Packed{dp + p.tiles, p.ntiles, p.tokens});
+        Packed{dp + p.tiles, p.ntiles, p.tokens, rest});
     return launch_status("fa_fwd_kernel (packed)");
 }
 
 template <int HD, int DT>
-int packed_bwd_impl(const void* dO, const void* q, const void* k, const void* v, const void* o, const float* lse, void* dq, void* dk, void* dv,
+int packed_bwd_impl(const void* dO, const void* q, const void* k, const void* v, const void* o, const float* lse, uint32_t* rest, void* dq, void* dk, void* dv,
                     const Workspace& w, const PlanHead& p, const int32_t* dp, float scale, const Lays& l, hipStream_t st) {
     const int g = p.H / p.KVH;
     if (p.nshort) {
         fa_short_bwd_kernel<HD, DT><<<dim3((unsigned)(((int64_t)p.nshort * (p.H + p.KVH) + 3) / 4)), dim3(256), 0, st>>>(
             (const u16*)q, (const u16*)k, (const u16*)v, (const u16*)o, (const u16*)dO, lse, (u16*)dq, (u16*)dk, (u16*)dv,
-            Packed{dp + p.shorts, p.nshort, p.tokens}, p.H, p.KVH, scale * kLog2e, scale, l.q, l.k, l.o, l.dq, l.dk);
+            Packed{dp + p.shorts, p.nshort, p.tokens, rest}, p.H, p.KVH, scale * kLog2e, scale, l.q, l.k, l.o, l.dq, l.dk);
         if (int e = launch_status("fa_short_bwd_kernel")) return e;
     }
     if (p.ntiles == 0) return 0;
     fa_bwd_dq_kernel<HD, DT, false, true><<<dim3((unsigned)(p.ntiles * g)), dim3(256), 0, st>>>(
         (const u16*)q, (const u16*)k, (const u16*)v, (const u16*)o, (const u16*)dO, lse, w.nL, w.nD, (u16*)dq, p.H, p.H, p.KVH, 0, 0, scale * kLog2e,
-        scale, l.q, l.k, l.o, l.dq, RopeArgs{}, Packed{dp + p.tiles, p.ntiles, p.tokens});
+        scale, l.q, l.k, l.o, l.dq, RopeArgs{}, Packed{dp + p.tiles, p.ntiles, p.tokens, rest});
     if (int e = launch_status("fa_bwd_dq_kernel (packed)")) return e;
     auto launch = [&](auto kern, int per) {
         kern<<<dim3((unsigned)((p.nunits + per - 1) / per)), dim3(256), 0, st>>>(
             (const u16*)q, (const u16*)k, (const u16*)v, (const u16*)dO, w.nL, w.nD, (u16*)dk, (u16*)dv, p.KVH, p.H, p.KVH, 0, 0, 0, scale * kLog2e,
-            scale, l.q, l.k, l.dk, 1, w.part, 1, Packed{dp + p.units, p.nunits, p.tokens});
+            scale, l.q, l.k, l.dk, 1, w.part, 1, Packed{dp + p.units, p.nunits, p.tokens, nullptr});
     };
     if (p.wpp == 1)
         launch(fa_bwd_dkdv_kernel<HD, DT, 1, false, true>, 4);
@@ -2450,17 +2553,17 @@ NNFA_API int nn_fa_packed_plan_info(const int32_t* plan, nn_fa_packed_info* info
     return 0;
 }
 
-NNFA_API int nn_fa_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* plan, const int32_t* device_plan,
-                              int64_t D, const int64_t* strides, int dtype, float scale, void* stream) {
+NNFA_API int nn_fa_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* rest, const int32_t* plan,
+                              const int32_t* device_plan, int64_t D, const int64_t* strides, int dtype, float scale, void* stream) {
     g_last_error.clear();
     PlanHead p;
     if (int e = take_plan(plan, device_plan, D, dtype, &p)) return e;
     if (p.tokens == 0) return 0;
     if (!q || !k || !v || !o || !lse) return fail(-1, "null pointer argument");
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)) return fail(-1, "inputs must be 16-byte aligned");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(rest)) return fail(-1, "inputs must be 16-byte aligned");
     Lays l;
     if (int e = take_packed_lays(strides, p, D, false, &l)) return e;
-    return NNFA_DISPATCH(packed_fwd_impl, D, dtype, q, k, v, o, lse, p, device_plan, scale, l, (hipStream_t)stream);
+    return NNFA_DISPATCH(packed_fwd_impl, D, dtype, q, k, v, o, lse, (uint32_t*)rest, p, device_plan, scale, l, (hipStream_t)stream);
 }
 
 NNFA_API size_t nn_fa_packed_bwd_workspace_size(const int32_t* plan, int64_t D) {
@@ -2470,15 +2573,15 @@ NNFA_API size_t nn_fa_packed_bwd_workspace_size(const int32_t* plan, int64_t D) 
     return carve_packed(nullptr, p, D).bytes;
 }
 
-NNFA_API int nn_fa_packed_bwd(const void* dO, const void* q, const void* k, const void* v, const void* o, const float* lse, void* dq, void* dk,
-                              void* dv, void* workspace, size_t workspace_bytes, const int32_t* plan, const int32_t* device_plan, int64_t D,
+NNFA_API int nn_fa_packed_bwd(const void* dO, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* rest,
+                              void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, const int32_t* plan, const int32_t* device_plan, int64_t D,
                               const int64_t* strides, int dtype, float scale, void* stream) {
     g_last_error.clear();
     PlanHead p;
     if (int e = take_plan(plan, device_plan, D, dtype, &p)) return e;
     if (p.tokens == 0) return 0;
     if (!dO || !q || !k || !v || !o || !lse || !dq || !dk || !dv) return fail(-1, "null pointer argument");
-    if (!aligned16(dO) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
+    if (!aligned16(dO) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(rest))
         return fail(-1, "inputs must be 16-byte aligned");
     if (!(scale > 0.f)) return fail(-1, "scale must be positive");
     if (!workspace) return fail(-1, "null workspace");
@@ -2487,7 +2590,7 @@ NNFA_API int nn_fa_packed_bwd(const void* dO, const void* q, const void* k, cons
     if (workspace_bytes < w.bytes) return fail(-1, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, w.bytes);
     Lays l;
     if (int e = take_packed_lays(strides, p, D, true, &l)) return e;
-    return NNFA_DISPATCH(packed_bwd_impl, D, dtype, dO, q, k, v, o, lse, dq, dk, dv, w, p, device_plan, scale, l, (hipStream_t)stream);
+    return NNFA_DISPATCH(packed_bwd_impl, D, dtype, dO, q, k, v, o, lse, (uint32_t*)rest, dq, dk, dv, w, p, device_plan, scale, l, (hipStream_t)stream);
 }
 
 #if NN_TIMELINE

@@ -861,7 +861,8 @@ void check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Plan&
               " KV heads, the tensors of " + std::to_string(q.size(0)) + ", " + std::to_string(q.size(1)) + " and " + std::to_string(k.size(1)));
 }
 
-T2 packed_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& plan, const Tensor& plan_host) {
+// (o, lse, for a backward what rounding o left, in bytes of o's shape).
+T3 packed_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& plan, const Tensor& plan_host, bool backward) {
     const Plan p(plan, plan_host);
     check_packed(q_, k_, v_, p);
     const c10::DeviceGuard guard(q_.device());
@@ -869,39 +870,42 @@ T2 packed_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor
     const S2 sq = packed_readable({&q}), sk = packed_readable({&k, &v});
     const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
     Tensor o = empty_of(q, q.sizes()), lse = empty_f32(q, {H, T});
-    if (T == 0) return {o, lse};
+    Tensor rest = at::empty(backward ? q.sizes() : at::IntArrayRef({0}), q.options().dtype(at::kChar));
+    if (T == 0) return {o, lse, rest};
     const S2 s[3] = {sq, sk, dense_packed(o)};
-    fa_done(nn_fa_packed_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(), p.at_host(), p.at_device(), D, s[0].data(),
-                             code(q), scale_of(D), stream_of(q)));
-    return {o, lse};
+    fa_done(nn_fa_packed_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(), backward ? rest.data_ptr() : nullptr,
+                             p.at_host(), p.at_device(), D, s[0].data(), code(q), scale_of(D), stream_of(q)));
+    return {o, lse, rest};
 }
 
-T3 packed_bwd(const Tensor& d_o_, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& o_, const Tensor& lse_, const Tensor& plan,
-              const Tensor& plan_host) {
+T3 packed_bwd(const Tensor& d_o_, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& o_, const Tensor& lse_, const Tensor& rest_,
+              const Tensor& plan, const Tensor& plan_host) {
     const Plan p(plan, plan_host);
     check_packed(q_, k_, v_, p);
-    check_on_device(q_, {&d_o_, &o_, &lse_});
+    check_on_device(q_, {&d_o_, &o_, &lse_, &rest_});
     const int64_t T = q_.size(0), H = q_.size(1), D = q_.size(2);
     need(d_o_.sizes() == q_.sizes() && d_o_.scalar_type() == q_.scalar_type() && o_.sizes() == q_.sizes() && o_.scalar_type() == q_.scalar_type(),
          "d_o and o must be of q's shape and type");
     need(lse_.sizes() == at::IntArrayRef({H, T}) && lse_.scalar_type() == at::kFloat, "lse must be a float32 tensor of shape (H, tokens)");
+    const bool has = rest_.numel() > 0;
+    need(rest_.scalar_type() == at::kChar && (!has || rest_.sizes() == q_.sizes()), "rest must be int8 of o's shape, or empty");
     const c10::DeviceGuard guard(q_.device());
     Tensor q = q_, d_o = d_o_, k = k_, v = v_;
     const S2 sq = packed_readable({&q, &d_o}), sk = packed_readable({&k, &v});
-    const Tensor o = dense(o_), lse = contig(lse_);
+    const Tensor o = dense(o_), lse = contig(lse_), rest = dense(rest_);
     Tensor dq = empty_of(q, q.sizes()), dk = empty_of(k, k.sizes()), dv = empty_of(v, v.sizes());
     if (T == 0) return {dq, dk, dv};
     const size_t n = nn_fa_packed_bwd_workspace_size(p.at_host(), D);
     Tensor ws = bytes(q, n);
     const S2 s[5] = {sq, sk, dense_packed(o), dense_packed(dq), dense_packed(dk)};
-    fa_done(nn_fa_packed_bwd(d_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
-                             dv.data_ptr(), ws.data_ptr(), n, p.at_host(), p.at_device(), D, s[0].data(), code(q), scale_of(D), stream_of(q)));
+    fa_done(nn_fa_packed_bwd(d_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(), has ? rest.data_ptr() : nullptr,
+                             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n, p.at_host(), p.at_device(), D, s[0].data(), code(q), scale_of(D), stream_of(q)));
     return {dq, dk, dv};
 }
-T3 packed_bwd_op(const Tensor& d_o, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& plan,
-                 const Tensor& plan_host) {
+T3 packed_bwd_op(const Tensor& d_o, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& rest,
+                 const Tensor& plan, const Tensor& plan_host) {
     refuse_capture_from_engine("flash_attn_packed backward op");
-    return packed_bwd(d_o, q, k, v, o, lse, plan, plan_host);
+    return packed_bwd(d_o, q, k, v, o, lse, rest, plan, plan_host);
 }
 
 // ---- norm and rotation of queries and keys ------------------------------------------------------
@@ -1089,14 +1093,14 @@ Tensor distill_call(const Tensor& logits, const Tensor& values, const Tensor& in
 
 struct PackedNode : torch::autograd::Function<PackedNode> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& plan, const Tensor& plan_host) {
-        Tensor q = q_, k = k_, v = v_, o, lse;
+        Tensor q = q_, k = k_, v = v_, o, lse, rest;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
             if (k.dim() == 3 && k.sizes() == v.sizes()) packed_readable({&k, &v});  // copies that the backward would make again
-            std::tie(o, lse) = packed_fwd(q, k, v, plan, plan_host);
+            std::tie(o, lse, rest) = packed_fwd(q, k, v, plan, plan_host, true);
         }
         ctx->set_materialize_grads(false);
-        ctx->save_for_backward({q, k, v, o, lse, plan, plan_host});
+        ctx->save_for_backward({q, k, v, o, lse, rest, plan, plan_host});
         return o;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -1107,14 +1111,14 @@ struct PackedNode : torch::autograd::Function<PackedNode> {
         const Tensor d_o = readable_grad(grads[0]);
         {
             const at::AutoDispatchBelowADInplaceOrView below;
-            std::tie(out[0], out[1], out[2]) = packed_bwd(d_o, t[0], t[1], t[2], t[3], t[4], t[5], t[6]);
+            std::tie(out[0], out[1], out[2]) = packed_bwd(d_o, t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7]);
         }
         for (int i = 0; i < 3; ++i) out[i] = once(out[i], "flash_attn_packed");
         return out;
     }
 };
 Tensor packed_call(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& plan, const Tensor& plan_host) {
-    if (!records(q) && !records(k) && !records(v)) return std::get<0>(packed_fwd(q, k, v, plan, plan_host));
+    if (!records(q) && !records(k) && !records(v)) return std::get<0>(packed_fwd(q, k, v, plan, plan_host, false));
     refuse_capture("flash_attn_packed");
     return PackedNode::apply(q, k, v, plan, plan_host);
 }

@@ -81,10 +81,10 @@ SIGNATURES: dict[str, tuple] = {
     "nn_fa_packed_plan_words": (_sz, [_i64p, _i64, _i64, _i64]),
     "nn_fa_packed_plan": (_int, [_i64p, _i64, _i64, _i64, _vp, _sz]),
     "nn_fa_packed_plan_info": (_int, [_vp, _i64p]),
-    "nn_fa_packed_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64p, _int, _f32, _vp]),
+    "nn_fa_packed_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64p, _int, _f32, _vp]),
     "nn_fa_packed_bwd_workspace_size": (_sz, [_vp, _i64]),
     "nn_fa_packed_bwd": (
-        _int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _i64, _i64p, _int, _f32, _vp]
+        _int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _i64, _i64p, _int, _f32, _vp]
     ),
     # include/nanonemo_rope.h
     "nn_rope_qk": (

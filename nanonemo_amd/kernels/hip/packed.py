@@ -9,7 +9,8 @@ token attends to its own sequence up to itself. The reference's model has batche
 
 A ``Packing`` holds how the kernels share the work out, on the host and on the device: tiles and units of the longest
 sequences first, long ones split where they would outlast the others. The kernels are the dense attention's, so a sequence's
-output and dq are the same bits as flash_attn's on it alone, and everything is deterministic.
+output is the same bits as flash_attn's on it alone, and everything is deterministic. The gradients are nearer to the formula's
+than the dense ones: the forward keeps what rounding its output to 16 bits took off, one byte a value, for rowsum(dO * o).
 
 fp16 or bf16, head_dim 32 or 64, sequences of 0 to 2^30 / (H hd) tokens. Once differentiable, in reverse mode (a tangent is
 refused); capturing a call that autograd records into a HIP graph is refused, as the dense attention's is; without autograd it
@@ -18,11 +19,13 @@ captures, with the packing that it was given.
 
 from __future__ import annotations
 
+import operator
+
 import torch
 from torch import Tensor
 from torch.autograd import forward_ad
 
-from nanonemo_amd.kernels.hip import eager, host, preload, refuse_capture, refuse_forward_ad
+from nanonemo_amd.kernels.hip import eager, host, preload, records, refuse_capture, refuse_forward_ad
 
 _POSITIONS = 15  # the word of a plan that says where the positions begin (NN_FA_PACKED_POSITIONS)
 
@@ -36,7 +39,7 @@ class Packing:
     """
 
     def __init__(self, lengths, heads: int, kv_heads: int, device: torch.device | str = "cuda"):
-        self.lengths = tuple(int(n) for n in (lengths.tolist() if isinstance(lengths, Tensor) else lengths))
+        self.lengths = tuple(operator.index(n) for n in (lengths.tolist() if isinstance(lengths, Tensor) else lengths))
         self.tokens, self.longest = sum(self.lengths), max(self.lengths, default=0)
         self.heads, self.kv_heads = heads, kv_heads
         self.plan_host = host().packed_plan(self.lengths, heads, kv_heads)
@@ -56,40 +59,44 @@ class Packing:
 
 
 @torch.library.custom_op("nanonemo::flash_attn_packed", mutates_args=())
-def _flash_attn_packed(q: Tensor, k: Tensor, v: Tensor, plan: Tensor, plan_host: Tensor) -> tuple[Tensor, Tensor]:
-    return host().packed_fwd(q, k, v, plan, plan_host)
+def _flash_attn_packed(q: Tensor, k: Tensor, v: Tensor, plan: Tensor, plan_host: Tensor, backward: bool) -> tuple[Tensor, Tensor, Tensor]:
+    return host().packed_fwd(q, k, v, plan, plan_host, backward)
 
 
 @_flash_attn_packed.register_fake
-def _(q, k, v, plan, plan_host):
+def _(q, k, v, plan, plan_host, backward):
     T, H, _ = q.shape
-    return torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty((H, T), dtype=torch.float32, device=q.device)
+    return (
+        torch.empty(q.shape, dtype=q.dtype, device=q.device),
+        torch.empty((H, T), dtype=torch.float32, device=q.device),
+        torch.empty(q.shape if backward else 0, dtype=torch.int8, device=q.device),
+    )
 
 
 @torch.library.custom_op("nanonemo::flash_attn_packed_bwd", mutates_args=())
 def _flash_attn_packed_bwd(
-    d_o: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, plan: Tensor, plan_host: Tensor
+    d_o: Tensor, q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, rest: Tensor, plan: Tensor, plan_host: Tensor
 ) -> tuple[Tensor, Tensor, Tensor]:
-    return host().packed_bwd(d_o, q, k, v, o, lse, plan, plan_host)
+    return host().packed_bwd(d_o, q, k, v, o, lse, rest, plan, plan_host)
 
 
 @_flash_attn_packed_bwd.register_fake
-def _(d_o, q, k, v, o, lse, plan, plan_host):
+def _(d_o, q, k, v, o, lse, rest, plan, plan_host):
     return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
 
 
 def _setup_context(ctx, inputs, output):
     refuse_capture("flash_attn_packed (autograd)")
-    q, k, v, plan, plan_host = inputs
+    q, k, v, plan, plan_host, _ = inputs
     ctx.save_for_backward(q, k, v, *output, plan, plan_host)
     ctx.set_materialize_grads(False)  # lse's gradient is ignored
 
 
-def _backward(ctx, d_o, _d_lse):
+def _backward(ctx, d_o, _d_lse, _d_rest=None):
     refuse_capture("flash_attn_packed backward")
     if d_o is None:
-        return (None,) * 5
-    return *_flash_attn_packed_bwd(d_o, *ctx.saved_tensors), None, None
+        return (None,) * 6
+    return *_flash_attn_packed_bwd(d_o, *ctx.saved_tensors), None, None, None
 
 
 _flash_attn_packed.register_autograd(_backward, setup_context=_setup_context)
@@ -103,7 +110,7 @@ def flash_attn_packed(q: Tensor, k: Tensor, v: Tensor, packing: Packing) -> Tens
     if eager(q, k, v):  # the same launches as the op's, as one autograd node of the host module
         return host().packed(q, k, v, packing.plan, packing.plan_host)
     refuse_capture("flash_attn_packed", q, k, v)
-    return _flash_attn_packed(q, k, v, packing.plan, packing.plan_host)[0]
+    return _flash_attn_packed(q, k, v, packing.plan, packing.plan_host, records(q, k, v))[0]
 
 
 preload()

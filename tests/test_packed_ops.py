@@ -121,29 +121,29 @@ def test_c_abi_rejects_bad_arguments_before_any_launch():
     assert L.nn_fa_packed_plan(_c(lengths), 2, 4, 2, plan, words - 1) != 0 and b"words" in L.nn_fa_last_error()
     assert L.nn_fa_packed_plan(_c(lengths), 2, 4, 2, None, words) != 0
     assert L.nn_fa_packed_plan_words(None, 2, 4, 2) == 0 and L.nn_fa_packed_plan_words(_c(lengths), -1, 4, 2) == 0
-    assert L.nn_fa_packed_fwd(16, 16, 16, 16, 16, plan, 16, 64, None, 1, 0.125, None) != 0 and b"not a plan" in L.nn_fa_last_error()
+    assert L.nn_fa_packed_fwd(16, 16, 16, 16, 16, None, plan, 16, 64, None, 1, 0.125, None) != 0 and b"not a plan" in L.nn_fa_last_error()
     assert L.nn_fa_packed_plan(_c(lengths), 2, 4, 2, plan, words) == 0
 
-    def fwd(q=16, o=16, lse=16, p=plan, dp=16, D=64, strides=None, dt=1):
+    def fwd(q=16, o=16, lse=16, rest=None, p=plan, dp=16, D=64, strides=None, dt=1):
         s = None if strides is None else (ctypes.c_int64 * 6)(*strides)
-        return L.nn_fa_packed_fwd(q, 16, 16, o, lse, p, dp, D, s, dt, 0.125, None), L.nn_fa_last_error().decode()
+        return L.nn_fa_packed_fwd(q, 16, 16, o, lse, rest, p, dp, D, s, dt, 0.125, None), L.nn_fa_last_error().decode()
 
-    for kw, msg in ((dict(q=None), "null"), (dict(lse=None), "null"), (dict(q=8), "16-byte"), (dict(p=None), "null plan"), (dict(dp=None), "null plan"), (dict(dp=20), "16-byte"),
+    for kw, msg in ((dict(q=None), "null"), (dict(lse=None), "null"), (dict(q=8), "16-byte"), (dict(rest=4), "16-byte"), (dict(p=None), "null plan"), (dict(dp=None), "null plan"), (dict(dp=20), "16-byte"),
                     (dict(D=48), "head_dim"), (dict(dt=2), "float16 or bfloat16"), (dict(strides=[64, 256, 64, 100, 64, 256]), "multiples of 8"),
                     (dict(strides=[64, 32, 64, 128, 64, 256]), "smaller than head_dim"), (dict(strides=[64, 1 << 28, 64, 128, 64, 256]), "too large")):
         rc, got = fwd(**kw)
         assert rc != 0 and msg in got, (kw, got)
 
-    def bwd(ws=256, n=1 << 20, scale=0.125, q=16):
-        return L.nn_fa_packed_bwd(16, q, 16, 16, 16, 16, 16, 16, 16, ws, n, plan, 16, 64, None, 1, scale, None), L.nn_fa_last_error().decode()
+    def bwd(ws=256, n=1 << 20, scale=0.125, q=16, rest=None):
+        return L.nn_fa_packed_bwd(16, q, 16, 16, 16, 16, rest, 16, 16, 16, ws, n, plan, 16, 64, None, 1, scale, None), L.nn_fa_last_error().decode()
 
-    for kw, msg in ((dict(ws=None), "null workspace"), (dict(ws=128), "256-byte"), (dict(n=8), "too small"), (dict(scale=0.0), "positive"), (dict(q=None), "null"), (dict(q=8), "16-byte")):
+    for kw, msg in ((dict(ws=None), "null workspace"), (dict(ws=128), "256-byte"), (dict(n=8), "too small"), (dict(scale=0.0), "positive"), (dict(q=None), "null"), (dict(q=8), "16-byte"), (dict(rest=8), "16-byte")):
         rc, got = bwd(**kw)
         assert rc != 0 and msg in got, (kw, got)
     words = L.nn_fa_packed_plan_words(_c([0, 0]), 2, 4, 2)  # nothing to do
     empty = (ctypes.c_int32 * words)()
     assert L.nn_fa_packed_plan(_c([0, 0]), 2, 4, 2, empty, words) == 0
-    assert L.nn_fa_packed_fwd(None, None, None, None, None, empty, 16, 64, None, 1, 0.125, None) == 0
+    assert L.nn_fa_packed_fwd(None, None, None, None, None, None, empty, 16, 64, None, 1, 0.125, None) == 0
     assert L.nn_fa_packed_bwd_workspace_size(empty, 64) == 0
 
 
@@ -194,8 +194,8 @@ def test_packing():
     assert (p.lengths, p.tokens, p.longest, p.heads, p.kv_heads, p.device.type) == ((3, 0, 5), 8, 5, 4, 2, "cpu")
     assert p.positions.tolist() == [0, 1, 2, 0, 1, 2, 3, 4] and p.positions.dtype == torch.int32
     assert _packing(torch.tensor([2, 2]), 4, 2).positions.tolist() == [0, 1, 0, 1] and _packing([], 4, 2).tokens == 0
-    for lengths in ([3, -2], [3.5, "x"]):
-        with pytest.raises((RuntimeError, ValueError)):
+    for lengths in ([3, -2], [3.5], ["x"], torch.tensor([1.0])):
+        with pytest.raises((RuntimeError, TypeError)):
             _packing(lengths, 4, 2)
 
 
@@ -204,7 +204,7 @@ def test_schemas_and_fakes():
     from nanonemo_amd.kernels.hip.qk_norm import qk_norm_rope
 
     ops = torch.ops.nanonemo
-    assert str(ops.flash_attn_packed.default._schema) == "nanonemo::flash_attn_packed(Tensor q, Tensor k, Tensor v, Tensor plan, Tensor plan_host) -> (Tensor, Tensor)"
+    assert str(ops.flash_attn_packed.default._schema) == "nanonemo::flash_attn_packed(Tensor q, Tensor k, Tensor v, Tensor plan, Tensor plan_host, bool backward) -> (Tensor, Tensor, Tensor)"
     assert str(ops.qk_norm_rope.default._schema) == (
         "nanonemo::qk_norm_rope(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor)")
 
