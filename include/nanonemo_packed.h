@@ -42,7 +42,7 @@ typedef struct {
 } nn_fa_packed_info;
 int nn_fa_packed_plan_info(const int32_t* plan, nn_fa_packed_info* info);
 
-/* Forward. strides: element strides {head, row} of q, of k and v, and of o (6 values; positive multiples of 8, rows at
+/* Forward; lse may be null where no backward follows. strides: element strides {head, row} of q, of k and v, and of o (6 values; positive multiples of 8, rows at
  * least D apart), or null for dense tensors. */
 int nn_fa_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* rest, const int32_t* plan,
                      const int32_t* device_plan, int64_t D, const int64_t* strides, int dtype, float scale, void* stream);

@@ -589,7 +589,7 @@ __global__ __launch_bounds__(256, 2) void fa_fwd_kernel(const u16* __restrict__ 
                     *reinterpret_cast<u32x2*>(op + 32 * dt + 8 * g + 4 * hh) = w;
                 }
         }
-        if (hh == 0) LSE[vec_row<PACKED>(pk, bh, h, start, T) + qrow] = (mb + fast_log2(ltot)) * kLn2;
+        if (hh == 0 && (!PACKED || LSE)) LSE[vec_row<PACKED>(pk, bh, h, start, T) + qrow] = (mb + fast_log2(ltot)) * kLn2;
     }
     NN_TL_END(kTlFwd);
 }
@@ -1590,7 +1590,7 @@ __global__ __launch_bounds__(256, 4) void fa_short_fwd_kernel(const u16* __restr
     const float ltot = pair_sum(lsum);
     if (pk.rest && qrow < T) store_row<HD, DT>(oacc, 1.f / ltot, hh, nullptr, pk.rest + ((size_t)(e.start + qrow) * H + h) * (HD / 4));
     store_rows<HD, DT>(oacc, 1.f / ltot, vb, O + lo.at(0, h) + (size_t)(e.start + 32 * e.qb) * lo.st, lo.st, T - 32 * e.qb, lane);
-    if (hh == 0 && qrow < T) LSE[(size_t)h * pk.tokens + e.start + qrow] = (mb + fast_log2(ltot)) * kLn2;
+    if (LSE && hh == 0 && qrow < T) LSE[(size_t)h * pk.tokens + e.start + qrow] = (mb + fast_log2(ltot)) * kLn2;
 }
 
 // Waves 0 .. count KVH - 1: dk and dv of 32 keys; the next count H: dq of 32 rows. Either computes D for its rows itself.
@@ -2559,7 +2559,7 @@ NNFA_API int nn_fa_packed_fwd(const void* q, const void* k, const void* v, void*
     PlanHead p;
     if (int e = take_plan(plan, device_plan, D, dtype, &p)) return e;
     if (p.tokens == 0) return 0;
-    if (!q || !k || !v || !o || !lse) return fail(-1, "null pointer argument");
+    if (!q || !k || !v || !o) return fail(-1, "null pointer argument");
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(rest)) return fail(-1, "inputs must be 16-byte aligned");
     Lays l;
     if (int e = take_packed_lays(strides, p, D, false, &l)) return e;

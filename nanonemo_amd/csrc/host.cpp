@@ -861,21 +861,27 @@ void check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Plan&
               " KV heads, the tensors of " + std::to_string(q.size(0)) + ", " + std::to_string(q.size(1)) + " and " + std::to_string(k.size(1)));
 }
 
-// (o, lse, for a backward what rounding o left, in bytes of o's shape).
-T3 packed_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& plan, const Tensor& plan_host, bool backward) {
+// o; and where they are given, lse and, for a backward, what rounding o left, in bytes of o's shape.
+Tensor packed_into(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& plan, const Tensor& plan_host, Tensor* lse, Tensor* rest) {
     const Plan p(plan, plan_host);
     check_packed(q_, k_, v_, p);
     const c10::DeviceGuard guard(q_.device());
     Tensor q = q_, k = k_, v = v_;
     const S2 sq = packed_readable({&q}), sk = packed_readable({&k, &v});
     const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
-    Tensor o = empty_of(q, q.sizes()), lse = empty_f32(q, {H, T});
-    Tensor rest = at::empty(backward ? q.sizes() : at::IntArrayRef({0}), q.options().dtype(at::kChar));
-    if (T == 0) return {o, lse, rest};
+    Tensor o = empty_of(q, q.sizes());
+    if (lse) *lse = empty_f32(q, {H, T});
+    if (rest) *rest = at::empty(q.sizes(), q.options().dtype(at::kChar));
+    if (T == 0) return o;
     const S2 s[3] = {sq, sk, dense_packed(o)};
-    fa_done(nn_fa_packed_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(), backward ? rest.data_ptr() : nullptr,
-                             p.at_host(), p.at_device(), D, s[0].data(), code(q), scale_of(D), stream_of(q)));
-    return {o, lse, rest};
+    fa_done(nn_fa_packed_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse ? lse->data_ptr<float>() : nullptr,
+                             rest ? rest->data_ptr() : nullptr, p.at_host(), p.at_device(), D, s[0].data(), code(q), scale_of(D), stream_of(q)));
+    return o;
+}
+T3 packed_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& plan, const Tensor& plan_host, bool backward) {
+    Tensor lse, rest;
+    const Tensor o = packed_into(q, k, v, plan, plan_host, &lse, backward ? &rest : nullptr);
+    return {o, lse, backward ? rest : at::empty({0}, q.options().dtype(at::kChar))};
 }
 
 T3 packed_bwd(const Tensor& d_o_, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& o_, const Tensor& lse_, const Tensor& rest_,
@@ -1118,7 +1124,7 @@ struct PackedNode : torch::autograd::Function<PackedNode> {
     }
 };
 Tensor packed_call(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& plan, const Tensor& plan_host) {
-    if (!records(q) && !records(k) && !records(v)) return std::get<0>(packed_fwd(q, k, v, plan, plan_host, false));
+    if (!records(q) && !records(k) && !records(v)) return packed_into(q, k, v, plan, plan_host, nullptr, nullptr);
     refuse_capture("flash_attn_packed");
     return PackedNode::apply(q, k, v, plan, plan_host);
 }

@@ -42,13 +42,14 @@ class Packing:
         self.lengths = tuple(operator.index(n) for n in (lengths.tolist() if isinstance(lengths, Tensor) else lengths))
         self.tokens, self.longest = sum(self.lengths), max(self.lengths, default=0)
         self.heads, self.kv_heads = heads, kv_heads
-        self.plan_host = host().packed_plan(self.lengths, heads, kv_heads)
         device = torch.device(device)
         if device.type == "cuda" and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("Packing: made while a HIP graph is captured, whose replays would copy it again from memory that is gone; make it before")
-        # (from pinned memory, which its allocator keeps until the copy has run: the host does not wait)
-        self.plan = self.plan_host.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else self.plan_host
-        self.positions = self.plan[int(self.plan_host[_POSITIONS]) :]
+        with torch.inference_mode(False):  # (autograd saves the plan, which it does with no inference tensor)
+            self.plan_host = host().packed_plan(self.lengths, heads, kv_heads)
+            # (from pinned memory, which its allocator keeps until the copy has run: the host does not wait)
+            self.plan = self.plan_host.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else self.plan_host
+            self.positions = self.plan[int(self.plan_host[_POSITIONS]) :]
 
     @property
     def device(self) -> torch.device:

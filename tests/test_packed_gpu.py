@@ -411,3 +411,75 @@ def test_gradients_carry_two_roundings(dtype):
             ratio = ((x.double() - ref).norm() / one).item()
             print(f"[err] {name} {ratio:.3f} roundings", flush=True)
             assert ratio <= 1.5, (name, lengths[:3], ratio)
+
+
+def test_packings_of_inference_mode_and_two_streams_at_once():
+    lengths, H, KVH, D = [700, 30, 129], 12, 4, 64
+    with torch.inference_mode():
+        packing = _packing(lengths, H, KVH)
+        q, k, v, do = _inputs(lengths, H, KVH, D, torch.bfloat16, seed=14)
+        inferred = _call(q, k, v, packing)
+    ins = [t.clone() for t in (q, k, v, do)]
+    ref = _run(*ins, packing)
+    assert torch.equal(ref[0], inferred)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for _ in range(4):
+        for st in streams:  # the same packing on both, their workspaces their own
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                outs.append(_run(*ins, packing))
+    for st in streams:
+        torch.cuda.current_stream().wait_stream(st)
+    for got in outs:
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+def test_packed_model_compiles_without_graph_breaks():
+    from nanonemo_amd.model import ModelConfig, NanoNemo
+
+    torch.manual_seed(0)
+    model = NanoNemo(ModelConfig(**SMALL, attn_kernel="hip_bthd", rope_kernel="hip", norm_kernel="hip", qk_norm=True)).cuda()
+    lengths = [100, 28, 1, 127]
+    packing = model.pack(lengths)
+    idx, y = (torch.randint(0, 512, (1, 256), device="cuda") for _ in range(2))
+
+    def loss(m):
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            return m(idx, y, None, packing)[1]
+
+    got, want = loss(torch.compile(model, fullgraph=True, backend="aot_eager")), loss(model)
+    # the compiled modules round weight gradients and the loss's logits as autocast does: bf16 logits of about 0.3 in both
+    torch.testing.assert_close(got, want, rtol=2e-3, atol=0)
+    got.backward()
+    assert all(p.grad is not None and p.grad.isfinite().all() for p in model.parameters())
+
+
+def test_evaluation_of_a_packed_model_captured_into_a_graph():
+    from nanonemo_amd.model import ModelConfig, NanoNemo
+
+    print("\n[case] packed model in a graph", flush=True)
+    torch.manual_seed(0)
+    model = NanoNemo(ModelConfig(**SMALL, attn_kernel="hip_bthd", rope_kernel="hip", norm_kernel="hip", emb_kernel="hip", qk_norm=True)).cuda()
+    packing = model.pack([100, 28, 1, 127])
+    idx = torch.randint(0, 512, (1, 256), device="cuda")
+
+    def run():
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+            return model(idx, packing=packing)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for i in range(4):
+        idx.copy_(torch.randint(0, 512, idx.shape, device="cuda"))
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, run()), i

@@ -128,7 +128,7 @@ def test_c_abi_rejects_bad_arguments_before_any_launch():
         s = None if strides is None else (ctypes.c_int64 * 6)(*strides)
         return L.nn_fa_packed_fwd(q, 16, 16, o, lse, rest, p, dp, D, s, dt, 0.125, None), L.nn_fa_last_error().decode()
 
-    for kw, msg in ((dict(q=None), "null"), (dict(lse=None), "null"), (dict(q=8), "16-byte"), (dict(rest=4), "16-byte"), (dict(p=None), "null plan"), (dict(dp=None), "null plan"), (dict(dp=20), "16-byte"),
+    for kw, msg in ((dict(q=None), "null"), (dict(o=None), "null"), (dict(q=8), "16-byte"), (dict(rest=4), "16-byte"), (dict(p=None), "null plan"), (dict(dp=None), "null plan"), (dict(dp=20), "16-byte"),
                     (dict(D=48), "head_dim"), (dict(dt=2), "float16 or bfloat16"), (dict(strides=[64, 256, 64, 100, 64, 256]), "multiples of 8"),
                     (dict(strides=[64, 32, 64, 128, 64, 256]), "smaller than head_dim"), (dict(strides=[64, 1 << 28, 64, 128, 64, 256]), "too large")):
         rc, got = fwd(**kw)
