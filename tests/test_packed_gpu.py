@@ -14,7 +14,8 @@ pytestmark = pytest.mark.gpu
 
 # lengths, H, KVH, hd: tile and unit edges with empty sequences; an odd group; one long sequence among short ones, whose pairs
 # are split; few tokens, a block for each unit; many sequences, a wave for each pair; lengths of 1 and 2; long and split, MQA; short
-# sequences alone, and many of them beside a longer one.
+# sequences alone, and many of them beside a longer one; a wave for each pair again, of single units that leave waves over and of
+# pairs; a long one split at head_dim 32; long pairs that are not.
 CASES = [
     ([63, 0, 64, 65, 1, 127, 128, 129, 0, 191, 192, 193, 0], 12, 4, 64),
     ([63, 64, 65, 1, 127, 128, 129, 300], 6, 2, 32),
@@ -27,8 +28,16 @@ CASES = [
     ([1, 31, 32, 33, 63, 64, 0, 2, 50] * 3, 12, 4, 64),
     ([40, 7, 64, 32, 5], 5, 1, 32),
     ([20, 64, 33] * 40 + [500], 8, 2, 64),
+    ([100] * 343, 9, 3, 64),
+    ([190, 129] * 130, 4, 4, 32),
+    ([3000], 12, 1, 32),
+    ([2100, 300], 32, 32, 64),
 ]
 IDS = [f"{len(c[0])}x{max(c[0])}-{c[1]}-{c[2]}-{c[3]}" for c in CASES]
+
+
+# What each case is there for: short tiles, splits, waves per pair (0: no longer sequences).
+KINDS = [(0, 0, 4), (0, 0, 4), (0, 1, 4), (0, 0, 4), (1, 0, 4), (1, 0, None), (0, 1, 4), (0, 0, 4), (1, 0, None), (1, 0, None), (1, 0, 4), (0, 0, 1), (0, 0, 1), (0, 1, 4), (0, 0, 4)]
 
 
 def _packing(lengths, H, KVH):
@@ -41,6 +50,15 @@ def _call(*args):
     from nanonemo_amd.kernels.hip.packed import flash_attn_packed
 
     return flash_attn_packed(*args)
+
+
+def test_the_cases_are_of_every_kind():
+    for (lengths, H, KVH, _), (few, split, wpp) in zip(CASES, KINDS):
+        w = _packing(lengths, H, KVH).plan_host
+        assert (w[16] > 0, w[10] > 0) == (few, split) and (wpp is None or w[11] == wpp), (lengths[:3], H, KVH, w[:18])
+    single = [_packing(c[0], c[1], c[2]).plan_host for c in (CASES[3], CASES[14])]
+    paired = [bool(w[w[13] + 7]) for w in single]
+    assert paired == [False, True]
 
 
 def _inputs(lengths, H, KVH, D, dtype, seed=0, mult=1.0):
