@@ -195,8 +195,8 @@ __device__ inline float sub_rn(float a, float b) {
 // Sequences of different lengths behind one another in one [tokens][heads][D] tensor (include/nanonemo_packed.h). Each is a
 // problem of its own to the kernels below: what a block works on, and where its sequence lies, is one entry of a list that the
 // host laid out and sorted (nn_fa_packed_plan), the tensors' pointers move to the sequence's first row, T is its length, and
-// the loops, masks and sums are those of the dense kernels. So a sequence's outputs are the same bits as a dense call's on it
-// alone (its dk and dv too where the same blocks share the work).
+// the loops, masks and sums are those of the dense kernels. So a sequence's o and lse are the same bits as a dense call's on it
+// alone (without rests, below, its dq too, and dk and dv where the same blocks share the work).
 struct PackedTile {  // forward and dQ: 128 query rows of one sequence, for the query heads of one KV head
     int start, len, qb, kvh;  // len 0: nothing to do (the list is padded to a multiple of 8)
 };
@@ -299,8 +299,7 @@ __device__ inline float dot_rest(u16x8 g, u16x8 o, u32x2 r, float acc) {
     return acc;
 }
 constexpr int kPairRows = 128;  // rows of a partial sum of packed dK/dV: the pair's two units
-// A forward or dQ block's batch, head and query block; packed: its sequence's start and length, and bh * T as the place of the
-// sequence's row 0 in the per-head fp32 vectors. Entry i of the packed list is for XCD i % 8 (block i goes to XCD i % 8), where
+// A forward or dQ block's batch, head and query block; packed: also its sequence's start and length. Entry i of the packed list is for XCD i % 8 (block i goes to XCD i % 8), where
 // the heads of its group follow one another and share its K and V tiles in that XCD's L2.
 struct Place {
     int bh, qb, b, h, kvh, start, T;
@@ -1461,13 +1460,19 @@ __global__ __launch_bounds__(256, 2) void fa_bwd_dq_kernel(const u16* __restrict
 // ------------------------------------------------------------------------------------------
 // Packed sequences of up to kShort tokens: one wave for each 32 query rows of a head (forward, dQ), one for each 32 keys of a KV
 // head (dK/dV). A block of the kernels above carries 128 rows and its barriers for them: 7872 blocks of 24 tokens on average
-// took 44 us, mostly latency, where these waves, independent of each other and more of them to a CU, take 17 (and the backward 50 instead of 89). The
-// arithmetic of a row is that of the kernels above in the same order, so its bits are too (dk and dv: sums over the group's
-// heads in one wave instead of four).
+// took 44 us, mostly latency, where these waves, independent of each other and more of them to a CU, take 17 (5.2 TB/s; the
+// backward 54 instead of 89, of which the rests are 4). The arithmetic of a row is that of the kernels above in the same order,
+// so its bits are too (dk and dv: sums over the group's heads in one wave instead of four).
 // Operands that need rows come straight from memory in their lanes' layout, those that need columns through the wave's own LDS
 // tile by DMA, whose rows past the sequence read as zeros. List entries: PackedTile with qb = the 32-row tile.
 // ------------------------------------------------------------------------------------------
 constexpr int kShort = 64;
+
+// This wave's copies have landed: nothing that reads them moves before it.
+__device__ inline void copies_landed() {
+    wait_vmem();
+    __asm__ volatile("" ::: "memory");
+}
 
 // A wave's 32 x HD result, held transposed (lane: row l32; element i of acc[dt]: column 32 dt + (i / 4) * 8 + 4 hh + i % 4),
 // times mul and rounded, to rows [0, left) of p: through the wave's own LDS tile, so that a store instruction writes whole rows.
@@ -1578,7 +1583,7 @@ __global__ __launch_bounds__(256, 4) void fa_short_fwd_kernel(const u16* __restr
             if (__builtin_amdgcn_ballot_w64(psum > kPsumMax)) rescale();
         }
         lsum += psum;
-        if (t == 0) wait_vmem();  // the V rows
+        if (t == 0) copies_landed();  // the V rows
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -1660,7 +1665,7 @@ __global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restr
         float* vec = vecS + wave * 64;
         fetch(0);
         for (int it = 0; it < n; ++it) {
-            wait_vmem();
+            copies_landed();
             const u16* qt = lds + (it & 1) * 2 * TILE;
             const u16* ot = qt + TILE;
             u16x8 qa[NS], oa[NS];
@@ -1739,7 +1744,7 @@ __global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restr
             for (int i = 0; i < 16; ++i) s[i] = 32 * t + (i >> 2) * 8 + (i & 3) > lim ? -INFINITY : s[i];
 #pragma unroll
             for (int i = 0; i < 16; ++i) dp[i] = fast_exp2(fmaf(s[i], sl2, nl2)) * dp[i];
-            if (t == 0) wait_vmem();  // the K rows
+            if (t == 0) copies_landed();  // the K rows
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const u16x8 sf = pack8<DT>(dp, 8 * half);
@@ -2389,7 +2394,7 @@ int plan_size(const int64_t* lengths, int64_t n, int64_t H, int64_t KVH, PlanSiz
             if (ns > 1) z.nsums += KVH, z.nslots += ns * KVH;
         }
     }
-    if (z.words() >= (int64_t)1 << 31) return fail(-1, "sizes too large");
+    if (z.nunits >= (int64_t)1 << 24 || z.words() >= (int64_t)1 << 31) return fail(-1, "sizes too large");
     *out = z;
     return 0;
 }

@@ -501,3 +501,24 @@ def test_evaluation_of_a_packed_model_captured_into_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, run()), i
+
+
+def test_offsets_past_32_bits():
+    """The last sequence of 2.9 million tokens, whose values lie past the 2^31st of q, o and the gradients."""
+    print("\n[case] 2.9 million packed tokens", flush=True)
+    H, KVH, D = 12, 4, 64
+    lengths = [1024] * 2800 + [20] * 30 + [300, 33]  # (many short ones, and a longer one behind them)
+    T = sum(lengths)
+    assert (T - 333) * H * D > 2**31
+    last = 333
+    tail = _inputs([300, 33], H, KVH, D, torch.bfloat16, seed=15)
+    q, k, v, do = (torch.zeros(T, n, D, dtype=torch.bfloat16, device="cuda") for n in (H, KVH, KVH, H))
+    for t, x in zip((q, k, v, do), tail):
+        t[-last:] = x
+    got = _run(q, k, v, do, _packing(lengths, H, KVH))
+    small = _packing([300, 33], H, KVH)
+    for name, x, y in zip(("o", "dq", "dk", "dv"), got, _run(*tail, small)):
+        assert not x[:-last].any(), name
+        # (which blocks share a sum goes by the batch: fp32 sums in another order, rounded to bf16)
+        torch.testing.assert_close(x[-last:].float(), y.float(), rtol=2**-7, atol=1e-5 * y.float().abs().max().item(), msg=name)
+    assert torch.equal(got[0][-last:], _call(*tail[:3], small))

@@ -270,3 +270,26 @@ def test_on_another_stream_and_captured_into_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, both())), i
+
+
+def test_offsets_past_32_bits():
+    print("\n[case] qk_norm of 2.9 million tokens", flush=True)
+    T, H, KVH, D = 2_900_000, 12, 4, 64
+    tail = _inputs((100,), H, KVH, D, torch.bfloat16, seed=9)
+    wq, wk = tail[2:4]
+    cos, sin = _tables(100, D)
+    q, k, dq, dk = (torch.zeros(T, n, D, dtype=torch.bfloat16, device="cuda") for n in (H, KVH, H, KVH))
+    assert (T - 100) * H * D > 2**31
+    for t, x in zip((q, k, dq, dk), (tail[0], tail[1], tail[4], tail[5])):
+        t[-100:] = x
+    pos = torch.zeros(T, dtype=torch.int32, device="cuda")
+    pos[-100:] = torch.arange(100, device="cuda")
+    outs = []
+    for ins, p, g in (((q, k), pos, (dq, dk)), (tail[:2], pos[-100:], tail[4:])):
+        leaves = [t.detach().requires_grad_() for t in (*ins, wq, wk)]
+        y = _call(*leaves, cos, sin, p)
+        outs.append([t.detach()[-100:] for t in y] + [t[-100:] if t.dim() > 1 else t for t in torch.autograd.grad(y, leaves, g)])
+    for a, b in zip(outs[0][:4], outs[1][:4]):
+        assert torch.equal(a, b)
+    for a, b in zip(outs[0][4:], outs[1][4:]):  # zeros add nothing; the fp32 sums' order goes by the size: 400 or 1200 terms
+        torch.testing.assert_close(a, b, rtol=0, atol=1200 * 2**-24 * 4 * b.abs().max().item())
