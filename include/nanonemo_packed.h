@@ -16,7 +16,7 @@
  * The work is laid out once for a batch, on the host: nn_fa_packed_plan fills `plan` (int32 words, in host memory), which the
  * caller copies to the device as it is (16-byte aligned) and keeps while it uses it, in both places. Its layout is the
  * library's own, but for the last `tokens` words, from word plan[NN_FA_PACKED_POSITIONS] on, which hold every row's position
- * in its sequence. A call given a device copy that differs from the host's may read and write out of bounds.
+ * in its sequence. A call whose device copy differs from the host's computes other values, within the tensors' bounds.
  */
 #ifndef NANONEMO_PACKED_H
 #define NANONEMO_PACKED_H
@@ -42,8 +42,8 @@ typedef struct {
 } nn_fa_packed_info;
 int nn_fa_packed_plan_info(const int32_t* plan, nn_fa_packed_info* info);
 
-/* Forward; lse may be null where no backward follows. strides: element strides {head, row} of q, of k and v, and of o (6 values; positive multiples of 8, rows at
- * least D apart), or null for dense tensors. */
+/* Forward; lse may be null where no backward follows. strides: element strides {head, row} of q, of k and v, and of o (6 values;
+ * positive multiples of 8, rows at least D apart), or null for dense tensors. */
 int nn_fa_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* rest, const int32_t* plan,
                      const int32_t* device_plan, int64_t D, const int64_t* strides, int dtype, float scale, void* stream);
 

@@ -212,9 +212,22 @@ struct PackedArg<true> {
     const void* list;  // PackedTile or PackedUnit
     int count;         // entries
     int tokens;        // of all sequences: the stride of the per-head vectors lse, -lse/scale and -D
+    int longest;       // sequence
+    int slots;         // partial sums
     uint32_t* rest;    // [tokens][H][HD] bytes: what rounding o to 16 bits took off (below), or null
 };
 using Packed = PackedArg<true>;
+constexpr int64_t kDkdvMaxSplit = 16;  // blocks that share a pair of units
+// The list lies in memory that a program can free or overwrite while a captured graph or another stream still reads it. A kernel
+// touches nothing for an entry that names no place in the tensors, so that such a mistake costs values and not the GPU.
+__device__ inline bool inside(const Packed& pk, int start, int len, int kvh, int KVH, int tile, int size) {
+    return (unsigned)len <= (unsigned)pk.longest && (unsigned)start <= (unsigned)(pk.tokens - len) && (unsigned)kvh < (unsigned)KVH &&
+           (unsigned)tile < (unsigned)((len + size - 1) / size);
+}
+__device__ inline bool inside(const Packed& pk, const PackedUnit& u, int KVH) {
+    return inside(pk, u.start, u.len, u.kvh, KVH, u.pj, 64) && (unsigned)u.sidx < (unsigned)u.nsplit && (unsigned)u.nsplit <= (unsigned)kDkdvMaxSplit &&
+           (u.nsplit == 1 || ((unsigned)u.slot < (unsigned)pk.slots));
+}
 // D = rowsum(dO * O) enters every dS, and an O of 16 bits puts an error of its own into it: with dS rounded to 16 bits before its
 // products, which the matrix unit asks for, and the gradients rounded once more, dq and dk come out 1.5 to 1.6 times as far from
 // the formula's as a single rounding; without O's share 1.4 (by arithmetic sqrt(2)). So a forward whose backward will be run
@@ -299,8 +312,9 @@ __device__ inline float dot_rest(u16x8 g, u16x8 o, u32x2 r, float acc) {
     return acc;
 }
 constexpr int kPairRows = 128;  // rows of a partial sum of packed dK/dV: the pair's two units
-// A forward or dQ block's batch, head and query block; packed: also its sequence's start and length. Entry i of the packed list is for XCD i % 8 (block i goes to XCD i % 8), where
-// the heads of its group follow one another and share its K and V tiles in that XCD's L2.
+// A forward or dQ block's batch, head and query block; packed: also its sequence's start and length. Entry i of the packed list
+// is for XCD i % 8 (block i goes to XCD i % 8), where the heads of its group follow one another and share its K and V tiles in
+// that XCD's L2.
 struct Place {
     int bh, qb, b, h, kvh, start, T;
 };
@@ -317,7 +331,7 @@ __device__ inline Place place(const PackedArg<PACKED>& pk, int BH, int H, int KV
     if constexpr (PACKED) {
         const int group = H / KVH, slot = (int)blockIdx.x >> 3, at = slot / group;
         const PackedTile e = static_cast<const PackedTile*>(pk.list)[at * 8 + ((int)blockIdx.x & 7)];
-        return {0, e.qb, 0, e.kvh * group + (slot - at * group), e.kvh, e.start, e.len};
+        return {0, e.qb, 0, e.kvh * group + (slot - at * group), e.kvh, e.start, inside(pk, e.start, e.len, e.kvh, KVH, e.qb, 128) ? e.len : 0};
     } else {
         const QBlk blk = qblock_of(blockIdx.x, BH, H / KVH, nqb);
         const int b = blk.bh / H, h = blk.bh - b * H;
@@ -694,7 +708,8 @@ __global__ __launch_bounds__(256, 1) void fa_bwd_dkdv_kernel(
     if constexpr (PACKED) {  // this wave's entry of the list (with every wave on one pair the block's)
         const int at = (int)blockIdx.x * PPB + (WPP == NW ? 0 : wave / WPP);
         active = at < pk.count;
-        const PackedUnit u = static_cast<const PackedUnit*>(pk.list)[min(at, pk.count - 1)];
+        PackedUnit u = static_cast<const PackedUnit*>(pk.list)[min(at, pk.count - 1)];
+        if (!inside(pk, u, KVH)) active = false, u = PackedUnit{0, 1, 0, 0, 1, 0, 0, 0};
         T = u.len, pj = u.pj, kvh = u.kvh, nsplit = u.nsplit, sidx = u.sidx, slot0 = u.slot, paired = u.paired;
         nkb = nqt = (T + 63) / 64, vecT = pk.tokens;
         Q += (size_t)u.start * lq.st, dO += (size_t)u.start * lq.st;
@@ -1192,9 +1207,10 @@ __global__ __launch_bounds__(256) void fa_bwd_dkdv_sum_kernel(const float* __res
 constexpr int kSumBlocks = 8;
 template <int HD, int DT>
 __global__ __launch_bounds__(256) void fa_packed_sum_kernel(const float* __restrict__ part, u16* __restrict__ dK, u16* __restrict__ dV,
-                                                            const PackedUnit* __restrict__ list, Lay ldk) {
+                                                            Packed pk, int KVH, Lay ldk) {
     using E = Elem<DT>;
-    const PackedUnit u = list[blockIdx.x];
+    const PackedUnit u = static_cast<const PackedUnit*>(pk.list)[blockIdx.x];
+    if (!inside(pk, u, KVH) || (unsigned)u.slot >= (unsigned)pk.slots || u.nsplit > pk.slots - u.slot) return;
     const int nkb = (u.len + 63) / 64;
     constexpr int kOne = kPairRows * HD;  // values of one gradient's partial sum
     const float* from = part + (size_t)u.slot * 2 * kOne;
@@ -1511,6 +1527,7 @@ __global__ __launch_bounds__(256, 4) void fa_short_fwd_kernel(const u16* __restr
     if (at >= pk.count) return;
     const int h = item - at * H, kvh = h / (H / KVH);
     const PackedTile e = static_cast<const PackedTile*>(pk.list)[at];
+    if (e.len > kShort || !inside(pk, e.start, e.len, 0, KVH, e.qb, 32)) return;
     const int T = e.len, nt = e.qb + 1, qrow = 32 * e.qb + l32;  // nt: 32-key sub-tiles with a visible key
     u16* vb = vS + wave * 2 * TILE;
     const u16* Vp = V + lk.at(0, kvh) + (size_t)e.start * lk.st;
@@ -1616,6 +1633,7 @@ __global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restr
     const int per = keys ? KVH : H, at = item / per;
     if (at >= pk.count) return;
     const PackedTile e = static_cast<const PackedTile*>(pk.list)[at];
+    if (e.len > kShort || !inside(pk, e.start, e.len, 0, KVH, e.qb, 32)) return;
     const int T = e.len, tile = e.qb;
     u16* lds = tS + wave * 4 * TILE;
     int roff[NS], coff[ND][2];
@@ -1808,7 +1826,7 @@ size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 // block's work is shared by up to 16 blocks whose fp32 partials are summed afterwards, as long as
 // every split keeps at least 8 of the pair's (query head, query tile) iterations (two per wave: a
 // block's fixed cost is about that much work).
-constexpr int64_t kDkdvFill = 256, kDkdvMaxSplit = 16, kDkdvMinIters = 8;
+constexpr int64_t kDkdvFill = 256, kDkdvMinIters = 8;
 int dkdv_split(int64_t B, int64_t H, int64_t KVH, int64_t T) {
     if (B <= 0 || KVH <= 0 || H < KVH || T <= 0) return 1;
     const int64_t nkb = (T + 63) / 64, base = B * KVH * ((nkb + 1) / 2);
@@ -2374,7 +2392,8 @@ int plan_size(const int64_t* lengths, int64_t n, int64_t H, int64_t KVH, PlanSiz
     }
     // (blocks of 256 threads, fewer than 2^32 threads to a launch; 32-bit words and split bounds)
     const int64_t most = g * ((z.longest + 63) / 64 + 1);
-    if (z.padded() * g >= (int64_t)1 << 24 || z.nshort * (H + KVH) >= (int64_t)1 << 24 || units * kDkdvMaxSplit >= (int64_t)1 << 28 || most * kDkdvMaxSplit >= (int64_t)1 << 31)
+    if (z.padded() * g >= (int64_t)1 << 24 || z.nshort * (H + KVH) >= (int64_t)1 << 24 || units * kDkdvMaxSplit >= (int64_t)1 << 28 ||
+        most * kDkdvMaxSplit >= (int64_t)1 << 31)
         return fail(-1, "sizes too large");
     // The dense kernels' choices (dkdv_waves_per_pair, dkdv_mode), for work that differs from pair to pair. A wave of its own for
     // each pair where there are enough of them and the longest does not outlast a wave's even share of all (65536 tokens in
@@ -2448,13 +2467,13 @@ int packed_fwd_impl(const void* q, const void* k, const void* v, void* o, float*
     const int g = p.H / p.KVH;
     if (p.nshort) {
         fa_short_fwd_kernel<HD, DT><<<dim3((unsigned)(((int64_t)p.nshort * p.H + 3) / 4)), dim3(256), 0, st>>>(
-            (const u16*)q, (const u16*)k, (const u16*)v, (u16*)o, lse, Packed{dp + p.shorts, p.nshort, p.tokens, rest}, p.H, p.KVH, scale * kLog2e, l.q, l.k, l.o);
+            (const u16*)q, (const u16*)k, (const u16*)v, (u16*)o, lse, Packed{dp + p.shorts, p.nshort, p.tokens, p.longest, p.nslots, rest}, p.H, p.KVH, scale * kLog2e, l.q, l.k, l.o);
         if (int e = launch_status("fa_short_fwd_kernel")) return e;
     }
     if (p.ntiles == 0) return 0;
     fa_fwd_kernel<HD, DT, false, true><<<dim3((unsigned)(p.ntiles * g)), dim3(256), 0, st>>>(
         (const u16*)q, (const u16*)k, (const u16*)v, (u16*)o, lse, p.H, p.H, p.KVH, 0, 0, scale * kLog2e, l.q, l.k, l.o, RopeArgs{},
-        Packed{dp + p.tiles, p.ntiles, p.tokens, rest});
+        Packed{dp + p.tiles, p.ntiles, p.tokens, p.longest, p.nslots, rest});
     return launch_status("fa_fwd_kernel (packed)");
 }
 
@@ -2465,18 +2484,18 @@ int packed_bwd_impl(const void* dO, const void* q, const void* k, const void* v,
     if (p.nshort) {
         fa_short_bwd_kernel<HD, DT><<<dim3((unsigned)(((int64_t)p.nshort * (p.H + p.KVH) + 3) / 4)), dim3(256), 0, st>>>(
             (const u16*)q, (const u16*)k, (const u16*)v, (const u16*)o, (const u16*)dO, lse, (u16*)dq, (u16*)dk, (u16*)dv,
-            Packed{dp + p.shorts, p.nshort, p.tokens, rest}, p.H, p.KVH, scale * kLog2e, scale, l.q, l.k, l.o, l.dq, l.dk);
+            Packed{dp + p.shorts, p.nshort, p.tokens, p.longest, p.nslots, rest}, p.H, p.KVH, scale * kLog2e, scale, l.q, l.k, l.o, l.dq, l.dk);
         if (int e = launch_status("fa_short_bwd_kernel")) return e;
     }
     if (p.ntiles == 0) return 0;
     fa_bwd_dq_kernel<HD, DT, false, true><<<dim3((unsigned)(p.ntiles * g)), dim3(256), 0, st>>>(
         (const u16*)q, (const u16*)k, (const u16*)v, (const u16*)o, (const u16*)dO, lse, w.nL, w.nD, (u16*)dq, p.H, p.H, p.KVH, 0, 0, scale * kLog2e,
-        scale, l.q, l.k, l.o, l.dq, RopeArgs{}, Packed{dp + p.tiles, p.ntiles, p.tokens, rest});
+        scale, l.q, l.k, l.o, l.dq, RopeArgs{}, Packed{dp + p.tiles, p.ntiles, p.tokens, p.longest, p.nslots, rest});
     if (int e = launch_status("fa_bwd_dq_kernel (packed)")) return e;
     auto launch = [&](auto kern, int per) {
         kern<<<dim3((unsigned)((p.nunits + per - 1) / per)), dim3(256), 0, st>>>(
             (const u16*)q, (const u16*)k, (const u16*)v, (const u16*)dO, w.nL, w.nD, (u16*)dk, (u16*)dv, p.KVH, p.H, p.KVH, 0, 0, 0, scale * kLog2e,
-            scale, l.q, l.k, l.dk, 1, w.part, 1, Packed{dp + p.units, p.nunits, p.tokens, nullptr});
+            scale, l.q, l.k, l.dk, 1, w.part, 1, Packed{dp + p.units, p.nunits, p.tokens, p.longest, p.nslots, nullptr});
     };
     if (p.wpp == 1)
         launch(fa_bwd_dkdv_kernel<HD, DT, 1, false, true>, 4);
@@ -2486,7 +2505,8 @@ int packed_bwd_impl(const void* dO, const void* q, const void* k, const void* v,
         launch(fa_bwd_dkdv_kernel<HD, DT, 4, false, true>, 1);
     if (int e = launch_status("fa_bwd_dkdv_kernel (packed)")) return e;
     if (p.nsums == 0) return 0;
-    fa_packed_sum_kernel<HD, DT><<<dim3((unsigned)p.nsums, kSumBlocks), dim3(256), 0, st>>>(w.part, (u16*)dk, (u16*)dv, (const PackedUnit*)(dp + p.sums), l.dk);
+    fa_packed_sum_kernel<HD, DT><<<dim3((unsigned)p.nsums, kSumBlocks), dim3(256), 0, st>>>(
+        w.part, (u16*)dk, (u16*)dv, Packed{dp + p.sums, p.nsums, p.tokens, p.longest, p.nslots, nullptr}, p.KVH, l.dk);
     return launch_status("fa_packed_sum_kernel");
 }
 

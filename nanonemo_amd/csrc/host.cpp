@@ -809,7 +809,7 @@ struct Plan {
     const Tensor &host, &device;
     nn_fa_packed_info info;
     Plan(const Tensor& device_, const Tensor& host_) : host(host_), device(device_) {
-        need(host.device().is_cpu() && host.scalar_type() == at::kInt && host.dim() == 1 && host.is_contiguous() && host.numel() >= 16 &&
+        need(host.device().is_cpu() && host.scalar_type() == at::kInt && host.dim() == 1 && host.is_contiguous() && host.numel() >= 32 &&
                  device.scalar_type() == at::kInt && device.sizes() == host.sizes() && device.is_contiguous(),
              "plan and plan_host must be a Packing's");
         fa_done(nn_fa_packed_plan_info(at_host(), &info));

@@ -32,7 +32,8 @@ _POSITIONS = 15  # the word of a plan that says where the positions begin (NN_FA
 
 class Packing:
     """How sequences of the given lengths (>= 0) lie in a packed batch, for attention with these heads on this device. Its
-    tensors are not to be changed.
+    tensors are not to be changed. They are copied on the device's current stream and, as any tensor's are, their memory is that
+    stream's: another stream waits for it before it uses them, and they are kept until it has, and as long as a captured graph.
 
     lengths    the lengths, a tuple;   tokens   their sum;   longest   the longest
     positions  (tokens,) int32 on the device: each token's position in its sequence

@@ -522,3 +522,29 @@ def test_offsets_past_32_bits():
         # (which blocks share a sum goes by the batch: fp32 sums in another order, rounded to bf16)
         torch.testing.assert_close(x[-last:].float(), y.float(), rtol=2**-7, atol=1e-5 * y.float().abs().max().item(), msg=name)
     assert torch.equal(got[0][-last:], _call(*tail[:3], small))
+
+
+# (whole blocks, short ones, a wave a pair beside short ones, shared pairs)
+@pytest.mark.parametrize("lengths", [[300, 1000, 5], [30] * 40, [700] * 60 + [20] * 400, [4096]])
+def test_a_list_that_was_overwritten_costs_values_only(lengths):
+    """A program that frees a packing while a captured graph or another stream still reads it: entries that lie outside the
+    tensors are passed over, and what else the memory holds stays as it was."""
+    print(f"\n[case] overwritten list of {len(lengths)} sequences", flush=True)
+    H, KVH, D = 12, 4, 64
+    q, k, v, do = _inputs(lengths, H, KVH, D, torch.bfloat16, seed=12)
+    packing = _packing(lengths, H, KVH)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    want = _run(q, k, v, do, packing)
+    mine = packing.plan.clone()
+    g = torch.Generator().manual_seed(13)
+    T = sum(lengths)
+    for low, high in ((2**31 - 1, 2**31), (-1, 0), (0, 1), (-(2**31), 2**31), (-2, T + 3), (-1, 40), (0, 4)):
+        packing.plan.copy_(torch.randint(low, high, mine.shape, generator=g).to(torch.int32))
+        o = _call(*leaves, packing)
+        torch.autograd.grad(o, leaves, do)
+        torch.cuda.synchronize()
+        for a, b in zip(leaves, (q, k, v)):
+            assert torch.equal(a.detach(), b)
+    packing.plan.copy_(mine)
+    for a, b in zip(_run(q, k, v, do, packing), want):
+        assert torch.equal(a, b)
