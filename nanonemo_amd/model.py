@@ -410,6 +410,8 @@ class NanoNemo(nn.Module):
     def _hidden_packed(self, idx: torch.Tensor, packing) -> torch.Tensor:
         if idx.numel() != packing.tokens:
             raise ValueError(f"{idx.numel()} tokens, but a packing of {packing.tokens}")
+        if not packing.tokens:
+            raise ValueError("a packing without tokens")
         x, delta = self.tok_emb(idx.reshape(1, -1)), None
         cos, sin = self.rope_cos[packing.positions], self.rope_sin[packing.positions]  # once for all blocks
         for blk in self.blocks:

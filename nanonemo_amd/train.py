@@ -35,7 +35,8 @@ CURVE_BOUND = 0.12
 
 def train_step(model, opt, batches, grad_clip: float = 1.0, amp_dtype=torch.bfloat16):
     """One optimizer step over the micro-batches ``batches`` [(x, y), ...] or, for a student, [(x, y, teacher), ...]
-    (``teacher_batches``), or of packed documents, [(x, y, None, packing), ...] (``packed_batches``); returns (loss, grad_norm) as device tensors (no host synchronisation)."""
+    (``teacher_batches``), or of packed documents, [(x, y, None, packing), ...] (``packed_batches``); returns (loss, grad_norm) as
+    device tensors (no host synchronisation)."""
     accum = len(batches)
     loss_sum = None
     for x, y, *more in batches:
@@ -149,6 +150,9 @@ def run(attn: str, steps: int, batch: int, seq: int, cfg_kwargs: dict, device: s
     torch.cuda.synchronize()
     dt = time.perf_counter() - t0 if t0 is not None else float("nan")
     tokens = sum(micro[0].numel() for micro in data[warmup:])
+    if docs:  # (a token's attention products go by its own document's length)
+        lengths = [n for micro in data for n in micro[3].lengths]
+        seq = round(sum(n * n for n in lengths) / sum(lengths))
     return [float(v) for v in torch.stack(losses).cpu()], tokens / dt, model.flops_per_token(seq)
 
 

@@ -294,6 +294,26 @@ def test_a_packed_model_is_the_model_on_each_sequence(qk_norm):
         model(idx, None, None, model.pack([65, 25]))
 
 
+def test_a_packing_without_tokens_is_refused_by_the_model():
+    from nanonemo_amd.model import ModelConfig, NanoNemo
+
+    model = NanoNemo(ModelConfig(n_layers=1, d_model=64, n_heads=2, n_kv_heads=1, d_ff=64, vocab_size=64, max_seq_len=32))
+    for lengths in ([], [0, 0]):
+        with pytest.raises(ValueError, match="without tokens"):
+            model(torch.zeros(1, 0, dtype=torch.long), None, None, model.pack(lengths))
+
+
+def test_a_plan_cut_short_is_refused():
+    from nanonemo_amd.kernels.hip import host
+    from nanonemo_amd.kernels.hip.packed import Packing
+
+    plan = Packing([5, 9], 2, 1, device="cpu").plan_host
+    q, k = torch.zeros(14, 2, 64, dtype=torch.bfloat16), torch.zeros(14, 1, 64, dtype=torch.bfloat16)
+    for n in (0, 16, 31, 32, len(plan) - 1):
+        with pytest.raises(RuntimeError, match="must be a Packing's"):
+            host().packed_fwd(q, k, k, plan[:n], plan[:n], False)
+
+
 def test_packed_batches():
     from nanonemo_amd.model import ModelConfig, NanoNemo
     from nanonemo_amd.train import packed_batches, synthetic_documents, teacher_batches, train_step
