@@ -490,11 +490,27 @@ T2 project_fwd(const Tensor& x, const std::vector<Tensor>& ws, bool turned) {
     return {at::mm(x, w.fwd[0].t()), w.bwd[0]};
 }
 
+// A call's plan: in host memory and, the same, on the tensors' device.
+struct Plan {
+    Tensor host, device;
+    nn_fa_packed_info info;
+    Plan(const Tensor& device_, const Tensor& host_) : host(contig(host_)), device(contig(device_)) {
+        need(host.device().is_cpu() && host.scalar_type() == at::kInt && host.dim() == 1 && host.numel() >= 32 &&
+                 device.scalar_type() == at::kInt && device.sizes() == host.sizes(),
+             "plan and plan_host must be a Packing's");
+        fa_done(nn_fa_packed_plan_info(at_host(), &info));
+        need(info.words == host.numel(), "plan and plan_host must be a Packing's");
+    }
+    const int32_t* at_host() const { return host.data_ptr<int32_t>(); }
+    const int32_t* at_device() const { return device.data_ptr<int32_t>(); }
+};
+
 // The attention layer (kernels/hip/layers.py): sizes, and the strides of its tensors for the library. q, k and v are
 // column ranges of one (B T, n) product, dq, dk and dv of another such buffer.
 struct LayerShape {
     int64_t B, T, H, KVH, D, nq, nk, n;
     int64_t fwd[9], bwd[15], rot[12], unrot[12];
+    int64_t packed[10];                                              // {head, row} of q and dO, k and v, o, dq, dk and dv
     LayerShape(int64_t B, int64_t T, int64_t H, int64_t KVH, int64_t D) : B(B), T(T), H(H), KVH(KVH), D(D) {
         nq = H * D, nk = KVH * D, n = nq + 2 * nk;
         const S3 dense{T * nq, D, nq}, wide{T * n, D, n};            // {batch, head, row}
@@ -507,14 +523,24 @@ struct LayerShape {
         put(bwd, {dense, wide, dense, wide, wide});                  // q and dO, k and v, o, dq, dk and dv
         put(rot, {wide_r, dense_r, wide_r, wide_r});                 // q out of the buffer, k in place
         put(unrot, {wide_r, wide_r, wide_r, wide_r});
+        const int64_t rows[5] = {nq, n, nq, n, n};
+        for (int i = 0; i < 5; ++i) packed[2 * i] = D, packed[2 * i + 1] = rows[i];
     }
     char* k(const Tensor& buf) const { return (char*)buf.data_ptr() + 2 * nq; }
     char* v(const Tensor& buf) const { return k(buf) + 2 * nk; }
+    // The plan of one row of sequences (a layer given one has B = 1).
+    Plan plan(const Tensor& x, const OptTensor& device, const OptTensor& host) const {
+        need(device && host, "a packed layer takes both of a Packing's plans");
+        const Plan p(*device, *host);
+        check_on_device(x, {&*device});
+        need(B == 1 && p.info.tokens == T && p.info.H == H && p.info.KVH == KVH, "the packing must be of the layer's tokens and heads");
+        return p;
+    }
 };
 
 std::vector<Tensor> attention_layer_fwd(const Tensor& x, const Tensor& cos, const Tensor& sin, int64_t B, int64_t T, int64_t H,
                                         int64_t KVH, const Tensor& wq, const Tensor& wk, const Tensor& wv, const Tensor& wo,
-                                        bool turned) {
+                                        bool turned, const OptTensor& plan, const OptTensor& plan_host) {
     const Inner inner;
     const c10::DeviceGuard guard(x.device());
     const LayerShape s(B, T, H, KVH, wq.size(0) / H);
@@ -526,15 +552,26 @@ std::vector<Tensor> attention_layer_fwd(const Tensor& x, const Tensor& cos, cons
     Tensor q = empty_of(x, {B * T, s.nq}), o = empty_of(x, {B * T, s.nq}), lse = empty_f32(x, {B, H, T});
     rope_done(nn_rope_qk_views(qkv.data_ptr(), q.data_ptr(), s.k(qkv), s.k(qkv), cos.data_ptr<float>(), sin.data_ptr<float>(), B, T, H,
                                KVH, s.D, s.rot, cos.size(0), dt, 0, st));
-    fa_done(nn_fa_fwd_views(q.data_ptr(), s.k(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(), B, H, KVH, T, s.D, s.fwd, dt,
-                            scale_of(s.D), st));
-    return {at::mm(o, w.fwd[1].t()), qkv, q, o, lse, w.bwd[0], w.bwd[1]};
+    Tensor rest;  // what rounding o left, where sequences are packed, as packed_into's
+    if (plan) {
+        rest = at::empty({turned ? T : 0, s.nq}, x.options().dtype(at::kChar));
+        const Plan p = s.plan(x, plan, plan_host);
+        fa_done(nn_fa_packed_fwd(q.data_ptr(), s.k(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(), turned ? rest.data_ptr() : nullptr,
+                                 p.at_host(), p.at_device(), s.D, s.packed, dt, scale_of(s.D), st));
+    } else {
+        fa_done(nn_fa_fwd_views(q.data_ptr(), s.k(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(), B, H, KVH, T, s.D, s.fwd, dt,
+                                scale_of(s.D), st));
+    }
+    std::vector<Tensor> out{at::mm(o, w.fwd[1].t()), qkv, q, o, lse, w.bwd[0], w.bwd[1]};
+    if (plan) out.push_back(rest);
+    return out;
 }
 
 // The gradients of x, wq, wk, wv and wo; undefined where not needed.
 std::vector<OptTensor> attention_layer_bwd(const Tensor& dy_, const Tensor& x, const Tensor& cos_, const Tensor& sin_, const Tensor& qkv_,
                                            const Tensor& q_, const Tensor& o_, const Tensor& lse_, const Tensor& w, const Tensor& wo,
-                                           int64_t B, int64_t T, int64_t H, int64_t KVH, bool need_x, bool need_qkv, bool need_o) {
+                                           int64_t B, int64_t T, int64_t H, int64_t KVH, bool need_x, bool need_qkv, bool need_o,
+                                           const OptTensor& rest_, const OptTensor& plan, const OptTensor& plan_host) {
     const Inner inner;
     check_on_device(x, {&dy_});
     const c10::DeviceGuard guard(x.device());
@@ -550,10 +587,21 @@ std::vector<OptTensor> attention_layer_bwd(const Tensor& dy_, const Tensor& x, c
     if (need_o) out[4] = wgrad(dy, o, {wo.size(0)})[0];
     if (!need_x && !need_qkv) return out;
     Tensor dqkv = at::empty_like(qkv);
-    const size_t n = nn_fa_bwd_workspace_size(B, H, KVH, T, s.D);
-    Tensor ws = bytes(x, n);
-    fa_done(nn_fa_bwd_views(d_o.data_ptr(), q.data_ptr(), s.k(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(), dqkv.data_ptr(),
-                            s.k(dqkv), s.v(dqkv), ws.data_ptr(), n, B, H, KVH, T, s.D, s.bwd, dt, scale_of(s.D), st));
+    if (plan) {
+        const Plan p = s.plan(x, plan, plan_host);
+        need(rest_.has_value(), "a packed layer's backward takes the forward's rests");
+        const Tensor rest = saved(*rest_, x, {rest_->size(0) ? T : 0, s.nq}, at::kChar);
+        const size_t n = nn_fa_packed_bwd_workspace_size(p.at_host(), s.D);
+        Tensor ws = bytes(x, n);
+        fa_done(nn_fa_packed_bwd(d_o.data_ptr(), q.data_ptr(), s.k(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(),
+                                 rest.numel() ? rest.data_ptr() : nullptr, dqkv.data_ptr(), s.k(dqkv), s.v(dqkv), ws.data_ptr(), n, p.at_host(),
+                                 p.at_device(), s.D, s.packed, dt, scale_of(s.D), st));
+    } else {
+        const size_t n = nn_fa_bwd_workspace_size(B, H, KVH, T, s.D);
+        Tensor ws = bytes(x, n);
+        fa_done(nn_fa_bwd_views(d_o.data_ptr(), q.data_ptr(), s.k(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(), dqkv.data_ptr(),
+                                s.k(dqkv), s.v(dqkv), ws.data_ptr(), n, B, H, KVH, T, s.D, s.bwd, dt, scale_of(s.D), st));
+    }
     rope_done(nn_rope_qk_views(dqkv.data_ptr(), dqkv.data_ptr(), s.k(dqkv), s.k(dqkv), cos.data_ptr<float>(), sin.data_ptr<float>(), B, T,
                                H, KVH, s.D, s.unrot, cos.size(0), dt, 1, st));
     if (need_x) out[0] = at::mm(dqkv, w);
@@ -803,21 +851,6 @@ Tensor packed_plan(const std::vector<int64_t>& lengths, int64_t H, int64_t KVH) 
     fa_done(nn_fa_packed_plan(lengths.data(), (int64_t)lengths.size(), H, KVH, plan.data_ptr<int32_t>(), n));
     return plan;
 }
-
-// A call's plan: in host memory and, the same, on the tensors' device.
-struct Plan {
-    const Tensor &host, &device;
-    nn_fa_packed_info info;
-    Plan(const Tensor& device_, const Tensor& host_) : host(host_), device(device_) {
-        need(host.device().is_cpu() && host.scalar_type() == at::kInt && host.dim() == 1 && host.is_contiguous() && host.numel() >= 32 &&
-                 device.scalar_type() == at::kInt && device.sizes() == host.sizes() && device.is_contiguous(),
-             "plan and plan_host must be a Packing's");
-        fa_done(nn_fa_packed_plan_info(at_host(), &info));
-        need(info.words == host.numel(), "plan and plan_host must be a Packing's");
-    }
-    const int32_t* at_host() const { return host.data_ptr<int32_t>(); }
-    const int32_t* at_device() const { return device.data_ptr<int32_t>(); }
-};
 
 using S2 = std::array<int64_t, 2>;
 // The {head, row} strides through which the kernels can read the (tokens, heads, hd) tensor's values in place, if they can (the
@@ -1266,8 +1299,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("wgrad_takes", wgrad_takes);
     m.def("rows_aligned", rows_aligned);
     m.def("project_fwd", project_fwd, nogil);
-    m.def("attention_layer_fwd", attention_layer_fwd, nogil);
-    m.def("attention_layer_bwd", attention_layer_bwd, nogil);
+    using py::arg;
+    const auto none = py::none();
+    m.def("attention_layer_fwd", attention_layer_fwd, nogil, arg("x"), arg("cos"), arg("sin"), arg("B"), arg("T"), arg("H"), arg("KVH"), arg("wq"),
+          arg("wk"), arg("wv"), arg("wo"), arg("turned"), arg("plan") = none, arg("plan_host") = none);
+    m.def("attention_layer_bwd", attention_layer_bwd, nogil, arg("dy"), arg("x"), arg("cos"), arg("sin"), arg("qkv"), arg("q"), arg("o"), arg("lse"),
+          arg("w"), arg("wo"), arg("B"), arg("T"), arg("H"), arg("KVH"), arg("need_x"), arg("need_qkv"), arg("need_o"), arg("rest") = none,
+          arg("plan") = none, arg("plan_host") = none);
     m.def("mlp_fwd", mlp_fwd, nogil);
     m.def("mlp_bwd", mlp_bwd, nogil);
     m.def("head_fwd", head_fwd, nogil);

@@ -211,14 +211,14 @@ class Attention(nn.Module):
 
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, packing=None) -> torch.Tensor:
         B, T, _ = x.shape
-        fusible = self.cfg.attn_kernel == "hip_bthd" and self.cfg.rope_kernel != "torch" and not self.cfg.qk_norm and packing is None
+        fusible = self.cfg.attn_kernel == "hip_bthd" and self.cfg.rope_kernel != "torch" and not self.cfg.qk_norm
         if fusible and x.is_cuda:
             from nanonemo_amd.kernels.hip import layers
 
             call = (x, cos, sin, self.H, self.KVH)
             ws = (self.wq, self.wk, self.wv, self.wo)
             if layers.can_fuse(*call, self.hd, *ws):  # the whole layer in this build's kernels, as one autograd node
-                return layers.attention_layer(*call, *ws)
+                return layers.attention_layer(*call, *ws, packing)
         q, k, v = _project(self.cfg, x, self.wq, self.wk, self.wv)
         q = q.view(B, T, self.H, self.hd)
         k = k.view(B, T, self.KVH, self.hd)

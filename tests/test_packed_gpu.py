@@ -548,3 +548,140 @@ def test_a_list_that_was_overwritten_costs_values_only(lengths):
     packing.plan.copy_(mine)
     for a, b in zip(_run(q, k, v, do, packing), want):
         assert torch.equal(a, b)
+
+
+LAYER = [([100, 1, 260, 0, 64, 33], 12, 4, 64), ([20] * 30, 2, 2, 64), ([700, 330], 8, 2, 32), ([130, 1, 65], 4, 1, 32)]
+
+
+def _layer(lengths, H, KVH, hd):
+    """An attention layer, its packing, and cos and sin of every token."""
+    from tests.test_layers_gpu import _attention
+
+    m, (cos, sin) = _attention(H, KVH, hd, max(lengths), rope_kernel="hip")
+    packing = _packing(lengths, H, KVH)
+    return m, packing, cos[packing.positions], sin[packing.positions]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths, H, KVH, hd", LAYER)
+def test_packed_attention_layer_matches_its_modules_and_float64(lengths, H, KVH, hd, dtype):
+    from tests.test_layers_gpu import _assert_close_to_float64, _attention64, _modules_only
+    from tests.test_layers_gpu import _run as run
+
+    print(f"\n[case] packed attention layer of {len(lengths)} sequences H={H} KVH={KVH} hd={hd} {dtype}", flush=True)
+    m, packing, cos, sin = _layer(lengths, H, KVH, hd)
+    T = sum(lengths)
+    x = torch.randn(1, T, H * hd, device="cuda").to(dtype).requires_grad_()
+    dy = torch.randn(1, T, H * hd, device="cuda").to(dtype)
+    got, ref = run(m, (x, cos, sin, packing), dy, dtype), run(_modules_only(m), (x, cos, sin, packing), dy, dtype)
+    ins = [t.detach().double().requires_grad_() for t in (x, m.wq.weight, m.wk.weight, m.wv.weight, m.wo.weight)]
+    # (the rows of each sequence's own tables are the first of the longest one's)
+    i = lengths.index(max(lengths))
+    a = sum(lengths[:i])
+    c, s = cos[a : a + lengths[i]], sin[a : a + lengths[i]]
+    y = torch.cat([_attention64(t, c, s, H, KVH, *ins[1:]) for t in ins[0].split(lengths, 1) if t.shape[1]], 1)
+    exact = (y.detach(), *torch.autograd.grad(y, ins, dy.double()))
+    # as the dense layer: weights, product, rotation of q and of k; P and O; the output weight, dO, dS, dq or dk, its rotation
+    _assert_close_to_float64(("y", "dx", "dwq", "dwk", "dwv", "dwo"), got, ref, exact, 13, dtype)
+    with torch.no_grad(), torch.autocast("cuda", dtype=dtype):
+        assert torch.equal(m(x, cos, sin, packing), got[0])
+
+
+def test_packed_attention_layer_is_one_node():
+    m, packing, cos, sin = _layer([70, 70], 4, 2, 64)
+    x = torch.randn(1, 140, 256, device="cuda", requires_grad=True)  # fp32 in, cast by the layer
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = m(x, cos, sin, packing)
+    node = y.grad_fn
+    while "View" in node.name():
+        node = node.next_functions[0][0]
+    assert node.name() == "_AttentionLayerBackward"
+
+
+def test_packed_attention_layer_frozen_parts_and_repeated_backward():
+    m, packing, cos, sin = _layer([70, 30, 40], 4, 2, 64)
+    x = torch.randn(1, 140, 256, device="cuda", requires_grad=True)
+    m.wk.weight.requires_grad_(False)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = m(x, cos, sin, packing)
+    y.float().square().sum().backward(retain_graph=True)
+    first = [t.grad.clone() for t in (x, m.wq.weight, m.wv.weight, m.wo.weight)]
+    assert m.wk.weight.grad is None
+    y.float().square().sum().backward()
+    for a, t in zip(first, (x, m.wq.weight, m.wv.weight, m.wo.weight)):
+        assert torch.equal(a + a, t.grad)
+    for p in m.parameters():
+        p.requires_grad_(False)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        (gx,) = torch.autograd.grad(m(x, cos, sin, packing).float().square().sum(), x)
+    assert torch.equal(gx, first[0])
+    m.wo.weight.requires_grad_(True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        (gw,) = torch.autograd.grad(m(x.detach(), cos, sin, packing).float().square().sum(), m.wo.weight)
+    assert torch.equal(gw, first[3])
+
+
+def test_packed_attention_layer_recorded_and_batched_backwards():
+    """They go through the modules' functions: first derivatives by the kernels, second and batched ones through the attention refused."""
+    from tests.test_layers_gpu import _modules_only
+
+    m, packing, cos, sin = _layer([20, 13], 4, 2, 32)
+    x = torch.randn(1, 33, 128, device="cuda", requires_grad=True)
+    out = []
+    for mod in (m, _modules_only(m)):
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            y = mod(x, cos, sin, packing)
+        (gw,) = torch.autograd.grad(y.float().sum(), mod.wo.weight, create_graph=True)
+        out.append(torch.autograd.grad(gw.square().sum(), x))
+    for a, b in zip(*out):
+        torch.testing.assert_close(a, b, rtol=5e-2, atol=5e-2 * b.abs().max().item())
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = m(x, cos, sin, packing)
+    (gx,) = torch.autograd.grad(y.float().sum(), x, create_graph=True)
+    # (as with PyTorch's own once_differentiable the graph of gx ends at the node that refuses: x is not in it, and a backward meets it)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        gx.square().sum().backward()
+    with pytest.raises(RuntimeError, match="batched gradients"):
+        torch.autograd.grad(y, x, torch.ones(2, *y.shape, device="cuda", dtype=y.dtype), is_grads_batched=True)
+
+
+def test_packed_attention_layer_refuses_another_batch_s_packing():
+    m, packing, cos, sin = _layer([20, 13], 4, 2, 32)
+    x = torch.randn(1, 33, 128, device="cuda", requires_grad=True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        for bad in (_packing([20, 12], 4, 2), _packing([20, 13], 4, 4), _packing([20, 13], 2, 2)):
+            with pytest.raises(RuntimeError, match="packing"):
+                m(x, cos, sin, bad)
+
+
+@pytest.mark.parametrize("what", ["layer", "flash_attn_packed", "qk_norm_rope"])
+def test_saved_tensors_are_checked_like_inputs(what):
+    """What a saved-tensor hook hands back reaches the kernels by address: dense or not it is read rightly, and a host tensor or
+    another type is an error before any launch."""
+    from nanonemo_amd.kernels.hip.qk_norm import qk_norm_rope
+    from tests.test_layers_gpu import _rel, _saved_through
+
+    m, packing, cos, sin = _layer([70, 30, 40], 4, 2, 64)
+    x = torch.randn(1, 140, 256, device="cuda").bfloat16().requires_grad_()
+    q, k, v = (torch.randn(140, h, 64, device="cuda").bfloat16().requires_grad_() for h in (4, 2, 2))
+    wq, wk = (torch.ones(64, device="cuda", requires_grad=True) for _ in range(2))
+
+    def f():
+        if what == "layer":
+            with torch.autocast("cuda", dtype=torch.bfloat16):
+                return m(x, cos, sin, packing), (x, *m.parameters())
+        if what == "flash_attn_packed":
+            return _call(q, k, v, packing), (q, k, v)
+        a, b = qk_norm_rope(q, k, wq, wk, cos, sin)
+        return torch.cat((a, b), 1), (q, k, wq, wk)
+
+    def spread(t):  # the same values, every second element of a buffer
+        return t if t.dim() == 0 else torch.stack((t, t), -1)[..., 0]
+
+    ref = _saved_through(lambda t: t, f)
+    for a, b in zip(_saved_through(spread, f), ref):
+        # (the library may take another product for other strides: two bf16 roundings apart)
+        assert torch.equal(a, b) or what == "layer" and _rel(a, b.double()) < 2 * 2.0**-8
+    for bad in (lambda t: t.cpu(), lambda t: t.float() if t.dtype == torch.bfloat16 else t):
+        with pytest.raises(RuntimeError):
+            _saved_through(bad, f)
