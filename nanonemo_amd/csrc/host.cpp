@@ -506,28 +506,39 @@ struct Plan {
 };
 
 // The attention layer (kernels/hip/layers.py): sizes, and the strides of its tensors for the library. q, k and v are
-// column ranges of one (B T, n) product, dq, dk and dv of another such buffer.
+// column ranges of one (B T, n) product, dq, dk and dv of another such buffer. A layer that normalises its heads keeps q and k as
+// the product had them, for the norm's backward, and has its keys behind v, in rows of nf: of v's stride, as the attention reads them.
 struct LayerShape {
-    int64_t B, T, H, KVH, D, nq, nk, n;
+    int64_t B, T, H, KVH, D, nq, nk, n, nf;
+    bool normed;
     int64_t fwd[9], bwd[15], rot[12], unrot[12];
     int64_t packed[10];                                              // {head, row} of q and dO, k and v, o, dq, dk and dv
-    LayerShape(int64_t B, int64_t T, int64_t H, int64_t KVH, int64_t D) : B(B), T(T), H(H), KVH(KVH), D(D) {
-        nq = H * D, nk = KVH * D, n = nq + 2 * nk;
-        const S3 dense{T * nq, D, nq}, wide{T * n, D, n};            // {batch, head, row}
+    int64_t norm[8], unnorm[12];                                     // {token, head} of q, k and the outputs; of both gradients, q, k and the results
+    LayerShape(int64_t B, int64_t T, int64_t H, int64_t KVH, int64_t D, bool normed) : B(B), T(T), H(H), KVH(KVH), D(D), normed(normed) {
+        nq = H * D, nk = KVH * D, n = nq + 2 * nk, nf = normed ? n + nk : n;
+        const S3 dense{T * nq, D, nq}, wide{T * n, D, n}, wide_f{T * nf, D, nf};  // {batch, head, row}
         const S3 dense_r{T * nq, nq, D}, wide_r{T * n, n, D};        // {batch, position, head}
         auto put = [](int64_t* to, std::initializer_list<S3> all) {
             for (const S3& s : all)
                 for (int64_t v : s) *to++ = v;
         };
-        put(fwd, {dense, wide, dense});                              // q, k and v, o
-        put(bwd, {dense, wide, dense, wide, wide});                  // q and dO, k and v, o, dq, dk and dv
+        put(fwd, {dense, wide_f, dense});                            // q, k and v, o
+        put(bwd, {dense, wide_f, dense, wide, wide});                // q and dO, k and v, o, dq, dk and dv
         put(rot, {wide_r, dense_r, wide_r, wide_r});                 // q out of the buffer, k in place
         put(unrot, {wide_r, wide_r, wide_r, wide_r});
-        const int64_t rows[5] = {nq, n, nq, n, n};
+        const int64_t rows[5] = {nq, nf, nq, n, n}, tokens[10] = {nf, nf, nq, nf, n, n, nf, nf, n, n};
         for (int i = 0; i < 5; ++i) packed[2 * i] = D, packed[2 * i + 1] = rows[i];
+        for (int i = 0; i < 4; ++i) norm[2 * i] = tokens[i], norm[2 * i + 1] = D;
+        for (int i = 0; i < 6; ++i) unnorm[2 * i] = tokens[4 + i], unnorm[2 * i + 1] = D;
     }
     char* k(const Tensor& buf) const { return (char*)buf.data_ptr() + 2 * nq; }
     char* v(const Tensor& buf) const { return k(buf) + 2 * nk; }
+    char* keys(const Tensor& qkv) const { return normed ? v(qkv) + 2 * nk : k(qkv); }  // as the attention takes them
+    void check_norms(const Tensor& x, const OptTensor& q, const OptTensor& k) const {
+        need(q && k, "a layer normalises both or neither of queries and keys");
+        check_on_device(x, {&*q, &*k});
+        for (const Tensor* w : {&*q, &*k}) need(w->scalar_type() == at::kFloat && w->dim() == 1 && w->size(0) == D, "weights must be float32 of head_dim values");
+    }
     // The plan of one row of sequences (a layer given one has B = 1).
     Plan plan(const Tensor& x, const OptTensor& device, const OptTensor& host) const {
         need(device && host, "a packed layer takes both of a Packing's plans");
@@ -540,26 +551,34 @@ struct LayerShape {
 
 std::vector<Tensor> attention_layer_fwd(const Tensor& x, const Tensor& cos, const Tensor& sin, int64_t B, int64_t T, int64_t H,
                                         int64_t KVH, const Tensor& wq, const Tensor& wk, const Tensor& wv, const Tensor& wo,
-                                        bool turned, const OptTensor& plan, const OptTensor& plan_host) {
+                                        bool turned, const OptTensor& plan, const OptTensor& plan_host, const OptTensor& q_norm,
+                                        const OptTensor& k_norm, double eps) {
     const Inner inner;
     const c10::DeviceGuard guard(x.device());
-    const LayerShape s(B, T, H, KVH, wq.size(0) / H);
+    const LayerShape s(B, T, H, KVH, wq.size(0) / H, q_norm.has_value());
     check_tables(cos, sin, T, s.D, x.device());
+    if (s.normed) s.check_norms(x, q_norm, k_norm);
     const int dt = code(x);
     void* st = stream_of(x);
     const Weights w = cast_weights(x, {{wq, wk, wv}, {wo}}, turned);
-    Tensor qkv = at::mm(x, w.fwd[0].t());
+    Tensor qkv = empty_of(x, {B * T, s.nf}), product = qkv.narrow(1, 0, s.n);
+    at::mm_out(product, x, w.fwd[0].t());
     Tensor q = empty_of(x, {B * T, s.nq}), o = empty_of(x, {B * T, s.nq}), lse = empty_f32(x, {B, H, T});
-    rope_done(nn_rope_qk_views(qkv.data_ptr(), q.data_ptr(), s.k(qkv), s.k(qkv), cos.data_ptr<float>(), sin.data_ptr<float>(), B, T, H,
-                               KVH, s.D, s.rot, cos.size(0), dt, 0, st));
+    if (s.normed)
+        qkn_done(nn_qk_norm_rope_fwd(qkv.data_ptr(), s.k(qkv), q_norm->data_ptr<float>(), k_norm->data_ptr<float>(), cos.data_ptr<float>(),
+                                     sin.data_ptr<float>(), cos.size(0), nullptr, 0, T, q.data_ptr(), s.keys(qkv), B * T, H, KVH, s.D, s.norm, (float)eps,
+                                     dt, st));
+    else
+        rope_done(nn_rope_qk_views(qkv.data_ptr(), q.data_ptr(), s.k(qkv), s.k(qkv), cos.data_ptr<float>(), sin.data_ptr<float>(), B, T, H,
+                                   KVH, s.D, s.rot, cos.size(0), dt, 0, st));
     Tensor rest;  // what rounding o left, where sequences are packed, as packed_into's
     if (plan) {
         rest = at::empty({turned ? T : 0, s.nq}, x.options().dtype(at::kChar));
         const Plan p = s.plan(x, plan, plan_host);
-        fa_done(nn_fa_packed_fwd(q.data_ptr(), s.k(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(), turned ? rest.data_ptr() : nullptr,
+        fa_done(nn_fa_packed_fwd(q.data_ptr(), s.keys(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(), turned ? rest.data_ptr() : nullptr,
                                  p.at_host(), p.at_device(), s.D, s.packed, dt, scale_of(s.D), st));
     } else {
-        fa_done(nn_fa_fwd_views(q.data_ptr(), s.k(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(), B, H, KVH, T, s.D, s.fwd, dt,
+        fa_done(nn_fa_fwd_views(q.data_ptr(), s.keys(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(), B, H, KVH, T, s.D, s.fwd, dt,
                                 scale_of(s.D), st));
     }
     std::vector<Tensor> out{at::mm(o, w.fwd[1].t()), qkv, q, o, lse, w.bwd[0], w.bwd[1]};
@@ -567,43 +586,56 @@ std::vector<Tensor> attention_layer_fwd(const Tensor& x, const Tensor& cos, cons
     return out;
 }
 
-// The gradients of x, wq, wk, wv and wo; undefined where not needed.
+// The gradients of x, wq, wk, wv, wo and of the norms' weights; undefined where not needed.
 std::vector<OptTensor> attention_layer_bwd(const Tensor& dy_, const Tensor& x, const Tensor& cos_, const Tensor& sin_, const Tensor& qkv_,
                                            const Tensor& q_, const Tensor& o_, const Tensor& lse_, const Tensor& w, const Tensor& wo,
                                            int64_t B, int64_t T, int64_t H, int64_t KVH, bool need_x, bool need_qkv, bool need_o,
-                                           const OptTensor& rest_, const OptTensor& plan, const OptTensor& plan_host) {
+                                           const OptTensor& rest_, const OptTensor& plan, const OptTensor& plan_host, const OptTensor& q_norm_,
+                                           const OptTensor& k_norm_, double eps, bool need_norms) {
     const Inner inner;
     check_on_device(x, {&dy_});
     const c10::DeviceGuard guard(x.device());
-    const LayerShape s(B, T, H, KVH, wo.size(1) / H);
+    const LayerShape s(B, T, H, KVH, wo.size(1) / H, q_norm_.has_value());
     check_tables(cos_, sin_, T, s.D, x.device());
     const Tensor cos = contig(cos_), sin = contig(sin_), lse = saved(lse_, x, {B, H, T}, at::kFloat);
-    const Tensor qkv = saved(qkv_, x, {B * T, s.n}), q = saved(q_, x, {B * T, s.nq}), o = saved(o_, x, {B * T, s.nq});
+    const Tensor qkv = saved(qkv_, x, {B * T, s.nf}), q = saved(q_, x, {B * T, s.nq}), o = saved(o_, x, {B * T, s.nq});
     const int dt = code(x);
     void* st = stream_of(x);
     const Tensor dy = contig(dy_);
-    std::vector<OptTensor> out(5);
-    Tensor d_o = need_x || need_qkv ? at::mm(dy, wo) : Tensor();
+    std::vector<OptTensor> out(7);
+    const bool inside = need_x || need_qkv || need_norms;
+    Tensor d_o = inside ? at::mm(dy, wo) : Tensor();
     if (need_o) out[4] = wgrad(dy, o, {wo.size(0)})[0];
-    if (!need_x && !need_qkv) return out;
-    Tensor dqkv = at::empty_like(qkv);
+    if (!inside) return out;
+    Tensor dqkv = empty_of(x, {B * T, s.n});
     if (plan) {
         const Plan p = s.plan(x, plan, plan_host);
         need(rest_.has_value(), "a packed layer's backward takes the forward's rests");
         const Tensor rest = saved(*rest_, x, {rest_->size(0) ? T : 0, s.nq}, at::kChar);
         const size_t n = nn_fa_packed_bwd_workspace_size(p.at_host(), s.D);
         Tensor ws = bytes(x, n);
-        fa_done(nn_fa_packed_bwd(d_o.data_ptr(), q.data_ptr(), s.k(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(),
+        fa_done(nn_fa_packed_bwd(d_o.data_ptr(), q.data_ptr(), s.keys(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(),
                                  rest.numel() ? rest.data_ptr() : nullptr, dqkv.data_ptr(), s.k(dqkv), s.v(dqkv), ws.data_ptr(), n, p.at_host(),
                                  p.at_device(), s.D, s.packed, dt, scale_of(s.D), st));
     } else {
         const size_t n = nn_fa_bwd_workspace_size(B, H, KVH, T, s.D);
         Tensor ws = bytes(x, n);
-        fa_done(nn_fa_bwd_views(d_o.data_ptr(), q.data_ptr(), s.k(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(), dqkv.data_ptr(),
+        fa_done(nn_fa_bwd_views(d_o.data_ptr(), q.data_ptr(), s.keys(qkv), s.v(qkv), o.data_ptr(), lse.data_ptr<float>(), dqkv.data_ptr(),
                                 s.k(dqkv), s.v(dqkv), ws.data_ptr(), n, B, H, KVH, T, s.D, s.bwd, dt, scale_of(s.D), st));
     }
-    rope_done(nn_rope_qk_views(dqkv.data_ptr(), dqkv.data_ptr(), s.k(dqkv), s.k(dqkv), cos.data_ptr<float>(), sin.data_ptr<float>(), B, T,
-                               H, KVH, s.D, s.unrot, cos.size(0), dt, 1, st));
+    if (s.normed) {
+        s.check_norms(x, q_norm_, k_norm_);
+        const Tensor q_norm = contig(*q_norm_), k_norm = contig(*k_norm_), dwq = at::empty_like(q_norm), dwk = at::empty_like(k_norm);
+        const size_t n = nn_qk_norm_rope_bwd_workspace_size(B * T, H, KVH, s.D);
+        Tensor ws = bytes(x, n);
+        qkn_done(nn_qk_norm_rope_bwd(dqkv.data_ptr(), s.k(dqkv), qkv.data_ptr(), s.k(qkv), q_norm.data_ptr<float>(), k_norm.data_ptr<float>(),
+                                     cos.data_ptr<float>(), sin.data_ptr<float>(), cos.size(0), nullptr, 0, T, dqkv.data_ptr(), s.k(dqkv),
+                                     dwq.data_ptr<float>(), dwk.data_ptr<float>(), ws.data_ptr(), n, B * T, H, KVH, s.D, s.unnorm, (float)eps, dt, st));
+        out[5] = dwq, out[6] = dwk;
+    } else {
+        rope_done(nn_rope_qk_views(dqkv.data_ptr(), dqkv.data_ptr(), s.k(dqkv), s.k(dqkv), cos.data_ptr<float>(), sin.data_ptr<float>(), B, T,
+                                   H, KVH, s.D, s.unrot, cos.size(0), dt, 1, st));
+    }
     if (need_x) out[0] = at::mm(dqkv, w);
     if (need_qkv) {
         auto dw = wgrad(dqkv, x, {s.nq, s.nk, s.nk});
@@ -1302,10 +1334,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     using py::arg;
     const auto none = py::none();
     m.def("attention_layer_fwd", attention_layer_fwd, nogil, arg("x"), arg("cos"), arg("sin"), arg("B"), arg("T"), arg("H"), arg("KVH"), arg("wq"),
-          arg("wk"), arg("wv"), arg("wo"), arg("turned"), arg("plan") = none, arg("plan_host") = none);
+          arg("wk"), arg("wv"), arg("wo"), arg("turned"), arg("plan") = none, arg("plan_host") = none, arg("q_norm") = none, arg("k_norm") = none,
+          arg("eps") = 0.0);
     m.def("attention_layer_bwd", attention_layer_bwd, nogil, arg("dy"), arg("x"), arg("cos"), arg("sin"), arg("qkv"), arg("q"), arg("o"), arg("lse"),
           arg("w"), arg("wo"), arg("B"), arg("T"), arg("H"), arg("KVH"), arg("need_x"), arg("need_qkv"), arg("need_o"), arg("rest") = none,
-          arg("plan") = none, arg("plan_host") = none);
+          arg("plan") = none, arg("plan_host") = none, arg("q_norm") = none, arg("k_norm") = none, arg("eps") = 0.0, arg("need_norms") = false);
     m.def("mlp_fwd", mlp_fwd, nogil);
     m.def("mlp_bwd", mlp_bwd, nogil);
     m.def("head_fwd", head_fwd, nogil);

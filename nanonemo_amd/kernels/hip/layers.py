@@ -9,6 +9,9 @@ product for the input's gradient and one call for the three weights'.
 That is 6 launches forward and 9 to 11 backward, where the modules take 27 in all: a cast, a product and a rounding
 per weight each way, three input gradients added in 16 bits. With a packing (kernels/hip/packed.py) the attention is
 nn_fa_packed_*, on the same strides: 652 k tokens/s of training on documents of about 300 tokens, module by module 630 k.
+With norms of the heads (``norms``) the rotation is nn_qk_norm_rope_*: q and k stay as the product wrote them, for the norm's
+backward, and its keys go behind v in the same rows, whose stride the attention wants of both (dense 661 -> 675 k tokens/s,
+packed 631 -> 646 k).
 
 MLP: one product for gate and up, SwiGLU on its two halves (nn_swiglu_*), the down product; backward, one call for
 the gate's and up's weight gradients and one product for the input's gradient. 4 launches forward and 6 to 8 backward
@@ -28,25 +31,30 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 from torch import Tensor, nn
+from torch.nn.modules import module as _module
 
 from nanonemo_amd.kernels.hip import host, records
 from nanonemo_amd.kernels.hip.flash_attn import _refuse_capture_with_autograd, flash_attn_bthd
 from nanonemo_amd.kernels.hip.linear import Stored, eligible, plain
 from nanonemo_amd.kernels.hip.packed import flash_attn_packed
+from nanonemo_amd.kernels.hip.qk_norm import qk_norm_rope
 from nanonemo_amd.kernels.hip.rope import rope_qk
 
 
-def can_fuse(x: Tensor, cos: Tensor, sin: Tensor, heads: int, kv_heads: int, hd: int, wq, wk, wv, wo) -> bool:
-    """Whether ``attention_layer`` can stand for the layer's modules called on x."""
+def can_fuse(x: Tensor, cos: Tensor, sin: Tensor, heads: int, kv_heads: int, hd: int, wq, wk, wv, wo, norms=()) -> bool:
+    """Whether ``attention_layer`` can stand for the layer's modules called on x. norms: its head norms' weights, for a layer that
+    has two, which ``plain_norms`` passed."""
     if not eligible(x) or x.dim() != 3 or hd not in (32, 64):
         return False
     B, T, d = x.shape
     if not (plain(wq, x, d) and plain(wk, x, d) and plain(wv, x, d) and plain(wo, x, heads * hd)):
         return False
     # the library's row offsets within a sequence, and the rotation kernel's index
-    if T * (heads + 2 * kv_heads) * hd >= 1 << 30 or B * T * (heads + kv_heads) * (hd // 16) >= 1 << 31:
+    if T * (heads + (3 if norms else 2) * kv_heads) * hd >= 1 << 30 or B * T * (heads + kv_heads) * (hd // 16) >= 1 << 31:
         return False
     if wq.weight.shape[0] != heads * hd or wk.weight.shape[0] != kv_heads * hd or wv.weight.shape[0] != kv_heads * hd:
+        return False
+    if any(w.device != x.device or w.shape != (hd,) or w.data_ptr() % 16 for w in norms):
         return False
     for t in (cos, sin):
         if type(t) is not Tensor or t.dtype is not torch.float32 or t.device != x.device or t.requires_grad \
@@ -55,13 +63,25 @@ def can_fuse(x: Tensor, cos: Tensor, sin: Tensor, heads: int, kv_heads: int, hd:
     return True
 
 
+def plain_norms(cls: type, *norms: nn.Module) -> bool:
+    """Whether these are untouched norms of that class with fp32 weights and one eps."""
+    for m in norms:
+        if type(m) is not cls or "forward" in m.__dict__ or m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks:
+            return False
+        w = m._parameters.get("weight")
+        if type(w) is not nn.Parameter or w.dtype is not torch.float32 or not w.is_contiguous() or m.eps != norms[0].eps:
+            return False
+    return not _module._has_any_global_hook()
+
+
 class _AttentionLayer(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, cos, sin, B, T, H, KVH, wq, wk, wv, wo, turned, packing):
-        plan = () if packing is None else (packing.plan, packing.plan_host)
-        y, qkv, q, o, lse, w, wo16, *rest = host().attention_layer_fwd(x, cos, sin, B, T, H, KVH, wq, wk, wv, wo, turned, *plan)
-        ctx.save_for_backward(x, cos, sin, qkv, q, o, lse, w, wo16, *rest, *plan)
-        ctx.weights, ctx.sizes, ctx.packing = (wq, wk, wv, wo), (B, T, H, KVH), packing
+    def forward(ctx, x, cos, sin, B, T, H, KVH, wq, wk, wv, wo, turned, packing, eps, *norms):
+        plan = (None, None) if packing is None else (packing.plan, packing.plan_host)
+        more = (*plan, *norms, eps) if norms else () if packing is None else plan
+        y, qkv, q, o, lse, w, wo16, *rest = host().attention_layer_fwd(x, cos, sin, B, T, H, KVH, wq, wk, wv, wo, turned, *more)
+        ctx.save_for_backward(x, cos, sin, qkv, q, o, lse, w, wo16, *(rest or (None,)), *plan, *norms)
+        ctx.weights, ctx.sizes, ctx.packing, ctx.eps = (wq, wk, wv, wo), (B, T, H, KVH), packing, eps
         return y
 
     @staticmethod
@@ -69,20 +89,23 @@ class _AttentionLayer(torch.autograd.Function):
         _refuse_capture_with_autograd("attention layer backward")
         x, cos, sin, qkv, q, o, lse, w, wo16, *packed = ctx.saved_tensors
         need = ctx.needs_input_grad
+        norms, wants = packed[3:], (*need[7:11], *need[14:])
         if torch.is_grad_enabled() or not host().ordinary(dy):
-            copies = (*w.split([m.shape[0] for m in ctx.weights[:3]]), wo16)
-            dx, *dws = _replayed(_modular, x, ctx.weights, copies, (need[0], *need[7:11]), dy,
-                                 (cos, sin, *ctx.sizes, ctx.packing))
-            return dx, None, None, None, None, None, None, *dws, None, None
-        dx, *dws = host().attention_layer_bwd(dy, x, cos, sin, qkv, q, o, lse, w, wo16, *ctx.sizes, need[0], any(need[7:10]), need[10], *packed)
-        return dx, None, None, None, None, None, None, *(g if n else None for g, n in zip(dws, need[7:11])), None, None
+            copies = (*w.split([m.shape[0] for m in ctx.weights[:3]]), wo16, *norms)
+            dx, *dws = _replayed(_modular, x, (*ctx.weights, *norms), copies, (need[0], *wants), dy, (cos, sin, *ctx.sizes, ctx.packing, ctx.eps))
+        else:
+            more = (*packed, ctx.eps, any(need[14:])) if norms else () if ctx.packing is None else packed
+            dx, *dws = host().attention_layer_bwd(dy, x, cos, sin, qkv, q, o, lse, w, wo16, *ctx.sizes, need[0], any(need[7:10]), need[10], *more)
+            dws = [g if n else None for g, n in zip(dws, wants)]
+        return dx, None, None, None, None, None, None, *dws[:4], None, None, None, *dws[4:]
 
 
-def _modular(x, wq, wk, wv, wo, cos, sin, B, T, H, KVH, packing):
+def _modular(x, wq, wk, wv, wo, *more):
     """The layer through differentiable functions, on (B T, d) x and weights of x's dtype."""
+    *norms, cos, sin, B, T, H, KVH, packing, eps = more
     D = wq.shape[0] // H
     q, k, v = (F.linear(x, w).view(B, T, -1, D) for w in (wq, wk, wv))
-    q, k = rope_qk(q, k, cos, sin)
+    q, k = qk_norm_rope(q, k, *norms, cos, sin, eps=eps) if norms else rope_qk(q, k, cos, sin)
     o = flash_attn_bthd(q, k, v) if packing is None else flash_attn_packed(*(t.flatten(0, 1) for t in (q, k, v)), packing)
     return F.linear(o.view(B * T, H * D), wo)
 
@@ -98,13 +121,13 @@ def _replayed(fn, x, weights, copies, need, dy, extra=()) -> list:
 
 
 def attention_layer(x: Tensor, cos: Tensor, sin: Tensor, heads: int, kv_heads: int, wq: nn.Linear, wk: nn.Linear,
-                    wv: nn.Linear, wo: nn.Linear, packing=None) -> Tensor:
+                    wv: nn.Linear, wo: nn.Linear, packing=None, norms: tuple[Tensor, ...] = (), eps: float = 0.0) -> Tensor:
     """wo(attention(rope(wq x), rope(wk x), wv x)) on x (B, T, d) in the autocast dtype, for calls that can_fuse; with a packing B
-    is 1, and cos and sin hold a row for each token."""
+    is 1, and cos and sin hold a row for each token. norms: the weights of norms of the heads before rope, of queries and of keys."""
     B, T, d = x.shape
     flat = x.to(torch.get_autocast_dtype("cuda")).reshape(B * T, d)
     y = _AttentionLayer.apply(flat, cos, sin, B, T, heads, kv_heads, wq.weight, wk.weight, wv.weight, wo.weight,
-                              records(flat, wq.weight, wk.weight, wv.weight), packing)
+                              records(flat, wq.weight, wk.weight, wv.weight, *norms), packing, eps, *norms)
     return y.view(B, T, -1)
 
 

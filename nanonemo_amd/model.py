@@ -187,10 +187,11 @@ class Attention(nn.Module):
 
             self._fa, self._packed = fa, flash_attn_packed
         if cfg.rope_kernel in ("hip", "fused"):
+            from nanonemo_amd.kernels.hip.layers import plain_norms
             from nanonemo_amd.kernels.hip.qk_norm import qk_norm_rope
             from nanonemo_amd.kernels.hip.rope import rope_k, rope_qk
 
-            self._rope_qk, self._rope_k, self._qk_norm_rope = rope_qk, rope_k, qk_norm_rope
+            self._rope_qk, self._rope_k, self._qk_norm_rope, self._plain_norms = rope_qk, rope_k, qk_norm_rope, plain_norms
 
     def _rotated(self, q, k, cos, sin):
         """q and k (B, T, heads, hd), normalised if the model does, and rotated."""
@@ -199,7 +200,9 @@ class Attention(nn.Module):
                 q, k = self.q_norm(q), self.k_norm(k)
             return rope(q, cos, sin, seq_dim=1), rope(k, cos, sin, seq_dim=1)
         if self.cfg.qk_norm:
-            return self._qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, eps=self.cfg.norm_eps)
+            if self._plain_norms(RMSNorm, self.q_norm, self.k_norm):
+                return self._qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, eps=self.q_norm.eps)
+            q, k = self.q_norm(q), self.k_norm(k)
         return self._rope_qk(q, k, cos, sin)  # in the projection layout, q and k in one launch
 
     def _attend_packed(self, q, k, v, packing):
@@ -211,14 +214,17 @@ class Attention(nn.Module):
 
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, packing=None) -> torch.Tensor:
         B, T, _ = x.shape
-        fusible = self.cfg.attn_kernel == "hip_bthd" and self.cfg.rope_kernel != "torch" and not self.cfg.qk_norm
+        fusible = self.cfg.attn_kernel == "hip_bthd" and self.cfg.rope_kernel != "torch"
+        if fusible and self.cfg.qk_norm:
+            fusible = self._plain_norms(RMSNorm, self.q_norm, self.k_norm)
         if fusible and x.is_cuda:
             from nanonemo_amd.kernels.hip import layers
 
             call = (x, cos, sin, self.H, self.KVH)
             ws = (self.wq, self.wk, self.wv, self.wo)
-            if layers.can_fuse(*call, self.hd, *ws):  # the whole layer in this build's kernels, as one autograd node
-                return layers.attention_layer(*call, *ws, packing)
+            norms, eps = ((self.q_norm.weight, self.k_norm.weight), self.q_norm.eps) if self.cfg.qk_norm else ((), 0.0)
+            if layers.can_fuse(*call, self.hd, *ws, norms):  # the whole layer in this build's kernels, as one autograd node
+                return layers.attention_layer(*call, *ws, packing, norms, eps)
         q, k, v = _project(self.cfg, x, self.wq, self.wk, self.wv)
         q = q.view(B, T, self.H, self.hd)
         k = k.view(B, T, self.KVH, self.hd)

@@ -293,3 +293,168 @@ def test_offsets_past_32_bits():
         assert torch.equal(a, b)
     for a, b in zip(outs[0][4:], outs[1][4:]):  # zeros add nothing; the fp32 sums' order goes by the size: 400 or 1200 terms
         torch.testing.assert_close(a, b, rtol=0, atol=1200 * 2**-24 * 4 * b.abs().max().item())
+
+
+def _layer(B, T, H, KVH, hd, lengths=None, **kw):
+    """An attention layer with norms, whose weights are not ones, and what it is called with beside x."""
+    from nanonemo_amd.kernels.hip.packed import Packing
+    from tests.test_layers_gpu import _attention
+
+    m, (cos, sin) = _attention(H, KVH, hd, T, rope_kernel="hip", qk_norm=True, **kw)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    with torch.no_grad():
+        for n in (m.q_norm, m.k_norm):
+            n.weight.copy_(1 + 0.3 * torch.randn(hd, device="cuda", generator=g))
+    if lengths is None:
+        return m, (cos, sin)
+    packing = Packing(lengths, H, KVH)
+    return m, (cos[packing.positions], sin[packing.positions], packing)
+
+
+def _layer64(x, cos, sin, H, KVH, eps, wq, wk, wv, wo, wqn, wkn):
+    _, T, _ = x.shape
+    c, s = cos[:T, None].double(), sin[:T, None].double()
+
+    def rot(t, w):
+        a, b = (w * t / torch.sqrt(t.square().mean(-1, keepdim=True) + eps)).chunk(2, -1)
+        return torch.cat((a * c - b * s, a * s + b * c), -1).transpose(1, 2)
+
+    q, k, v = ((x @ w.t()).view(*x.shape[:2], h, -1) for w, h in ((wq, H), (wk, KVH), (wv, KVH)))
+    q, k, v = rot(q, wqn), rot(k, wkn), v.transpose(1, 2)
+    k, v = (t.repeat_interleave(H // KVH, 1) for t in (k, v))
+    future = torch.ones(T, T, dtype=torch.bool, device=x.device).triu(1)
+    p = ((q @ k.transpose(2, 3).contiguous()) / q.shape[-1] ** 0.5).masked_fill(future, -float("inf")).softmax(-1)
+    return (p @ v).transpose(1, 2).reshape(*x.shape[:2], -1) @ wo.t()
+
+
+def _parts(m):
+    return m.wq.weight, m.wk.weight, m.wv.weight, m.wo.weight, m.q_norm.weight, m.k_norm.weight
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B, T, H, KVH, hd, lengths", [(2, 200, 12, 4, 64, None), (3, 65, 2, 2, 64, None), (1, 700, 8, 2, 32, None),
+                                                       (1, 458, 12, 4, 64, [100, 1, 260, 0, 64, 33]), (1, 196, 4, 1, 32, [130, 1, 65])])
+def test_attention_layer_with_norms_matches_float64(B, T, H, KVH, hd, lengths, dtype):
+    from tests.test_layers_gpu import _modules_only, _rel
+
+    print(f"\n[case] attention layer with norms B={B} T={T} H={H} KVH={KVH} hd={hd} {lengths} {dtype}", flush=True)
+    m, more = _layer(B, T if lengths is None else max(lengths), H, KVH, hd, lengths)
+    x = torch.randn(B, T, H * hd, device="cuda").to(dtype).requires_grad_()
+    dy = torch.randn(B, T, H * hd, device="cuda").to(dtype)
+
+    def run(mod):
+        with torch.autocast("cuda", dtype=dtype):
+            y = mod(x, *more)
+        return y, (y.detach(), *torch.autograd.grad(y, (x, *_parts(mod)), dy))
+
+    y, got = run(m)
+    node = y.grad_fn
+    while "View" in node.name():
+        node = node.next_functions[0][0]
+    assert node.name() == "_AttentionLayerBackward"
+    ref = run(_modules_only(m))[1]
+    ins = [t.detach().double().requires_grad_() for t in (x, *_parts(m))]
+    if lengths is None:
+        y = _layer64(ins[0], *more, H, KVH, m.q_norm.eps, *ins[1:])
+    else:
+        i = lengths.index(max(lengths))
+        c, s = (t.split(lengths)[i] for t in more[:2])
+        y = torch.cat([_layer64(t, c, s, H, KVH, m.q_norm.eps, *ins[1:]) for t in ins[0].split(lengths, 1) if t.shape[1]], 1)
+    exact = (y.detach(), *torch.autograd.grad(y, ins, dy.double()))
+    # The 16-bit roundings on the longest path, each of u in the 2-norm, as the layer without norms has them (the norm rounds with
+    # the rotation): weights, product, rotation of q and of k; P and O; the output weight, dO, dS, dq or dk, its rotation. And no
+    # term may be worse than in the modules, which round more; but the 2-norm of n independent errors of equal size is itself only
+    # within 1 / sqrt(2 n) of its mean (one standard deviation), the ratio of two within 1 / sqrt(n): four of those are allowed, 0.5
+    # for the norms' 64 weights and 0.01 for the other tensors.
+    u = 2.0**-8 if dtype == torch.bfloat16 else 2.0**-11
+    for name, a, b, e in zip(("y", "dx", "dwq", "dwk", "dwv", "dwo", "dq_norm", "dk_norm"), got, ref, exact):
+        mine, theirs = _rel(a, e), _rel(b, e)
+        print(f"  {name}: {mine:.2e}, modules {theirs:.2e}, bound {13**0.5 * u:.2e}", flush=True)
+        assert mine <= 13**0.5 * u, name
+        assert mine <= (1.1 + 4 * a.numel() ** -0.5) * theirs, name
+    with torch.no_grad(), torch.autocast("cuda", dtype=dtype):
+        assert torch.equal(m(x, *more), got[0])
+
+
+@pytest.mark.parametrize("lengths", [None, [70, 30, 40]])
+def test_attention_layer_with_norms_frozen_parts_and_repeated_backward(lengths):
+    m, more = _layer(1, 140, 4, 2, 64, lengths)
+    x = torch.randn(1, 140, 256, device="cuda", requires_grad=True)  # fp32 in, cast by the layer
+
+    def loss():
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            return m(x, *more).float().square().sum()
+
+    y = loss()
+    y.backward(retain_graph=True)
+    all_ = (x, *_parts(m))
+    first = [t.grad.clone() for t in all_]
+    y.backward()
+    for a, t in zip(first, all_):
+        assert torch.equal(a + a, t.grad)
+    for i in range(len(all_)):  # each alone: the others' gradients are not formed
+        for j, t in enumerate(all_):
+            t.requires_grad_(i == j)
+        (g,) = torch.autograd.grad(loss(), all_[i])
+        assert torch.equal(g, first[i]), i
+
+
+@pytest.mark.parametrize("lengths", [None, [20, 13]])
+def test_attention_layer_with_norms_recorded_backward(lengths):
+    from tests.test_layers_gpu import _modules_only
+
+    m, more = _layer(1, 33, 4, 2, 32, lengths)
+    x = torch.randn(1, 33, 128, device="cuda", requires_grad=True)
+    out = []
+    for mod in (m, _modules_only(m)):
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            y = mod(x, *more)
+        gs = torch.autograd.grad(y.float().sum(), (x, *_parts(mod)), create_graph=True)
+        out.append([*(g.detach() for g in gs), *torch.autograd.grad(gs[4].square().sum(), x)])  # (through wo's gradient)
+    for a, b in zip(*out):
+        torch.testing.assert_close(a, b, rtol=5e-2, atol=5e-2 * b.abs().max().item())
+
+
+def test_norms_with_hooks_are_called():
+    """A hook on a head norm, another norm in its place, or its weight in another type, runs as a module."""
+    from nanonemo_amd.model import RMSNorm
+
+    m, more = _layer(1, 40, 4, 2, 64)
+    x = torch.randn(1, 40, 256, device="cuda").bfloat16()
+
+    def run():
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+            return m(x, *more)
+
+    plain, seen = run(), []
+    h = m.k_norm.register_forward_hook(lambda _, ins, out: seen.append(out.shape))
+    hooked = run()
+    assert seen == [(1, 40, 2, 64)]
+    h.remove()
+    u = 2.0**-8  # one rounding more of q and of k: each of their scores' terms and its sum at random
+    assert (hooked.float() - plain.float()).norm() <= 4 * u * plain.float().norm()
+    assert torch.equal(run(), plain)
+
+    class Half(RMSNorm):
+        def forward(self, t):
+            return 0 * super().forward(t)
+
+    m.q_norm = Half(64, 1e-5).cuda()
+    uniform = run()  # queries of zeros: the mean of the values so far
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        v = m.wv(x).view(1, 40, 2, 64).float()
+        mean = (v.cumsum(1) / torch.arange(1, 41, device="cuda").view(1, 40, 1, 1)).repeat_interleave(2, 2).bfloat16()
+        want = m.wo(mean.view(1, 40, 256)).float()
+    assert (uniform.float() - want).norm() <= 3 * u * want.norm()
+
+
+def test_attention_layer_with_norms_refuses_norms_of_other_sizes():
+    from nanonemo_amd.kernels.hip import host
+
+    m, (cos, sin) = _layer(1, 40, 4, 2, 64)
+    x = torch.randn(40, 256, device="cuda").bfloat16()
+    call = (x, cos, sin, 1, 40, 4, 2, m.wq.weight, m.wk.weight, m.wv.weight, m.wo.weight, False, None, None)
+    good = m.q_norm.weight
+    for bad in ((good[:32], good), (good, good.half()), (good.cpu(), good), (good, None)):
+        with pytest.raises(RuntimeError):
+            host().attention_layer_fwd(*call, *bad, 1e-5)
