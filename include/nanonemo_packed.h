@@ -11,7 +11,8 @@
  *
  * rest: tokens * H * D bytes, or null. The forward writes into it what rounding o to 16 bits took off each value, in 8 bits, and
  * a backward that is given it computes D = rowsum(dO * o) from both: dq and dk then carry the rounding of dS and their own, and
- * none of o's. Without it dq is the same bits as nn_fa_bwd's.
+ * none of o's. Without it dq is the same bits as nn_fa_bwd's. (Sequences that the plan gives to a wave as one tile of 32 rows need
+ * none: their rests are left as they were, and D is formed in the backward.)
  *
  * The work is laid out once for a batch, on the host: nn_fa_packed_plan fills `plan` (int32 words, in host memory), which the
  * caller copies to the device as it is (16-byte aligned) and keeps while it uses it, in both places. Its layout is the

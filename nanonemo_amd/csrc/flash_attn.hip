@@ -196,7 +196,7 @@ __device__ inline float sub_rn(float a, float b) {
 // problem of its own to the kernels below: what a block works on, and where its sequence lies, is one entry of a list that the
 // host laid out and sorted (nn_fa_packed_plan), the tensors' pointers move to the sequence's first row, T is its length, and
 // the loops, masks and sums are those of the dense kernels. So a sequence's o and lse are the same bits as a dense call's on it
-// alone (without rests, below, its dq too, and dk and dv where the same blocks share the work).
+// alone (without rests, below, its dq too, and dk and dv where the same blocks share the work; sequences of one tile aside).
 struct PackedTile {  // forward and dQ: 128 query rows of one sequence, for the query heads of one KV head
     int start, len, qb, kvh;  // len 0: nothing to do (the list is padded to a multiple of 8)
 };
@@ -1477,8 +1477,8 @@ __global__ __launch_bounds__(256, 2) void fa_bwd_dq_kernel(const u16* __restrict
 // Packed sequences of up to kShort tokens: one wave for each 32 query rows of a head (forward, dQ), one for each 32 keys of a KV
 // head (dK/dV). A block of the kernels above carries 128 rows and its barriers for them: 7872 blocks of 24 tokens on average
 // took 44 us, mostly latency, where these waves, independent of each other and more of them to a CU, take 17 (5.2 TB/s; the
-// backward 54 instead of 89, of which the rests are 4). The arithmetic of a row is that of the kernels above in the same order,
-// so its bits are too (dk and dv: sums over the group's heads in one wave instead of four).
+// backward 44 instead of 89). The arithmetic of a row is that of the kernels above in the same order, so its bits are too (dk and
+// dv: sums over the group's heads in one wave instead of four; but for the backward of one tile, below).
 // Operands that need rows come straight from memory in their lanes' layout, those that need columns through the wave's own LDS
 // tile by DMA, whose rows past the sequence read as zeros. List entries: PackedTile with qb = the 32-row tile.
 // ------------------------------------------------------------------------------------------
@@ -1610,32 +1610,155 @@ __global__ __launch_bounds__(256, 4) void fa_short_fwd_kernel(const u16* __restr
             }
     }
     const float ltot = pair_sum(lsum);
-    if (pk.rest && qrow < T) store_row<HD, DT>(oacc, 1.f / ltot, hh, nullptr, pk.rest + ((size_t)(e.start + qrow) * H + h) * (HD / 4));
+    if (pk.rest && T > 32 && qrow < T) store_row<HD, DT>(oacc, 1.f / ltot, hh, nullptr, pk.rest + ((size_t)(e.start + qrow) * H + h) * (HD / 4));
     store_rows<HD, DT>(oacc, 1.f / ltot, vb, O + lo.at(0, h) + (size_t)(e.start + 32 * e.qb) * lo.st, lo.st, T - 32 * e.qb, lane);
     if (LSE && hh == 0 && qrow < T) LSE[(size_t)h * pk.tokens + e.start + qrow] = (mb + fast_log2(ltot)) * kLn2;
 }
 
-// Waves 0 .. count KVH - 1: dk and dv of 32 keys; the next count H: dq of 32 rows. Either computes D for its rows itself.
+// Backward, sequences of one tile (up to 32 tokens): a wave for each of them and KV head computes all of dq, dk and dv. With all keys of
+// a row at hand, D = rowsum(p * dp) and p's own sum, 1 but for the forward's rounding of p before it summed them, are formed in
+// fp32. rowsum(dO * o), whose o comes of rounded p, is less near: dq and dk of such sequences were 1.48 to 1.55 single roundings off
+// the formula's, and are 1.41 to 1.45, which is what dS's and their own come to. Neither o nor its rests are read, nor written for
+// them. For each head:
+//   S^T = K Q^T, dP^T = V dO^T     (lane: a query row)     P, D, dS^T
+//   S = Q K^T, dP = dO V^T         (lane: a key)           P, dS
+//   dV^T += dO^T P, dK^T += Q^T dS, dQ^T = K^T dS^T
+// Products are repeated rather than turned round: 28 matrix instructions a head take a fifth of its bytes' time. 16384 tokens in 1006
+// sequences: 28.4 us (4.7 TB/s) where the waves below took 52; 65536 in 11964 227 for 481. (Sequences of two tiles in the same
+// way, a wave a tile: 81 us for 52, more rows for each wave one after another and no registers for them.)
+// lds: K; Q and dO of this head and of the next.
 template <int HD, int DT>
-__global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restrict__ Q, const u16* __restrict__ K, const u16* __restrict__ V,
-                                                              const u16* __restrict__ O, const u16* __restrict__ dO, const float* __restrict__ LSE,
-                                                              u16* __restrict__ dQ, u16* __restrict__ dK, u16* __restrict__ dV, Packed pk, int H, int KVH,
-                                                              float sl2, float scale, Lay lq, Lay lk, Lay lo, Lay ldq, Lay ldk) {
+__device__ __forceinline__ void one_tile_bwd(int item, u16* lds, const u16* __restrict__ Q, const u16* __restrict__ K,
+                                             const u16* __restrict__ V, const u16* __restrict__ dO, const float* __restrict__ LSE,
+                                             u16* __restrict__ dQ, u16* __restrict__ dK, u16* __restrict__ dV, const Packed& pk, int H, int KVH,
+                                             float sl2, float scale, const Lay& lq, const Lay& lk, const Lay& ldq, const Lay& ldk) {
     using E = Elem<DT>;
     constexpr int NS = HD / 16, ND = HD / 32, TILE = 32 * HD;
-    __shared__ __attribute__((aligned(16))) u16 tS[4 * 4 * TILE];  // per wave: two Q and two dO tiles, or the K rows
-    __shared__ __attribute__((aligned(16))) float vecS[4 * 64];    // per wave: -lse/scale | -D
-    const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5, g16 = (lane >> 4) & 1;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = H / KVH;
-    int item = (int)blockIdx.x * 4 + wave;
-    const bool keys = item < pk.count * KVH;
-    if (!keys) item -= pk.count * KVH;
-    const int per = keys ? KVH : H, at = item / per;
+    const int lane = threadIdx.x, l32 = lane & 31, hh = lane >> 5, g16 = (lane >> 4) & 1, group = H / KVH;
+    const int at = item / KVH, kvh = item - at * KVH;
     if (at >= pk.count) return;
+    const PackedTile e = static_cast<const PackedTile*>(pk.list)[at];
+    if (e.len > 32 || !inside(pk, e.start, e.len, 0, KVH, e.qb, 32)) return;
+    const int T = e.len, last = min(l32, T - 1);
+    int roff[NS], coff[ND][2];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) roff[s] = row_off<HD>(l32, 16 * s + 8 * hh);
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) coff[dt][x] = col_off<HD>(8 * x + 4 * hh, 32 * dt + 16 * g16, lane);
+    const size_t koff = lk.at(0, kvh) + (size_t)e.start * lk.st, row = koff + (size_t)last * lk.st + 8 * hh;
+    const DmaOffs<HD, 32, 1> fo = dma_offsets<HD, 32, 1>(lane, 0, lq.st), ko = dma_offsets<HD, 32, 1>(lane, 0, lk.st);
+    u16x8 kf[NS], vf[NS];  // (keys past T: the last's, masked or not stored)
+#pragma unroll
+    for (int s = 0; s < NS; ++s) kf[s] = ld8(K + row + 16 * s), vf[s] = ld8(V + row + 16 * s);
+    dma_rows<HD, 32, 1>(K + koff, lk.st, 0, T, lds, 0, ko);
+    float lse = 0.f;
+    auto fetch = [&](int g) {  // Q, dO and lse of the group's head g
+        const int h = kvh * group + g;
+        u16* to = lds + (1 + (g & 1) * 2) * TILE;
+        const size_t off = lq.at(0, h) + (size_t)e.start * lq.st;
+        dma_rows<HD, 32, 1>(Q + off, lq.st, 0, T, to, 0, fo);
+        dma_rows<HD, 32, 1>(dO + off, lq.st, 0, T, to + TILE, 0, fo);
+        lse = LSE[(size_t)h * pk.tokens + e.start + last];
+    };
+    f32x16 dk[ND], dv[ND];
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) dk[dt] = dv[dt] = f32x16{};
+    const int lim = last - 4 * hh;  // (lane: a row) key offsets beyond this are masked
+    const float per = 1.f / sl2;
+    fetch(0);
+    for (int g = 0; g < group; ++g) {
+        copies_landed();
+        u16* qt = lds + (1 + (g & 1) * 2) * TILE;
+        const u16* ot = qt + TILE;
+        u16x8 qa[NS], oa[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qa[s] = ld8(qt + roff[s]), oa[s] = ld8(ot + roff[s]);
+        const float nl2 = -lse * kLog2e;
+        if (g + 1 < group) fetch(g + 1);
+        f32x16 p = f32x16{}, dp = f32x16{};
+#pragma unroll
+        for (int ks = 0; ks < NS; ++ks) {
+            p = E::mfma(kf[ks], qa[ks], p);
+            dp = E::mfma(vf[ks], oa[ks], dp);
+        }
+        float d = 0.f, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            p[i] = (i >> 2) * 8 + (i & 3) > lim ? 0.f : fast_exp2(fmaf(p[i], sl2, nl2));
+            d = fmaf(p[i], dp[i], d), l += p[i];
+        }
+        l = pair_sum(l);
+        const float inv = 1.f / l;
+        d = pair_sum(d) * inv;
+        u16x8 sf[2];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dp[i] = p[i] * inv * (dp[i] - d);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) sf[half] = pack8<DT>(dp, 8 * half);
+        const int nls = __float_as_int(l32 < T ? (nl2 - fast_log2(l)) * per : -INFINITY), nd = __float_as_int(l32 < T ? -d : 0.f);  // (p of rows past T: 0)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {  // row (i / 4) * 8 + 4 hh + i % 4's, from its lane
+            const int from = 4 * ((i >> 2) * 8 + (i & 3)) + 16 * hh;
+            p[i] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, nls));
+            dp[i] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, nd));
+        }
+#pragma unroll
+        for (int ks = 0; ks < NS; ++ks) {
+            p = E::mfma(qa[ks], kf[ks], p);
+            dp = E::mfma(oa[ks], vf[ks], dp);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            p[i] = fast_exp2(((i >> 2) * 8 + (i & 3) >= l32 - 4 * hh ? p[i] : -INFINITY) * sl2);  // (lane: a key) rows before it see none of it
+            dp[i] *= p[i];
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const u16x8 pf = pack8<DT>(p, 8 * half), df = pack8<DT>(dp, 8 * half);
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) {
+                const u16 *oc = ot + half * 16 * HD, *qc = qt + half * 16 * HD;
+                dv[dt] = E::mfma(cat4(ld_tr(oc + coff[dt][0]), ld_tr(oc + coff[dt][1])), pf, dv[dt]);
+                dk[dt] = E::mfma(cat4(ld_tr(qc + coff[dt][0]), ld_tr(qc + coff[dt][1])), df, dk[dt]);
+            }
+        }
+        f32x16 dq[ND];
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) dq[dt] = f32x16{};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const u16* kc = lds + half * 16 * HD;
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) dq[dt] = E::mfma(cat4(ld_tr(kc + coff[dt][0]), ld_tr(kc + coff[dt][1])), sf[half], dq[dt]);
+        }
+        // (through the Q tile, which has been read)
+        store_rows<HD, DT>(dq, scale, qt, dQ + ldq.at(0, kvh * group + g) + (size_t)e.start * ldq.st, ldq.st, T, lane);
+    }
+    const size_t off = ldk.at(0, kvh) + (size_t)e.start * ldk.st;
+    store_rows<HD, DT>(dk, scale, lds, dK + off, ldk.st, T, lane);
+    store_rows<HD, DT>(dv, 1.f, lds + TILE, dV + off, ldk.st, T, lane);
+}
+
+// Backward, sequences of two tiles. Of the first `pairs` entries of the list, items 0 .. pairs KVH - 1: dk and dv of 32 keys; the
+// next pairs H: dq of 32 rows. Either computes D for its rows itself.
+template <int HD, int DT>
+__device__ __forceinline__ void two_tile_bwd(int item, int pairs, u16* lds, const u16* __restrict__ Q, const u16* __restrict__ K,
+                                             const u16* __restrict__ V, const u16* __restrict__ O, const u16* __restrict__ dO,
+                                             const float* __restrict__ LSE, u16* __restrict__ dQ, u16* __restrict__ dK, u16* __restrict__ dV,
+                                             const Packed& pk, int H, int KVH, float sl2, float scale, const Lay& lq, const Lay& lk, const Lay& lo,
+                                             const Lay& ldq, const Lay& ldk) {
+    using E = Elem<DT>;
+    constexpr int NS = HD / 16, ND = HD / 32, TILE = 32 * HD;
+    float* vec = reinterpret_cast<float*>(lds + 4 * TILE);  // lds: two Q and two dO tiles, or the K rows; -lse/scale | -D
+    const int lane = threadIdx.x, l32 = lane & 31, hh = lane >> 5, g16 = (lane >> 4) & 1, group = H / KVH;
+    const bool keys = item < pairs * KVH;
+    if (!keys) item -= pairs * KVH;
+    const int per = keys ? KVH : H, at = item / per;
     const PackedTile e = static_cast<const PackedTile*>(pk.list)[at];
     if (e.len > kShort || !inside(pk, e.start, e.len, 0, KVH, e.qb, 32)) return;
     const int T = e.len, tile = e.qb;
-    u16* lds = tS + wave * 4 * TILE;
     int roff[NS], coff[ND][2];
 #pragma unroll
     for (int s = 0; s < NS; ++s) roff[s] = row_off<HD>(l32, 16 * s + 8 * hh);
@@ -1680,7 +1803,6 @@ __global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restr
         f32x16 dk[ND], dv[ND];
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) dk[dt] = dv[dt] = f32x16{};
-        float* vec = vecS + wave * 64;
         fetch(0);
         for (int it = 0; it < n; ++it) {
             copies_landed();
@@ -1772,6 +1894,24 @@ __global__ __launch_bounds__(256, 2) void fa_short_bwd_kernel(const u16* __restr
             }
         }
         store_rows<HD, DT>(dq, scale, lds + 2 * TILE, dQ + ldq.at(0, h) + (size_t)(e.start + 32 * tile) * ldq.st, ldq.st, T - 32 * tile, lane);
+    }
+}
+
+// A wave an item, a block a wave: those of two tiles first, which take longer. 16384 tokens in 678 sequences of 24 on average 44 us.
+// (A launch for each kind: 52; 4096 tokens in 135 sequences 26 us for 17.)
+template <int HD, int DT>
+__global__ __launch_bounds__(64, 2) void fa_short_bwd_kernel(const u16* __restrict__ Q, const u16* __restrict__ K, const u16* __restrict__ V,
+                                                             const u16* __restrict__ O, const u16* __restrict__ dO, const float* __restrict__ LSE,
+                                                             u16* __restrict__ dQ, u16* __restrict__ dK, u16* __restrict__ dV, Packed pk, int pairs,
+                                                             int H, int KVH, float sl2, float scale, Lay lq, Lay lk, Lay lo, Lay ldq, Lay ldk) {
+    __shared__ __attribute__((aligned(16))) u16 lds[5 * 32 * HD];  // 20 KB: eight blocks to a CU
+    const int item = (int)blockIdx.x, first = pairs * (H + KVH);
+    if (item < first) {
+        two_tile_bwd<HD, DT>(item, pairs, lds, Q, K, V, O, dO, LSE, dQ, dK, dV, pk, H, KVH, sl2, scale, lq, lk, lo, ldq, ldk);
+    } else {
+        Packed rest = pk;
+        rest.list = static_cast<const PackedTile*>(pk.list) + pairs, rest.count = pk.count - pairs;
+        one_tile_bwd<HD, DT>(item - first, lds, Q, K, V, dO, LSE, dQ, dK, dV, rest, H, KVH, sl2, scale, lq, lk, ldq, ldk);
     }
 }
 
@@ -2330,7 +2470,8 @@ struct PlanHead {
     int32_t wpp;                    // waves per entry of the dK/dV list: 1 or 4
     int32_t tiles, units, sums, positions;  // words where they begin
     int32_t nshort, shorts;                 // 32-row tiles of the short sequences, and the word where they begin
-    int32_t unused[14];
+    int32_t npairs;                         // of these the first, of sequences of two tiles
+    int32_t unused[13];
 };
 static_assert(sizeof(PlanHead) == 128 && offsetof(PlanHead, positions) == 4 * NN_FA_PACKED_POSITIONS, "32 words");
 
@@ -2361,7 +2502,7 @@ constexpr int64_t kShortWaves = 1024;
 
 struct PlanSize {
     PlanRule rule;
-    int64_t tokens = 0, longest = 0, ntiles = 0, nunits = 0, nsums = 0, nslots = 0, nshort = 0;
+    int64_t tokens = 0, longest = 0, ntiles = 0, nunits = 0, nsums = 0, nslots = 0, nshort = 0, npairs = 0;
     int64_t padded() const { return (ntiles + 7) / 8 * 8; }
     int64_t words() const { return 32 + 4 * (padded() + nshort) + 8 * (nunits + nsums) + tokens; }
 };
@@ -2371,17 +2512,17 @@ int plan_size(const int64_t* lengths, int64_t n, int64_t H, int64_t KVH, PlanSiz
     if (n < 0 || (n > 0 && !lengths)) return fail(-1, "invalid list of lengths");
     if (int e = check_dims(1, H, KVH, 1, 64, kBF16)) return e;
     PlanSize z;
-    int64_t pairs = 0, units = 0, work = 0, few = 0;
+    int64_t pairs = 0, units = 0, work = 0, few = 0, two = 0;
     const int64_t g = H / KVH;
     for (int64_t i = 0; i < n; ++i) {
         const int64_t len = lengths[i];
         if (len < 0) return fail(-1, "sequence %lld has the length %lld", (long long)i, (long long)len);
         if (len >= (int64_t)1 << 30 || (z.tokens += len) >= (int64_t)1 << 30) return fail(-1, "sizes too large");
         z.longest = std::max(z.longest, len);
-        if (len <= kShort) few += (len + 31) / 32;
+        if (len <= kShort) few += (len + 31) / 32, two += len > 32 ? 2 : 0;
     }
     const int64_t upto = z.longest <= kShort || few * H >= kShortWaves ? kShort : 0;
-    if (upto) z.nshort = few;
+    if (upto) z.nshort = few, z.npairs = two;
     for (int64_t i = 0; i < n; ++i) {
         const int64_t len = lengths[i];
         if (len <= upto) continue;
@@ -2482,9 +2623,10 @@ int packed_bwd_impl(const void* dO, const void* q, const void* k, const void* v,
                     const Workspace& w, const PlanHead& p, const int32_t* dp, float scale, const Lays& l, hipStream_t st) {
     const int g = p.H / p.KVH;
     if (p.nshort) {
-        fa_short_bwd_kernel<HD, DT><<<dim3((unsigned)(((int64_t)p.nshort * (p.H + p.KVH) + 3) / 4)), dim3(256), 0, st>>>(
+        const int64_t items = (int64_t)p.npairs * (p.H + p.KVH) + (int64_t)(p.nshort - p.npairs) * p.KVH;
+        fa_short_bwd_kernel<HD, DT><<<dim3((unsigned)items), dim3(64), 0, st>>>(
             (const u16*)q, (const u16*)k, (const u16*)v, (const u16*)o, (const u16*)dO, lse, (u16*)dq, (u16*)dk, (u16*)dv,
-            Packed{dp + p.shorts, p.nshort, p.tokens, p.longest, p.nslots, rest}, p.H, p.KVH, scale * kLog2e, scale, l.q, l.k, l.o, l.dq, l.dk);
+            Packed{dp + p.shorts, p.nshort, p.tokens, p.longest, p.nslots, rest}, p.npairs, p.H, p.KVH, scale * kLog2e, scale, l.q, l.k, l.o, l.dq, l.dk);
         if (int e = launch_status("fa_short_bwd_kernel")) return e;
     }
     if (p.ntiles == 0) return 0;
@@ -2527,7 +2669,7 @@ NNFA_API int nn_fa_packed_plan(const int64_t* lengths, int64_t n, int64_t H, int
     p.magic = kPlanMagic, p.words = (int32_t)words, p.n = (int32_t)std::min<int64_t>(n, INT32_MAX), p.H = (int32_t)H, p.KVH = (int32_t)KVH;
     p.tokens = (int32_t)z.tokens, p.longest = (int32_t)z.longest;
     p.ntiles = (int32_t)z.padded(), p.nunits = (int32_t)z.nunits, p.nsums = (int32_t)z.nsums, p.nslots = (int32_t)z.nslots, p.wpp = r.wpp;
-    p.nshort = (int32_t)z.nshort;
+    p.nshort = (int32_t)z.nshort, p.npairs = (int32_t)z.npairs;
     p.tiles = 32, p.units = p.tiles + 4 * p.ntiles, p.sums = p.units + 8 * p.nunits, p.shorts = p.sums + 8 * p.nsums;
     p.positions = p.shorts + 4 * p.nshort;
     memcpy(plan, &p, sizeof p);
@@ -2558,7 +2700,9 @@ NNFA_API int nn_fa_packed_plan(const int64_t* lengths, int64_t n, int64_t H, int
     std::sort(tile0, tile, [](const PackedTile& a, const PackedTile& b) {
         return a.qb != b.qb ? a.qb > b.qb : a.start != b.start ? a.start < b.start : a.kvh < b.kvh;
     });
-    std::sort(few0, few, [](const PackedTile& a, const PackedTile& b) { return a.qb != b.qb ? a.qb > b.qb : a.start < b.start; });
+    std::sort(few0, few, [](const PackedTile& a, const PackedTile& b) {
+        return (a.len > 32) != (b.len > 32) ? a.len > 32 : a.qb != b.qb ? a.qb > b.qb : a.start < b.start;
+    });
     std::sort(unit0, unit, [&](const PackedUnit& a, const PackedUnit& b) {
         const int64_t wa = r.iters((a.len + 63) / 64, a.pj) * b.nsplit, wb = r.iters((b.len + 63) / 64, b.pj) * a.nsplit;
         if (wa != wb) return wa > wb;

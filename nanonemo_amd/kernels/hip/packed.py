@@ -10,7 +10,8 @@ token attends to its own sequence up to itself. The reference's model has batche
 A ``Packing`` holds how the kernels share the work out, on the host and on the device: tiles and units of the longest
 sequences first, long ones split where they would outlast the others. The kernels are the dense attention's, so a sequence's
 output is the same bits as flash_attn's on it alone, and everything is deterministic. The gradients are nearer to the formula's
-than the dense ones: the forward keeps what rounding its output to 16 bits took off, one byte a value, for rowsum(dO * o).
+than the dense ones: the forward keeps what rounding its output to 16 bits took off, one byte a value, for rowsum(dO * o) (where
+a wave has a sequence's whole rows in the backward, up to 32 tokens, it keeps nothing: those bytes are left as they were).
 
 fp16 or bf16, head_dim 32 or 64, sequences of 0 to 2^30 / (H hd) tokens. Once differentiable, in reverse mode (a tangent is
 refused); capturing a call that autograd records into a HIP graph is refused, as the dense attention's is; without autograd it
