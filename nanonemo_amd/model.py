@@ -214,6 +214,8 @@ class Attention(nn.Module):
 
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, packing=None) -> torch.Tensor:
         B, T, _ = x.shape
+        if packing is not None and (B != 1 or len(cos) != T or len(sin) != T):
+            raise ValueError(f"a packing's tokens are one row, with a row of cos and sin for each, not {B} rows of {T} with {len(cos)}")
         fusible = self.cfg.attn_kernel == "hip_bthd" and self.cfg.rope_kernel != "torch"
         if fusible and self.cfg.qk_norm:
             fusible = self._plain_norms(RMSNorm, self.q_norm, self.k_norm)

@@ -303,6 +303,24 @@ def test_a_packing_without_tokens_is_refused_by_the_model():
             model(torch.zeros(1, 0, dtype=torch.long), None, None, model.pack(lengths))
 
 
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_a_packed_attention_layer_takes_one_row_and_its_tokens_tables(qk_norm):
+    """Two rows would take the tables' first rows each, whole tables those of a single sequence."""
+    from nanonemo_amd.model import Attention, ModelConfig, rope_tables
+
+    torch.manual_seed(0)
+    m = Attention(ModelConfig(**SMALL, qk_norm=qk_norm))
+    lengths = [13, 7]
+    packing, x = _packing(lengths, 4, 2), torch.randn(1, 20, 128)
+    tables = rope_tables(32, 64, 10000.0)
+    cos, sin = (t[packing.positions] for t in tables)
+    alone = torch.cat([m(t, *tables) for t in x.split(lengths, 1)], 1)
+    torch.testing.assert_close(m(x, cos, sin, packing), alone, rtol=1e-4, atol=1e-5)
+    for bad in ((x.view(2, 10, 128), cos, sin), (x, *tables), (x, cos, tables[1]), (x, cos[:19], sin[:19])):
+        with pytest.raises(ValueError, match="one row, with a row of cos and sin for each"):
+            m(*bad, packing)
+
+
 def test_a_plan_cut_short_is_refused():
     from nanonemo_amd.kernels.hip import host
     from nanonemo_amd.kernels.hip.packed import Packing
