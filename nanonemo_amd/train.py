@@ -58,6 +58,8 @@ def teacher_batches(teacher, batches, k: int, temperature: float = 2.0, weight: 
     suit the teacher's heads too."""
     out = []
     for x, y, *more in batches:
+        if more and more[0] is not None:
+            raise ValueError("a micro-batch has a teacher already")
         with torch.autocast(x.device.type, dtype=amp_dtype, enabled=amp_dtype is not None):
             out.append((x, y, teacher.teach(x, k, temperature, weight, *more[1:]), *more[1:]))
     return out

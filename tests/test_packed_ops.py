@@ -352,3 +352,17 @@ def test_packed_batches():
     for some in (batches[:2], teacher_batches(model, batches[:2], 3, amp_dtype=None)):
         loss, norm = train_step(student, opt, some, amp_dtype=None)
         assert loss.isfinite() and norm > 0
+
+
+def test_a_micro_batch_that_has_a_teacher_gets_no_other():
+    from nanonemo_amd.model import ModelConfig, NanoNemo
+    from nanonemo_amd.train import packed_batches, synthetic_documents, teacher_batches
+
+    model = NanoNemo(ModelConfig(**SMALL))
+    packed = packed_batches(model, synthetic_documents(1, 80, 20, 97), 80)
+    x, y = (torch.randint(0, 97, (2, 16)) for _ in range(2))
+    for batches in ([(x, y)], [(x, y, None)], packed):
+        taught = teacher_batches(model, batches, 3, amp_dtype=None)
+        assert all(t[2].indices.shape == (*t[0].shape, 3) and t[3:] == b[3:] for t, b in zip(taught, batches))
+        with pytest.raises(ValueError, match="has a teacher already"):
+            teacher_batches(model, taught, 3, amp_dtype=None)
