@@ -200,7 +200,7 @@ class Attention(nn.Module):
                 q, k = self.q_norm(q), self.k_norm(k)
             return rope(q, cos, sin, seq_dim=1), rope(k, cos, sin, seq_dim=1)
         if self.cfg.qk_norm:
-            if self._plain_norms(RMSNorm, self.q_norm, self.k_norm):
+            if self.hd <= 256 and self._plain_norms(RMSNorm, self.q_norm, self.k_norm):  # (the kernel's limit)
                 return self._qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, eps=self.q_norm.eps)
             q, k = self.q_norm(q), self.k_norm(k)
         return self._rope_qk(q, k, cos, sin)  # in the projection layout, q and k in one launch

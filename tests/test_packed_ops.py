@@ -366,3 +366,20 @@ def test_a_micro_batch_that_has_a_teacher_gets_no_other():
         assert all(t[2].indices.shape == (*t[0].shape, 3) and t[3:] == b[3:] for t, b in zip(taught, batches))
         with pytest.raises(ValueError, match="has a teacher already"):
             teacher_batches(model, taught, 3, amp_dtype=None)
+
+
+@pytest.mark.parametrize("hd", [256, 272])
+def test_heads_past_the_norm_kernel_s_size_are_normalised_by_their_modules(hd):
+    """The rotation's kernel takes larger heads than the norm's with the rotation, whose calls they would make an error."""
+    from nanonemo_amd.model import Attention, ModelConfig, rope, rope_tables
+
+    torch.manual_seed(0)
+    sizes = dict(d_model=2 * hd, n_heads=2, n_kv_heads=1, d_ff=32, vocab_size=32, max_seq_len=9, qk_norm=True)
+    plain, m = Attention(ModelConfig(**sizes)), Attention(ModelConfig(**sizes, rope_kernel="hip"))
+    m.load_state_dict(plain.state_dict())
+    with_norm = []
+    m._rope_qk = lambda q, k, cos, sin: (rope(q, cos, sin, 1), rope(k, cos, sin, 1))  # (there is no GPU here)
+    m._qk_norm_rope = lambda q, k, wq, wk, cos, sin, eps: with_norm.append(hd) or m._rope_qk(m.q_norm(q), m.k_norm(k), cos, sin)
+    x, tables = torch.randn(2, 9, 2 * hd), rope_tables(hd, 9, 10000.0)
+    torch.testing.assert_close(m(x, *tables), plain(x, *tables), rtol=1e-5, atol=1e-6)
+    assert bool(with_norm) == (hd <= 256)
