@@ -383,3 +383,32 @@ def test_heads_past_the_norm_kernel_s_size_are_normalised_by_their_modules(hd):
     x, tables = torch.randn(2, 9, 2 * hd), rope_tables(hd, 9, 10000.0)
     torch.testing.assert_close(m(x, *tables), plain(x, *tables), rtol=1e-5, atol=1e-6)
     assert bool(with_norm) == (hd <= 256)
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_shares_of_split_pairs(seed):
+    """A pair's blocks keep 8 iterations (query head, query tile) each at least, and their shares of each of its units, in the
+    kernel's arithmetic, are the unit's iterations once. Pairs alone are split, and where that takes 64 iterations off a block."""
+    rng = random.Random(seed)
+    H, KVH = rng.choice([(12, 4), (4, 1), (8, 8), (16, 2), (1, 1), (12, 1)])
+    lengths = [rng.choice([2048, 4096, 8192, 20000])] + [rng.randint(1, rng.choice([100, 600, 2000])) for _ in range(rng.choice([0, 3, 30]))]
+    w, g = _plan(lengths, H, KVH), H // KVH
+    upto = 64 if w[16] else 0
+    # (query head, query tile) iterations of all units of 64 keys over 256 CUs
+    even = sum(g * nkb * (nkb + 1) // 2 * KVH for nkb in (-(-n // 64) for n in lengths if n > upto)) // 256
+    split = 0
+    for i in range(w[8]):
+        _, n, pj, _, ns, sidx, _, paired = w[w[13] + 8 * i : w[13] + 8 * i + 8]
+        nkb = -(-n // 64)
+        both = paired and nkb - 1 - pj > pj
+        units = [g * (nkb - pj)] + ([g * (pj + 1)] if both else [])
+        assert paired or ns == 1
+        if ns > 1:
+            split += sidx == 0
+            assert sum(units) // ns >= 8 and sum(units) - even >= 64
+        if sidx == 0:
+            for it in units:
+                shares = [(s * it // ns, (s + 1) * it // ns) for s in range(ns)]
+                assert shares[0][0] == 0 and shares[-1][1] == it and all(a[1] == b[0] and a[0] <= a[1] for a, b in zip(shares, shares[1:]))
+                assert (ns + 1) * it < 2**31
+    assert split == w[9]
