@@ -714,3 +714,59 @@ def test_gradients_of_short_sequences_carry_two_roundings_alone(most, dtype):
         print(f"  {name} of sequences of up to {most}, {dtype}: {(off / once).item():.3f} roundings, two are {(least / once).item():.3f}", flush=True)
         # (values between two steps, which fp32's errors of some 2^-22 send the other way, are one in 2^13 or fewer)
         assert off <= 1.02 * least, name
+
+
+@pytest.mark.parametrize("lengths", [[300, 1000, 5], [30] * 40 + [50] * 20, [700] * 60 + [20] * 400, [4096]])
+def test_a_list_that_was_overwritten_leaves_the_memory_around_the_tensors(lengths):
+    """What the kernels write lies side by side with rows of a pattern between: none of it changes, nor does what they read,
+    whatever the list holds (random words; the list's own, some of them one off or another entry's)."""
+    import ctypes
+
+    from nanonemo_amd.kernels.hip import check, lib
+
+    print(f"\n[case] overwritten list of {len(lengths)} sequences among guards", flush=True)
+    H, KVH, D = 12, 4, 64
+    ins = _inputs(lengths, H, KVH, D, torch.bfloat16, seed=16)
+    packing = _packing(lengths, H, KVH)
+    host, words, T, L = packing.plan_host.data_ptr(), len(packing.plan), sum(lengths), lib()
+    ws = L.nn_fa_packed_bwd_workspace_size(host, D)
+    q, kv = 2 * T * H * D, 2 * T * KVH * D
+    names = ("q", "k", "v", "do", "plan", "o", "lse", "rest", "dq", "dk", "dv", "ws")
+    sizes = dict(zip(names, (q, kv, kv, q, 4 * words, q, 4 * H * T, q // 2, q, kv, kv, ws)))
+    guard, at, end = 1 << 16, {}, 1 << 16
+    for n in names:
+        at[n] = end
+        end = (end + sizes[n] + guard + 255) // 256 * 256
+    memory = torch.full((end,), 0x5A, dtype=torch.uint8, device="cuda")
+    for n, t in zip(names, ins):
+        memory[at[n] : at[n] + sizes[n]] = t.flatten().view(torch.uint8)
+    # (everything but what the kernels may write, and the list)
+    kept = torch.ones(end, dtype=torch.bool, device="cuda")
+    for n in names[4:]:
+        kept[at[n] : at[n] + sizes[n]] = False
+    before = memory[kept]
+    a = {n: memory.data_ptr() + at[n] for n in names}
+    plan = memory[at["plan"] : at["plan"] + 4 * words].view(torch.int32)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def run():
+        s = ctypes.c_float(D**-0.5)
+        check(L.nn_fa_packed_fwd(a["q"], a["k"], a["v"], a["o"], a["lse"], a["rest"], host, a["plan"], D, None, 1, s, stream))
+        check(L.nn_fa_packed_bwd(a["do"], a["q"], a["k"], a["v"], a["o"], a["lse"], a["rest"], a["dq"], a["dk"], a["dv"], a["ws"], ws, host, a["plan"],
+                                 D, None, 1, s, stream))
+        torch.cuda.synchronize()
+
+    g = torch.Generator().manual_seed(17)
+    mine = packing.plan_host
+    lists = [torch.randint(low, high, mine.shape, generator=g).to(torch.int32)
+             for low, high in ((2**31 - 1, 2**31), (-1, 0), (0, 1), (-(2**31), 2**31), (-2, T + 3), (-1, 40), (0, 4))]
+    lists += [mine + torch.randint(-1, 2, mine.shape, generator=g, dtype=torch.int32) * (torch.rand(mine.shape, generator=g) < 0.2) for _ in range(4)]
+    lists += [torch.where(torch.rand(mine.shape, generator=g) < 0.2, mine[torch.randperm(words, generator=g)], mine) for _ in range(4)]
+    for i, bad in enumerate([*lists, mine]):
+        plan.copy_(bad)
+        run()
+        assert torch.equal(memory[kept], before), i
+        assert torch.equal(plan.cpu(), bad), i
+    want = _run(*ins, packing)
+    for n, t in zip(("o", "dq", "dk", "dv"), want):
+        assert torch.equal(memory[at[n] : at[n] + sizes[n]].view(torch.bfloat16), t.flatten()), n
