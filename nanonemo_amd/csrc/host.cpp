@@ -240,7 +240,7 @@ T3 bthd_bwd(const Tensor& d_o_, const Tensor& q_, const Tensor& k_, const Tensor
 }
 
 // The RoPE tables: float32 (T_max >= T, hd/2), on the inputs' GPU. Checked before any launch, since the library reads
-// them through raw device pointers (a host table would be read as device memory).
+// them through raw device pointers (a host table would be read as device memory), and at 16-byte boundaries (dense).
 void check_tables(const Tensor& cos, const Tensor& sin, int64_t T, int64_t D, c10::Device device) {
     need(cos.is_cuda() && sin.is_cuda() && cos.device() == device && sin.device() == device && cos.scalar_type() == at::kFloat &&
              sin.scalar_type() == at::kFloat && cos.sizes() == sin.sizes() && cos.dim() == 2 && cos.size(1) == D / 2 && cos.size(0) >= T,
@@ -253,7 +253,7 @@ T3 bthd_rope_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Ten
     check_attention(q, k, v, 1);
     const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3);
     check_tables(cos_, sin_, T, D, q.device());
-    const Tensor cos = contig(cos_), sin = contig(sin_);
+    const Tensor cos = dense(cos_), sin = dense(sin_);
     Tensor o = empty_of(q, q.sizes()), q_rot = empty_of(q, q.sizes()), lse = empty_f32(q, {B, H, T});
     if (empty_problem(q)) return {o, lse, q_rot};
     const c10::DeviceGuard guard(q.device());
@@ -268,7 +268,7 @@ T3 bthd_rope_bwd(const Tensor& d_o_, const Tensor& q_, const Tensor& k_, const T
     const Tensor d_o = contig(d_o_), q = contig(q_), k = contig(k_), v = contig(v_), o = contig(o_), lse = contig(lse_);
     check_backward(d_o, q, k, v, o, lse, 1);
     check_tables(cos_, sin_, q.size(1), q.size(3), q.device());
-    const Tensor cos = contig(cos_), sin = contig(sin_);
+    const Tensor cos = dense(cos_), sin = dense(sin_);
     const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3), KVH = k.size(2);
     Tensor dq = empty_of(q, q.sizes()), dk = empty_of(k, k.sizes()), dv = empty_of(v, v.sizes());
     if (empty_problem(q)) return {dq, dk, dv};
@@ -318,7 +318,7 @@ T2 rope(const Tensor& q_, const Tensor& k_, const Tensor& cos_, const Tensor& si
     need(cos_.scalar_type() == at::kFloat && sin_.scalar_type() == at::kFloat && cos_.sizes() == sin_.sizes() && cos_.dim() == 2 &&
              cos_.size(1) == D / 2 && cos_.size(0) >= T,
          "cos/sin must be float32 (T_max >= T, hd/2) tables");
-    const Tensor q = contig(q_), k = contig(k_), cos = contig(cos_), sin = contig(sin_);
+    const Tensor q = contig(q_), k = contig(k_), cos = dense(cos_), sin = dense(sin_);
     Tensor qo = empty_of(q, q.sizes()), ko = empty_of(k, k.sizes());
     if (q.numel() == 0 && k.numel() == 0) return {qo, ko};
     const c10::DeviceGuard guard(q.device());
@@ -549,14 +549,15 @@ struct LayerShape {
     }
 };
 
-std::vector<Tensor> attention_layer_fwd(const Tensor& x, const Tensor& cos, const Tensor& sin, int64_t B, int64_t T, int64_t H,
+std::vector<Tensor> attention_layer_fwd(const Tensor& x, const Tensor& cos_, const Tensor& sin_, int64_t B, int64_t T, int64_t H,
                                         int64_t KVH, const Tensor& wq, const Tensor& wk, const Tensor& wv, const Tensor& wo,
                                         bool turned, const OptTensor& plan, const OptTensor& plan_host, const OptTensor& q_norm,
                                         const OptTensor& k_norm, double eps) {
     const Inner inner;
     const c10::DeviceGuard guard(x.device());
     const LayerShape s(B, T, H, KVH, wq.size(0) / H, q_norm.has_value());
-    check_tables(cos, sin, T, s.D, x.device());
+    check_tables(cos_, sin_, T, s.D, x.device());
+    const Tensor cos = dense(cos_), sin = dense(sin_);
     if (s.normed) s.check_norms(x, q_norm, k_norm);
     const int dt = code(x);
     void* st = stream_of(x);
@@ -597,7 +598,7 @@ std::vector<OptTensor> attention_layer_bwd(const Tensor& dy_, const Tensor& x, c
     const c10::DeviceGuard guard(x.device());
     const LayerShape s(B, T, H, KVH, wo.size(1) / H, q_norm_.has_value());
     check_tables(cos_, sin_, T, s.D, x.device());
-    const Tensor cos = contig(cos_), sin = contig(sin_), lse = saved(lse_, x, {B, H, T}, at::kFloat);
+    const Tensor cos = dense(cos_), sin = dense(sin_), lse = saved(lse_, x, {B, H, T}, at::kFloat);
     const Tensor qkv = saved(qkv_, x, {B * T, s.nf}), q = saved(q_, x, {B * T, s.nq}), o = saved(o_, x, {B * T, s.nq});
     const int dt = code(x);
     void* st = stream_of(x);
@@ -625,7 +626,7 @@ std::vector<OptTensor> attention_layer_bwd(const Tensor& dy_, const Tensor& x, c
     }
     if (s.normed) {
         s.check_norms(x, q_norm_, k_norm_);
-        const Tensor q_norm = contig(*q_norm_), k_norm = contig(*k_norm_), dwq = at::empty_like(q_norm), dwk = at::empty_like(k_norm);
+        const Tensor q_norm = dense(*q_norm_), k_norm = dense(*k_norm_), dwq = at::empty_like(q_norm), dwk = at::empty_like(k_norm);
         const size_t n = nn_qk_norm_rope_bwd_workspace_size(B * T, H, KVH, s.D);
         Tensor ws = bytes(x, n);
         qkn_done(nn_qk_norm_rope_bwd(dqkv.data_ptr(), s.k(dqkv), qkv.data_ptr(), s.k(qkv), q_norm.data_ptr<float>(), k_norm.data_ptr<float>(),

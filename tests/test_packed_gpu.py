@@ -716,6 +716,75 @@ def test_gradients_of_short_sequences_carry_two_roundings_alone(most, dtype):
         assert off <= 1.02 * least, name
 
 
+def _shifted(t):
+    """The same values one element into a buffer, off the 16-byte boundaries of which the kernels read."""
+    return torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_attention_layer_takes_tables_off_a_boundary(qk_norm, packed):
+    """As the norm's own call does: in the fused layer, in its recorded backward, module by module, and negated lazily."""
+    from tests.test_layers_gpu import _attention, _modules_only
+
+    print(f"\n[case] attention layer, tables off a boundary, qk_norm={qk_norm} packed={packed}", flush=True)
+    lengths = [20, 13] if packed else None
+    m, (cos, sin) = _attention(4, 2, 64, 33, rope_kernel="hip", qk_norm=qk_norm)
+    more = ()
+    if packed:
+        more = (_packing(lengths, 4, 2),)
+        cos, sin = cos[more[0].positions], sin[more[0].positions]
+    x = torch.randn(1, 33, 256, device="cuda").bfloat16().requires_grad_()
+    dy = torch.randn(1, 33, 256, device="cuda").bfloat16()
+
+    def run(mod, c, s, **kw):
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            y = mod(x, c, s, *more)
+        return (y.detach(), *(g.detach() for g in torch.autograd.grad(y, (x, *mod.parameters()), dy, **kw)))
+
+    odd = [_shifted(t) for t in (cos, sin)]
+    assert all(t.is_contiguous() and t.data_ptr() % 16 for t in odd)
+    lazy = [torch._neg_view(-t) for t in (cos, sin)]
+    assert all(t.is_neg() and t.is_contiguous() for t in lazy)
+    for mod, kw in ((m, {}), (_modules_only(m), {}), (m, dict(create_graph=True))):
+        want = run(mod, cos, sin, **kw)
+        for tables in (odd, lazy):
+            for a, b in zip(run(mod, *tables, **kw), want):
+                assert torch.equal(a, b)
+
+
+def test_rotations_take_tables_off_a_boundary():
+    from nanonemo_amd.kernels.hip.flash_attn import flash_attn_bthd_rope
+    from nanonemo_amd.kernels.hip.rope import rope_k, rope_qk
+    from nanonemo_amd.model import rope_tables
+
+    print("\n[case] rotations, tables off a boundary", flush=True)
+    q, k, v = (torch.randn(2, 33, h, 64, device="cuda").bfloat16().requires_grad_() for h in (4, 2, 2))
+    tables = [t.cuda() for t in rope_tables(64, 40, 10000.0)]
+    for f in (lambda *t: torch.cat(rope_qk(q, k, *t), 2), lambda *t: rope_k(k, *t), lambda *t: flash_attn_bthd_rope(q, k, v, *t)):
+        outs = []
+        for t in (tables, [_shifted(t) for t in tables]):
+            y = f(*t)
+            outs.append((y.detach(), *torch.autograd.grad(y.float().square().sum(), (q, k, v), allow_unused=True)))
+        for a, b in zip(*outs):
+            assert a is None and b is None or torch.equal(a, b)
+
+
+def test_the_layer_s_norms_come_back_from_saved_tensor_hooks_off_a_boundary():
+    from tests.test_layers_gpu import _attention, _saved_through
+
+    m, (cos, sin) = _attention(4, 2, 64, 33, rope_kernel="hip", qk_norm=True)
+    x = torch.randn(1, 33, 256, device="cuda").bfloat16().requires_grad_()
+
+    def f():
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            return m(x, cos, sin), (x, *m.parameters())
+
+    ref = _saved_through(lambda t: t, f)
+    for a, b in zip(_saved_through(lambda t: _shifted(t) if t.dim() == 1 and t.dtype == torch.float32 else t, f), ref):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("lengths", [[300, 1000, 5], [30] * 40 + [50] * 20, [700] * 60 + [20] * 400, [4096]])
 def test_a_list_that_was_overwritten_leaves_the_memory_around_the_tensors(lengths):
     """What the kernels write lies side by side with rows of a pattern between: none of it changes, nor does what they read,
