@@ -1956,7 +1956,7 @@ struct Workspace {
     float* nD;
     float* nL;
     float* part;  // dK / dV split partials (nsplit > 1 only)
-    int nsplit;
+    int nsplit = 1;  // (packed: each list entry has its own)
     size_t bytes;
 };
 
@@ -2594,7 +2594,6 @@ int take_packed_lays(const int64_t* strides, const PlanHead& p, int64_t D, bool 
 Workspace carve_packed(void* base, const PlanHead& p, int64_t D) {
     const size_t vec = round256(4 * (size_t)p.H * p.tokens);
     Workspace w;
-    w.nsplit = p.nslots > 0 ? 2 : 1;
     w.nD = (float*)base;
     w.nL = (float*)((char*)base + vec);
     w.part = (float*)((char*)base + 2 * vec);

@@ -289,13 +289,6 @@ def check_distill(rc: int) -> None:
         raise RuntimeError(msg or f"nanonemo_distill call failed with code {rc}")
 
 
-def check_qk_norm(rc: int) -> None:
-    """Raise RuntimeError with the library's message when an nn_qk_norm_* entry point returns non-zero."""
-    if rc != 0:
-        msg = lib().nn_qk_norm_last_error().decode(errors="replace")
-        raise RuntimeError(msg or f"nanonemo_qk_norm call failed with code {rc}")
-
-
 def check_rmsnorm(rc: int) -> None:
     """Raise RuntimeError with the library's message when an nn_add_rmsnorm_* entry point returns non-zero."""
     if rc != 0:
