@@ -1624,7 +1624,7 @@ __global__ __launch_bounds__(256, 4) void fa_short_fwd_kernel(const u16* __restr
 //   S = Q K^T, dP = dO V^T         (lane: a key)           P, dS
 //   dV^T += dO^T P, dK^T += Q^T dS, dQ^T = K^T dS^T
 // Products are repeated rather than turned round: 28 matrix instructions a head take a fifth of its bytes' time. 16384 tokens in 1006
-// sequences: 28.4 us (4.7 TB/s) where the waves below took 52; 65536 in 11964 227 for 481. (Sequences of two tiles in the same
+// sequences: 28.4 us (3.9 TB/s) where the waves below took 52; 65536 in 11964 227 for 481. (Sequences of two tiles in the same
 // way, a wave a tile: 81 us for 52, more rows for each wave one after another and no registers for them.)
 // lds: K; Q and dO of this head and of the next.
 template <int HD, int DT>

@@ -8,10 +8,10 @@ and the backward writes dq, dk and dv as column ranges of one buffer, rotates th
 product for the input's gradient and one call for the three weights'.
 That is 6 launches forward and 9 to 11 backward, where the modules take 27 in all: a cast, a product and a rounding
 per weight each way, three input gradients added in 16 bits. With a packing (kernels/hip/packed.py) the attention is
-nn_fa_packed_*, on the same strides: 652 k tokens/s of training on documents of about 300 tokens, module by module 630 k.
+nn_fa_packed_*, on the same strides: 666 k tokens/s of training on documents of about 300 tokens, module by module 643 k.
 With norms of the heads (``norms``) the rotation is nn_qk_norm_rope_*: q and k stay as the product wrote them, for the norm's
-backward, and its keys go behind v in the same rows, whose stride the attention wants of both (dense 661 -> 675 k tokens/s,
-packed 631 -> 646 k).
+backward, and its keys go behind v in the same rows, whose stride the attention wants of both (dense 674 -> 689 k tokens/s,
+packed 644 -> 660 k).
 
 MLP: one product for gate and up, SwiGLU on its two halves (nn_swiglu_*), the down product; backward, one call for
 the gate's and up's weight gradients and one product for the input's gradient. 4 launches forward and 6 to 8 backward

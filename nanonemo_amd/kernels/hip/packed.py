@@ -107,7 +107,8 @@ _flash_attn_packed.register_autograd(_backward, setup_context=_setup_context)
 
 def flash_attn_packed(q: Tensor, k: Tensor, v: Tensor, packing: Packing) -> Tensor:
     """Causal GQA attention within each of the packing's sequences: q (tokens, H, hd), k and v (tokens, KVH, hd), fp16 or bf16,
-    -> (tokens, H, hd), contiguous. Column ranges of a projection are read in place where q is one, or k and v both are."""
+    -> (tokens, H, hd), contiguous. Column ranges of a projection are read in place where q is one, or k and v both are;
+    in the backward q is copied unless the gradient of the output has its strides."""
     if forward_ad._current_level >= 0:
         refuse_forward_ad("flash_attn_packed", q, k, v)
     if eager(q, k, v):  # the same launches as the op's, as one autograd node of the host module
